@@ -42,7 +42,7 @@ extern "C" {
 #define NT_DTYPE_F16 1
 #define NT_DTYPE_BF16 2
 #define NT_DTYPE_E5M2 3 /* GEMM bias (c) only: OCP float8_e5m2 */
-#define NT_DTYPE_E4M3 4 /* GEMM bias (c) only: OCP float8_e4m3fn */
+#define NT_DTYPE_E4M3 4 /* GEMM bias (c) and key/value caches: OCP float8_e4m3fn */
 
 /* Manifest check: returns NT_ABI_VERSION. Replaces the reference's ABI field of
  * its built manifest (reference src/ninetoothed/compiler/runtime.py:1485-1503). */
@@ -402,6 +402,76 @@ int nt_attention_ws_bf16(const void* q, const int64_t* q_strides, const void* k,
                          const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
                          int o_dtype, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int64_t D,
                          float q_scale, int causal, hipStream_t stream, void* workspace, int64_t workspace_bytes);
+
+/* ---------------------------------------------------------------------------
+ * Operators around a paged key/value cache (no counterpart in the reference, whose attention
+ * application takes dense [B, H, S, D] tensors only): the steps of a program that answers with
+ * a model, beside nt_attention_*.  Three strides of a packed tensor are those of (token, head,
+ * element), of a cache those of (page, slot, head) with elements side by side.  Sequences are packed
+ * one behind another along the token axis: `starts` [sequences + 1] int32 on the device holds where
+ * each begins, clamped to the tensor's tokens; rows behind the last sequence are left alone.
+ *
+ * Rotation by position: pair i < pairs of a head's first 2 * pairs elements, (a, b) = x[i],
+ * x[i + pairs], or x[2 i], x[2 i + 1] with `interleaved`, becomes
+ *   (a c - b s, b c + a s),  c, s = magnitude * cos, sin(position * freqs[i]),
+ * in fp32 with the angle reduced in fp64, rounded once; the other elements are copied.  `inverse`
+ * turns back: with it the gradient of y gives the gradient of x.  `positions` are
+ * int32 or int64 (position_bits); a token of negative position is left alone.  out may be x.
+ * dim <= 512; dtype F32, F16 or BF16. */
+int nt_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t* out_strides, int dtype,
+              const void* positions, int64_t position_stride, int position_bits, const double* freqs,
+              int64_t tokens, int64_t heads, int64_t dim, int64_t pairs, int interleaved, int inverse,
+              float magnitude, hipStream_t stream);
+
+/* New tokens' k (rotated as above by their position) and v into a paged cache.  Token i of sequence
+ * b gets position lengths[b] + i: slot position % page_size of page tables[b][position / page_size].
+ * A token past its table's width, or of a page outside [0, pages), is not stored.  Two sequences
+ * may share pages, but no page into which this call writes for both.
+ * cache_dtype is dtype (F16 or BF16), or NT_DTYPE_E4M3 with k_scale, v_scale [pages, heads] (contiguous):
+ * stored is x / scale, with scale the least power of two (from 2^-64 on) for which 448 scale is
+ * at least the page's largest finite value.  A page whose slot 0 is among the new tokens takes a
+ * scale afresh; else the scale only grows, and what the page held before the new slots is divided to match.
+ * Infinities are stored as NaN.  dim a multiple of 4 up to 128; pages of 8 bits up to 128 slots. */
+int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
+                    void* k_cache, const int64_t* kc_strides, void* v_cache, const int64_t* vc_strides,
+                    int cache_dtype, float* k_scale, float* v_scale, const int32_t* tables, int64_t table_stride,
+                    const int32_t* lengths, const int32_t* starts, const double* freqs, int64_t tokens,
+                    int64_t sequences, int64_t heads, int64_t dim, int64_t pages, int64_t page_size,
+                    int64_t table_width, int64_t pairs, int interleaved, float magnitude, hipStream_t stream);
+
+/* Attention of packed prompts: o_i = sum_j p_ij v_j, p the softmax of scale q_i . k_j over the keys j
+ * of i's sequence, with `causal` those with j <= i + (its keys - its queries).  Head h of q reads head
+ * h / (heads / kv_heads) of k and v.  A query that sees no key gives zeros.  dtype F16 or BF16 (all
+ * tensors), dim <= 128, any strides (unit element strides, strides of multiples of 8 and 16-byte
+ * aligned tensors take vector loads). */
+int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides, int dtype,
+                        const int32_t* q_starts, const int32_t* k_starts, int64_t q_tokens, int64_t k_tokens,
+                        int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, float scale, int causal,
+                        hipStream_t stream);
+
+/* Attention of one query a sequence ([sequences, heads, dim]) over the first lengths[b] keys (at most
+ * page_size * table_width) of its pages: as above, not causal, with the cache's layouts and types;
+ * E4M3 values count times their page's and head's scale (not negative; a v scale below 2^-64 counts
+ * as 2^-64).  Keys of a page outside [0, pages) do not count; without keys the output is zero.
+ * dim a multiple of 16 up to 128; caches 16-byte aligned, with strides of multiples of 16 bytes.
+ * The workspace (16-byte aligned, nt_cache_attention_workspace_size bytes, 0: none needed) holds
+ * partial states of sequences whose keys are split over workgroups; nothing between calls. */
+int64_t nt_cache_attention_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
+                                          int64_t page_size, int64_t table_width);
+int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,
+                       const void* v_cache, const int64_t* v_strides, int cache_dtype, const float* k_scale,
+                       const float* v_scale, void* o, const int64_t* o_strides, int dtype, const int32_t* tables,
+                       int64_t table_stride, const int32_t* lengths, int64_t sequences, int64_t heads,
+                       int64_t kv_heads, int64_t dim, int64_t pages, int64_t page_size, int64_t table_width,
+                       float scale, hipStream_t stream, void* workspace, int64_t workspace_bytes);
+
+/* The same with their arguments in one array, in order: an int64 for each (pointers as their address,
+ * a float as its bits), an array of strides as its three values. */
+int nt_rotary_packed(const int64_t* v);
+int nt_cache_append_packed(const int64_t* v);
+int nt_prompt_attention_packed(const int64_t* v);
+int nt_cache_attention_packed(const int64_t* v);
 
 /* ---------------------------------------------------------------------------
  * Generic kernels for programs that match none of the families above.  They replace

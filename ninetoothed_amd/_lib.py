@@ -24,7 +24,7 @@ DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
 DTYPE_E5M2 = 3  # GEMM bias (c) only
-DTYPE_E4M3 = 4
+DTYPE_E4M3 = 4  # GEMM bias (c), key/value caches
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -97,13 +97,22 @@ _SIGNATURES = {
         for t in ("f16", "bf16")
     },
     "nt_attention_workspace_size": (_I64,) * 5 + (_I, _I),
+    "nt_rotary": (_P, _I64P, _P, _I64P, _I, _P, _I64, _I, _P, _I64, _I64, _I64, _I64, _I, _I, _F, _P),
+    "nt_cache_append": (_P, _I64P, _P, _I64P, _I, _P, _I64P, _P, _I64P, _I, _P, _P, _P, _I64, _P, _P, _P) + (_I64,) * 8
+                       + (_I, _F, _P),
+    "nt_prompt_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P) + (_I64,) * 6 + (_F, _I, _P),
+    "nt_cache_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P, _P, _I64P, _I, _P, _I64, _P) + (_I64,) * 7
+                          + (_F, _P, _P, _I64),
+    "nt_cache_attention_workspace_size": (_I64,) * 6,
+    **{f"nt_{op}_packed": (_I64P,) for op in ("rotary", "cache_append", "prompt_attention", "cache_attention")},
     "nt_rtc_compile": (ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_P), _I64P, ctypes.c_char_p, _I64),
     "nt_rtc_free": (_P,),
     "nt_rtc_load": (_P, ctypes.c_char_p, ctypes.POINTER(_P)),
     "nt_rtc_launch": (_P, ctypes.c_uint32, ctypes.c_uint32, ctypes.POINTER(_P), _P),
 }
 _RESTYPES = {"nt_conv2d_workspace_size": ctypes.c_int64, "nt_attention_workspace_size": ctypes.c_int64,
-             "nt_gemm_workspace_size": ctypes.c_int64, "nt_rtc_free": None}
+             "nt_gemm_workspace_size": ctypes.c_int64, "nt_cache_attention_workspace_size": ctypes.c_int64,
+             "nt_rtc_free": None}
 
 _lock = threading.Lock()
 _library = None

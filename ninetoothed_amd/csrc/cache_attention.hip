@@ -1,0 +1,632 @@
+// Attention of one query a sequence over a paged key/value cache, in 16 bits or in 8 with a scale
+// for each page and head.
+#include "packed.h"
+#include "mfma_core.h"
+
+#include <algorithm>
+
+namespace nt {
+namespace ca {
+
+constexpr int NW = 4;        // waves per workgroup
+constexpr int BN = 32;       // keys a wave takes at a time
+constexpr int BLOCK = NW * BN;
+constexpr int BQ = 16;       // query rows: heads that share a head of k and v
+constexpr float RESCALE_LOG2 = 8.0f;
+constexpr float LEAST_SCALE = 0x1p-64f;  // a smaller v scale (or none) counts as this one
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf162_t __attribute__((ext_vector_type(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct mma16;
+template <>
+struct mma16<f16_t> {
+  typedef half8 frag;
+  __device__ __forceinline__ static floatx4 mma(frag a, frag b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{lo, hi}, half2_t));
+  }
+  template <bool HIGH>
+  __device__ __forceinline__ static uint32_t of_e4m3(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
+  }
+};
+template <>
+struct mma16<bf16_t> {
+  typedef bf16x8 frag;
+  __device__ __forceinline__ static floatx4 mma(frag a, frag b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{lo, hi}, bf162_t));
+  }
+  template <bool HIGH>
+  __device__ __forceinline__ static uint32_t of_e4m3(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+  }
+};
+// Eight e4m3 values (two dwords) as eight of type T: exact, in either type.
+template <typename T>
+__device__ __forceinline__ u32x4 wide8(uint32_t lo, uint32_t hi) {
+  return u32x4{mma16<T>::template of_e4m3<false>(lo), mma16<T>::template of_e4m3<true>(lo),
+               mma16<T>::template of_e4m3<false>(hi), mma16<T>::template of_e4m3<true>(hi)};
+}
+template <int WORDS>
+struct Words {
+  uint32_t w[WORDS];
+};
+
+}  // namespace ca
+
+struct CacheArgs {
+  const void *q, *k, *v;
+  void* o;
+  const float *k_scale, *v_scale;
+  int64_t qs[3], os[3];  // sequence, head, element
+  int64_t ks[3], vs[3];  // page, slot, head (elements side by side)
+  const int32_t *tables, *lengths;
+  int64_t table_stride, pages;
+  int sequences, kv_heads, group, dim, page_size, table_width, row_blocks, workgroups;
+  float scale_log2;
+  float *part_o, *part_ml;  // of partial states, two a workgroup: [slot][row][DM], [slot][row][2]
+};
+
+// The work is a line of blocks of 128 keys: sequence by sequence, head by head (and block of 16
+// query rows), one block at least for each.  Every workgroup takes an equal stretch of the line,
+// so that sequences of very different lengths fill the chip evenly; where the stretch starts, the
+// workgroups find out for themselves from the lengths.
+struct Line {
+  int64_t share;
+  __device__ __forceinline__ static int keys(const CacheArgs& g, int b) {
+    return min(max(g.lengths[b], 0), g.table_width * g.page_size);
+  }
+  __device__ __forceinline__ static int blocks(const CacheArgs& g, int b) {
+    return max(1, (keys(g, b) + ca::BLOCK - 1) / ca::BLOCK);
+  }
+};
+// Blocks of all sequences before `upto` and of all (in blocks of one head), by the 256 lanes.
+__device__ __forceinline__ void line_sums(const CacheArgs& g, int upto, int64_t* sums, int64_t& before, int64_t& all) {
+  int64_t mine = 0, mine_before = 0;
+  for (int b = threadIdx.x; b < g.sequences; b += 256) {
+    const int n = Line::blocks(g, b);
+    mine += n;
+    mine_before += b < upto ? n : 0;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    mine += __shfl_xor(mine, off, 64);
+    mine_before += __shfl_xor(mine_before, off, 64);
+  }
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    sums[wave] = mine;
+    sums[4 + wave] = mine_before;
+  }
+  __syncthreads();
+  all = sums[0] + sums[1] + sums[2] + sums[3];
+  before = sums[4] + sums[5] + sums[6] + sums[7];
+}
+__device__ __forceinline__ int64_t line_share(const CacheArgs& g, int64_t all_blocks) {
+  return max((int64_t)1, cdiv(all_blocks, g.workgroups));
+}
+
+// Per sequence and head of k and v, for the heads of q that share it (rows i):
+//   s_ij = scale q_i . (kq_j ks_j),  o_i = sum_j p_ij (vq_j vs_j) / sum_j p_ij,  p_ij = exp(s_ij - m_i)
+// over its cached keys; an empty sequence gives zeros.
+// HBM-bound: each cached element is read once, 4 group flops for each.  The rows of a group are
+// the columns of 16 x 16 x 32 products, so that MHA to MQA read the cache once: S^T = K Q^T, with
+// keys as the rows, and O^T += V^T P^T.  Every wave takes 32 keys at a time straight into registers,
+// the next 32 in flight meanwhile; P^T goes from the scores' registers to the second product as it
+// is, and V, read eight keys by DM / 16 neighbouring elements a lane, is transposed by byte permutes.
+// 8 bits: e4m3 widens exactly, so k's scale multiplies the score and v's enters the weight:
+//   w_ij = exp2(s_ij + log2 vs_j - M_i),  o_i = sum_j w_ij vq_j / sum_j w_ij / vs_j,
+// with M the running max of the exponents: w stays within 2^8 for any scales, is rounded to fp16
+// (11 bits, also for bf16 queries) for the product with v, and its sum stays in fp32.
+// ONE_PAGE: pages are whole multiples of 32 keys, so that a wave's 32 keys lie in one page and
+// their address is uniform; else each key's page is looked up.
+template <typename T, bool EIGHT, int DM, bool ONE_PAGE>
+__global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs g) {
+  using namespace ca;
+  typedef typename std::conditional<EIGHT, f16_t, T>::type P;  // the type of V^T P^T
+  typedef mma16<T> MQ;
+  typedef mma16<P> MP;
+  constexpr int ES = EIGHT ? 1 : 2;
+  constexpr int STEPS = DM / 32;                   // products over the elements of q and k
+  constexpr int KL = DM * ES / 64;                 // 16-byte loads of a key a lane
+  constexpr int DL = DM / 16, VW = DL * ES / 4;    // elements of v a lane, and their words
+  constexpr int OROW = DM + 4;
+  __shared__ float merge_o[NW][BQ * OROW];
+  __shared__ float merge_ml[NW][2][BQ];
+  __shared__ int64_t sums[8];
+  __shared__ int64_t key_at[NW][2][2][ONE_PAGE ? 1 : BN];
+  __shared__ float key_scale[NW][2][3][ONE_PAGE || !EIGHT ? 1 : BN];
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int D = g.dim;
+
+  const int lines = g.kv_heads * g.row_blocks;  // of a sequence
+  int64_t none, all;
+  line_sums(g, 0, sums, none, all);
+  const int64_t share = line_share(g, all * lines);
+  int64_t at = blockIdx.x * share;
+  const int64_t stop = min(at + share, all * lines);
+  if (at >= stop) return;
+  const int64_t begin = at;
+  // The sequence of the stretch's first block, and the line's length up to it: each lane
+  // holds the sum of a run of sequences, whose prefix tells the run that holds `at`.
+  int b;
+  int64_t seq0;  // blocks of the line before sequence b
+  {
+    const int run = (g.sequences + 63) / 64;
+    int64_t mine = 0;
+    for (int i = 0; i < run; ++i) {
+      const int s = lane * run + i;
+      if (s < g.sequences) mine += Line::blocks(g, s);
+    }
+    mine *= lines;
+    int64_t upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t other = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += other;
+    }
+    const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
+    seq0 = __shfl(upto - mine, who, 64);
+    b = who * run;
+    for (;; ++b) {
+      const int64_t n = (int64_t)Line::blocks(g, b) * lines;
+      if (seq0 + n > at) break;
+      seq0 += n;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+  }
+
+  while (at < stop) {
+    const int len = Line::keys(g, b), nblk = Line::blocks(g, b);
+    const int64_t inside = at - seq0;
+    const int line = (int)(inside / nblk), blk0 = (int)(inside % nblk);
+    const int blk1 = (int)min((int64_t)nblk, blk0 + (stop - at));
+    const int h = line / g.row_blocks, rb = line % g.row_blocks;
+    const int rows = min(BQ, g.group - rb * BQ);
+    const int head0 = h * g.group + rb * BQ;
+
+    typename MQ::frag qf[STEPS];
+    {
+      const uint16_t* Q = (const uint16_t*)g.q + b * g.qs[0] + (head0 + col) * g.qs[1];
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        uint16_t x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = EIGHT ? (s >> 1) * 64 + quad * 16 + (s & 1) * 8 + e : s * 32 + quad * 8 + e;
+          x[e] = col < rows && d < D ? Q[d * g.qs[2]] : (uint16_t)0;
+        }
+        qf[s] = __builtin_bit_cast(typename MQ::frag, *(const u32x4*)x);
+      }
+    }
+    floatx4 acc[DL];
+#pragma unroll
+    for (int c = 0; c < DL; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    const int32_t* table = g.tables + b * g.table_stride;
+    const char* kbase = (const char*)g.k + h * g.ks[2] * ES;
+    const char* vbase = (const char*)g.v + h * g.vs[2] * ES;
+    const int tiles = (len + BN - 1) / BN;
+    const int t_end = min(blk1 * NW, tiles);
+
+    struct Tile {
+      u32x4 k[2][KL];
+      Words<VW> v[8];
+      float kf, lv, rv;  // ONE_PAGE: k's factor, log2 and reciprocal of v's scale
+      bool ok;
+    };
+    auto scales = [&](int64_t page, float& kf, float& lv, float& rv) {
+      const float ks = g.k_scale[page * g.kv_heads + h], vs = fmaxf(g.v_scale[page * g.kv_heads + h], LEAST_SCALE);
+      kf = ks * g.scale_log2;
+      lv = __builtin_amdgcn_logf(vs);
+      rv = 1.0f / vs;
+    };
+    auto load = [&](Tile& x, int t, int buf) {
+      const int k0 = t * BN, last = min(BN, len - k0) - 1;  // (keys past the end repeat the last one)
+      int64_t page = 0;
+      const char *kp = kbase, *vp = vbase;
+      x.ok = true;
+      if (ONE_PAGE) {
+        page = table[k0 / g.page_size];
+        x.ok = page >= 0 && page < g.pages;
+        if (!x.ok) page = 0;
+        const int slot = k0 % g.page_size;
+        kp += (page * g.ks[0] + slot * g.ks[1]) * ES;
+        vp += (page * g.vs[0] + slot * g.vs[1]) * ES;
+        if (EIGHT) scales(page, x.kf, x.lv, x.rv);
+      } else {
+        // Each lane looks up key lane % 32; the wave's lanes then take what they need of them.
+        const int key = k0 + min(lane & 31, last), n = key / g.page_size;
+        page = table[n];
+        const bool ok = page >= 0 && page < g.pages;
+        if (!ok) page = 0;
+        const int slot = key - n * g.page_size;
+        if (lane < 32) {
+          key_at[wave][buf][0][lane] = (page * g.ks[0] + slot * g.ks[1]) * ES;
+          key_at[wave][buf][1][lane] = (page * g.vs[0] + slot * g.vs[1]) * ES;
+          if (EIGHT) {
+            float kf, lv, rv;
+            scales(page, kf, lv, rv);
+            key_scale[wave][buf][0][lane] = kf;
+            key_scale[wave][buf][1][lane] = lv;
+            key_scale[wave][buf][2][lane] = rv;
+          }
+        }
+        x.ok = !__builtin_amdgcn_ballot_w64(!ok);
+        wave_lds_order();
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int key = kb * 16 + col;
+        const char* row = ONE_PAGE ? kp + min(key, last) * (int)(g.ks[1] * ES) : kbase + key_at[wave][buf][0][ONE_PAGE ? 0 : key];
+#pragma unroll
+        for (int u = 0; u < KL; ++u) {
+          const int d = (EIGHT ? u * 64 + quad * 16 : u * 32 + quad * 8);
+          x.k[kb][u] = D == DM || d < D ? *(const u32x4*)(row + d * ES) : u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = (e >> 2) * 16 + quad * 4 + (e & 3);
+        const char* row = ONE_PAGE ? vp + min(key, last) * (int)(g.vs[1] * ES) : vbase + key_at[wave][buf][1][ONE_PAGE ? 0 : key];
+        const int d = col * DL;  // (elements past D reach outputs past D only)
+        x.v[e] = *(const Words<VW>*)(row + (D == DM || d < D ? d : 0) * ES);
+      }
+    };
+    auto compute = [&](Tile& x, int t, int buf) {
+      if (ONE_PAGE && !x.ok) return;
+      floatx4 s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        s[kb] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+          u32x4 w;
+          if (EIGHT) {
+            const u32x4 r = x.k[kb][st >> 1];
+            w = st & 1 ? wide8<T>(r[2], r[3]) : wide8<T>(r[0], r[1]);
+          } else {
+            w = x.k[kb][st];
+          }
+          s[kb] = MQ::mma(__builtin_bit_cast(typename MQ::frag, w), qf[st], s[kb]);
+        }
+      }
+      const int k0 = t * BN;
+      float y[8], rv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = (e >> 2) * 16 + quad * 4 + (e & 3);
+        if (!EIGHT) {
+          y[e] = s[e >> 2][e & 3] * g.scale_log2;
+        } else if (ONE_PAGE) {
+          y[e] = __builtin_fmaf(s[e >> 2][e & 3], x.kf, x.lv);
+          rv[e] = x.rv;
+        } else {
+          y[e] = __builtin_fmaf(s[e >> 2][e & 3], key_scale[wave][buf][0][ONE_PAGE || !EIGHT ? 0 : key],
+                                key_scale[wave][buf][1][ONE_PAGE || !EIGHT ? 0 : key]);
+          rv[e] = key_scale[wave][buf][2][ONE_PAGE || !EIGHT ? 0 : key];
+        }
+      }
+      if (k0 + BN > len) {  // (the last key's row stands in for those past it: nothing of it counts twice)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + (e >> 2) * 16 + quad * 4 + (e & 3) >= len) {
+            y[e] = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) x.v[e].w[w] = 0u;
+          }
+      }
+      if (!ONE_PAGE && !x.ok) {  // keys of no page: no weight, and nothing of what was read for them
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int n = min(k0 + (e >> 2) * 16 + quad * 4 + (e & 3), len - 1) / g.page_size;
+          if (table[n] < 0 || table[n] >= g.pages) {
+            y[e] = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) x.v[e].w[w] = 0u;
+          }
+        }
+      }
+      float mx = y[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, y[e]);
+      if (__builtin_amdgcn_ballot_w64(mx > m + RESCALE_LOG2)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const bool grow = mx > m + RESCALE_LOG2;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+        l *= alpha;
+#pragma unroll
+        for (int c = 0; c < DL; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[c][r] *= alpha;
+        if (grow) m = mx;
+      }
+      const float shift = m == -INFINITY ? 0.f : m;  // (no key of the wave counted yet: weights of 0)
+      u32x4 pw;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(y[e] - shift), p1 = __builtin_amdgcn_exp2f(y[e + 1] - shift);
+        l = EIGHT ? __builtin_fmaf(p0, rv[e], l) : l + p0;
+        l = EIGHT ? __builtin_fmaf(p1, rv[e + 1], l) : l + p1;
+        pw[e >> 1] = MP::pack(p0, p1);
+      }
+      const typename MP::frag pf = __builtin_bit_cast(typename MP::frag, pw);
+      if (EIGHT) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t tr[2][4];  // [keys 0-3, 4-7][element]: four keys' bytes of one element
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t a0 = x.v[4 * q].w[w], a1 = x.v[4 * q + 1].w[w], a2 = x.v[4 * q + 2].w[w], a3 = x.v[4 * q + 3].w[w];
+            const uint32_t l01 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), h01 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
+            const uint32_t l23 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), h23 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+            tr[q][0] = __builtin_amdgcn_perm(l23, l01, 0x05040100u);
+            tr[q][1] = __builtin_amdgcn_perm(l23, l01, 0x07060302u);
+            tr[q][2] = __builtin_amdgcn_perm(h23, h01, 0x05040100u);
+            tr[q][3] = __builtin_amdgcn_perm(h23, h01, 0x07060302u);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[4 * w + e] = MP::mma(__builtin_bit_cast(typename MP::frag, wide8<P>(tr[0][e], tr[1][e])), pf, acc[4 * w + e]);
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+            u32x4 a;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = __builtin_amdgcn_perm(x.v[2 * j + 1].w[w], x.v[2 * j].w[w], sel);
+            acc[2 * w + e] = MP::mma(__builtin_bit_cast(typename MP::frag, a), pf, acc[2 * w + e]);
+          }
+      }
+    };
+    {
+      int t = blk0 * NW + wave;
+      Tile x, y;
+      if (t < t_end) load(x, t, 0);
+      while (t < t_end) {
+        if (t + NW < t_end) load(y, t + NW, 1);
+        compute(x, t, 0);
+        t += NW;
+        if (t >= t_end) break;
+        if (t + NW < t_end) load(x, t + NW, 0);
+        compute(y, t, 1);
+        t += NW;
+      }
+    }
+
+    // The waves' states through LDS, then the output, or a partial state where the keys go on in
+    // another workgroup's stretch.
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < DL; ++c) merge_o[wave][col * OROW + (quad * 4 + r) * DL + c] = acc[c][r];
+    if (quad == 0) {
+      merge_ml[wave][0][col] = m;
+      merge_ml[wave][1][col] = l;
+    }
+    __syncthreads();
+    const bool whole = blk0 == 0 && blk1 == nblk;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (at == begin ? 0 : 1);
+    for (int e = tid; e < rows * DM; e += NW * 64) {
+      const int r = e / DM, d = e % DM;
+      float mm = merge_ml[0][0][r];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) mm = fmaxf(mm, merge_ml[w][0][r]);
+      float sum = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = merge_ml[w][0][r], sc = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
+        sum += merge_ml[w][1][r] * sc;
+        o += merge_o[w][r * OROW + d] * sc;
+      }
+      if (whole) {
+        if (d < D)
+          ((uint16_t*)g.o)[b * g.os[0] + (head0 + r) * g.os[1] + d * g.os[2]] =
+              elem<T>::from_float(sum == 0.f ? 0.f : o / sum);
+      } else {
+        g.part_o[(slot * BQ + r) * DM + d] = o;
+        if (d == 0) {
+          g.part_ml[(slot * BQ + r) * 2] = mm;
+          g.part_ml[(slot * BQ + r) * 2 + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    at += blk1 - blk0;
+    if (at - seq0 == (int64_t)nblk * lines) {
+      seq0 = at;
+      ++b;
+    }
+  }
+}
+
+// Joins the partial states of one sequence, head and block of rows, where its keys were split.
+template <typename T, int DM>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs g) {
+  using namespace ca;
+  __shared__ int64_t sums[8];
+  const int lines = g.kv_heads * g.row_blocks, b = blockIdx.x / lines, line = blockIdx.x % lines;
+  int64_t before, all;
+  line_sums(g, b, sums, before, all);
+  const int64_t share = line_share(g, all * lines);
+  const int nblk = Line::blocks(g, b);
+  const int64_t from = before * lines + (int64_t)line * nblk, to = from + nblk;
+  const int64_t w0 = from / share, w1 = (to - 1) / share;
+  if (w0 == w1) return;  // written by its one workgroup
+  const int h = line / g.row_blocks, rb = line % g.row_blocks, rows = min(BQ, g.group - rb * BQ);
+  const int64_t slot0 = 2 * w0 + (from == w0 * share ? 0 : 1);
+  for (int e = threadIdx.x; e < rows * DM; e += 256) {
+    const int r = e / DM, d = e % DM;
+    float mm = g.part_ml[(slot0 * BQ + r) * 2];
+    for (int64_t w = w0 + 1; w <= w1; ++w) mm = fmaxf(mm, g.part_ml[(2 * w * BQ + r) * 2]);
+    float sum = 0.f, o = 0.f;
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t slot = w == w0 ? slot0 : 2 * w;
+      const float mw = g.part_ml[(slot * BQ + r) * 2], sc = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
+      sum += g.part_ml[(slot * BQ + r) * 2 + 1] * sc;
+      o += g.part_o[(slot * BQ + r) * DM + d] * sc;
+    }
+    if (d < g.dim)
+      ((uint16_t*)g.o)[b * g.os[0] + (h * g.group + rb * BQ + r) * g.os[1] + d * g.os[2]] =
+          elem<T>::from_float(sum == 0.f ? 0.f : o / sum);
+  }
+}
+
+// Workgroups of a launch: 512 (two a CU), or fewer where the longest possible sequences have fewer
+// blocks; partial states only where a sequence can have more than one block.
+static int64_t cache_workgroups(int64_t lines, int64_t most_keys) {
+  return std::min<int64_t>(512, lines * std::max<int64_t>(1, cdiv(most_keys, ca::BLOCK)));
+}
+static int64_t cache_part_floats(int64_t workgroups, int64_t dm) { return workgroups * 2 * ca::BQ * (dm + 2); }
+
+template <typename T, bool EIGHT, int DM>
+static void cache_launch(const CacheArgs& g, bool join, hipStream_t stream) {
+  const dim3 grid((unsigned)g.workgroups), block(ca::NW * 64);
+  if (g.page_size % ca::BN == 0)
+    hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, true>), grid, block, 0, stream, g);
+  else
+    hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, false>), grid, block, 0, stream, g);
+  if (join)
+    hipLaunchKernelGGL((cache_join_kernel<T, DM>), dim3((unsigned)(g.sequences * g.kv_heads * g.row_blocks)), dim3(256), 0,
+                       stream, g);
+}
+
+}  // namespace nt
+
+extern "C" int64_t nt_cache_attention_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
+                                                     int64_t page_size, int64_t table_width) {
+  if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim > 128 || page_size <= 0 ||
+      table_width <= 0 || page_size * table_width <= nt::ca::BLOCK)
+    return 0;
+  const int64_t lines = sequences * kv_heads * nt::cdiv(heads / kv_heads, nt::ca::BQ);
+  return nt::cache_part_floats(nt::cache_workgroups(lines, page_size * table_width), dim <= 64 ? 64 : 128) * 4;
+}
+
+extern "C" int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,
+                                  const void* v_cache, const int64_t* v_strides, int cache_dtype, const float* k_scale,
+                                  const float* v_scale, void* o, const int64_t* o_strides, int dtype,
+                                  const int32_t* tables, int64_t table_stride, const int32_t* lengths,
+                                  int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages,
+                                  int64_t page_size, int64_t table_width, float scale, hipStream_t stream,
+                                  void* workspace, int64_t workspace_bytes) {
+  const bool eight = cache_dtype == NT_DTYPE_E4M3;
+  const int es = eight ? 1 : 2;
+  if (sequences < 0 || heads < 0 || kv_heads < 0 || dim < 0 || dim > 128 || dim % 16 || pages < 0 || page_size < 1 ||
+      table_width < 0 || sequences > (1 << 24) || heads > (1 << 20) || page_size > 0x7fffff00LL ||
+      table_width > 0x7fffff00LL || page_size * table_width > 0x7fffff00LL)
+    return NT_ERR_INVALID;
+  if ((dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || (!eight && cache_dtype != dtype)) return NT_ERR_INVALID;
+  if (sequences * heads * dim == 0) return 0;
+  if (kv_heads == 0 || heads % kv_heads) return NT_ERR_INVALID;
+  if (pages == 0) table_width = 0;  // no keys: every output is zero
+  if (!q || !o || !q_strides || !k_strides || !v_strides || !o_strides || !lengths) return NT_ERR_INVALID;
+  if (table_width > 0 && (!k_cache || !v_cache || !tables || (eight && (!k_scale || !v_scale)))) return NT_ERR_INVALID;
+  // Rows of 16-byte vectors; a page's slots within 32-bit byte offsets.
+  for (int i = 0; i < 3; ++i)
+    if (k_strides[i] * es % 16 || v_strides[i] * es % 16) return NT_ERR_INVALID;
+  if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || k_strides[1] < 0 || v_strides[1] < 0 ||
+      k_strides[1] * es * nt::ca::BN > 0x7fffffffLL || v_strides[1] * es * nt::ca::BN > 0x7fffffffLL)
+    return NT_ERR_INVALID;
+  nt::CacheArgs g{};
+  g.q = q;
+  g.k = k_cache;
+  g.v = v_cache;
+  g.o = o;
+  g.k_scale = k_scale;
+  g.v_scale = v_scale;
+  for (int i = 0; i < 3; ++i) {
+    g.qs[i] = q_strides[i];
+    g.os[i] = o_strides[i];
+    g.ks[i] = k_strides[i];
+    g.vs[i] = v_strides[i];
+  }
+  g.tables = tables;
+  g.lengths = lengths;
+  g.table_stride = table_stride;
+  g.pages = pages;
+  g.sequences = (int)sequences;
+  g.kv_heads = (int)kv_heads;
+  g.group = (int)(heads / kv_heads);
+  g.dim = (int)dim;
+  g.page_size = (int)page_size;
+  g.table_width = (int)table_width;
+  g.row_blocks = (int)nt::cdiv(g.group, nt::ca::BQ);
+  g.scale_log2 = scale * 1.44269504088896340736f;
+  const int64_t lines = sequences * kv_heads * g.row_blocks, dm = dim <= 64 ? 64 : 128;
+  if (lines > 0x7fffffffLL) return NT_ERR_INVALID;
+  const int64_t need = nt_cache_attention_workspace_size(sequences, heads, kv_heads, dim, page_size, table_width);
+  if (need > 0 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return NT_ERR_INVALID;
+  g.workgroups = (int)nt::cache_workgroups(lines, page_size * table_width);
+  g.part_o = (float*)workspace;
+  g.part_ml = g.part_o ? g.part_o + (int64_t)g.workgroups * 2 * nt::ca::BQ * dm : nullptr;
+  const bool join = need > 0;
+#define NT_CACHE(T, E)                                     \
+  if (dim <= 64)                                           \
+    nt::cache_launch<T, E, 64>(g, join, stream);           \
+  else                                                     \
+    nt::cache_launch<T, E, 128>(g, join, stream);
+  if (dtype == NT_DTYPE_F16) {
+    if (eight) {
+      NT_CACHE(nt::f16_t, true)
+    } else {
+      NT_CACHE(nt::f16_t, false)
+    }
+  } else {
+    if (eight) {
+      NT_CACHE(nt::bf16_t, true)
+    } else {
+      NT_CACHE(nt::bf16_t, false)
+    }
+  }
+#undef NT_CACHE
+  return nt::launch_status();
+}
+
+extern "C" int nt_cache_attention_packed(const int64_t* v) {
+  if (!v) return NT_ERR_INVALID;
+  nt::Packed p{v};
+  const void* q = p.ptr<const void>();
+  const int64_t* qs = p.array(3);
+  const void* k_cache = p.ptr<const void>();
+  const int64_t* ks = p.array(3);
+  const void* v_cache = p.ptr<const void>();
+  const int64_t* vs = p.array(3);
+  int cache_dtype = p.i();
+  const float* k_scale = p.ptr<const float>();
+  const float* v_scale = p.ptr<const float>();
+  void* o = p.ptr<void>();
+  const int64_t* os = p.array(3);
+  int dtype = p.i();
+  const int32_t* tables = p.ptr<const int32_t>();
+  int64_t table_stride = p.i64();
+  const int32_t* lengths = p.ptr<const int32_t>();
+  int64_t sequences = p.i64();
+  int64_t heads = p.i64();
+  int64_t kv_heads = p.i64();
+  int64_t dim = p.i64();
+  int64_t pages = p.i64();
+  int64_t page_size = p.i64();
+  int64_t table_width = p.i64();
+  float scale = p.f();
+  hipStream_t stream = (hipStream_t)p.ptr<void>();
+  void* workspace = p.ptr<void>();
+  int64_t workspace_bytes = p.i64();
+  return nt_cache_attention(q, qs, k_cache, ks, v_cache, vs, cache_dtype, k_scale, v_scale, o, os, dtype, tables,
+                            table_stride, lengths, sequences, heads, kv_heads, dim, pages, page_size, table_width,
+                            scale, stream, workspace, workspace_bytes);
+}

@@ -1,0 +1,80 @@
+// Sequences packed one behind another along a token axis, and the rotation of head elements by
+// position: what the kernels over a paged key/value cache share.
+#pragma once
+
+#include "nt_common.h"
+
+namespace nt {
+
+constexpr float E4M3_MAX = 448.0f;
+
+// Work over packed sequences is dealt out in units of `per` rows (a row: a token, or a token's
+// share of a group of heads) that no two sequences share.  How many there are is known on the
+// device only, so sequence b's units get the numbers from first_unit(b) on, with
+//   first_unit(b) = starts[b] * rows / per + extra * b,
+// which leaves room for every unit of b below first_unit(b + 1) as long as b has at most
+// floor(its rows / per) + extra of them: the grid needs tokens * rows / per + extra * sequences
+// numbers, a few of which stay idle, and no unit needs a prefix sum over the sequences.
+struct UnitMap {
+  const int32_t* starts;  // [sequences + 1]
+  int64_t tokens;         // rows of the packed tensor: starts are clamped to [0, tokens]
+  int sequences, rows, per, extra;
+};
+
+__host__ __device__ __forceinline__ int64_t unit_count(const UnitMap& u) {
+  return u.tokens * u.rows / u.per + (int64_t)u.extra * u.sequences;
+}
+
+__device__ __forceinline__ int64_t clamped_start(const UnitMap& u, int b) {
+  const int64_t s = u.starts[b];
+  return s < 0 ? 0 : s > u.tokens ? u.tokens : s;
+}
+__device__ __forceinline__ int64_t first_unit(const UnitMap& u, int b) {
+  return clamped_start(u, b) * u.rows / u.per + (int64_t)u.extra * b;
+}
+
+// The sequence whose range of unit numbers holds `id` (the last b with first_unit(b) <= id), by
+// a 64-way search: the lanes of a wave probe together, so up to 64 sequences take one load
+// and up to 4096 two.  The answer is the same in every lane.
+__device__ __forceinline__ int find_sequence(const UnitMap& u, int64_t id) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = u.sequences;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const uint64_t below = __builtin_amdgcn_ballot_w64(at < hi && (lane == 0 || first_unit(u, at) <= id));
+    const int n = 63 - __builtin_clzll(below);  // (starts that do not rise give some b, and its bounds hold)
+    lo += n * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// cos and sin of position * frequency, times `magnitude`.  The angle is reduced to a part of a
+// turn in 64 bits (a position of a million times a frequency of 1 leaves 2^-4 of a turn to 32
+// bits), its cosine and sine are taken in 32.
+__device__ __forceinline__ float2 rotation(double position, double frequency, float magnitude) {
+  const double turns = position * frequency * 0.15915494309189533577;
+  float s, c;
+  sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+  return float2{c * magnitude, s * magnitude};
+}
+
+// The arguments of an entry point from its packed form: one int64 each, in order (pointers as
+// their address, a float as its bits), an array of strides as its values.
+struct Packed {
+  const int64_t* v;
+  int64_t i64() { return *v++; }
+  int i() { return (int)*v++; }
+  float f() { return __builtin_bit_cast(float, (uint32_t)*v++); }
+  const int64_t* array(int n) { return (v += n) - n; }
+  template <typename P>
+  P* ptr() { return (P*)(uintptr_t)*v++; }
+};
+
+// N neighbouring elements as they lie in memory.
+template <typename S, int N>
+struct alignas(sizeof(S) * N) Vec {
+  S e[N];
+};
+
+}  // namespace nt

@@ -1,0 +1,507 @@
+// Attention over packed prompts: sequences of different lengths one behind another, heads of q
+// that share heads of k and v, causal or not.
+#include "packed.h"
+#include "mfma_core.h"
+
+#include <algorithm>
+
+namespace nt {
+namespace pa {
+
+constexpr int NW = 8;              // waves per workgroup, two per SIMD
+constexpr int BM = NW * 32;        // query rows per workgroup
+constexpr int BN = 64;             // keys per tile
+constexpr float RESCALE_LOG2 = 8.0f;
+// V^T rows: 64 keys + 8 pad.  Within each 16-key slice the keys lie in the order in which a
+// lane's P^T slots take them (0-3, 8-11 | 4-7, 12-15), so that a fragment is 16 contiguous bytes.
+constexpr int VT_STRIDE = BN + 8;
+__host__ __device__ constexpr int vt_pos(int kq) { return (kq >> 2) * 16 + ((kq & 1) << 3) + ((kq & 2) << 1); }
+
+template <int DM>
+struct Geo {
+  static constexpr int DH = DM / 64, DSUB = DM / 16, DBLK = DM / 32;
+  static constexpr int K_ELEMS = DH * BN * TILE_K;      // K tile [d-half][key][64 d]
+  static constexpr int BUF = K_ELEMS + DM * VT_STRIDE;  // + V^T tile [d][64 keys + pad]
+  static constexpr int CPR = DM / 8;                    // 16-byte chunks per key row
+  static constexpr int K_LOADS = BN * CPR / 256;
+  static constexpr int KEYS_PER_LOAD = 256 / CPR;
+};
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf162_t __attribute__((ext_vector_type(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, f16_t>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{lo, hi}, half2_t));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{lo, hi}, bf162_t));
+}
+
+// The magnitude bits of infinity in the 16-bit types: above it lie the NaN.
+template <typename T>
+constexpr uint32_t inf_bits = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
+template <typename T>
+constexpr uint32_t one_bits = std::is_same<T, f16_t>::value ? 0x3c00u : 0x3f80u;
+
+// Eight packed values with zeros for the infinities and NaN.
+template <typename T>
+__device__ __forceinline__ u32x4 finite8(u32x4 w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = ((w[i] & 0x7fffu) < inf_bits<T> ? w[i] & 0xffffu : 0u) |
+           (((w[i] >> 16) & 0x7fffu) < inf_bits<T> ? w[i] & 0xffff0000u : 0u);
+  return w;
+}
+
+}  // namespace pa
+
+struct PromptArgs {
+  const void *q, *k, *v;
+  void* o;
+  int64_t qs[3], ks[3], vs[3], os[3];  // token, head, element
+  UnitMap map;                         // of q's rows: tokens * group
+  const int32_t* k_starts;
+  int64_t k_tokens, units;
+  int kv_heads, group, dim, causal;
+  float scale_log2;  // softmax scale * log2(e)
+};
+
+// Workgroup id -> (unit, head of k and v).  Ids go to the 8 XCDs round-robin, each with its own
+// L2: when the heads divide by 8, XCD x walks heads x, x + 8, ..., so that a head's K and V stay
+// in one L2; and units run from the last to the first, the long causal ones of a sequence first.
+__device__ __forceinline__ void prompt_order(const PromptArgs& g, int64_t id, int64_t& unit, int& head) {
+  unit = g.units - 1 - id / g.kv_heads;
+  head = (int)(id % g.kv_heads);
+}
+
+// Per row i of a sequence (a token and a head of its group) over the keys j it may see:
+//   s_ij = scale q_i . k_j,  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i);
+// causal: j <= i + (keys - queries).  A row that sees no key gives zeros.
+// MFMA-bound: 4 dim flops a head and visible pair.  A workgroup takes 256 rows, a group's heads
+// side by side for each token, so that short sequences fill its rows and share K and V; eight waves
+// of 32 rows, two a SIMD.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: a lane holds
+// one row, its max and sum take no LDS, and P^T goes from the score registers to the second product
+// as it is.  Keys stream through two LDS stages of 64, fetched by waves 0-3 (K) and 4-7 (V,
+// transposed in registers on the way).
+//   - Scores stay unscaled in fp32 until exp2(s scale - m): q is not rounded a second time.
+//   - m is raised only where a tile's max passes it by 2^8 (o and l are rescaled then): p stays
+//     within 2^8 and keeps its relative precision; o / l is the same.
+//   - p is rounded to the operands' type for the product; its row sums are of the rounded p.
+//   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
+//     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: where a tile
+//     that some row masks holds one (the fetching waves look), the product is taken of the finite
+//     values and the others are added, one by one, to the rows that see them.
+// VEC: unit element strides, 16-byte aligned rows; else element by element.
+template <typename T, int DM, bool VEC>
+__global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_attention_kernel(
+    PromptArgs g) {
+  using namespace pa;
+  using G = Geo<DM>;
+  typedef typename mfma_traits<T>::frag frag;
+  constexpr int STAGE_ELEMS = NW * 32 * 65 * 2;  // output staging, fp32
+  constexpr int SMEM = 2 * G::BUF > STAGE_ELEMS ? 2 * G::BUF : STAGE_ELEMS;
+  __shared__ __attribute__((aligned(16))) uint16_t smem[SMEM];
+  __shared__ int odd_v[2];  // a stage's V holds an infinity or a NaN
+  char* lds = (char*)smem;
+
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t unit;
+  int head;
+  prompt_order(g, blockIdx.x, unit, head);
+  const int b = find_sequence(g.map, unit);
+  const int64_t q_begin = clamped_start(g.map, b);
+  const int Sq = (int)max((int64_t)0, clamped_start(g.map, b + 1) - q_begin);
+  const int64_t r0_64 = (unit - first_unit(g.map, b)) * BM;
+  const int64_t rows_64 = (int64_t)Sq * g.group;
+  if (r0_64 < 0 || r0_64 >= rows_64) return;
+  const int r0 = (int)r0_64, rows = (int)rows_64, D = g.dim;
+  auto k_clamp = [&](int64_t s) { return s < 0 ? 0 : s > g.k_tokens ? g.k_tokens : s; };
+  const int64_t k_begin = k_clamp(g.k_starts[b]);
+  const int Sk = (int)max((int64_t)0, k_clamp(g.k_starts[b + 1]) - k_begin);
+  const int offset = Sk - Sq;  // causal: token i sees keys up to i + offset
+
+  const int rw = r0 + wave * 32;  // first row of this wave
+  const int row = rw + (lane & 31);
+  const int tok = row / g.group;
+  const int qhead = head * g.group + (row - tok * g.group);
+  const int64_t es_q = VEC ? 1 : g.qs[2], es_k = VEC ? 1 : g.ks[2], es_v = VEC ? 1 : g.vs[2];
+  frag qf[G::DSUB];
+  {
+    const uint16_t* Q = (const uint16_t*)g.q + (q_begin + tok) * g.qs[0] + qhead * g.qs[1];
+#pragma unroll
+    for (int dd = 0; dd < G::DSUB; ++dd) {
+      u32x4 raw = {0u, 0u, 0u, 0u};
+      const int d = dd * 16 + half * 8;
+      if (VEC) {
+        if (row < rows && d < D) raw = *(const u32x4*)(Q + d);
+      } else {
+        uint16_t tmp[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) tmp[u] = row < rows && d + u < D ? Q[(d + u) * es_q] : (uint16_t)0;
+        raw = *(const u32x4*)tmp;
+      }
+      qf[dd] = __builtin_bit_cast(frag, raw);
+    }
+  }
+  // The last key a row sees, and how many tiles the workgroup and this wave need.
+  const int last = g.causal ? tok + offset : Sk - 1;
+  int nkt = (Sk + BN - 1) / BN, nkt_w = nkt, full_w = Sk / BN;
+  if (g.causal) {
+    const int end = (min(r0 + BM, rows) - 1) / g.group + offset, end_w = (min(rw + 32, rows) - 1) / g.group + offset;
+    nkt = end < 0 ? 0 : min(nkt, end / BN + 1);
+    nkt_w = end_w < 0 ? 0 : min(nkt, end_w / BN + 1);
+    const int begin_w = rw / g.group + offset;  // every row of the wave sees the tiles before it
+    full_w = begin_w < 0 ? 0 : min(full_w, (begin_w + 1) / BN);
+  }
+  if (rw >= rows) nkt_w = 0;
+  const int full_block = g.causal ? max(0, r0 / g.group + offset + 1) / BN : nkt;  // tiles no row masks causally
+
+  // Tile loaders: waves 0-3 K, waves 4-7 V.
+  const int lt = tid & 255;
+  const bool k_role = wave < 4, v_role = wave >= 4 && (lt >> 4) < DM / 8;
+  const uint16_t* Kb = (const uint16_t*)g.k + k_begin * g.ks[0] + head * g.ks[1];
+  const uint16_t* Vb = (const uint16_t*)g.v + k_begin * g.vs[0] + head * g.vs[1];
+  const int ks2b = (int)g.ks[0] * 2, vs2b = (int)g.vs[0] * 2;
+  // A tile's rows as a buffer that ends with the sequence: keys past it read as zeros.
+  auto tile_rows = [&](const uint16_t* base, int64_t stride, int stride2b, int k0) {
+    const int n = min(Sk - k0, BN);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (n > 0 ? k0 * stride : 0)), (short)0,
+                                             n > 0 ? (n - 1) * stride2b + D * 2 : 0, 0x00020000);
+  };
+  const int kr = lt / G::CPR, kc = lt % G::CPR;
+  const int vK = kr * ks2b + kc * 16;
+  int k_st[G::K_LOADS];
+#pragma unroll
+  for (int i = 0; i < G::K_LOADS; ++i) {
+    const int key = i * G::KEYS_PER_LOAD + kr;
+    k_st[i] = ((kc >> 3) * BN * TILE_K + key * TILE_K + swz(key, kc & 7) * 8) * 2;
+  }
+  const int kq = lt & 15, db = lt >> 4;
+  const int vV = kq * 4 * vs2b + db * 16;
+  const int v_st = (G::K_ELEMS + db * 8 * VT_STRIDE + vt_pos(kq)) * 2;
+  u32x4 rl[4 > G::K_LOADS ? 4 : G::K_LOADS];
+  auto element_row = [&](const uint16_t* base, int64_t stride, int64_t es, int key, int d) {
+    uint16_t tmp[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) tmp[u] = key < Sk && d + u < D ? base[key * stride + (d + u) * es] : (uint16_t)0;
+    return *(const u32x4*)tmp;
+  };
+  auto load_tile = [&](int kt) {
+    const int k0 = kt * BN;
+    if (k_role) {
+      const __amdgpu_buffer_rsrc_t rsK = tile_rows(Kb, g.ks[0], ks2b, k0);
+#pragma unroll
+      for (int i = 0; i < G::K_LOADS; ++i) {
+        if (VEC)
+          rl[i] = kc * 8 < D ? __builtin_amdgcn_raw_buffer_load_b128(rsK, vK, i * G::KEYS_PER_LOAD * ks2b, 0)
+                             : u32x4{0u, 0u, 0u, 0u};
+        else
+          rl[i] = element_row(Kb, g.ks[0], es_k, k0 + i * G::KEYS_PER_LOAD + kr, kc * 8);
+      }
+    }
+    if (v_role) {
+      const __amdgpu_buffer_rsrc_t rsV = tile_rows(Vb, g.vs[0], vs2b, k0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (VEC)
+          rl[r] = __builtin_amdgcn_raw_buffer_load_b128(rsV, vV, r * vs2b, 0);
+        else
+          rl[r] = element_row(Vb, g.vs[0], es_v, k0 + kq * 4 + r, db * 8);
+      }
+    }
+  };
+  auto store_tile = [&](int kt) {
+    char* base = lds + (kt & 1) * (G::BUF * 2);
+    if (k_role) {
+#pragma unroll
+      for (int i = 0; i < G::K_LOADS; ++i) *(u32x4*)(base + k_st[i]) = rl[i];
+    }
+    if (v_role) {
+      if (kt >= full_block) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            most = max(most, max(rl[r][w] & 0x7fffu, (rl[r][w] >> 16) & 0x7fffu));
+        if (most >= inf_bits<T>) {
+          odd_v[kt & 1] = 1;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) rl[r] = finite8<T>(rl[r]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = j >> 1;
+        const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+        *(u32x2*)(base + v_st + j * VT_STRIDE * 2) = u32x2{__builtin_amdgcn_perm(rl[1][d], rl[0][d], sel),
+                                                           __builtin_amdgcn_perm(rl[3][d], rl[2][d], sel)};
+      }
+    }
+  };
+
+  floatx16 o_acc[G::DBLK], l_acc;
+  // The infinities and NaN of tile kt's V, left out of the product, added where their key is seen.
+  auto add_odd = [&](int kt) {
+#pragma unroll 1
+    for (int key = kt * BN; key < min(Sk, kt * BN + BN); ++key) {
+      int64_t es = es_v;
+      if (!VEC) asm volatile("" : "+s"(es));  // (the addresses of a row are not kept over the loop)
+#pragma unroll
+      for (int i = 0; i < G::DBLK; ++i) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int d = i * 32 + r4 * 8 + half * 4;  // acc_row(4 r4, lane)
+          uint16_t x[4] = {0, 0, 0, 0};
+          if (VEC) {
+            if (d < D) *(u32x2*)x = *(const u32x2*)(Vb + key * g.vs[0] + d);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (d + u < D) x[u] = Vb[key * g.vs[0] + (d + u) * es];
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if ((x[u] & 0x7fffu) >= inf_bits<T> && key <= last) o_acc[i][4 * r4 + u] += elem<T>::to_float(x[u]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  };
+  float m = 0.f;  // the first tile sets it to its max
+#pragma unroll
+  for (int r = 0; r < 16; ++r) l_acc[r] = 0.f;
+#pragma unroll
+  for (int i = 0; i < G::DBLK; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o_acc[i][r] = 0.f;
+  const uint32_t one2 = one_bits<T> | one_bits<T> << 16;
+  const frag ones = __builtin_bit_cast(frag, u32x4{one2, one2, one2, one2});
+  const float c = g.scale_log2;
+
+  if (tid < 2) odd_v[tid] = 0;
+  __syncthreads();
+  if (nkt > 0) {
+    load_tile(0);
+    store_tile(0);
+    if (nkt > 1) load_tile(1);
+  }
+  int kt = 0;
+  for (; kt < nkt_w; ++kt) {
+    __syncthreads();
+    if (kt + 1 < nkt) {
+      store_tile(kt + 1);
+      if (kt + 2 < nkt) load_tile(kt + 2);
+    }
+    const int k0 = kt * BN;
+    const uint16_t* sK = smem + (kt & 1) * G::BUF;
+    const uint16_t* sVt = sK + G::K_ELEMS;
+    floatx16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+    for (int dd = 0; dd < G::DSUB; ++dd) {
+      const int chunk = (dd & 3) * 2 + half;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int kr2 = kb * 32 + (lane & 31);
+        const frag kf = *(const frag*)(sK + (dd >> 2) * BN * TILE_K + kr2 * TILE_K + swz(kr2, chunk) * 8);
+        s[kb] = mfma_traits<T>::mma(kf, qf[dd], s[kb]);
+      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], c, -m);
+    const bool masked = kt >= full_w;
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + kb * 32 + acc_row(r, lane);
+          if (key >= Sk || key > last) s[kb][r] = -INFINITY;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const bool grow = (kt == 0 && mx != -INFINITY) || mx > RESCALE_LOG2;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float delta = grow ? mx : 0.f, alpha = kt == 0 ? 1.f : __builtin_amdgcn_exp2f(-delta);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) l_acc[r] *= alpha;
+#pragma unroll
+      for (int i = 0; i < G::DBLK; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[i][r] *= alpha;
+      m += delta;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] -= delta;
+    }
+    frag pf[BN / 16];
+#pragma unroll
+    for (int t = 0; t < BN / 16; ++t) {
+      u32x4 w;
+#pragma unroll
+      for (int sl = 0; sl < 4; ++sl) {
+        const int e = 8 * (t & 1) + 2 * sl;
+        w[sl] = pack2<T>(__builtin_amdgcn_exp2f(s[t >> 1][e]), __builtin_amdgcn_exp2f(s[t >> 1][e + 1]));
+      }
+      pf[t] = __builtin_bit_cast(frag, w);
+    }
+    auto v_frag = [&](int t, int i) {
+      return *(const u32x4*)(sVt + (i * 32 + (lane & 31)) * VT_STRIDE + t * 16 + half * 8);
+    };
+#pragma unroll
+    for (int t = 0; t < BN / 16; ++t) l_acc = mfma_traits<T>::mma(ones, pf[t], l_acc);
+#pragma unroll
+    for (int t = 0; t < BN / 16; ++t)
+#pragma unroll
+      for (int i = 0; i < G::DBLK; ++i)
+        o_acc[i] = mfma_traits<T>::mma(__builtin_bit_cast(frag, v_frag(t, i)), pf[t], o_acc[i]);
+    if (g.causal && odd_v[kt & 1]) add_odd(kt);
+  }
+  for (; kt < nkt; ++kt) {
+    __syncthreads();
+    if (kt + 1 < nkt) {
+      store_tile(kt + 1);
+      if (kt + 2 < nkt) load_tile(kt + 2);
+    }
+  }
+  __syncthreads();  // the output staging below reuses the K and V stages
+
+  // o = acc / l through LDS, 64 elements at a time, so that a lane writes four neighbours.
+  constexpr int ST = 65;
+  float* stage = reinterpret_cast<float*>(smem) + wave * (32 * ST);
+  const float inv = l_acc[0] != 0.f ? 1.0f / l_acc[0] : 0.f;
+#pragma unroll
+  for (int ps = 0; ps < DM / 64; ++ps) {
+#pragma unroll
+    for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) stage[(lane & 31) * ST + jb * 32 + acc_row(r, lane)] = o_acc[ps * 2 + jb][r] * inv;
+    wave_lds_order();
+#pragma unroll 2
+    for (int e0 = 0; e0 < 32 * 16; e0 += 64) {
+      const int e = e0 + lane, lr = e >> 4, d0 = ps * 64 + (e & 15) * 4;
+      const int orow = rw + lr;
+      if (orow < rows && d0 < D) {
+        const int ot = orow / g.group;
+        const float* sp = stage + lr * ST + (e & 15) * 4;
+        uint16_t* O = (uint16_t*)g.o + (q_begin + ot) * g.os[0] + (head * g.group + (orow - ot * g.group)) * g.os[1];
+        if (VEC) {
+          *(u32x2*)(O + d0) = u32x2{pack2<T>(sp[0], sp[1]), pack2<T>(sp[2], sp[3])};
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (d0 + u < D) O[(d0 + u) * g.os[2]] = elem<T>::from_float(sp[u]);
+        }
+      }
+    }
+    wave_lds_order();
+  }
+}
+
+template <typename T>
+static int prompt_launch(PromptArgs g, hipStream_t stream) {
+  auto rows_ok = [&](const void* p, const int64_t* s) {
+    return s[2] == 1 && s[0] >= 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && (uintptr_t)p % 16 == 0;
+  };
+  // A tile's keys are addressed with 32-bit buffer offsets.
+  auto span_ok = [&](const int64_t* s) { return 2 * pa::BN * s[0] * 2 < 0x7fffffffLL; };
+  const bool vec = g.dim % 8 == 0 && rows_ok(g.q, g.qs) && rows_ok(g.k, g.ks) && rows_ok(g.v, g.vs) &&
+                   rows_ok(g.o, g.os) && span_ok(g.ks) && span_ok(g.vs);
+  g.map.rows = g.group;
+  g.map.per = pa::BM;
+  g.map.extra = 1;
+  g.units = unit_count(g.map);
+  if (g.units * g.kv_heads > 0x7fffffffLL) return NT_ERR_INVALID;
+  const dim3 grid((unsigned)(g.units * g.kv_heads)), block(pa::NW * 64);
+#define NT_PROMPT(DM)                                                                      \
+  if (vec)                                                                                 \
+    hipLaunchKernelGGL((prompt_attention_kernel<T, DM, true>), grid, block, 0, stream, g); \
+  else                                                                                     \
+    hipLaunchKernelGGL((prompt_attention_kernel<T, DM, false>), grid, block, 0, stream, g);
+  if (g.dim <= 64) {
+    NT_PROMPT(64)
+  } else {
+    NT_PROMPT(128)
+  }
+#undef NT_PROMPT
+  return launch_status();
+}
+
+}  // namespace nt
+
+extern "C" int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                   const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
+                                   int dtype, const int32_t* q_starts, const int32_t* k_starts, int64_t q_tokens,
+                                   int64_t k_tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
+                                   float scale, int causal, hipStream_t stream) {
+  if (q_tokens < 0 || k_tokens < 0 || sequences < 0 || heads < 0 || kv_heads < 0 || dim < 0 || dim > 128 ||
+      (dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || k_tokens > 0x7fffff00LL || sequences > (1 << 30))
+    return NT_ERR_INVALID;
+  if (q_tokens * sequences * heads * dim == 0) return 0;
+  if (kv_heads == 0 || heads % kv_heads || q_tokens * (heads / kv_heads) > 0x7fffff00LL) return NT_ERR_INVALID;
+  if (!q || !o || !q_strides || !o_strides || !q_starts || !k_starts || !k_strides || !v_strides) return NT_ERR_INVALID;
+  if (k_tokens > 0 && (!k || !v)) return NT_ERR_INVALID;
+  nt::PromptArgs g{};
+  g.q = q;
+  g.k = k;
+  g.v = v;
+  g.o = o;
+  for (int i = 0; i < 3; ++i) {
+    g.qs[i] = q_strides[i];
+    g.ks[i] = k_strides[i];
+    g.vs[i] = v_strides[i];
+    g.os[i] = o_strides[i];
+  }
+  g.map.starts = q_starts;
+  g.map.tokens = q_tokens;
+  g.map.sequences = (int)sequences;
+  g.k_starts = k_starts;
+  g.k_tokens = k_tokens;
+  g.kv_heads = (int)kv_heads;
+  g.group = (int)(heads / kv_heads);
+  g.dim = (int)dim;
+  g.causal = causal != 0;
+  g.scale_log2 = scale * 1.44269504088896340736f;
+  return dtype == NT_DTYPE_F16 ? nt::prompt_launch<nt::f16_t>(g, stream) : nt::prompt_launch<nt::bf16_t>(g, stream);
+}
+
+extern "C" int nt_prompt_attention_packed(const int64_t* packed) {
+  if (!packed) return NT_ERR_INVALID;
+  nt::Packed p{packed};
+  const void* q = p.ptr<const void>();
+  const int64_t* qs = p.array(3);
+  const void* k = p.ptr<const void>();
+  const int64_t* ks = p.array(3);
+  const void* v = p.ptr<const void>();
+  const int64_t* vs = p.array(3);
+  void* o = p.ptr<void>();
+  const int64_t* os = p.array(3);
+  int dtype = p.i();
+  const int32_t* q_starts = p.ptr<const int32_t>();
+  const int32_t* k_starts = p.ptr<const int32_t>();
+  int64_t q_tokens = p.i64();
+  int64_t k_tokens = p.i64();
+  int64_t sequences = p.i64();
+  int64_t heads = p.i64();
+  int64_t kv_heads = p.i64();
+  int64_t dim = p.i64();
+  float scale = p.f();
+  int causal = p.i();
+  hipStream_t stream = (hipStream_t)p.ptr<void>();
+  return nt_prompt_attention(q, qs, k, ks, v, vs, o, os, dtype, q_starts, k_starts, q_tokens, k_tokens, sequences,
+                             heads, kv_heads, dim, scale, causal, stream);
+}

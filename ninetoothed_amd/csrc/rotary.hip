@@ -1,0 +1,611 @@
+// Rotation of head elements by token position, and keys and values appended to a paged cache
+// with that rotation on the way.
+#include "packed.h"
+
+#include <algorithm>
+
+namespace nt {
+
+struct RotaryArgs {
+  const void* x;
+  void* out;
+  int64_t xs[3], os[3];  // token, head, element
+  const void* positions;
+  int64_t position_stride;
+  const double* freqs;
+  int64_t tokens;
+  int heads, dim, pairs, heads_per_wave;
+  int long_positions, interleaved, inverse;
+  float magnitude;
+  int units, per_head;     // of a head: vectors of pairs, and those plus vectors that are copied
+  uint32_t per_head_magic;  // ceil(2^32 / per_head), for per_head above 1
+};
+
+constexpr int ROTARY_PAIRS = 256;  // dim <= 512
+
+// y = x with pair i of the first 2 pairs elements turned by the angle position * freqs[i]:
+//   (a, b) -> (a cos - b sin, b cos + a sin),  a, b = x[i], x[i + pairs] or x[2i], x[2i + 1]
+// (inverse: the angle negated, which is the transpose and so the gradient).
+// Bound by HBM: x read and y written once.  A wave takes one token and some of its heads; its
+// lanes compute one angle each and pass cos and sin through LDS, so the angles cost a token, not
+// a head, and every lane then loads two 16-byte vectors (a and b of N pairs) for a rotation.
+// The loads of U items are in flight together, the first of them before the angles.
+// UNIT: unit element strides and N-element aligned rows; else one pair at a time by strides.
+template <typename T, int N, bool UNIT>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
+  typedef typename elem<T>::storage S;
+  constexpr int U = N > 1 ? 4 : 2;
+  __shared__ float2 turn_all[4][ROTARY_PAIRS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t token = (int64_t)blockIdx.x * 4 + wave;
+  if (token >= g.tokens) return;
+  const int64_t at = token * g.position_stride;
+  const int64_t position =
+      g.long_positions ? ((const int64_t*)g.positions)[at] : (int64_t)((const int32_t*)g.positions)[at];
+  if (position < 0) return;
+  float2* turn = turn_all[wave];
+  const int head0 = blockIdx.y * g.heads_per_wave;
+  const int nheads = min(g.heads - head0, g.heads_per_wave);
+  const int items = nheads * g.per_head;
+  const S* x = (const S*)g.x + token * g.xs[0] + head0 * g.xs[1];
+  S* out = (S*)g.out + token * g.os[0] + head0 * g.os[1];
+  const int second = g.interleaved ? N : g.pairs;  // where an item's second vector starts
+
+  Vec<S, N> a[U], b[U];
+  int head[U], first[U];
+  bool turned[U];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int item = base + i * 64 + lane;
+      if (item >= items) break;
+      head[i] = g.per_head == 1 ? item : (int)__umulhi((uint32_t)item, g.per_head_magic);
+      const int unit = item - head[i] * g.per_head;
+      turned[i] = unit < g.units;
+      first[i] = turned[i] ? (g.interleaved ? 2 * N * unit : N * unit) : 2 * g.pairs + (unit - g.units) * N;
+      const S* row = x + head[i] * g.xs[1];
+      if (UNIT) {
+        a[i] = *(const Vec<S, N>*)(row + first[i]);
+        if (turned[i]) b[i] = *(const Vec<S, N>*)(row + first[i] + second);
+      } else {
+        a[i].e[0] = row[first[i] * g.xs[2]];
+        if (turned[i]) b[i].e[0] = row[(first[i] + second) * g.xs[2]];
+      }
+    }
+  };
+  load(0);
+  for (int p = lane; p < g.pairs; p += 64) {
+    float2 cs = rotation((double)position, g.freqs[p], g.magnitude);
+    if (g.inverse) cs.y = -cs.y;
+    turn[p] = cs;
+  }
+  wave_lds_order();
+  for (int base = 0; base < items; base += 64 * U) {
+    if (base) load(base);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (base + i * 64 + lane >= items) break;
+      S* row = out + head[i] * g.os[1];
+      if (turned[i]) {
+        const int pair = g.interleaved ? first[i] >> 1 : first[i];
+        if (g.interleaved && N > 1) {  // a holds the first N / 2 pairs, b the others
+#pragma unroll
+          for (int e = 0; e < N; e += 2) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              Vec<S, N>& v = w ? b[i] : a[i];
+              const float2 cs = turn[pair + w * (N / 2) + e / 2];
+              const float p = elem<T>::to_float(v.e[e]), q = elem<T>::to_float(v.e[e + 1 < N ? e + 1 : e]);
+              v.e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
+              v.e[e + 1 < N ? e + 1 : e] = elem<T>::from_float(q * cs.x + p * cs.y);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float2 cs = turn[pair + e];
+            const float p = elem<T>::to_float(a[i].e[e]), q = elem<T>::to_float(b[i].e[e]);
+            a[i].e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
+            b[i].e[e] = elem<T>::from_float(q * cs.x + p * cs.y);
+          }
+        }
+      }
+      if (UNIT) {
+        *(Vec<S, N>*)(row + first[i]) = a[i];
+        if (turned[i]) *(Vec<S, N>*)(row + first[i] + second) = b[i];
+      } else {
+        row[first[i] * g.os[2]] = a[i].e[0];
+        if (turned[i]) row[(first[i] + second) * g.os[2]] = b[i].e[0];
+      }
+    }
+  }
+}
+
+// Rows of `elements`-element vectors: unit element stride, and every row starts on a vector.
+static bool rows_of(const void* p, const int64_t* s, int elements, int bytes) {
+  return s[2] == 1 && s[0] % elements == 0 && s[1] % elements == 0 && (uintptr_t)p % (uint64_t)(elements * bytes) == 0;
+}
+
+template <typename T>
+static int rotary_launch(RotaryArgs g, hipStream_t stream) {
+  constexpr int bytes = sizeof(typename elem<T>::storage), full = 16 / bytes;
+  auto fits = [&](int n) {
+    return g.pairs % n == 0 && (g.dim - 2 * g.pairs) % n == 0 && rows_of(g.x, g.xs, n, bytes) &&
+           rows_of(g.out, g.os, n, bytes);
+  };
+  const int n = fits(full) ? full : fits(full / 2) ? full / 2 : 1;
+  g.units = g.pairs / n;
+  g.per_head = g.units + (g.dim - 2 * g.pairs) / n;
+  g.per_head_magic = (uint32_t)(((1ull << 32) + g.per_head - 1) / g.per_head);
+  // A wave takes all of a token's heads where tokens alone fill the chip, else fewer of them.
+  const int64_t want = std::max<int64_t>(1, 4096 / std::max<int64_t>(1, g.tokens));
+  int64_t splits = std::min<int64_t>({want, (int64_t)g.heads, std::max<int64_t>(1, (int64_t)g.heads * g.per_head / 64)});
+  // (an item number stays below 2^16, so that the multiplied division is exact)
+  splits = std::max<int64_t>(splits, cdiv((int64_t)g.heads * g.per_head, 32768));
+  splits = std::min<int64_t>(splits, g.heads);
+  g.heads_per_wave = (int)cdiv(g.heads, splits);
+  const int64_t blocks = cdiv(g.tokens, 4), parts = cdiv(g.heads, g.heads_per_wave);
+  if (blocks > 0x7fffffffLL || parts > 65535) return NT_ERR_INVALID;
+  const dim3 grid((unsigned)blocks, (unsigned)parts), block(256);
+  if (n == full)
+    hipLaunchKernelGGL((rotary_kernel<T, full, true>), grid, block, 0, stream, g);
+  else if (n == full / 2)
+    hipLaunchKernelGGL((rotary_kernel<T, full / 2, true>), grid, block, 0, stream, g);
+  else
+    hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, block, 0, stream, g);
+  return launch_status();
+}
+
+struct AppendArgs {
+  const void* x[2];  // k, v: [tokens, heads, dim]
+  void* cache[2];
+  float* scale[2];           // [pages, heads] of an 8-bit cache
+  int64_t xs[2][3], cs[2][3];  // token, head, element; page, slot, head (elements side by side)
+  const int32_t *tables, *lengths;
+  const double* freqs;
+  UnitMap map;
+  int64_t table_stride, pages;
+  int heads, dim, pairs, page_size, table_width, heads_per_block, interleaved;
+  float magnitude;
+};
+
+// The tokens [first, first + count) of the packed tensors that a unit takes, at the positions
+// from `position` on.
+struct AppendUnit {
+  int64_t first;
+  uint32_t position;  // (31 bits of cached tokens and 31 bits of new ones)
+  int count, sequence;
+};
+__device__ __forceinline__ AppendUnit append_unit(const AppendArgs& g, int64_t id) {
+  AppendUnit u;
+  u.sequence = find_sequence(g.map, id);
+  const int64_t begin = clamped_start(g.map, u.sequence), end = clamped_start(g.map, u.sequence + 1);
+  const int64_t cached = g.lengths[u.sequence], block = g.map.per;
+  const int64_t which = cached / block + (id - first_unit(g.map, u.sequence));  // of the sequence's blocks of positions
+  const int64_t from = max(cached, which * block), to = min(cached + (end - begin), (which + 1) * block);
+  u.position = (uint32_t)from;
+  u.first = begin + (from - cached);
+  u.count = cached < 0 || id < first_unit(g.map, u.sequence) || to <= from ? 0 : (int)(to - from);
+  return u;
+}
+// The page of a position, or -1 where the table or the cache has none.
+__device__ __forceinline__ int64_t page_of(const AppendArgs& g, int sequence, uint32_t position) {
+  const uint32_t n = position / (uint32_t)g.page_size;
+  if (n >= (uint32_t)g.table_width) return -1;
+  const int64_t page = g.tables[sequence * g.table_stride + n];
+  return page < 0 || page >= g.pages ? -1 : page;
+}
+
+// One row's item: 2 N elements, N pairs to turn or 2 N neighbours to copy.
+template <typename T, int N>
+struct AppendItem {
+  int d0, d1;  // where its two vectors of N start
+  int pair;    // its first pair, or -1
+};
+template <typename T, int N>
+__device__ __forceinline__ AppendItem<T, N> append_item(int unit, int pairs, int interleaved) {
+  const bool turned = unit * N < pairs;
+  const int d0 = turned && !interleaved ? unit * N : 2 * N * unit;
+  return {d0, turned && !interleaved ? d0 + pairs : d0 + N, turned ? unit * N : -1};
+}
+template <typename T, int N, bool UNIT>
+__device__ __forceinline__ void append_load(const typename elem<T>::storage* row, int64_t es, const AppendItem<T, N>& it,
+                                            const float2* turn, int interleaved, float (&y)[2 * N]) {
+  typedef typename elem<T>::storage S;
+  Vec<S, N> a, b;
+  if (UNIT) {
+    a = *(const Vec<S, N>*)(row + it.d0);
+    b = *(const Vec<S, N>*)(row + it.d1);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      a.e[e] = row[(it.d0 + e) * es];
+      b.e[e] = row[(it.d1 + e) * es];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    y[e] = elem<T>::to_float(a.e[e]);
+    y[N + e] = elem<T>::to_float(b.e[e]);
+  }
+  if (it.pair < 0) return;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float2 cs = turn[it.pair + e];
+    // (a register array is indexed by constants only: both layouts are written out)
+    if (interleaved) {
+      const float p = y[2 * e], q = y[2 * e + 1];
+      y[2 * e] = p * cs.x - q * cs.y;
+      y[2 * e + 1] = q * cs.x + p * cs.y;
+    } else {
+      const float p = y[e], q = y[N + e];
+      y[e] = p * cs.x - q * cs.y;
+      y[N + e] = q * cs.x + p * cs.y;
+    }
+  }
+}
+
+// The angles of a unit's tokens: turn[token * pairs + pair].
+__device__ __forceinline__ void append_turns(const AppendArgs& g, const AppendUnit& u, float2* turn) {
+  for (int i = threadIdx.x; i < u.count * g.pairs; i += 256) {
+    const int t = i / g.pairs;
+    turn[i] = rotation((double)(u.position + t), g.freqs[i - t * g.pairs], g.magnitude);
+  }
+}
+
+// Keys (turned by position) and values into pages of their own 16-bit type.  Bound by HBM: each
+// element read and written once.  A workgroup takes up to `per` positions of one sequence and some
+// heads of k or of v: the angles are then taken once for those heads.
+template <typename T, int N, bool UNIT>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
+  typedef typename elem<T>::storage S;
+  extern __shared__ float2 turn[];
+  const AppendUnit u = append_unit(g, blockIdx.x);
+  if (u.count == 0) return;
+  const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
+  const int nheads = min(g.heads - head0, g.heads_per_block);
+  const int pairs = which == 0 ? g.pairs : 0;
+  if (pairs) {
+    append_turns(g, u, turn);
+    __syncthreads();
+  }
+  const int per_row = g.dim / (2 * N), per_token = per_row * nheads, items = u.count * per_token;
+  const S* x = (const S*)g.x[which] + u.first * g.xs[which][0] + head0 * g.xs[which][1];
+  S* cache = (S*)g.cache[which] + head0 * g.cs[which][2];
+  for (int i = threadIdx.x; i < items; i += 256) {
+    const int t = i / per_token, r = i - t * per_token, h = r / per_row;
+    const AppendItem<T, N> it = append_item<T, N>(r - h * per_row, pairs, g.interleaved);
+    const uint32_t position = u.position + t;
+    const int64_t page = page_of(g, u.sequence, position);
+    float y[2 * N];
+    append_load<T, N, UNIT>(x + t * g.xs[which][0] + h * g.xs[which][1], g.xs[which][2], it, turn + t * g.pairs,
+                            g.interleaved, y);
+    if (page < 0) continue;
+    S* row = cache + page * g.cs[which][0] + (int64_t)(position % (uint32_t)g.page_size) * g.cs[which][1] + h * g.cs[which][2];
+    Vec<S, N> a, b;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      a.e[e] = elem<T>::from_float(y[e]);
+      b.e[e] = elem<T>::from_float(y[N + e]);
+    }
+    if (UNIT) {
+      *(Vec<S, N>*)(row + it.d0) = a;
+      *(Vec<S, N>*)(row + it.d1) = b;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        row[it.d0 + e] = a.e[e];
+        row[it.d1 + e] = b.e[e];
+      }
+    }
+  }
+}
+
+// e4m3 from fp32, to nearest even; |x| <= 448 but for NaN, which stays one.
+__device__ __forceinline__ uint8_t e4m3_of(float x) {
+  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false);
+}
+// The exponent of the least power of two that 448 times is at least x (x finite, not negative):
+// x = m 2^e with m in [0.5, 1), and 448 = 0.875 * 2^9.  Held in the range in which a scale's
+// reciprocal and logarithm are ordinary numbers too.
+__device__ __forceinline__ int fitting_exponent(float x) {
+  if (x == 0.f) return -64;
+  int e;
+  const float m = frexpf(x, &e);
+  return max(-64, e - 9 + (m > 0.875f ? 1 : 0));
+}
+
+// The same into pages of e4m3 with a scale for each page and head.  The scale is a power of two,
+// the least that fits the page's largest value: the values of an 8-bit float lose nothing by that
+// (but for one binade of subnormals), and where a later token makes a page's scale grow, what
+// the page already holds is divided exactly.  A scale is taken afresh when a page is begun (its slot 0
+// is among the new tokens); else it only grows.  Infinities and NaN are stored as NaN, which is
+// all that e4m3 has of them, and do not count for the scale.
+// A workgroup takes the new tokens of one page and some heads of k or of v: per head the values
+// are turned and held in registers (HOLD items a lane, the rest is turned again), their largest
+// found, then stored.
+template <typename T, int N, bool UNIT>
+__global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
+  typedef typename elem<T>::storage S;
+  constexpr int HOLD = N == 8 ? 4 : 8;
+  extern __shared__ float2 turn[];
+  __shared__ float largest[2][4];
+  const AppendUnit u = append_unit(g, blockIdx.x);
+  if (u.count == 0) return;
+  const int64_t page = page_of(g, u.sequence, u.position);
+  if (page < 0) return;
+  const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
+  const int nheads = min(g.heads - head0, g.heads_per_block);
+  const int pairs = which == 0 ? g.pairs : 0;
+  if (pairs) {
+    append_turns(g, u, turn);
+    __syncthreads();
+  }
+  const int slot0 = (int)(u.position % (uint32_t)g.page_size);
+  const int per_row = g.dim / (2 * N), items = u.count * per_row;
+  for (int h = 0; h < nheads; ++h) {
+    const S* x = (const S*)g.x[which] + u.first * g.xs[which][0] + (head0 + h) * g.xs[which][1];
+    uint8_t* cache = (uint8_t*)g.cache[which] + page * g.cs[which][0] + (head0 + h) * g.cs[which][2];
+    float* scale_at = g.scale[which] + page * g.heads + head0 + h;
+    const float old = *scale_at;
+    float held[HOLD][2 * N];
+    float most = 0.f;
+    auto load = [&](int i, float (&y)[2 * N]) {
+      const int t = i / per_row;
+      append_load<T, N, UNIT>(x + t * g.xs[which][0], g.xs[which][2], append_item<T, N>(i - t * per_row, pairs, g.interleaved),
+                              turn + t * g.pairs, g.interleaved, y);
+    };
+    auto look = [&](const float (&y)[2 * N]) {
+#pragma unroll
+      for (int e = 0; e < 2 * N; ++e) {
+        const float m = fabsf(y[e]);
+        most = m < INFINITY ? fmaxf(most, m) : most;
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k) {
+      const int i = k * 256 + threadIdx.x;
+      if (i < items) {
+        load(i, held[k]);
+        look(held[k]);
+      }
+    }
+    for (int i = HOLD * 256 + threadIdx.x; i < items; i += 256) {
+      float y[2 * N];
+      load(i, y);
+      look(y);
+    }
+    most = wave_max(most);
+    if ((threadIdx.x & 63) == 0) largest[h & 1][threadIdx.x >> 6] = most;
+    __syncthreads();  // (also: every lane has read the old scale)
+    most = fmaxf(fmaxf(largest[h & 1][0], largest[h & 1][1]), fmaxf(largest[h & 1][2], largest[h & 1][3]));
+    const float fitting = ldexpf(1.0f, fitting_exponent(most));
+    const float scale = slot0 ? fmaxf(old, fitting) : fitting, inverse = 1.0f / scale;
+    if (threadIdx.x == 0) *scale_at = scale;
+    if (slot0 && scale != old) {  // what the page held follows its scale
+      const float ratio = old * inverse;
+      for (int i = threadIdx.x; i < slot0 * (g.dim / 4); i += 256) {
+        const int t = i / (g.dim / 4), d = (i - t * (g.dim / 4)) * 4;
+        uint8_t* row = cache + t * g.cs[which][1] + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          row[e] = e4m3_of(__builtin_amdgcn_cvt_f32_fp8((int)row[e], 0) * ratio);
+      }
+    }
+    auto store = [&](int i, const float (&y)[2 * N]) {
+      const int t = i / per_row;
+      const AppendItem<T, N> it = append_item<T, N>(i - t * per_row, pairs, g.interleaved);
+      uint8_t* row = cache + (slot0 + t) * g.cs[which][1];
+      Vec<uint8_t, N> v[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float q = y[w * N + e] * inverse;
+          v[w].e[e] = e4m3_of(fabsf(q) < INFINITY ? q : NAN);
+        }
+      if (UNIT) {
+        *(Vec<uint8_t, N>*)(row + it.d0) = v[0];
+        *(Vec<uint8_t, N>*)(row + it.d1) = v[1];
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          row[it.d0 + e] = v[0].e[e];
+          row[it.d1 + e] = v[1].e[e];
+        }
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k) {
+      const int i = k * 256 + threadIdx.x;
+      if (i < items) store(i, held[k]);
+    }
+    for (int i = HOLD * 256 + threadIdx.x; i < items; i += 256) {
+      float y[2 * N];
+      load(i, y);
+      store(i, y);
+    }
+  }
+}
+
+template <typename T>
+static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
+  auto fits = [&](int n) {
+    bool ok = g.pairs % n == 0 && (g.dim - 2 * g.pairs) % (2 * n) == 0;
+    for (int w = 0; w < 2; ++w) {
+      ok = ok && rows_of(g.x[w], g.xs[w], n, 2) && (uintptr_t)g.cache[w] % (uint64_t)(n * (eight ? 1 : 2)) == 0;
+      for (int i = 0; i < 3; ++i) ok = ok && g.cs[w][i] % n == 0;
+    }
+    return ok;
+  };
+  const int n = fits(8) ? 8 : fits(4) ? 4 : 1;
+  // A unit is a page of an 8-bit cache, else 64 positions; its angles take at most 64 KiB of LDS.
+  g.map.per = eight ? g.page_size : 64;
+  g.map.rows = 1;
+  g.map.extra = 2;
+  const int64_t units = unit_count(g.map);
+  // All heads of a unit share its angles where there are enough units (and k and v) for that.
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.heads, 2048 / std::max<int64_t>(1, units)));
+  g.heads_per_block = (int)cdiv(g.heads, parts);
+  const int64_t y = cdiv(g.heads, g.heads_per_block);
+  if (units > 0x7fffffffLL || y > 65535) return NT_ERR_INVALID;
+  const dim3 grid((unsigned)units, (unsigned)y, 2), block(256);
+  const size_t lds = (size_t)std::min<int64_t>(g.map.per, g.map.tokens) * g.pairs * sizeof(float2);
+#define NT_APPEND(kernel)                                                                  \
+  if (n == 8)                                                                              \
+    hipLaunchKernelGGL((kernel<T, 8, true>), grid, block, lds, stream, g);                 \
+  else if (n == 4)                                                                         \
+    hipLaunchKernelGGL((kernel<T, 4, true>), grid, block, lds, stream, g);                 \
+  else                                                                                     \
+    hipLaunchKernelGGL((kernel<T, 1, false>), grid, block, lds, stream, g);
+  if (eight) {
+    NT_APPEND(append8_kernel)
+  } else {
+    NT_APPEND(append_kernel)
+  }
+#undef NT_APPEND
+  return launch_status();
+}
+
+}  // namespace nt
+
+extern "C" int nt_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t* out_strides, int dtype,
+                         const void* positions, int64_t position_stride, int position_bits, const double* freqs,
+                         int64_t tokens, int64_t heads, int64_t dim, int64_t pairs, int interleaved, int inverse,
+                         float magnitude, hipStream_t stream) {
+  if (tokens < 0 || heads < 0 || dim < 0 || pairs < 0 || dim > 2 * nt::ROTARY_PAIRS || 2 * pairs > dim ||
+      heads > (1 << 20) || !nt::valid_dtype(dtype) || (position_bits != 32 && position_bits != 64))
+    return NT_ERR_INVALID;
+  if (tokens * heads * dim == 0) return 0;
+  if (!x || !out || !x_strides || !out_strides || !positions || (pairs && !freqs)) return NT_ERR_INVALID;
+  nt::RotaryArgs g{};
+  g.x = x;
+  g.out = out;
+  for (int i = 0; i < 3; ++i) {
+    g.xs[i] = x_strides[i];
+    g.os[i] = out_strides[i];
+  }
+  g.positions = positions;
+  g.position_stride = position_stride;
+  g.long_positions = position_bits == 64;
+  g.freqs = freqs;
+  g.tokens = tokens;
+  g.heads = (int)heads;
+  g.dim = (int)dim;
+  g.pairs = (int)pairs;
+  g.interleaved = interleaved != 0;
+  g.inverse = inverse != 0;
+  g.magnitude = magnitude;
+  if (dtype == NT_DTYPE_F32) return nt::rotary_launch<float>(g, stream);
+  if (dtype == NT_DTYPE_F16) return nt::rotary_launch<nt::f16_t>(g, stream);
+  return nt::rotary_launch<nt::bf16_t>(g, stream);
+}
+
+extern "C" int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                               int dtype, void* k_cache, const int64_t* kc_strides, void* v_cache,
+                               const int64_t* vc_strides, int cache_dtype, float* k_scale, float* v_scale,
+                               const int32_t* tables, int64_t table_stride, const int32_t* lengths,
+                               const int32_t* starts, const double* freqs, int64_t tokens, int64_t sequences,
+                               int64_t heads, int64_t dim, int64_t pages, int64_t page_size, int64_t table_width,
+                               int64_t pairs, int interleaved, float magnitude, hipStream_t stream) {
+  const bool eight = cache_dtype == NT_DTYPE_E4M3;
+  if (tokens < 0 || sequences < 0 || heads < 0 || dim < 0 || pages < 0 || page_size < 1 || table_width < 0 ||
+      pairs < 0 || 2 * pairs > dim || dim > 128 || dim % 4 || heads > 65535 || sequences > (1 << 30) || tokens > 0x7fffffffLL ||
+      page_size > (eight ? 128 : (1 << 30)) || table_width > (1 << 30))
+    return NT_ERR_INVALID;
+  if ((dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || (!eight && cache_dtype != dtype)) return NT_ERR_INVALID;
+  if (tokens * sequences * heads * dim * pages * table_width == 0) return 0;
+  if (!k || !v || !k_strides || !v_strides || !k_cache || !v_cache || !kc_strides || !vc_strides || !tables || !lengths ||
+      !starts || (pairs && !freqs) || (eight && (!k_scale || !v_scale)))
+    return NT_ERR_INVALID;
+  nt::AppendArgs g{};
+  g.x[0] = k;
+  g.x[1] = v;
+  g.cache[0] = k_cache;
+  g.cache[1] = v_cache;
+  g.scale[0] = k_scale;
+  g.scale[1] = v_scale;
+  for (int i = 0; i < 3; ++i) {
+    g.xs[0][i] = k_strides[i];
+    g.xs[1][i] = v_strides[i];
+    g.cs[0][i] = kc_strides[i];
+    g.cs[1][i] = vc_strides[i];
+  }
+  g.tables = tables;
+  g.lengths = lengths;
+  g.freqs = freqs;
+  g.map.starts = starts;
+  g.map.tokens = tokens;
+  g.map.sequences = (int)sequences;
+  g.table_stride = table_stride;
+  g.pages = pages;
+  g.heads = (int)heads;
+  g.dim = (int)dim;
+  g.pairs = (int)pairs;
+  g.page_size = (int)page_size;
+  g.table_width = (int)table_width;
+  g.interleaved = interleaved != 0;
+  g.magnitude = magnitude;
+  return dtype == NT_DTYPE_F16 ? nt::append_launch<nt::f16_t>(g, eight, stream)
+                               : nt::append_launch<nt::bf16_t>(g, eight, stream);
+}
+
+extern "C" int nt_rotary_packed(const int64_t* v) {
+  if (!v) return NT_ERR_INVALID;
+  nt::Packed p{v};
+  const void* x = p.ptr<const void>();
+  const int64_t* xs = p.array(3);
+  void* out = p.ptr<void>();
+  const int64_t* os = p.array(3);
+  int dtype = p.i();
+  const void* positions = p.ptr<const void>();
+  int64_t position_stride = p.i64();
+  int position_bits = p.i();
+  const double* freqs = p.ptr<const double>();
+  int64_t tokens = p.i64();
+  int64_t heads = p.i64();
+  int64_t dim = p.i64();
+  int64_t pairs = p.i64();
+  int interleaved = p.i();
+  int inverse = p.i();
+  float magnitude = p.f();
+  hipStream_t stream = (hipStream_t)p.ptr<void>();
+  return nt_rotary(x, xs, out, os, dtype, positions, position_stride, position_bits, freqs, tokens, heads, dim,
+                   pairs, interleaved, inverse, magnitude, stream);
+}
+
+extern "C" int nt_cache_append_packed(const int64_t* packed) {
+  if (!packed) return NT_ERR_INVALID;
+  nt::Packed p{packed};
+  const void* k = p.ptr<const void>();
+  const int64_t* ks = p.array(3);
+  const void* v = p.ptr<const void>();
+  const int64_t* vs = p.array(3);
+  int dtype = p.i();
+  void* k_cache = p.ptr<void>();
+  const int64_t* kcs = p.array(3);
+  void* v_cache = p.ptr<void>();
+  const int64_t* vcs = p.array(3);
+  int cache_dtype = p.i();
+  float* k_scale = p.ptr<float>();
+  float* v_scale = p.ptr<float>();
+  const int32_t* tables = p.ptr<const int32_t>();
+  int64_t table_stride = p.i64();
+  const int32_t* lengths = p.ptr<const int32_t>();
+  const int32_t* starts = p.ptr<const int32_t>();
+  const double* freqs = p.ptr<const double>();
+  int64_t tokens = p.i64();
+  int64_t sequences = p.i64();
+  int64_t heads = p.i64();
+  int64_t dim = p.i64();
+  int64_t pages = p.i64();
+  int64_t page_size = p.i64();
+  int64_t table_width = p.i64();
+  int64_t pairs = p.i64();
+  int interleaved = p.i();
+  float magnitude = p.f();
+  hipStream_t stream = (hipStream_t)p.ptr<void>();
+  return nt_cache_append(k, ks, v, vs, dtype, k_cache, kcs, v_cache, vcs, cache_dtype, k_scale, v_scale, tables,
+                         table_stride, lengths, starts, freqs, tokens, sequences, heads, dim, pages, page_size,
+                         table_width, pairs, interleaved, magnitude, stream);
+}

@@ -18,6 +18,7 @@ reference's error type, ``src/ninetoothed/compiler/runtime.py:31-35``).
 """
 
 import ctypes
+import math
 import struct
 
 from ninetoothed_amd import _lib
@@ -552,3 +553,411 @@ def bind_attention(q, k, v, o, causal=False, q_scale=LOG2E, config=0):
 def attention(q, k, v, o, causal=False, q_scale=LOG2E, config=0):
     bind_attention(q, k, v, o, causal, q_scale, config)(q, k, v, o)
     return o
+
+
+# ------------------------------------------- around a paged key/value cache
+# The steps of a program that answers with a model: queries rotated by position, keys and values
+# appended to a paged cache, attention over packed prompts, attention of one new token a sequence over
+# what the cache holds.  They go through the packed entry points (one array of arguments, its constant
+# values packed at bind time); ``<op>(...)`` keeps the launchers it has bound by the call's
+# metadata, as a Handle does, so a serving loop may call it directly.
+_POINTER, _STREAM = object(), object()
+_bound_launchers = {}
+_MAX_BOUND = 4096  # (prompts come in ever new lengths: the launchers are dropped when there are so many)
+
+
+def _bind_packed(name, device, arguments):
+    """launch(tensors): the packed entry point ``name`` with ``arguments`` in order, where each
+    ``_POINTER`` takes the data pointer of the next of ``tensors`` (None: null) and ``_STREAM`` the
+    device's current stream.  Launches on ``device`` whatever the current device is."""
+    import torch
+
+    values, pointers, streams = [], [], []
+    for a in arguments:
+        if a is _POINTER:
+            pointers.append(len(values))
+        elif a is _STREAM:
+            streams.append(len(values))
+        if a is _POINTER or a is _STREAM:
+            values.append(0)
+        elif isinstance(a, tuple):
+            values.extend(a)
+        else:
+            values.append(_float_bits(a) if isinstance(a, float) else int(a))
+    template, slots, streams = struct.pack(f"<{len(values)}q", *values), tuple(pointers), tuple(streams)
+    fn = getattr(_lib.load(), name)
+    addr = _packed_address(name)
+    stream = _stream_of(device)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    current = torch._C._cuda_getDevice
+
+    def run(tensors):
+        if addr is not None:
+            return _fastkey.call(addr, template, slots, tensors, streams, (stream() or 0,))
+        args = list(values)
+        for slot, t in zip(slots, tensors):
+            args[slot] = 0 if t is None else t.data_ptr()
+        args[streams[0]] = stream() or 0
+        return fn(_lib.int64_array(args))
+
+    def launch(tensors):
+        if current() == index:
+            code = run(tensors)
+        else:
+            with torch.cuda.device(index):
+                code = run(tensors)
+        if code:
+            _raise(code, name)
+
+    return launch
+
+
+def _launch_bound(bind, tensors, options):
+    """Launch ``bind(*tensors, *options)`` on ``tensors``, bound once per metadata and options."""
+    key = None
+    if _fastkey is not None:
+        try:
+            given = _fastkey.key(tuple([t for t in tensors if t is not None]))
+            if given is not None:
+                key = (bind, given, tuple([t is None for t in tensors]), options)
+                launch = _bound_launchers.get(key)
+                if launch is not None:
+                    launch(*tensors)
+                    return
+        except TypeError:  # an unhashable option: the checks report it
+            key = None
+    launch = bind(*tensors, *options)
+    launch(*tensors)
+    if key is not None:
+        if len(_bound_launchers) >= _MAX_BOUND:
+            _bound_launchers.clear()
+        _bound_launchers[key] = launch
+
+
+def _check_written(t, name):
+    """A tensor a kernel writes has no two elements in one place."""
+    reach = 0
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride <= reach:
+            raise ValueError(f"{name} has elements that share memory")
+        reach += stride * (size - 1)
+
+
+def _check_index(t, name, shape, dtypes):
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+
+
+def _check_contiguous(t, name):
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _check_frequencies(freqs, dim):
+    import torch
+
+    if freqs.dtype != torch.float64:
+        raise TypeError("freqs must be torch.float64")
+    if freqs.dim() != 1 or 2 * freqs.shape[0] > dim:
+        raise ValueError(f"freqs must be 1-D, one for each pair of at most {dim} elements")
+    _check_contiguous(freqs, "freqs")
+
+
+def rotary_frequencies(dim, base=10000.0, factor=1.0, original_length=None, low=1.0, high=32.0, device="cuda"):
+    """The frequencies (radians a position, ``torch.float64``, [dim // 2]) of a rotation of ``dim``
+    elements: ``base ** (-2 i / dim)``, for contexts ``factor`` times as long as trained.
+
+    Without ``original_length`` every frequency is divided by ``factor``.  With it, those that make
+    at least ``high`` turns over that length keep their value, those that make at most ``low`` are
+    divided, and between the two the share that is divided falls linearly in the turns.  A scaled base is ``base``; a
+    factor on cosine and sine is the ``magnitude`` of :func:`rotary` and :func:`cache_append`."""
+    import torch
+
+    if dim < 2 or dim % 2:
+        raise ValueError("the rotated part must be a positive even number of elements")
+    if not (base > 0 and factor > 0 and high > low):
+        raise ValueError("base and factor must be positive, and high above low")
+    freqs = float(base) ** -(torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if original_length is None:
+        freqs = freqs / factor
+    else:
+        kept = ((original_length / (2 * math.pi) * freqs - low) / (high - low)).clamp(0.0, 1.0)
+        freqs = freqs * (kept + (1.0 - kept) / factor)
+    return freqs.to(device)
+
+
+def check_rotary(x, positions, freqs, out, interleaved=False, inverse=False, magnitude=1.0):
+    import torch
+
+    if x.dim() != 3 or out.shape != x.shape:
+        raise ValueError("rotary expects matching [tokens, heads, dim] tensors")
+    if x.dtype != out.dtype:
+        raise TypeError("rotary input and output must share one dtype")
+    code = _lib.dtype_code(x.dtype)
+    tokens, heads, dim = x.shape
+    if dim > 512 or heads > 1 << 20:
+        raise ValueError("rotary head dim must be <= 512")
+    _check_index(positions, "positions", (tokens,), (torch.int32, torch.int64))
+    _check_frequencies(freqs, dim)
+    _check_written(out, "out")
+    float(magnitude)
+    return code
+
+
+def bind_rotary(x, positions, freqs, out, interleaved=False, inverse=False, magnitude=1.0):
+    """launch(x, positions, freqs, out): out = x [tokens, heads, dim] with the first 2 * len(freqs)
+    elements of each head rotated by position.
+
+    Pair i is (x[i], x[i + len(freqs)]), with ``interleaved`` (x[2 i], x[2 i + 1]); its angle is
+    positions[token] * freqs[i], reduced in 64 bits.  The products are in fp32, rounded once.
+    ``magnitude`` scales cosine and sine.  The other elements are copied; a token whose position is
+    negative keeps what ``out`` held.  ``inverse`` turns back: applied to the gradient of ``out``
+    it gives the gradient of ``x``.  ``out`` may be ``x`` itself and else must not overlap it."""
+    code = check_rotary(x, positions, freqs, out, interleaved, inverse, magnitude)
+    device = _check_device(x, positions, freqs, out)
+    tokens, heads, dim = x.shape
+    same_strides = x.stride() == out.stride()
+    launch = _bind_packed("nt_rotary_packed", device, (
+        _POINTER, x.stride(), _POINTER, out.stride(), code, _POINTER, positions.stride(0),
+        positions.element_size() * 8, _POINTER, tokens, heads, dim, freqs.shape[0], bool(interleaved), bool(inverse),
+        float(magnitude), _STREAM))
+
+    def call(x, positions, freqs, out):
+        if not same_strides and x.data_ptr() == out.data_ptr():
+            raise ValueError("rotary in place needs input and output of the same strides")
+        launch((x, out, positions, freqs))
+
+    return call
+
+
+def rotary(x, positions, freqs, out, interleaved=False, inverse=False, magnitude=1.0):
+    _launch_bound(bind_rotary, (x, positions, freqs, out), (interleaved, inverse, magnitude))
+    return out
+
+
+def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, heads, dim):
+    """The element-type code of a pair of caches for tokens of ``dtype``."""
+    import torch
+
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("a key/value cache takes torch.float16 or torch.bfloat16 tokens")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("caches must be matching [pages, page_size, heads, dim] tensors")
+    pages, page_size = k_cache.shape[:2]
+    if k_cache.shape[2:] != (heads, dim):
+        raise ValueError(f"caches must hold {heads} heads of {dim}, not {tuple(k_cache.shape[2:])}")
+    if k_cache.dtype != v_cache.dtype:
+        raise TypeError("k and v caches must share one dtype")
+    eight = k_cache.dtype == torch.float8_e4m3fn
+    if not eight and k_cache.dtype != dtype:
+        raise TypeError(f"caches must be {dtype} or torch.float8_e4m3fn")
+    if dim % 16 or not 0 < dim <= 128:
+        raise ValueError("a cache's head dim must be a multiple of 16 up to 128")
+    if page_size < 1 or (eight and page_size > 128):
+        raise ValueError("pages must have at least one slot, and at most 128 in 8 bits")
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("caches must have elements side by side")
+    if (k_scale is None) == eight or (v_scale is None) == eight:
+        raise ValueError("k_scale and v_scale belong to 8-bit caches, and both are needed there")
+    if eight:
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            _check_index(t, name, (pages, heads), (torch.float32,))
+            _check_contiguous(t, name)
+    return _lib.DTYPE_E4M3 if eight else _lib.dtype_code(dtype)
+
+
+def _check_tables(tables, lengths):
+    import torch
+
+    if tables.dim() != 2:
+        raise ValueError("tables must be [sequences, pages of each]")
+    _check_index(tables, "tables", tables.shape, (torch.int32,))
+    if tables.shape[1] > 1 and tables.stride(1) != 1:
+        raise ValueError("a sequence's page numbers must lie side by side")
+    _check_index(lengths, "lengths", tables.shape[:1], (torch.int32,))
+    _check_contiguous(lengths, "lengths")
+
+
+def _check_starts(starts, name, sequences=None):
+    import torch
+
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError(f"{name} must be [sequences + 1]")
+    _check_index(starts, name, starts.shape if sequences is None else (sequences + 1,), (torch.int32,))
+    _check_contiguous(starts, name)
+
+
+def check_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=None, v_scale=None, freqs=None,
+                       interleaved=False, magnitude=1.0):
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("cache_append expects matching [tokens, heads, dim] tensors")
+    if k.dtype != v.dtype:
+        raise TypeError("k and v must share one dtype")
+    tokens, heads, dim = k.shape
+    if tokens > 0x7FFFFFFF or heads > 65535:
+        raise ValueError("cache_append takes less than 2^31 tokens of at most 65535 heads")
+    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, heads, dim)
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _check_written(t, name)
+    _check_tables(tables, lengths)
+    _check_starts(starts, "starts", tables.shape[0])
+    if freqs is not None:
+        _check_frequencies(freqs, dim)
+    float(magnitude)
+    return cache_code
+
+
+def bind_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=None, v_scale=None, freqs=None,
+                      interleaved=False, magnitude=1.0):
+    """launch(k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs): the packed
+    tokens' k, v [tokens, heads, dim] into the sequences' pages of the caches [pages, page_size, heads,
+    dim] (or any permutation of such storage that leaves elements side by side).
+
+    Sequence b's tokens are rows starts[b] to starts[b + 1]; the first goes to position lengths[b] (the
+    number it has in the cache already; the caller counts on), which is slot position % page_size of
+    page tables[b, position // page_size].  k is rotated by its position on the way (``freqs`` None:
+    not at all), as :func:`bind_rotary` rotates.  Tokens past a table's width or of a page number the
+    cache does not have are not stored; a page may be written for one sequence only.
+
+    Caches of ``torch.float8_e4m3fn`` hold x / scale with a scale for each page and head (k_scale,
+    v_scale [pages, heads], fp32): the least power of two that fits the page's largest value to 448,
+    taken afresh when the page's slot 0 is written, and growing (the slots before the new ones then
+    follow) when a later token needs it.  Infinities are stored as NaN."""
+    cache_code = check_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs,
+                                    interleaved, magnitude)
+    device = _check_device(k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs)
+    tokens, heads, dim = k.shape
+    pages, page_size = k_cache.shape[:2]
+    launch = _bind_packed("nt_cache_append_packed", device, (
+        _POINTER, k.stride(), _POINTER, v.stride(), _lib.dtype_code(k.dtype), _POINTER, k_cache.stride()[:3], _POINTER,
+        v_cache.stride()[:3], cache_code, _POINTER, _POINTER, _POINTER, tables.stride(0), _POINTER, _POINTER, _POINTER,
+        tokens, tables.shape[0], heads, dim, pages, page_size, tables.shape[1],
+        0 if freqs is None else freqs.shape[0], bool(interleaved), float(magnitude), _STREAM))
+
+    def call(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=None, v_scale=None, freqs=None):
+        launch((k, v, k_cache, v_cache, k_scale, v_scale, tables, lengths, starts, freqs))
+
+    return call
+
+
+def cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=None, v_scale=None, freqs=None,
+                 interleaved=False, magnitude=1.0):
+    _launch_bound(bind_cache_append, (k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs),
+                  (interleaved, magnitude))
+
+
+def _check_heads(heads, kv_heads):
+    if kv_heads == 0 or heads % kv_heads:
+        raise ValueError("the heads of q must be a multiple of those of k and v")
+
+
+def check_prompt_attention(q, k, v, out, q_starts, k_starts, causal=True, scale=None):
+    import torch
+
+    if not q.dim() == k.dim() == v.dim() == 3 or out.shape != q.shape or v.shape != k.shape:
+        raise ValueError("prompt_attention expects [tokens, heads, dim] tensors, out as q and v as k")
+    if not q.dtype == k.dtype == v.dtype == out.dtype or q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("prompt_attention q, k, v and out must share one dtype, torch.float16 or torch.bfloat16")
+    if k.shape[2] != q.shape[2] or not 0 < q.shape[2] <= 128:
+        raise ValueError("prompt_attention head dims must be one and <= 128")
+    _check_heads(q.shape[1], k.shape[1])
+    if q.shape[0] * (q.shape[1] // k.shape[1]) > 0x7FFFFF00 or k.shape[0] > 0x7FFFFF00:
+        raise ValueError("prompt_attention takes less than 2^31 rows")
+    _check_starts(q_starts, "q_starts")
+    _check_starts(k_starts, "k_starts", q_starts.shape[0] - 1)
+    _check_written(out, "out")
+    if scale is not None:
+        float(scale)
+    return _lib.dtype_code(q.dtype)
+
+
+def bind_prompt_attention(q, k, v, out, q_starts, k_starts, causal=True, scale=None):
+    """launch(q, k, v, out, q_starts, k_starts): attention of packed sequences, q and out [q tokens,
+    heads, dim], k and v [k tokens, kv_heads, dim] with heads a multiple of kv_heads (head h reads
+    h // (heads // kv_heads)).
+
+    Sequence b is rows q_starts[b] to q_starts[b + 1] of q and k_starts[b] to k_starts[b + 1] of k, v
+    (one tensor may serve as both where they agree).  ``causal``: query i sees the keys up to
+    i + (keys - queries), so that the last query sees them all.  ``scale`` defaults to
+    dim ** -0.5.  Scores, softmax and sums are in fp32, the weights rounded to the inputs' type for the
+    product with v.  A query without keys gives zeros; rows behind the last sequence are left alone."""
+    code = check_prompt_attention(q, k, v, out, q_starts, k_starts, causal, scale)
+    device = _check_device(q, k, v, out, q_starts, k_starts)
+    dim = q.shape[2]
+    launch = _bind_packed("nt_prompt_attention_packed", device, (
+        _POINTER, q.stride(), _POINTER, k.stride(), _POINTER, v.stride(), _POINTER, out.stride(), code, _POINTER,
+        _POINTER, q.shape[0], k.shape[0], q_starts.shape[0] - 1, q.shape[1], k.shape[1], dim,
+        float(dim ** -0.5 if scale is None else scale), bool(causal), _STREAM))
+
+    def call(q, k, v, out, q_starts, k_starts):
+        launch((q, k, v, out, q_starts, k_starts))
+
+    return call
+
+
+def prompt_attention(q, k, v, out, q_starts, k_starts, causal=True, scale=None):
+    _launch_bound(bind_prompt_attention, (q, k, v, out, q_starts, k_starts), (causal, scale))
+    return out
+
+
+def check_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=None, v_scale=None, scale=None):
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError("cache_attention expects matching [sequences, heads, dim] tensors")
+    if q.dtype != out.dtype:
+        raise TypeError("cache_attention q and out must share one dtype")
+    if k_cache.dim() != 4:
+        raise ValueError("caches must be [pages, page_size, heads, dim] tensors")
+    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, k_cache.shape[2], q.shape[2])
+    _check_heads(q.shape[1], k_cache.shape[2])
+    _check_tables(tables, lengths)
+    if tables.shape[0] != q.shape[0]:
+        raise ValueError("tables must have a row for each sequence of q")
+    if k_cache.shape[1] * tables.shape[1] > 0x7FFFFF00:
+        raise ValueError("cache_attention takes less than 2^31 keys a sequence")
+    vector = 16 // k_cache.element_size()
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if any(st % vector for st, size in zip(t.stride()[:3], t.shape) if size > 1):
+            raise ValueError(f"{name} rows must start on 16 bytes")
+    _check_written(out, "out")
+    if scale is not None:
+        float(scale)
+    return cache_code
+
+
+def bind_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=None, v_scale=None, scale=None):
+    """launch(q, k_cache, v_cache, tables, lengths, out, k_scale, v_scale): attention of one query a
+    sequence, q and out [sequences, heads, dim], over the first lengths[b] keys of its pages, in caches
+    as :func:`bind_cache_append` fills them (lengths here count the new token too).
+
+    heads is a multiple of the caches' heads, ``scale`` defaults to dim ** -0.5.  8-bit caches count
+    times their scales (any that are not negative).  Scores, softmax and sums are in fp32; the weights are
+    rounded to the cache's type (to fp16 for 8-bit caches) for the product with v.  Lengths past a table's
+    pages are cut, page numbers the cache does not have hold no keys, and without keys the output is zero.
+    A call takes a workspace for keys that are split over workgroups from torch's allocator."""
+    cache_code = check_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale, v_scale, scale)
+    device = _check_device(q, k_cache, v_cache, tables, lengths, out, k_scale, v_scale)
+    import torch
+
+    sequences, heads, dim = q.shape
+    pages, page_size, kv_heads = k_cache.shape[:3]
+    width = tables.shape[1] if pages else 0
+    nbytes = int(_lib.load().nt_cache_attention_workspace_size(sequences, heads, kv_heads, dim, page_size, width))
+    # (a size of one may have any stride: the kernels take none for it)
+    strides = [tuple(st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape)) for t in (k_cache, v_cache)]
+    launch = _bind_packed("nt_cache_attention_packed", device, (
+        _POINTER, q.stride(), _POINTER, strides[0], _POINTER, strides[1], cache_code, _POINTER, _POINTER, _POINTER,
+        out.stride(), _lib.dtype_code(q.dtype), _POINTER, tables.stride(0), _POINTER, sequences, heads, kv_heads, dim,
+        pages, page_size, width, float(dim ** -0.5 if scale is None else scale), _STREAM, _POINTER, nbytes))
+
+    def call(q, k_cache, v_cache, tables, lengths, out, k_scale=None, v_scale=None):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        launch((q, k_cache, v_cache, k_scale, v_scale, out, tables, lengths, ws))
+
+    return call
+
+
+def cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=None, v_scale=None, scale=None):
+    _launch_bound(bind_cache_attention, (q, k_cache, v_cache, tables, lengths, out, k_scale, v_scale), (scale,))
+    return out
