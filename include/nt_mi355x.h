@@ -458,7 +458,7 @@ int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, 
  * The workspace (16-byte aligned, nt_cache_attention_workspace_size bytes, 0: none needed) holds
  * partial states of sequences whose keys are split over workgroups; nothing between calls. */
 int64_t nt_cache_attention_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
-                                          int64_t page_size, int64_t table_width);
+                                          int64_t page_size, int64_t table_width, int cache_dtype);
 int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,
                        const void* v_cache, const int64_t* v_strides, int cache_dtype, const float* k_scale,
                        const float* v_scale, void* o, const int64_t* o_strides, int dtype, const int32_t* tables,

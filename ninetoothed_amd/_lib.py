@@ -103,7 +103,7 @@ _SIGNATURES = {
     "nt_prompt_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P) + (_I64,) * 6 + (_F, _I, _P),
     "nt_cache_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P, _P, _I64P, _I, _P, _I64, _P) + (_I64,) * 7
                           + (_F, _P, _P, _I64),
-    "nt_cache_attention_workspace_size": (_I64,) * 6,
+    "nt_cache_attention_workspace_size": (_I64,) * 6 + (_I,),
     **{f"nt_{op}_packed": (_I64P,) for op in ("rotary", "cache_append", "prompt_attention", "cache_attention")},
     "nt_rtc_compile": (ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_P), _I64P, ctypes.c_char_p, _I64),
     "nt_rtc_free": (_P,),

@@ -59,6 +59,23 @@ struct Words {
   uint32_t w[WORDS];
 };
 
+// A wave's 32 keys in LDS, k and v: rows of DM elements of ES bytes, in 16-byte chunks that are
+// XORed by key so that the 16 keys of a fragment read fall on 16 distinct bank groups (64 banks of 4
+// bytes: a 64-, 128- or 256-byte row takes a quarter, a half or all of them).
+template <int DM, int ES>
+struct Geo {
+  static constexpr int ROW = DM * ES, CHUNKS = ROW / 16, TILE = BN * ROW, STAGE = 2 * TILE;
+  static constexpr int LOADS = TILE / 1024, KEYS = BN / LOADS;  // of k or v, and the keys of each
+  static constexpr int STAGES = 2, RING = STAGES * STAGE;
+  static constexpr int OROW = DM + 4, MERGE = BQ * OROW * 4;  // a wave's state, for the merge
+  static constexpr int LDS = NW * (RING > MERGE ? RING : MERGE);
+  __device__ __forceinline__ static int swizzle(int key) {
+    return ROW == 256 ? key & 15 : ROW == 128 ? (key >> 1) & 7 : (key >> 2) & 3;
+  }
+};
+typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
+typedef const __attribute__((address_space(4))) float* ScalarFloats;
+
 }  // namespace ca
 
 struct CacheArgs {
@@ -70,6 +87,7 @@ struct CacheArgs {
   const int32_t *tables, *lengths;
   int64_t table_stride, pages;
   int sequences, kv_heads, group, dim, page_size, table_width, row_blocks, workgroups;
+  int page_shift;  // page_size = 16 << page_shift, or -1
   float scale_log2;
   float *part_o, *part_ml;  // of partial states, two a workgroup: [slot][row][DM], [slot][row][2]
 };
@@ -118,31 +136,33 @@ __device__ __forceinline__ int64_t line_share(const CacheArgs& g, int64_t all_bl
 // over its cached keys; an empty sequence gives zeros.
 // HBM-bound: each cached element is read once, 4 group flops for each.  The rows of a group are
 // the columns of 16 x 16 x 32 products, so that MHA to MQA read the cache once: S^T = K Q^T, with
-// keys as the rows, and O^T += V^T P^T.  Every wave takes 32 keys at a time straight into registers,
-// the next 32 in flight meanwhile; P^T goes from the scores' registers to the second product as it
+// keys as the rows, and O^T += V^T P^T.  Every wave streams 32 keys at a time through two LDS stages
+// of its own (loads that bypass the registers, no barrier in the loop), so that 8 KiB (8 bits) or 16 a
+// wave are under way while it computes.  P^T goes from the scores' registers to the second product as it
 // is, and V, read eight keys by DM / 16 neighbouring elements a lane, is transposed by byte permutes.
 // 8 bits: e4m3 widens exactly, so k's scale multiplies the score and v's enters the weight:
 //   w_ij = exp2(s_ij + log2 vs_j - M_i),  o_i = sum_j w_ij vq_j / sum_j w_ij / vs_j,
 // with M the running max of the exponents: w stays within 2^8 for any scales, is rounded to fp16
 // (11 bits, also for bf16 queries) for the product with v, and its sum stays in fp32.
-// ONE_PAGE: pages are whole multiples of 32 keys, so that a wave's 32 keys lie in one page and
-// their address is uniform; else each key's page is looked up.
-template <typename T, bool EIGHT, int DM, bool ONE_PAGE>
+// SIXTEENS: pages are whole multiples of 16 keys, so that a load's keys lie in one page and its
+// address and scale are uniform; else each key's page is looked up.
+template <typename T, bool EIGHT, int DM, bool SIXTEENS>
 __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs g) {
   using namespace ca;
   typedef typename std::conditional<EIGHT, f16_t, T>::type P;  // the type of V^T P^T
   typedef mma16<T> MQ;
   typedef mma16<P> MP;
   constexpr int ES = EIGHT ? 1 : 2;
-  constexpr int STEPS = DM / 32;                   // products over the elements of q and k
-  constexpr int KL = DM * ES / 64;                 // 16-byte loads of a key a lane
-  constexpr int DL = DM / 16, VW = DL * ES / 4;    // elements of v a lane, and their words
-  constexpr int OROW = DM + 4;
-  __shared__ float merge_o[NW][BQ * OROW];
+  using G = Geo<DM, ES>;
+  constexpr int STEPS = DM / 32;                 // products over the elements of q and k
+  constexpr int KL = DM * ES / 64;               // 16-byte reads of a key a lane
+  constexpr int DL = DM / 16, VW = DL * ES / 4;  // elements of v a lane, and their words
+  constexpr int NKEYS = SIXTEENS ? 1 : BN;
+  __shared__ __attribute__((aligned(1024))) char ring[G::LDS];
   __shared__ float merge_ml[NW][2][BQ];
   __shared__ int64_t sums[8];
-  __shared__ int64_t key_at[NW][2][2][ONE_PAGE ? 1 : BN];
-  __shared__ float key_scale[NW][2][3][ONE_PAGE || !EIGHT ? 1 : BN];
+  __shared__ int64_t key_at[NW][2][NKEYS];             // where each key's k and v lie
+  __shared__ float key_scale[NW][G::STAGES][3][NKEYS];  // k's factor, log2 and reciprocal of v's scale
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = g.dim;
@@ -184,6 +204,27 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
     b = __builtin_amdgcn_readfirstlane(b);
   }
 
+  // Where this lane's 16 bytes of each load lie behind the load's first key, and where its fragments
+  // lie in a stage.  Elements past D read as zeros (SIXTEENS: past the buffer's end).
+  const uint32_t ring_w = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring + wave * G::RING;
+  const char* ring_p = ring + wave * G::RING;
+  const int kst = (int)(g.ks[1] * ES), vst = (int)(g.vs[1] * ES);
+  int kv_key[G::LOADS], kv_byte[G::LOADS];
+#pragma unroll
+  for (int u = 0; u < G::LOADS; ++u) {
+    kv_key[u] = u * G::KEYS + lane / G::CHUNKS;
+    kv_byte[u] = ((lane % G::CHUNKS) ^ G::swizzle(kv_key[u])) * 16;
+  }
+  auto k_frag = [&](int stage, int kb, int u) {
+    const int key = kb * 16 + col, chunk = u * 4 + quad;
+    return *(const u32x4*)(ring_p + stage * G::STAGE + key * G::ROW + ((chunk ^ G::swizzle(key)) * 16));
+  };
+  auto v_words = [&](int stage, int e) {
+    const int key = (e >> 2) * 16 + quad * 4 + (e & 3), byte = col * DL * ES;
+    return *(const Words<VW>*)(ring_p + stage * G::STAGE + G::TILE + key * G::ROW +
+                               (((byte >> 4) ^ G::swizzle(key)) * 16) + (byte & 15));
+  };
+
   while (at < stop) {
     const int len = Line::keys(g, b), nblk = Line::blocks(g, b);
     const int64_t inside = at - seq0;
@@ -192,6 +233,99 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
     const int h = line / g.row_blocks, rb = line % g.row_blocks;
     const int rows = min(BQ, g.group - rb * BQ);
     const int head0 = h * g.group + rb * BQ;
+
+    const ScalarInts table = (ScalarInts)(uintptr_t)(g.tables + b * g.table_stride);
+    const char* kbase = (const char*)g.k + h * g.ks[2] * ES;
+    const char* vbase = (const char*)g.v + h * g.vs[2] * ES;
+    const int tiles = (len + BN - 1) / BN;
+    const int t0 = blk0 * NW + wave, t_end = min(blk1 * NW, tiles);
+    const int nt = t0 < t_end ? (t_end - t0 + NW - 1) / NW : 0;  // this wave's tiles: t0 + j NW
+
+    // The scale of a page's head as a factor of scores, and what v's adds to exponents and sums.
+    struct Scales {
+      float kf, lv, rv;
+    };
+    auto scales = [&](float ks, float vs) {
+      vs = fmaxf(vs, LEAST_SCALE);
+      return Scales{ks * g.scale_log2, __builtin_amdgcn_logf(vs), 1.0f / vs};
+    };
+    auto page_number = [&](int sixteen) {  // of 16 keys; -1: none
+      const int n = g.page_shift >= 0 ? sixteen >> g.page_shift : sixteen / (g.page_size >> 4);
+      const int32_t page = n < g.table_width ? table[n] : -1;
+      return page >= 0 && page < g.pages ? page : -1;
+    };
+    // SIXTEENS: the pages of the tiles that come next (looked up ahead), and the scales of those
+    // under way.
+    int next_page[2];
+    Scales sc[G::STAGES][2];
+    bool real[G::STAGES][2];
+    auto look = [&](int j) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) next_page[kb] = j < nt ? page_number(2 * (t0 + j * NW) + kb) : -1;
+    };
+    auto issue = [&](int j, int stage) {
+      const int k0 = (t0 + j * NW) * BN;
+      const uint32_t to = ring_w + (uint32_t)(stage * G::STAGE);
+      if (SIXTEENS) {
+        u32x4 rk[2], rv[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const int first = k0 + kb * 16, n = min(16, len - first);
+          const bool ok = next_page[kb] >= 0 && n > 0;
+          const int64_t page = ok ? next_page[kb] : 0;
+          const int slot = first - (g.page_shift >= 0 ? (first >> (g.page_shift + 4)) << (g.page_shift + 4)
+                                                      : first / g.page_size * g.page_size);
+          // (a buffer ends with the last key: what lies past it, or in no page, reads as zeros)
+          rk[kb] = buffer_of(kbase + (page * g.ks[0] + slot * g.ks[1]) * ES, ok ? (n - 1) * kst + D * ES : 0);
+          rv[kb] = buffer_of(vbase + (page * g.vs[0] + slot * g.vs[1]) * ES, ok ? (n - 1) * vst + D * ES : 0);
+          real[stage][kb] = ok;
+          if (EIGHT) {
+            sc[stage][kb] = scales(((ScalarFloats)(uintptr_t)g.k_scale)[page * g.kv_heads + h],
+                                   ((ScalarFloats)(uintptr_t)g.v_scale)[page * g.kv_heads + h]);
+            if (!ok) sc[stage][kb] = Scales{0.f, 0.f, 1.0f};
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int u = 0; u < G::LOADS; ++u) {
+            const int kb = u * G::KEYS / 16, st = w ? vst : kst;
+            const int off = kv_byte[u] < D * ES ? (kv_key[u] - kb * 16) * st + kv_byte[u] : 0x7fffffff;
+            buffer_to_lds(w ? rv[kb] : rk[kb], to + w * G::TILE + u * 1024, off, 0);
+          }
+        look(j + 1);
+      } else {
+        // Lane i looks up key i % 32; then each lane takes what its loads need.  (Keys past the end
+        // repeat the last one.)
+        const int key = min(k0 + (lane & 31), len - 1), n = key / g.page_size;
+        const int32_t found = g.tables[b * g.table_stride + n];
+        const bool ok = found >= 0 && found < g.pages;
+        const int64_t page = ok ? found : 0;
+        const int slot = key - n * g.page_size;
+        if (lane < 32) {
+          key_at[wave][0][lane & (NKEYS - 1)] = (page * g.ks[0] + slot * g.ks[1]) * ES;
+          key_at[wave][1][lane & (NKEYS - 1)] = (page * g.vs[0] + slot * g.vs[1]) * ES;
+          Scales x{g.scale_log2, 0.f, 1.0f};
+          if (EIGHT && ok) x = scales(g.k_scale[page * g.kv_heads + h], g.v_scale[page * g.kv_heads + h]);
+          key_scale[wave][stage][0][lane & (NKEYS - 1)] = x.kf;
+          key_scale[wave][stage][1][lane & (NKEYS - 1)] = ok ? x.lv : -INFINITY;  // (a key of no page)
+          key_scale[wave][stage][2][lane & (NKEYS - 1)] = x.rv;
+        }
+        wave_lds_order();
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int u = 0; u < G::LOADS; ++u)
+            global_to_lds((w ? vbase : kbase) + key_at[wave][w][kv_key[u] & (NKEYS - 1)] +
+                              (kv_byte[u] < D * ES ? kv_byte[u] : 0),
+                          to + w * G::TILE + u * 1024);
+        wave_lds_order();
+      }
+    };
+    if (SIXTEENS) look(0);
+#pragma unroll
+    for (int j = 0; j < G::STAGES; ++j)
+      if (j < nt) issue(j, j);
 
     typename MQ::frag qf[STEPS];
     {
@@ -212,129 +346,51 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
     for (int c = 0; c < DL; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    const int32_t* table = g.tables + b * g.table_stride;
-    const char* kbase = (const char*)g.k + h * g.ks[2] * ES;
-    const char* vbase = (const char*)g.v + h * g.vs[2] * ES;
-    const int tiles = (len + BN - 1) / BN;
-    const int t_end = min(blk1 * NW, tiles);
-
-    struct Tile {
-      u32x4 k[2][KL];
-      Words<VW> v[8];
-      float kf, lv, rv;  // ONE_PAGE: k's factor, log2 and reciprocal of v's scale
-      bool ok;
-    };
-    auto scales = [&](int64_t page, float& kf, float& lv, float& rv) {
-      const float ks = g.k_scale[page * g.kv_heads + h], vs = fmaxf(g.v_scale[page * g.kv_heads + h], LEAST_SCALE);
-      kf = ks * g.scale_log2;
-      lv = __builtin_amdgcn_logf(vs);
-      rv = 1.0f / vs;
-    };
-    auto load = [&](Tile& x, int t, int buf) {
-      const int k0 = t * BN, last = min(BN, len - k0) - 1;  // (keys past the end repeat the last one)
-      int64_t page = 0;
-      const char *kp = kbase, *vp = vbase;
-      x.ok = true;
-      if (ONE_PAGE) {
-        page = table[k0 / g.page_size];
-        x.ok = page >= 0 && page < g.pages;
-        if (!x.ok) page = 0;
-        const int slot = k0 % g.page_size;
-        kp += (page * g.ks[0] + slot * g.ks[1]) * ES;
-        vp += (page * g.vs[0] + slot * g.vs[1]) * ES;
-        if (EIGHT) scales(page, x.kf, x.lv, x.rv);
-      } else {
-        // Each lane looks up key lane % 32; the wave's lanes then take what they need of them.
-        const int key = k0 + min(lane & 31, last), n = key / g.page_size;
-        page = table[n];
-        const bool ok = page >= 0 && page < g.pages;
-        if (!ok) page = 0;
-        const int slot = key - n * g.page_size;
-        if (lane < 32) {
-          key_at[wave][buf][0][lane] = (page * g.ks[0] + slot * g.ks[1]) * ES;
-          key_at[wave][buf][1][lane] = (page * g.vs[0] + slot * g.vs[1]) * ES;
-          if (EIGHT) {
-            float kf, lv, rv;
-            scales(page, kf, lv, rv);
-            key_scale[wave][buf][0][lane] = kf;
-            key_scale[wave][buf][1][lane] = lv;
-            key_scale[wave][buf][2][lane] = rv;
-          }
-        }
-        x.ok = !__builtin_amdgcn_ballot_w64(!ok);
-        wave_lds_order();
-      }
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const int key = kb * 16 + col;
-        const char* row = ONE_PAGE ? kp + min(key, last) * (int)(g.ks[1] * ES) : kbase + key_at[wave][buf][0][ONE_PAGE ? 0 : key];
-#pragma unroll
-        for (int u = 0; u < KL; ++u) {
-          const int d = (EIGHT ? u * 64 + quad * 16 : u * 32 + quad * 8);
-          x.k[kb][u] = D == DM || d < D ? *(const u32x4*)(row + d * ES) : u32x4{0u, 0u, 0u, 0u};
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int key = (e >> 2) * 16 + quad * 4 + (e & 3);
-        const char* row = ONE_PAGE ? vp + min(key, last) * (int)(g.vs[1] * ES) : vbase + key_at[wave][buf][1][ONE_PAGE ? 0 : key];
-        const int d = col * DL;  // (elements past D reach outputs past D only)
-        x.v[e] = *(const Words<VW>*)(row + (D == DM || d < D ? d : 0) * ES);
-      }
-    };
-    auto compute = [&](Tile& x, int t, int buf) {
-      if (ONE_PAGE && !x.ok) return;
+    auto compute = [&](int j, int stage) {
+      const int k0 = (t0 + j * NW) * BN;
+      if (j + 1 < nt)
+        wait_loads<3 * G::LOADS>();  // k's have ended: v's and the next tile's may be under way
+      else
+        wait_loads<G::LOADS>();
       floatx4 s[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         s[kb] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-          u32x4 w;
+        for (int u = 0; u < KL; ++u) {
+          u32x4 w = k_frag(stage, kb, u);
+          if (!SIXTEENS && D != DM && (u * 4 + quad) * 16 >= D * ES) w = u32x4{0u, 0u, 0u, 0u};
           if (EIGHT) {
-            const u32x4 r = x.k[kb][st >> 1];
-            w = st & 1 ? wide8<T>(r[2], r[3]) : wide8<T>(r[0], r[1]);
+            s[kb] = MQ::mma(__builtin_bit_cast(typename MQ::frag, wide8<T>(w[0], w[1])), qf[(2 * u) % STEPS], s[kb]);
+            s[kb] = MQ::mma(__builtin_bit_cast(typename MQ::frag, wide8<T>(w[2], w[3])), qf[(2 * u + 1) % STEPS], s[kb]);
           } else {
-            w = x.k[kb][st];
+            s[kb] = MQ::mma(__builtin_bit_cast(typename MQ::frag, w), qf[u % STEPS], s[kb]);
           }
-          s[kb] = MQ::mma(__builtin_bit_cast(typename MQ::frag, w), qf[st], s[kb]);
         }
       }
-      const int k0 = t * BN;
       float y[8], rv[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int key = (e >> 2) * 16 + quad * 4 + (e & 3);
-        if (!EIGHT) {
-          y[e] = s[e >> 2][e & 3] * g.scale_log2;
-        } else if (ONE_PAGE) {
-          y[e] = __builtin_fmaf(s[e >> 2][e & 3], x.kf, x.lv);
-          rv[e] = x.rv;
+        const int kb = e >> 2, key = kb * 16 + quad * 4 + (e & 3);
+        if (SIXTEENS) {
+          y[e] = EIGHT ? __builtin_fmaf(s[kb][e & 3], sc[stage][kb].kf, sc[stage][kb].lv) : s[kb][e & 3] * g.scale_log2;
+          rv[e] = sc[stage][kb].rv;
         } else {
-          y[e] = __builtin_fmaf(s[e >> 2][e & 3], key_scale[wave][buf][0][ONE_PAGE || !EIGHT ? 0 : key],
-                                key_scale[wave][buf][1][ONE_PAGE || !EIGHT ? 0 : key]);
-          rv[e] = key_scale[wave][buf][2][ONE_PAGE || !EIGHT ? 0 : key];
+          y[e] = __builtin_fmaf(s[kb][e & 3], key_scale[wave][stage][0][key & (NKEYS - 1)],
+                                key_scale[wave][stage][1][key & (NKEYS - 1)]);
+          rv[e] = key_scale[wave][stage][2][key & (NKEYS - 1)];
         }
       }
-      if (k0 + BN > len) {  // (the last key's row stands in for those past it: nothing of it counts twice)
+      const bool cut = k0 + BN > len || (SIXTEENS && !(real[stage][0] && real[stage][1]));
+      if (cut) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (k0 + (e >> 2) * 16 + quad * 4 + (e & 3) >= len) {
-            y[e] = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < VW; ++w) x.v[e].w[w] = 0u;
-          }
+          if (k0 + (e >> 2) * 16 + quad * 4 + (e & 3) >= len || (SIXTEENS && !real[stage][e >> 2])) y[e] = -INFINITY;
       }
-      if (!ONE_PAGE && !x.ok) {  // keys of no page: no weight, and nothing of what was read for them
+      if (!SIXTEENS) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int n = min(k0 + (e >> 2) * 16 + quad * 4 + (e & 3), len - 1) / g.page_size;
-          if (table[n] < 0 || table[n] >= g.pages) {
-            y[e] = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < VW; ++w) x.v[e].w[w] = 0u;
-          }
-        }
+        for (int e = 0; e < 8; ++e)
+          if (key_scale[wave][stage][1][((e >> 2) * 16 + quad * 4 + (e & 3)) & (NKEYS - 1)] == -INFINITY) y[e] = -INFINITY;
       }
       float mx = y[0];
 #pragma unroll
@@ -361,13 +417,28 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
         pw[e >> 1] = MP::pack(p0, p1);
       }
       const typename MP::frag pf = __builtin_bit_cast(typename MP::frag, pw);
+      if (j + 1 < nt)
+        wait_loads<2 * G::LOADS>();
+      else
+        wait_loads<0>();
+      Words<VW> v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = v_words(stage, e);
+        if (!SIXTEENS) {  // keys past the end or of no page: nothing of what was read for them
+          const int key = (e >> 2) * 16 + quad * 4 + (e & 3);
+          const bool out = k0 + key >= len || key_scale[wave][stage][1][key & (NKEYS - 1)] == -INFINITY;
+#pragma unroll
+          for (int w = 0; w < VW; ++w) v[e].w[w] = out ? 0u : v[e].w[w];
+        }
+      }
       if (EIGHT) {
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t tr[2][4];  // [keys 0-3, 4-7][element]: four keys' bytes of one element
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const uint32_t a0 = x.v[4 * q].w[w], a1 = x.v[4 * q + 1].w[w], a2 = x.v[4 * q + 2].w[w], a3 = x.v[4 * q + 3].w[w];
+            const uint32_t a0 = v[4 * q].w[w], a1 = v[4 * q + 1].w[w], a2 = v[4 * q + 2].w[w], a3 = v[4 * q + 3].w[w];
             const uint32_t l01 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), h01 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
             const uint32_t l23 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), h23 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
             tr[q][0] = __builtin_amdgcn_perm(l23, l01, 0x05040100u);
@@ -377,7 +448,7 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            acc[4 * w + e] = MP::mma(__builtin_bit_cast(typename MP::frag, wide8<P>(tr[0][e], tr[1][e])), pf, acc[4 * w + e]);
+            acc[(4 * w + e) % DL] = MP::mma(__builtin_bit_cast(typename MP::frag, wide8<P>(tr[0][e], tr[1][e])), pf, acc[(4 * w + e) % DL]);
         }
       } else {
 #pragma unroll
@@ -387,34 +458,31 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
             const uint32_t sel = e ? 0x07060302u : 0x05040100u;
             u32x4 a;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[j] = __builtin_amdgcn_perm(x.v[2 * j + 1].w[w], x.v[2 * j].w[w], sel);
-            acc[2 * w + e] = MP::mma(__builtin_bit_cast(typename MP::frag, a), pf, acc[2 * w + e]);
+            for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(v[2 * i + 1].w[w], v[2 * i].w[w], sel);
+            acc[(2 * w + e) % DL] = MP::mma(__builtin_bit_cast(typename MP::frag, a), pf, acc[(2 * w + e) % DL]);
           }
       }
+      // Every LDS read of this stage has returned before it is filled again.
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (j + G::STAGES < nt) issue(j + G::STAGES, stage);
     };
-    {
-      int t = blk0 * NW + wave;
-      Tile x, y;
-      if (t < t_end) load(x, t, 0);
-      while (t < t_end) {
-        if (t + NW < t_end) load(y, t + NW, 1);
-        compute(x, t, 0);
-        t += NW;
-        if (t >= t_end) break;
-        if (t + NW < t_end) load(x, t + NW, 0);
-        compute(y, t, 1);
-        t += NW;
-      }
+    static_assert(G::STAGES == 2, "the waits count one tile under way behind the current one");
+    for (int j = 0; j < nt; j += 2) {
+      compute(j, 0);
+      if (j + 1 < nt) compute(j + 1, 1);
     }
 
     // The waves' states through LDS, then the output, or a partial state where the keys go on in
     // another workgroup's stretch.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    __syncthreads();  // other waves may still read their stages, which the states cover
+    float* merge_o = (float*)ring;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < DL; ++c) merge_o[wave][col * OROW + (quad * 4 + r) * DL + c] = acc[c][r];
+      for (int c = 0; c < DL; ++c)
+        merge_o[wave * (G::MERGE / 4) + col * G::OROW + (quad * 4 + r) * DL + c] = acc[c][r];
     if (quad == 0) {
       merge_ml[wave][0][col] = m;
       merge_ml[wave][1][col] = l;
@@ -430,9 +498,9 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
       float sum = 0.f, o = 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float mw = merge_ml[w][0][r], sc = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
-        sum += merge_ml[w][1][r] * sc;
-        o += merge_o[w][r * OROW + d] * sc;
+        const float mw = merge_ml[w][0][r], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
+        sum += merge_ml[w][1][r] * f;
+        o += merge_o[w * (G::MERGE / 4) + r * G::OROW + d] * f;
       }
       if (whole) {
         if (d < D)
@@ -487,17 +555,18 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs g) {
   }
 }
 
-// Workgroups of a launch: 512 (two a CU), or fewer where the longest possible sequences have fewer
-// blocks; partial states only where a sequence can have more than one block.
-static int64_t cache_workgroups(int64_t lines, int64_t most_keys) {
-  return std::min<int64_t>(512, lines * std::max<int64_t>(1, cdiv(most_keys, ca::BLOCK)));
+// Workgroups of a launch: as many as the CUs' LDS holds at once, or fewer where the longest
+// possible sequences have fewer blocks; partial states only where a sequence can have more than one.
+static int64_t cache_workgroups(int64_t lines, int64_t most_keys, bool eight, bool wide) {
+  const int64_t a_cu = eight ? (wide ? 2 : 3) : (wide ? 1 : 2);
+  return std::min<int64_t>(256 * a_cu, lines * std::max<int64_t>(1, cdiv(most_keys, ca::BLOCK)));
 }
 static int64_t cache_part_floats(int64_t workgroups, int64_t dm) { return workgroups * 2 * ca::BQ * (dm + 2); }
 
 template <typename T, bool EIGHT, int DM>
 static void cache_launch(const CacheArgs& g, bool join, hipStream_t stream) {
   const dim3 grid((unsigned)g.workgroups), block(ca::NW * 64);
-  if (g.page_size % ca::BN == 0)
+  if (g.page_size % 16 == 0)
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, true>), grid, block, 0, stream, g);
   else
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, false>), grid, block, 0, stream, g);
@@ -509,12 +578,13 @@ static void cache_launch(const CacheArgs& g, bool join, hipStream_t stream) {
 }  // namespace nt
 
 extern "C" int64_t nt_cache_attention_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
-                                                     int64_t page_size, int64_t table_width) {
+                                                     int64_t page_size, int64_t table_width, int cache_dtype) {
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim > 128 || page_size <= 0 ||
       table_width <= 0 || page_size * table_width <= nt::ca::BLOCK)
     return 0;
   const int64_t lines = sequences * kv_heads * nt::cdiv(heads / kv_heads, nt::ca::BQ);
-  return nt::cache_part_floats(nt::cache_workgroups(lines, page_size * table_width), dim <= 64 ? 64 : 128) * 4;
+  return nt::cache_part_floats(nt::cache_workgroups(lines, page_size * table_width, cache_dtype == NT_DTYPE_E4M3, dim > 64),
+                               dim <= 64 ? 64 : 128) * 4;
 }
 
 extern "C" int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,
@@ -566,12 +636,15 @@ extern "C" int nt_cache_attention(const void* q, const int64_t* q_strides, const
   g.page_size = (int)page_size;
   g.table_width = (int)table_width;
   g.row_blocks = (int)nt::cdiv(g.group, nt::ca::BQ);
+  g.page_shift = -1;
+  for (int i = 0; i < 27; ++i)
+    if (page_size == 16LL << i) g.page_shift = i;
   g.scale_log2 = scale * 1.44269504088896340736f;
   const int64_t lines = sequences * kv_heads * g.row_blocks, dm = dim <= 64 ? 64 : 128;
   if (lines > 0x7fffffffLL) return NT_ERR_INVALID;
-  const int64_t need = nt_cache_attention_workspace_size(sequences, heads, kv_heads, dim, page_size, table_width);
+  const int64_t need = nt_cache_attention_workspace_size(sequences, heads, kv_heads, dim, page_size, table_width, cache_dtype);
   if (need > 0 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return NT_ERR_INVALID;
-  g.workgroups = (int)nt::cache_workgroups(lines, page_size * table_width);
+  g.workgroups = (int)nt::cache_workgroups(lines, page_size * table_width, eight, dim > 64);
   g.part_o = (float*)workspace;
   g.part_ml = g.part_o ? g.part_o + (int64_t)g.workgroups * 2 * nt::ca::BQ * dm : nullptr;
   const bool join = need > 0;

@@ -71,6 +71,35 @@ struct Packed {
   P* ptr() { return (P*)(uintptr_t)*v++; }
 };
 
+// Buffer resource of `bytes` bytes from `base` on (uniform: in scalar registers): reads past its
+// end give zeros.
+__device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
+  const uint64_t p = (uint64_t)base;
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p),
+               (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32) & 0xffffu),
+               (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+// 16 bytes a lane, from buffer `rs` at offset + soffset or from an address of each lane's own, into
+// LDS at lds_addr + 16 * lane.  Nothing waits for them but wait_loads.
+__device__ __forceinline__ void buffer_to_lds(u32x4 rs, uint32_t lds_addr, int offset, int soffset) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(offset), "s"(rs),
+                 "s"(__builtin_amdgcn_readfirstlane(soffset))
+               : "memory", "m0");
+}
+__device__ __forceinline__ void global_to_lds(const void* p, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(p)
+               : "memory", "m0");
+}
+// Until at most N of the wave's loads are under way (they end in order).
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
 // N neighbouring elements as they lie in memory.
 template <typename S, int N>
 struct alignas(sizeof(S) * N) Vec {

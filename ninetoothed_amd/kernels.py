@@ -943,7 +943,8 @@ def bind_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=None
     sequences, heads, dim = q.shape
     pages, page_size, kv_heads = k_cache.shape[:3]
     width = tables.shape[1] if pages else 0
-    nbytes = int(_lib.load().nt_cache_attention_workspace_size(sequences, heads, kv_heads, dim, page_size, width))
+    nbytes = int(_lib.load().nt_cache_attention_workspace_size(sequences, heads, kv_heads, dim, page_size, width,
+                                                               cache_code))
     # (a size of one may have any stride: the kernels take none for it)
     strides = [tuple(st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape)) for t in (k_cache, v_cache)]
     launch = _bind_packed("nt_cache_attention_packed", device, (

@@ -197,7 +197,8 @@ def test_entry_points_reject_before_they_launch():
 
 def test_workspace_size():
     size = _lib.load().nt_cache_attention_workspace_size
-    assert size(4, 8, 8, 128, 16, 8) == 0  # at most one block of keys a sequence
-    assert size(0, 8, 8, 128, 16, 100) == 0
-    assert size(1, 8, 8, 128, 16, 100) > 0
-    assert size(100, 32, 8, 128, 32, 1000) < 32 << 20
+    for cache in (_lib.DTYPE_F16, _lib.DTYPE_E4M3):
+        assert size(4, 8, 8, 128, 16, 8, cache) == 0  # at most one block of keys a sequence
+        assert size(0, 8, 8, 128, 16, 100, cache) == 0
+        assert size(1, 8, 8, 128, 16, 100, cache) > 0
+        assert size(100, 32, 8, 128, 32, 1000, cache) < 32 << 20
