@@ -11,6 +11,7 @@ namespace ca {
 constexpr int NW = 4;        // waves per workgroup
 constexpr int BN = 32;       // keys a wave takes at a time
 constexpr int BLOCK = NW * BN;
+constexpr int MOST_PARTS = 768;  // workgroups of a head
 constexpr int BQ = 16;       // query rows: heads that share a head of k and v
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr float LEAST_SCALE = 0x1p-64f;  // a smaller v scale (or none) counts as this one
@@ -86,49 +87,84 @@ struct CacheArgs {
   int64_t ks[3], vs[3];  // page, slot, head (elements side by side)
   const int32_t *tables, *lengths;
   int64_t table_stride, pages;
-  int sequences, kv_heads, group, dim, page_size, table_width, row_blocks, workgroups;
+  int sequences, kv_heads, group, dim, page_size, table_width, row_blocks, parts;
+  int q_vectors, join_rows;
   int page_shift;  // page_size = 16 << page_shift, or -1
   float scale_log2;
-  float *part_o, *part_ml;  // of partial states, two a workgroup: [slot][row][DM], [slot][row][2]
+  float *part_o, *part_ml;  // partial states, two a workgroup: [slot][row][DM], [slot][row][2]
 };
 
-// The work is a line of blocks of 128 keys: sequence by sequence, head by head (and block of 16
-// query rows), one block at least for each.  Every workgroup takes an equal stretch of the line,
-// so that sequences of very different lengths fill the chip evenly; where the stretch starts, the
-// workgroups find out for themselves from the lengths.
-struct Line {
-  int64_t share;
-  __device__ __forceinline__ static int keys(const CacheArgs& g, int b) {
-    return min(max(g.lengths[b], 0), g.table_width * g.page_size);
-  }
-  __device__ __forceinline__ static int blocks(const CacheArgs& g, int b) {
-    return max(1, (keys(g, b) + ca::BLOCK - 1) / ca::BLOCK);
-  }
-};
-// Blocks of all sequences before `upto` and of all (in blocks of one head), by the 256 lanes.
-__device__ __forceinline__ void line_sums(const CacheArgs& g, int upto, int64_t* sums, int64_t& before, int64_t& all) {
-  int64_t mine = 0, mine_before = 0;
-  for (int b = threadIdx.x; b < g.sequences; b += 256) {
-    const int n = Line::blocks(g, b);
-    mine += n;
-    mine_before += b < upto ? n : 0;
-  }
+// The work of a head of k and v is a line of blocks of 128 keys: sequence by sequence (and block of
+// 16 query rows), one block at least for each.  `parts` workgroups a head take equal stretches of it,
+// so that sequences of very different lengths fill the chip evenly; where a stretch starts, the
+// workgroups find out for themselves from the lengths.  The workgroups of all heads that take one
+// stretch run side by side: their keys lie side by side in memory.
+__device__ __forceinline__ int line_keys(const CacheArgs& g, int b) {
+  return min(max(g.lengths[b], 0), g.table_width * g.page_size);
+}
+__device__ __forceinline__ int line_blocks(int keys) { return max(1, (keys + ca::BLOCK - 1) / ca::BLOCK); }
+// The sum of n over the workgroup's lanes, and over those before this one.  `sums`: four of LDS,
+// not in use before the last barrier.
+__device__ __forceinline__ void line_scan(int n, int* sums, int& before, int& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int upto = n;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    mine += __shfl_xor(mine, off, 64);
-    mine_before += __shfl_xor(mine_before, off, 64);
+  for (int off = 1; off < 64; off <<= 1) {
+    const int other = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += other;
   }
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-    sums[wave] = mine;
-    sums[4 + wave] = mine_before;
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  before = upto - n;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    before += w < wave ? sums[w] : 0;
+    all += sums[w];
+  }
+}
+// The line's length, and the sequence (and its keys) in which position `at(length)` lies, with the
+// line's length before it; or of sequence `which`, if that is not negative.
+struct LinePlace {
+  int length, sequence, keys, before;
+};
+template <typename At>
+__device__ __forceinline__ LinePlace line_place(const CacheArgs& g, int which, int* lds, At&& at_of) {
+  const int tid = threadIdx.x;
+  int keys = tid < g.sequences ? line_keys(g, tid) : 0;
+  int n = tid < g.sequences ? line_blocks(keys) * g.row_blocks : 0;
+  LinePlace p{};
+  int before, sum;
+  line_scan(n, lds, before, sum);
+  p.length = sum;
+  for (int b0 = 256; b0 < g.sequences; b0 += 256) {  // (the length of a long batch's line comes first)
+    int more = b0 + tid < g.sequences ? line_blocks(line_keys(g, b0 + tid)) * g.row_blocks : 0;
+    int unused, total;
+    __syncthreads();
+    line_scan(more, lds, unused, total);
+    p.length += total;
+  }
+  const int at = at_of(p.length);
+  for (int b0 = 0, base = 0; b0 < g.sequences;) {
+    const bool here = which < 0 ? base + before <= at && at < base + before + n : b0 + tid == which;
+    if (here) {
+      lds[4] = b0 + tid;
+      lds[5] = keys;
+      lds[6] = base + before;
+    }
+    base += sum;
+    if (which < 0 ? at < base : which < b0 + 256) break;
+    b0 += 256;
+    keys = b0 + tid < g.sequences ? line_keys(g, b0 + tid) : 0;
+    n = b0 + tid < g.sequences ? line_blocks(keys) * g.row_blocks : 0;
+    __syncthreads();
+    line_scan(n, lds, before, sum);
   }
   __syncthreads();
-  all = sums[0] + sums[1] + sums[2] + sums[3];
-  before = sums[4] + sums[5] + sums[6] + sums[7];
-}
-__device__ __forceinline__ int64_t line_share(const CacheArgs& g, int64_t all_blocks) {
-  return max((int64_t)1, cdiv(all_blocks, g.workgroups));
+  p.sequence = __builtin_amdgcn_readfirstlane(lds[4]);
+  p.keys = __builtin_amdgcn_readfirstlane(lds[5]);
+  p.before = __builtin_amdgcn_readfirstlane(lds[6]);
+  return p;
 }
 
 // Per sequence and head of k and v, for the heads of q that share it (rows i):
@@ -160,49 +196,23 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
   constexpr int NKEYS = SIXTEENS ? 1 : BN;
   __shared__ __attribute__((aligned(1024))) char ring[G::LDS];
   __shared__ float merge_ml[NW][2][BQ];
-  __shared__ int64_t sums[8];
+  __shared__ int line_lds[8];
   __shared__ int64_t key_at[NW][2][NKEYS];             // where each key's k and v lie
   __shared__ float key_scale[NW][G::STAGES][3][NKEYS];  // k's factor, log2 and reciprocal of v's scale
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = g.dim;
 
-  const int lines = g.kv_heads * g.row_blocks;  // of a sequence
-  int64_t none, all;
-  line_sums(g, 0, sums, none, all);
-  const int64_t share = line_share(g, all * lines);
-  int64_t at = blockIdx.x * share;
-  const int64_t stop = min(at + share, all * lines);
+  const int h = blockIdx.x % g.kv_heads, part = blockIdx.x / g.kv_heads;
+  int share = 0;
+  const LinePlace place = line_place(g, -1, line_lds, [&](int length) {
+    share = (length + g.parts - 1) / g.parts;
+    return min(part * share, length - 1);  // (a workgroup past the end has nothing to do)
+  });
+  int at = part * share;
+  const int begin = at, stop = min(at + share, place.length);
   if (at >= stop) return;
-  const int64_t begin = at;
-  // The sequence of the stretch's first block, and the line's length up to it: each lane
-  // holds the sum of a run of sequences, whose prefix tells the run that holds `at`.
-  int b;
-  int64_t seq0;  // blocks of the line before sequence b
-  {
-    const int run = (g.sequences + 63) / 64;
-    int64_t mine = 0;
-    for (int i = 0; i < run; ++i) {
-      const int s = lane * run + i;
-      if (s < g.sequences) mine += Line::blocks(g, s);
-    }
-    mine *= lines;
-    int64_t upto = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t other = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += other;
-    }
-    const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
-    seq0 = __shfl(upto - mine, who, 64);
-    b = who * run;
-    for (;; ++b) {
-      const int64_t n = (int64_t)Line::blocks(g, b) * lines;
-      if (seq0 + n > at) break;
-      seq0 += n;
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-  }
+  int b = place.sequence, len = place.keys, seq0 = place.before;  // seq0: blocks of the line before sequence b
 
   // Where this lane's 16 bytes of each load lie behind the load's first key, and where its fragments
   // lie in a stage.  Elements past D read as zeros (SIXTEENS: past the buffer's end).
@@ -226,11 +236,8 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
   };
 
   while (at < stop) {
-    const int len = Line::keys(g, b), nblk = Line::blocks(g, b);
-    const int64_t inside = at - seq0;
-    const int line = (int)(inside / nblk), blk0 = (int)(inside % nblk);
-    const int blk1 = (int)min((int64_t)nblk, blk0 + (stop - at));
-    const int h = line / g.row_blocks, rb = line % g.row_blocks;
+    const int nblk = line_blocks(len), inside = at - seq0, rb = g.row_blocks == 1 ? 0 : inside / nblk, blk0 = inside - rb * nblk;
+    const int blk1 = min(nblk, blk0 + (stop - at));
     const int rows = min(BQ, g.group - rb * BQ);
     const int head0 = h * g.group + rb * BQ;
 
@@ -241,13 +248,13 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
     const int t0 = blk0 * NW + wave, t_end = min(blk1 * NW, tiles);
     const int nt = t0 < t_end ? (t_end - t0 + NW - 1) / NW : 0;  // this wave's tiles: t0 + j NW
 
-    // The scale of a page's head as a factor of scores, and what v's adds to exponents and sums.
+    // The scales of a page's head; as a factor of scores, and what v's adds to exponents and sums.
     struct Scales {
       float kf, lv, rv;
     };
     auto scales = [&](float ks, float vs) {
       vs = fmaxf(vs, LEAST_SCALE);
-      return Scales{ks * g.scale_log2, __builtin_amdgcn_logf(vs), 1.0f / vs};
+      return Scales{ks * g.scale_log2, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
     };
     auto page_number = [&](int sixteen) {  // of 16 keys; -1: none
       const int n = g.page_shift >= 0 ? sixteen >> g.page_shift : sixteen / (g.page_size >> 4);
@@ -257,7 +264,7 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
     // SIXTEENS: the pages of the tiles that come next (looked up ahead), and the scales of those
     // under way.
     int next_page[2];
-    Scales sc[G::STAGES][2];
+    float k_sc[G::STAGES][2], v_sc[G::STAGES][2];
     bool real[G::STAGES][2];
     auto look = [&](int j) {
 #pragma unroll
@@ -280,9 +287,8 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
           rv[kb] = buffer_of(vbase + (page * g.vs[0] + slot * g.vs[1]) * ES, ok ? (n - 1) * vst + D * ES : 0);
           real[stage][kb] = ok;
           if (EIGHT) {
-            sc[stage][kb] = scales(((ScalarFloats)(uintptr_t)g.k_scale)[page * g.kv_heads + h],
-                                   ((ScalarFloats)(uintptr_t)g.v_scale)[page * g.kv_heads + h]);
-            if (!ok) sc[stage][kb] = Scales{0.f, 0.f, 1.0f};
+            k_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.k_scale)[page * g.kv_heads + h];
+            v_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.v_scale)[page * g.kv_heads + h];
           }
         }
 #pragma unroll
@@ -332,13 +338,19 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
       const uint16_t* Q = (const uint16_t*)g.q + b * g.qs[0] + (head0 + col) * g.qs[1];
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        uint16_t x[8];
+        const int d = EIGHT ? (s >> 1) * 64 + quad * 16 + (s & 1) * 8 : s * 32 + quad * 8;  // (D: whole 16s)
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if (col < rows && d < D) {
+          if (g.q_vectors) {
+            w = *(const u32x4*)(Q + d);
+          } else {
+            uint16_t x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = EIGHT ? (s >> 1) * 64 + quad * 16 + (s & 1) * 8 + e : s * 32 + quad * 8 + e;
-          x[e] = col < rows && d < D ? Q[d * g.qs[2]] : (uint16_t)0;
+            for (int e = 0; e < 8; ++e) x[e] = Q[(d + e) * g.qs[2]];
+            w = *(const u32x4*)x;
+          }
         }
-        qf[s] = __builtin_bit_cast(typename MQ::frag, *(const u32x4*)x);
+        qf[s] = __builtin_bit_cast(typename MQ::frag, w);
       }
     }
     floatx4 acc[DL];
@@ -369,12 +381,18 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
         }
       }
       float y[8], rv[8];
+      Scales sc[2];
+      if (SIXTEENS && EIGHT) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          sc[kb] = real[stage][kb] ? scales(k_sc[stage][kb], v_sc[stage][kb]) : Scales{0.f, 0.f, 1.0f};
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int kb = e >> 2, key = kb * 16 + quad * 4 + (e & 3);
         if (SIXTEENS) {
-          y[e] = EIGHT ? __builtin_fmaf(s[kb][e & 3], sc[stage][kb].kf, sc[stage][kb].lv) : s[kb][e & 3] * g.scale_log2;
-          rv[e] = sc[stage][kb].rv;
+          y[e] = EIGHT ? __builtin_fmaf(s[kb][e & 3], sc[kb].kf, sc[kb].lv) : s[kb][e & 3] * g.scale_log2;
+          rv[e] = EIGHT ? sc[kb].rv : 1.0f;
         } else {
           y[e] = __builtin_fmaf(s[kb][e & 3], key_scale[wave][stage][0][key & (NKEYS - 1)],
                                 key_scale[wave][stage][1][key & (NKEYS - 1)]);
@@ -516,75 +534,155 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
     }
     __syncthreads();
     at += blk1 - blk0;
-    if (at - seq0 == (int64_t)nblk * lines) {
+    if (at - seq0 == nblk * g.row_blocks && at < stop) {
       seq0 = at;
-      ++b;
+      len = line_keys(g, ++b);
     }
   }
 }
 
-// Joins the partial states of one sequence, head and block of rows, where its keys were split.
+// Joins the partial states of a sequence's query rows, where its keys were split.  A workgroup takes
+// join_rows of them.  Many states: row by row, the weight of each state first, a lane for each, then
+// groups of lanes that each sum some of the outputs, 16 bytes a lane.  Few: a group of lanes a row.
 template <typename T, int DM>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs g) {
   using namespace ca;
-  __shared__ int64_t sums[8];
-  const int lines = g.kv_heads * g.row_blocks, b = blockIdx.x / lines, line = blockIdx.x % lines;
-  int64_t before, all;
-  line_sums(g, b, sums, before, all);
-  const int64_t share = line_share(g, all * lines);
-  const int nblk = Line::blocks(g, b);
-  const int64_t from = before * lines + (int64_t)line * nblk, to = from + nblk;
-  const int64_t w0 = from / share, w1 = (to - 1) / share;
-  if (w0 == w1) return;  // written by its one workgroup
-  const int h = line / g.row_blocks, rb = line % g.row_blocks, rows = min(BQ, g.group - rb * BQ);
-  const int64_t slot0 = 2 * w0 + (from == w0 * share ? 0 : 1);
-  for (int e = threadIdx.x; e < rows * DM; e += 256) {
-    const int r = e / DM, d = e % DM;
-    float mm = g.part_ml[(slot0 * BQ + r) * 2];
-    for (int64_t w = w0 + 1; w <= w1; ++w) mm = fmaxf(mm, g.part_ml[(2 * w * BQ + r) * 2]);
-    float sum = 0.f, o = 0.f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slot = w == w0 ? slot0 : 2 * w;
-      const float mw = g.part_ml[(slot * BQ + r) * 2], sc = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
-      sum += g.part_ml[(slot * BQ + r) * 2 + 1] * sc;
-      o += g.part_o[(slot * BQ + r) * DM + d] * sc;
+  constexpr int LANES = DM / 4, GROUPS = 256 / LANES, FEW = 8;
+  __shared__ int line_lds[8];
+  __shared__ float factor[MOST_PARTS], wave_m[4], wave_l[4];
+  __shared__ float4 part[GROUPS][LANES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int chunks = (min(g.group, BQ) + g.join_rows - 1) / g.join_rows;
+  int id = blockIdx.x;
+  const int chunk = id % chunks;
+  id /= chunks;
+  const int rb = id % g.row_blocks;
+  id /= g.row_blocks;
+  const int h = id % g.kv_heads, b = id / g.kv_heads;
+  const LinePlace place = line_place(g, b, line_lds, [](int) { return 0; });
+  const int share = (place.length + g.parts - 1) / g.parts, nblk = line_blocks(place.keys);
+  const int from = place.before + rb * nblk, to = from + nblk;
+  const int p0 = from / share, n = (to - 1) / share - p0 + 1;
+  if (n == 1) return;  // written by its one workgroup
+  const int begins = from == p0 * share ? 0 : 1;
+  const int row0 = chunk * g.join_rows, row1 = min(min(row0 + g.join_rows, BQ), g.group - rb * BQ);
+  const int group = tid / LANES, at = tid % LANES;
+  auto slot = [&](int i, int r) {  // of the i-th state
+    const int64_t workgroup = (int64_t)(p0 + i) * g.kv_heads + h;
+    return (2 * workgroup + (i == 0 ? begins : 0)) * BQ + r;
+  };
+  auto out = [&](int r) {
+    return (uint16_t*)g.o + b * g.os[0] + (h * g.group + rb * BQ + r) * g.os[1];
+  };
+  if (n <= FEW) {
+    for (int r = row0 + group; r < row1; r += GROUPS) {
+      float2 ml[FEW];
+      float4 x[FEW];
+#pragma unroll
+      for (int i = 0; i < FEW; ++i) {
+        if (i < n) {
+          ml[i] = *(const float2*)(g.part_ml + slot(i, r) * 2);
+          x[i] = *(const float4*)(g.part_o + slot(i, r) * DM + at * 4);
+        }
+      }
+      float mm = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < FEW; ++i)
+        if (i < n) mm = fmaxf(mm, ml[i].x);
+#pragma unroll
+      for (int i = 0; i < FEW; ++i) {
+        if (i < n) {
+          const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - mm);
+          sum += ml[i].y * f;
+          o[0] += x[i].x * f;
+          o[1] += x[i].y * f;
+          o[2] += x[i].z * f;
+          o[3] += x[i].w * f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (at * 4 + e < g.dim) out(r)[(at * 4 + e) * g.os[2]] = elem<T>::from_float(sum == 0.f ? 0.f : o[e] / sum);
     }
-    if (d < g.dim)
-      ((uint16_t*)g.o)[b * g.os[0] + (h * g.group + rb * BQ + r) * g.os[1] + d * g.os[2]] =
-          elem<T>::from_float(sum == 0.f ? 0.f : o / sum);
+    return;
+  }
+  for (int r = row0; r < row1; ++r) {
+    float mm = -INFINITY;
+    for (int i = tid; i < n; i += 256) mm = fmaxf(mm, g.part_ml[slot(i, r) * 2]);
+    mm = wave_max(mm);
+    if (lane == 0) wave_m[wave] = mm;
+    __syncthreads();
+    mm = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
+    float sum = 0.f;
+    for (int i = tid; i < n; i += 256) {
+      const float2 ml = *(const float2*)(g.part_ml + slot(i, r) * 2);
+      const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
+      factor[i] = f;
+      sum += ml.y * f;
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) wave_l[wave] = sum;
+    __syncthreads();
+    sum = wave_l[0] + wave_l[1] + wave_l[2] + wave_l[3];
+    float4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = group; i < n; i += GROUPS) {
+      const float4 x = *(const float4*)(g.part_o + slot(i, r) * DM + at * 4);
+      const float f = factor[i];
+      o.x += x.x * f;
+      o.y += x.y * f;
+      o.z += x.z * f;
+      o.w += x.w * f;
+    }
+    part[group][at] = o;
+    __syncthreads();
+    if (tid < DM && tid < g.dim) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) x += ((const float*)&part[i][0])[tid];
+      out(r)[tid * g.os[2]] = elem<T>::from_float(sum == 0.f ? 0.f : x / sum);
+    }
+    __syncthreads();
   }
 }
 
-// Workgroups of a launch: as many as the CUs' LDS holds at once, or fewer where the longest
-// possible sequences have fewer blocks; partial states only where a sequence can have more than one.
-static int64_t cache_workgroups(int64_t lines, int64_t most_keys, bool eight, bool wide) {
+// Workgroups a head: all heads' together as many as the CUs' LDS holds at once, or fewer where the
+// longest possible sequences have fewer blocks; partial states only where a sequence can have
+// more than one.
+static int64_t cache_parts(int64_t kv_heads, int64_t blocks, bool eight, bool wide) {
   const int64_t a_cu = eight ? (wide ? 2 : 3) : (wide ? 1 : 2);
-  return std::min<int64_t>(256 * a_cu, lines * std::max<int64_t>(1, cdiv(most_keys, ca::BLOCK)));
+  return std::max<int64_t>(1, std::min<int64_t>({256 * a_cu / kv_heads, blocks, (int64_t)ca::MOST_PARTS}));
 }
-static int64_t cache_part_floats(int64_t workgroups, int64_t dm) { return workgroups * 2 * ca::BQ * (dm + 2); }
 
 template <typename T, bool EIGHT, int DM>
-static void cache_launch(const CacheArgs& g, bool join, hipStream_t stream) {
-  const dim3 grid((unsigned)g.workgroups), block(ca::NW * 64);
+static void cache_launch(const CacheArgs& g, int64_t join_grid, hipStream_t stream) {
+  const dim3 grid((unsigned)(g.parts * g.kv_heads)), block(ca::NW * 64);
   if (g.page_size % 16 == 0)
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, true>), grid, block, 0, stream, g);
   else
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, false>), grid, block, 0, stream, g);
-  if (join)
-    hipLaunchKernelGGL((cache_join_kernel<T, DM>), dim3((unsigned)(g.sequences * g.kv_heads * g.row_blocks)), dim3(256), 0,
-                       stream, g);
+  if (join_grid)
+    hipLaunchKernelGGL((cache_join_kernel<T, DM>), dim3((unsigned)join_grid), dim3(256), 0, stream, g);
 }
 
 }  // namespace nt
 
+// The parts of a head of k and v, and the floats of their partial states.
+static int64_t cache_plan(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size,
+                          int64_t table_width, int cache_dtype, int64_t& parts) {
+  const int64_t blocks = std::max<int64_t>(1, nt::cdiv(page_size * table_width, nt::ca::BLOCK));
+  const int64_t line = sequences * nt::cdiv(heads / kv_heads, nt::ca::BQ) * blocks;
+  parts = nt::cache_parts(kv_heads, line, cache_dtype == NT_DTYPE_E4M3, dim > 64);
+  return blocks == 1 ? 0 : parts * kv_heads * 2 * nt::ca::BQ * ((dim <= 64 ? 64 : 128) + 2);
+}
+
 extern "C" int64_t nt_cache_attention_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
                                                      int64_t page_size, int64_t table_width, int cache_dtype) {
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim > 128 || page_size <= 0 ||
-      table_width <= 0 || page_size * table_width <= nt::ca::BLOCK)
+      table_width <= 0)
     return 0;
-  const int64_t lines = sequences * kv_heads * nt::cdiv(heads / kv_heads, nt::ca::BQ);
-  return nt::cache_part_floats(nt::cache_workgroups(lines, page_size * table_width, cache_dtype == NT_DTYPE_E4M3, dim > 64),
-                               dim <= 64 ? 64 : 128) * 4;
+  int64_t parts;
+  return 4 * cache_plan(sequences, heads, kv_heads, dim, page_size, table_width, cache_dtype, parts);
 }
 
 extern "C" int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,
@@ -640,19 +738,26 @@ extern "C" int nt_cache_attention(const void* q, const int64_t* q_strides, const
   for (int i = 0; i < 27; ++i)
     if (page_size == 16LL << i) g.page_shift = i;
   g.scale_log2 = scale * 1.44269504088896340736f;
-  const int64_t lines = sequences * kv_heads * g.row_blocks, dm = dim <= 64 ? 64 : 128;
-  if (lines > 0x7fffffffLL) return NT_ERR_INVALID;
-  const int64_t need = nt_cache_attention_workspace_size(sequences, heads, kv_heads, dim, page_size, table_width, cache_dtype);
+  // (the line of a head's blocks is counted in 32 bits)
+  if (sequences * heads > 0x7fffffffLL ||
+      sequences * g.row_blocks * (page_size * table_width / nt::ca::BLOCK + 1) > 0x70000000LL)
+    return NT_ERR_INVALID;
+  int64_t parts;
+  const int64_t need = 4 * cache_plan(sequences, heads, kv_heads, dim, page_size, table_width, cache_dtype, parts);
   if (need > 0 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return NT_ERR_INVALID;
-  g.workgroups = (int)nt::cache_workgroups(lines, page_size * table_width, eight, dim > 64);
+  g.parts = (int)parts;
   g.part_o = (float*)workspace;
-  g.part_ml = g.part_o ? g.part_o + (int64_t)g.workgroups * 2 * nt::ca::BQ * dm : nullptr;
-  const bool join = need > 0;
+  g.part_ml = workspace ? g.part_o + parts * kv_heads * 2 * nt::ca::BQ * (dim <= 64 ? 64 : 128) : nullptr;
+  // A workgroup joins one row, or where those are many, all of a head's.
+  const int most_rows = std::min<int>(g.group, nt::ca::BQ);
+  g.join_rows = sequences * heads > 1024 ? most_rows : 1;
+  const int64_t join_grid = need > 0 ? sequences * kv_heads * g.row_blocks * nt::cdiv(most_rows, g.join_rows) : 0;
+  g.q_vectors = q_strides[2] == 1 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 && (uintptr_t)q % 16 == 0;
 #define NT_CACHE(T, E)                                     \
   if (dim <= 64)                                           \
-    nt::cache_launch<T, E, 64>(g, join, stream);           \
+    nt::cache_launch<T, E, 64>(g, join_grid, stream);           \
   else                                                     \
-    nt::cache_launch<T, E, 128>(g, join, stream);
+    nt::cache_launch<T, E, 128>(g, join_grid, stream);
   if (dtype == NT_DTYPE_F16) {
     if (eight) {
       NT_CACHE(nt::f16_t, true)

@@ -914,8 +914,9 @@ def check_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=Non
     _check_tables(tables, lengths)
     if tables.shape[0] != q.shape[0]:
         raise ValueError("tables must have a row for each sequence of q")
-    if k_cache.shape[1] * tables.shape[1] > 0x7FFFFF00:
-        raise ValueError("cache_attention takes less than 2^31 keys a sequence")
+    keys, blocks = k_cache.shape[1] * tables.shape[1], q.shape[0] * -(-q.shape[1] // (16 * k_cache.shape[2]))
+    if keys > 0x7FFFFF00 or blocks * (keys // 128 + 1) > 0x70000000 or q.shape[0] * q.shape[1] > 0x7FFFFFFF:
+        raise ValueError("cache_attention takes less than 2^31 keys a sequence, and 2^37 in all")
     vector = 16 // k_cache.element_size()
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         if any(st % vector for st, size in zip(t.stride()[:3], t.shape) if size > 1):
