@@ -44,6 +44,40 @@ constexpr uint32_t inf_bits = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
 template <typename T>
 constexpr uint32_t one_bits = std::is_same<T, f16_t>::value ? 0x3c00u : 0x3f80u;
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// x of lane l ^ 32, and the larger of the two.  (v_permlane32_swap of two copies of x leaves the
+// low half's values in the first and the high half's in the second, in both halves; the VALU
+// write of its operands needs wait states before it.)
+__device__ __forceinline__ void both_halves(float x, float& lo, float& hi) {
+  lo = x;
+  hi = x;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo), "+v"(hi));
+}
+__device__ __forceinline__ float max_halves(float x) {
+  float lo, hi;
+  both_halves(x, lo, hi);
+  return fmaxf(lo, hi);
+}
+__device__ __forceinline__ float other_half(float x) {
+  float lo, hi;
+  both_halves(x, lo, hi);
+  return (threadIdx.x & 32) ? lo : hi;
+}
+// acc plus the two packed values of w, in fp32.
+template <typename T>
+__device__ __forceinline__ float add2(uint32_t w, float acc) {
+  const uint32_t one2 = one_bits<T> | one_bits<T> << 16;
+  if constexpr (std::is_same<T, f16_t>::value)
+    acc = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, w), __builtin_bit_cast(half2_t, one2), acc, false);
+  else
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf162_t, w), __builtin_bit_cast(bf162_t, one2), acc, false);
+  return acc;
+}
+
 // Eight packed values with zeros for the infinities and NaN.
 template <typename T>
 __device__ __forceinline__ u32x4 finite8(u32x4 w) {
@@ -67,12 +101,85 @@ struct PromptArgs {
   float scale_log2;  // softmax scale * log2(e)
 };
 
-// Workgroup id -> (unit, head of k and v).  Ids go to the 8 XCDs round-robin, each with its own
-// L2: when the heads divide by 8, XCD x walks heads x, x + 8, ..., so that a head's K and V stay
-// in one L2; and units run from the last to the first, the long causal ones of a sequence first.
-__device__ __forceinline__ void prompt_order(const PromptArgs& g, int64_t id, int64_t& unit, int& head) {
-  unit = g.units - 1 - id / g.kv_heads;
-  head = (int)(id % g.kv_heads);
+// The block of rows a workgroup takes: longest first.  Up to 64 sequences: a lane for each, which
+// counts its blocks of at least so many key tiles; the number of tiles of the wanted block is found by
+// bisection, so the last workgroups of a launch are its shortest.  More sequences: from the last
+// block to the first.
+struct PromptBlock {
+  int64_t q_begin, k_begin;
+  int head, r0, rows, Sq, Sk;  // rows: of the sequence; 0: nothing to do
+};
+__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
+  using namespace pa;
+  PromptBlock p{};
+  // Ids go to the 8 XCDs round-robin, each with its own L2: where the heads divide by 8, an XCD
+  // keeps to the K and V of heads of its own.
+  p.head = (int)(blockIdx.x % g.kv_heads);
+  const int64_t id = blockIdx.x / g.kv_heads;
+  auto k_clamp = [&](int64_t s) { return s < 0 ? 0 : s > g.k_tokens ? g.k_tokens : s; };
+  auto sequence = [&](int b) {
+    p.q_begin = clamped_start(g.map, b);
+    p.k_begin = k_clamp(g.k_starts[b]);
+    p.Sq = (int)max((int64_t)0, clamped_start(g.map, b + 1) - p.q_begin);
+    p.Sk = (int)max((int64_t)0, k_clamp(g.k_starts[b + 1]) - p.k_begin);
+    p.rows = p.Sq * g.group;
+  };
+  if (g.map.sequences > 64) {
+    const int64_t unit = g.units - 1 - id;
+    const int b = find_sequence(g.map, unit);
+    sequence(b);
+    const int64_t r0 = (unit - first_unit(g.map, b)) * BM;
+    if (r0 < 0 || r0 >= p.rows) p.rows = 0;
+    p.r0 = (int)r0;
+    return p;
+  }
+  const int lane = threadIdx.x & 63;
+  int rows = 0, Sk = 0, offset = 0;
+  if (lane < g.map.sequences) {
+    sequence(lane);
+    rows = p.rows;
+    Sk = p.Sk;
+    offset = Sk - p.Sq;
+  }
+  const int blocks = (rows + BM - 1) / BM, tiles = (Sk + BN - 1) / BN;
+  auto at_least = [&](int n) {  // this lane's blocks of at least n tiles
+    if (n <= 0) return blocks;
+    if (n > tiles) return 0;
+    if (!g.causal) return blocks;
+    const int64_t from = ((int64_t)(n - 1) * BN - offset) * g.group;  // the first row that needs them
+    return from <= 0 ? blocks : from >= rows ? 0 : blocks - (int)(from / BM);
+  };
+  auto sum = [&](int x) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    return x;
+  };
+  p.rows = 0;
+  if (id >= sum(blocks)) return p;
+  int lo = 0, hi = tiles;  // of the wanted block: lo <= its tiles <= hi
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) hi = max(hi, __shfl_xor(hi, off, 64));
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sum(at_least(mid)) > id)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const int more = at_least(lo + 1), here = at_least(lo) - more;
+  int upto = here;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int other = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += other;
+  }
+  const int rank = (int)id - sum(more);  // among the blocks of as many tiles
+  const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rank));
+  // (a sequence's blocks grow in tiles: those of exactly `lo` end before its last `more`)
+  const int block = blocks - more - (upto - rank);
+  p.r0 = __builtin_amdgcn_readfirstlane(__shfl(block, who, 64)) * BM;
+  sequence(__builtin_amdgcn_readfirstlane(who));
+  return p;
 }
 
 // Per row i of a sequence (a token and a head of its group) over the keys j it may see:
@@ -82,19 +189,300 @@ __device__ __forceinline__ void prompt_order(const PromptArgs& g, int64_t id, in
 // side by side for each token, so that short sequences fill its rows and share K and V; eight waves
 // of 32 rows, two a SIMD.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: a lane holds
 // one row, its max and sum take no LDS, and P^T goes from the score registers to the second product
-// as it is.  Keys stream through two LDS stages of 64, fetched by waves 0-3 (K) and 4-7 (V,
-// transposed in registers on the way).
+// as it is.
 //   - Scores stay unscaled in fp32 until exp2(s scale - m): q is not rounded a second time.
 //   - m is raised only where a tile's max passes it by 2^8 (o and l are rescaled then): p stays
 //     within 2^8 and keeps its relative precision; o / l is the same.
 //   - p is rounded to the operands' type for the product; its row sums are of the rounded p.
 //   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
-//     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: where a tile
-//     that some row masks holds one (the fetching waves look), the product is taken of the finite
-//     values and the others are added, one by one, to the rows that see them.
-// VEC: unit element strides, 16-byte aligned rows; else element by element.
-template <typename T, int DM, bool VEC>
-__global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_attention_kernel(
+//     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: rows of a
+//     tile that is masked and holds one are taken key by key, each over the keys that it sees.
+// A wave's 32 rows, one to a lane and its other half, which share its elements: the same sums key by key
+// over the `keys` first keys, those up to each row's `last`.  For rows whose masked keys hold
+// infinities or NaN; slow.
+template <typename T, int DM>
+__device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char* K, const char* V, uint16_t* O,
+                                                   int64_t ks2b, int64_t vs2b, int keys, int last, bool valid, int D,
+                                                   float scale_log2) {
+  constexpr int N = DM / 2;  // elements of a lane
+  const int d0 = ((threadIdx.x >> 5) & 1) * N;
+  float o[N], m = -INFINITY, l = 0.f;
+  u32x4 q[N / 8];
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i)
+    q[i] = valid && d0 + i * 8 < D ? *(const u32x4*)(Q + d0 + i * 8) : u32x4{0u, 0u, 0u, 0u};
+  auto value = [](const u32x4& x, int e) { return elem<T>::to_float((uint16_t)(x[e >> 1] >> ((e & 1) * 16))); };
+#pragma unroll 1
+  for (int key = 0; key < keys; ++key) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) {
+      const u32x4 k = d0 + i * 8 < D ? *(const u32x4*)(K + key * ks2b + (d0 + i * 8) * 2) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = __builtin_fmaf(value(q[i], e), value(k, e), s);
+    }
+    s = (s + pa::other_half(s)) * scale_log2;
+    const bool seen = key <= last;
+    const float m_new = seen ? fmaxf(m, s) : m;
+    const float shift = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - shift), p = seen ? __builtin_amdgcn_exp2f(s - shift) : 0.f;
+    m = m_new;
+    l = l * alpha + p;
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) {
+      const u32x4 v = d0 + i * 8 < D ? *(const u32x4*)(V + key * vs2b + (d0 + i * 8) * 2) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (seen) o[i * 8 + e] = __builtin_fmaf(p, value(v, e), o[i * 8 + e] * alpha);
+    }
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    if (valid && d0 + i < D)
+      *(u32x2*)(O + d0 + i) = u32x2{pa::pack2<T>(o[i] * inv, o[i + 1] * inv), pa::pack2<T>(o[i + 2] * inv, o[i + 3] * inv)};
+}
+
+// Unit element strides and 16-byte aligned rows.  K and V stream by direct loads into three LDS stages
+// of 64 keys each.  The two waves of a SIMD work half a tile apart, kept there by a barrier for each half:
+// while one has the matrix core (the products of a tile's scores and of the tile before with V), the
+// other turns its scores into weights.  A load is issued two halves before the barrier that ends it.
+// LDS: K [key][DM] in 16-byte chunks XORed by key, so that the 16 keys of a fragment read fall on 16
+// distinct bank groups; V [key][DM] in 64-byte chunks XORed by key, for the 4 keys of a transposing read.
+template <typename T, int DM>
+__global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_stream_kernel(
+    PromptArgs g) {
+  using namespace pa;
+  typedef typename mfma_traits<T>::frag frag;
+  constexpr int DSUB = DM / 16, DBLK = DM / 32, ROW = DM * 2, CHUNKS = ROW / 16, TILE = BN * ROW;
+  constexpr int STAGES = 3, LPW = TILE / 1024 / NW, KEYS = 1024 / ROW;  // loads a wave and operand, keys of each
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGES * TILE];  // K's stages, then V's
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const PromptBlock blk = prompt_block(g);
+  if (blk.rows == 0) return;
+  const int r0 = blk.r0, rows = blk.rows, Sk = blk.Sk, head = blk.head, D = g.dim;
+  const int offset = Sk - blk.Sq;  // causal: token i sees keys up to i + offset
+  const int rw = r0 + wave * 32;   // first row of this wave
+  const int row = rw + (lane & 31), tok = row / g.group;
+  const int qhead = head * g.group + (row - tok * g.group);
+
+  // The last key a row sees, and how many tiles the workgroup and this wave need.
+  const int last = g.causal ? tok + offset : Sk - 1;
+  int nkt = (Sk + BN - 1) / BN, nkt_w = nkt, full_w = Sk / BN;
+  if (g.causal) {
+    const int end = (min(r0 + BM, rows) - 1) / g.group + offset, end_w = (min(rw + 32, rows) - 1) / g.group + offset;
+    nkt = end < 0 ? 0 : min(nkt, end / BN + 1);
+    nkt_w = end_w < 0 ? 0 : min(nkt, end_w / BN + 1);
+    const int begin_w = rw / g.group + offset;  // every row of the wave sees the tiles before it
+    full_w = begin_w < 0 ? 0 : min(full_w, (begin_w + 1) / BN);
+  }
+  if (rw >= rows) nkt_w = 0;
+
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const char* Kb = (const char*)((const uint16_t*)g.k + blk.k_begin * g.ks[0] + head * g.ks[1]);
+  const char* Vb = (const char*)((const uint16_t*)g.v + blk.k_begin * g.vs[0] + head * g.vs[1]);
+  const int ks2b = (int)g.ks[0] * 2, vs2b = (int)g.vs[0] * 2;
+  auto k_swz = [](int key) { return DM == 128 ? key & 15 : (key >> 1) & 7; };
+  auto v_swz = [](int key) { return DM == 128 ? key & 3 : (key >> 1) & 1; };
+  int vk[LPW], vv[LPW];
+#pragma unroll
+  for (int u = 0; u < LPW; ++u) {
+    const int key = (wave * LPW + u) * KEYS + lane / CHUNKS, p = lane % CHUNKS;
+    const int kc = p ^ k_swz(key), vc = (((p >> 2) ^ v_swz(key)) << 2) | (p & 3);
+    vk[u] = kc * 8 < D ? key * ks2b + kc * 16 : 0x7fffffff;  // (elements past D: past the buffer's end, zeros)
+    vv[u] = vc * 8 < D ? key * vs2b + vc * 16 : 0x7fffffff;
+  }
+  // A tile's rows as a buffer that ends with the sequence: keys past it read as zeros.
+  auto issue = [&](const char* base, int64_t stride2b, const int (&off)[LPW], int t, uint32_t to) {
+    const int n = t < nkt ? min(Sk - t * BN, BN) : 0;
+    const u32x4 rs = buffer_of(base + (n > 0 ? (int64_t)t * BN * stride2b : 0), n > 0 ? (n - 1) * (int)stride2b + D * 2 : 0);
+#pragma unroll
+    for (int u = 0; u < LPW; ++u) buffer_to_lds(rs, lds_at + to + (wave * LPW + u) * 1024, off[u], 0);
+  };
+  auto issue_k = [&](int t, int stage) { issue(Kb, ks2b, vk, t, stage * TILE); };
+  auto issue_v = [&](int t, int stage) { issue(Vb, vs2b, vv, t, (STAGES + stage) * TILE); };
+  issue_k(0, 0);
+  issue_k(1, 1);
+  issue_v(0, 0);
+
+  const float c = fabsf(g.scale_log2);
+  const uint32_t flip = g.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes to q's signs)
+  frag qf[DSUB];
+  {
+    const uint16_t* Q = (const uint16_t*)g.q + (blk.q_begin + tok) * g.qs[0] + qhead * g.qs[1];
+#pragma unroll
+    for (int dd = 0; dd < DSUB; ++dd) {
+      const int d = dd * 16 + half * 8;
+      u32x4 raw = {0u, 0u, 0u, 0u};
+      if (row < rows && d < D) raw = *(const u32x4*)(Q + d);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) raw[w] ^= flip;
+      qf[dd] = __builtin_bit_cast(frag, raw);
+    }
+  }
+  int k_rd[DSUB], v_rd[DBLK];
+#pragma unroll
+  for (int dd = 0; dd < DSUB; ++dd) k_rd[dd] = (lane & 31) * ROW + (((2 * dd + half) ^ k_swz(lane & 31)) * 16);
+  {
+    const int gq = lane >> 4, r = (lane & 15) >> 2, q = lane & 3;
+#pragma unroll
+    for (int i = 0; i < DBLK; ++i)
+      v_rd[i] = STAGES * TILE + (4 * (gq >> 1) + r) * ROW + ((i ^ v_swz(r)) * 64) + (16 * (gq & 1) + 4 * q) * 2;
+  }
+
+  floatx16 o_acc[DBLK], s[2];
+  frag pf[BN / 16];
+  float m = 0.f, l = 0.f;  // m: the first tile sets it to its max; l: of this lane's half of the keys
+#pragma unroll
+  for (int i = 0; i < DBLK; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o_acc[i][r] = 0.f;
+
+  auto scores = [&](int stage) {
+    const char* base = lds + stage * TILE;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+    for (int dd = 0; dd < DSUB; ++dd)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        s[kb] = mfma_traits<T>::mma(*(const frag*)(base + k_rd[dd] + kb * (32 * ROW)), qf[dd], s[kb]);
+  };
+  auto v_frag = [&](const char* base, int t, int i) {
+    typedef short v4i16 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4i16* lds_v4;
+    const char* p = base + v_rd[i] + t * (16 * ROW);
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)p));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(p + 8 * ROW)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  bool odd = false;  // a tile that this wave masks holds an infinite or NaN v
+  auto values = [&](int kt, int stage) {
+    const char* base = lds + stage * TILE;
+    if (g.causal && kt >= full_w) {
+      uint32_t most = 0;
+#pragma unroll 4
+      for (int i = 0; i < TILE / 1024; ++i) {
+        const u32x4 x = *(const u32x4*)(base + STAGES * TILE + i * 1024 + lane * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = max(most, max(x[w] & 0x7fffu, (x[w] >> 16) & 0x7fffu));
+      }
+      odd |= __builtin_amdgcn_ballot_w64(most >= inf_bits<T>) != 0;
+    }
+#pragma unroll
+    for (int t = 0; t < BN / 16; ++t)
+#pragma unroll
+      for (int i = 0; i < DBLK; ++i)
+        o_acc[i] = mfma_traits<T>::mma(__builtin_bit_cast(frag, v_frag(base, t, i)), pf[t], o_acc[i]);
+  };
+  auto weights = [&](int kt) {
+    if (kt >= full_w) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kt * BN + kb * 32 + acc_row(r, lane);
+          if (key >= Sk || key > last) s[kb][r] = -INFINITY;
+        }
+    }
+    float mx = max3(s[0][0], s[0][1], s[0][2]);
+#pragma unroll
+    for (int e = 3; e < 31; e += 2) mx = max3(mx, s[e >> 4][e & 15], s[(e + 1) >> 4][(e + 1) & 15]);
+    mx = max_halves(fmaxf(mx, s[1][15]));
+    const float over = __builtin_fmaf(mx, c, -m);
+    const bool grow = (kt == 0 && mx != -INFINITY) || over > RESCALE_LOG2;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float delta = grow ? over : 0.f, alpha = kt == 0 ? 1.f : __builtin_amdgcn_exp2f(-delta);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DBLK; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[i][r] *= alpha;
+      m += delta;
+    }
+#pragma unroll
+    for (int t = 0; t < BN / 16; ++t) {
+      u32x4 w;
+#pragma unroll
+      for (int sl = 0; sl < 4; ++sl) {
+        const int e = 8 * (t & 1) + 2 * sl;
+        w[sl] = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][e], c, -m)),
+                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][e + 1], c, -m)));
+        l = add2<T>(w[sl], l);
+      }
+      pf[t] = __builtin_bit_cast(frag, w);
+    }
+  };
+  // No access to LDS and no product moves over the end of a half.
+  auto end_half = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  const bool second = wave >= NW / 2;
+  wait_loads<0>();
+  end_half();
+  if (second) end_half();
+  for (int t = 0, at = 0; t <= nkt; ++t) {  // at: t % 3, the stage of tile t
+    const int next = at == 2 ? 0 : at + 1, before = at == 0 ? 2 : at - 1;
+    // (the stages filled now were read for the last time two halves ago)
+    if (second) {
+      issue_k(t + 2, before);
+      issue_v(t + 1, next);
+    }
+    __builtin_amdgcn_s_setprio(1);
+    if (t > 0 && t - 1 < nkt_w) values(t - 1, before);
+    if (t < nkt_w) scores(at);
+    __builtin_amdgcn_s_setprio(0);
+    if (second) wait_loads<2 * LPW>();
+    end_half();
+    if (t == nkt) break;
+    if (!second) {
+      issue_k(t + 2, before);
+      issue_v(t + 1, next);
+    }
+    if (t < nkt_w) weights(t);
+    if (!second) wait_loads<2 * LPW>();
+    end_half();
+    at = next;
+  }
+  if (!second) end_half();
+
+  uint16_t* O = (uint16_t*)g.o + (blk.q_begin + tok) * g.os[0] + qhead * g.os[1];
+  if (odd) {
+    const uint16_t* Q = (const uint16_t*)g.q + (blk.q_begin + tok) * g.qs[0] + qhead * g.qs[1];
+    prompt_rows_by_key<T, DM>(Q, Kb, Vb, O, ks2b, vs2b, min(Sk, nkt_w * BN), row < rows ? last : -1, row < rows, D,
+                              g.scale_log2);
+    return;
+  }
+  l += other_half(l);
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  if (row < rows) {
+#pragma unroll
+    for (int i = 0; i < DBLK; ++i)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int d = i * 32 + r4 * 8 + half * 4;
+        if (d < D)
+          *(u32x2*)(O + d) = u32x2{pack2<T>(o_acc[i][4 * r4] * inv, o_acc[i][4 * r4 + 1] * inv),
+                                   pack2<T>(o_acc[i][4 * r4 + 2] * inv, o_acc[i][4 * r4 + 3] * inv)};
+      }
+  }
+}
+
+// Any strides, element by element: keys and values through registers into two LDS stages of 64 keys,
+// waves 0-3 fetching K and 4-7 V, transposed in registers on the way.  (Here a tile that any row of the
+// workgroup masks gets its infinities and NaN taken out as it is stored.)
+template <typename T, int DM>
+__global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_elements_kernel(
     PromptArgs g) {
   using namespace pa;
   using G = Geo<DM>;
@@ -107,26 +495,17 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
 
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int64_t unit;
-  int head;
-  prompt_order(g, blockIdx.x, unit, head);
-  const int b = find_sequence(g.map, unit);
-  const int64_t q_begin = clamped_start(g.map, b);
-  const int Sq = (int)max((int64_t)0, clamped_start(g.map, b + 1) - q_begin);
-  const int64_t r0_64 = (unit - first_unit(g.map, b)) * BM;
-  const int64_t rows_64 = (int64_t)Sq * g.group;
-  if (r0_64 < 0 || r0_64 >= rows_64) return;
-  const int r0 = (int)r0_64, rows = (int)rows_64, D = g.dim;
-  auto k_clamp = [&](int64_t s) { return s < 0 ? 0 : s > g.k_tokens ? g.k_tokens : s; };
-  const int64_t k_begin = k_clamp(g.k_starts[b]);
-  const int Sk = (int)max((int64_t)0, k_clamp(g.k_starts[b + 1]) - k_begin);
+  const PromptBlock blk = prompt_block(g);
+  if (blk.rows == 0) return;
+  const int r0 = blk.r0, rows = blk.rows, Sq = blk.Sq, Sk = blk.Sk, head = blk.head, D = g.dim;
+  const int64_t q_begin = blk.q_begin, k_begin = blk.k_begin;
   const int offset = Sk - Sq;  // causal: token i sees keys up to i + offset
 
   const int rw = r0 + wave * 32;  // first row of this wave
   const int row = rw + (lane & 31);
   const int tok = row / g.group;
   const int qhead = head * g.group + (row - tok * g.group);
-  const int64_t es_q = VEC ? 1 : g.qs[2], es_k = VEC ? 1 : g.ks[2], es_v = VEC ? 1 : g.vs[2];
+  const int64_t es_q = g.qs[2], es_k = g.ks[2], es_v = g.vs[2];
   frag qf[G::DSUB];
   {
     const uint16_t* Q = (const uint16_t*)g.q + (q_begin + tok) * g.qs[0] + qhead * g.qs[1];
@@ -134,14 +513,10 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     for (int dd = 0; dd < G::DSUB; ++dd) {
       u32x4 raw = {0u, 0u, 0u, 0u};
       const int d = dd * 16 + half * 8;
-      if (VEC) {
-        if (row < rows && d < D) raw = *(const u32x4*)(Q + d);
-      } else {
-        uint16_t tmp[8];
+      uint16_t tmp[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) tmp[u] = row < rows && d + u < D ? Q[(d + u) * es_q] : (uint16_t)0;
-        raw = *(const u32x4*)tmp;
-      }
+      for (int u = 0; u < 8; ++u) tmp[u] = row < rows && d + u < D ? Q[(d + u) * es_q] : (uint16_t)0;
+      raw = *(const u32x4*)tmp;
       qf[dd] = __builtin_bit_cast(frag, raw);
     }
   }
@@ -163,15 +538,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   const bool k_role = wave < 4, v_role = wave >= 4 && (lt >> 4) < DM / 8;
   const uint16_t* Kb = (const uint16_t*)g.k + k_begin * g.ks[0] + head * g.ks[1];
   const uint16_t* Vb = (const uint16_t*)g.v + k_begin * g.vs[0] + head * g.vs[1];
-  const int ks2b = (int)g.ks[0] * 2, vs2b = (int)g.vs[0] * 2;
-  // A tile's rows as a buffer that ends with the sequence: keys past it read as zeros.
-  auto tile_rows = [&](const uint16_t* base, int64_t stride, int stride2b, int k0) {
-    const int n = min(Sk - k0, BN);
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (n > 0 ? k0 * stride : 0)), (short)0,
-                                             n > 0 ? (n - 1) * stride2b + D * 2 : 0, 0x00020000);
-  };
   const int kr = lt / G::CPR, kc = lt % G::CPR;
-  const int vK = kr * ks2b + kc * 16;
   int k_st[G::K_LOADS];
 #pragma unroll
   for (int i = 0; i < G::K_LOADS; ++i) {
@@ -179,7 +546,6 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     k_st[i] = ((kc >> 3) * BN * TILE_K + key * TILE_K + swz(key, kc & 7) * 8) * 2;
   }
   const int kq = lt & 15, db = lt >> 4;
-  const int vV = kq * 4 * vs2b + db * 16;
   const int v_st = (G::K_ELEMS + db * 8 * VT_STRIDE + vt_pos(kq)) * 2;
   u32x4 rl[4 > G::K_LOADS ? 4 : G::K_LOADS];
   auto element_row = [&](const uint16_t* base, int64_t stride, int64_t es, int key, int d) {
@@ -191,25 +557,13 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   auto load_tile = [&](int kt) {
     const int k0 = kt * BN;
     if (k_role) {
-      const __amdgpu_buffer_rsrc_t rsK = tile_rows(Kb, g.ks[0], ks2b, k0);
 #pragma unroll
-      for (int i = 0; i < G::K_LOADS; ++i) {
-        if (VEC)
-          rl[i] = kc * 8 < D ? __builtin_amdgcn_raw_buffer_load_b128(rsK, vK, i * G::KEYS_PER_LOAD * ks2b, 0)
-                             : u32x4{0u, 0u, 0u, 0u};
-        else
-          rl[i] = element_row(Kb, g.ks[0], es_k, k0 + i * G::KEYS_PER_LOAD + kr, kc * 8);
-      }
+      for (int i = 0; i < G::K_LOADS; ++i)
+        rl[i] = element_row(Kb, g.ks[0], es_k, k0 + i * G::KEYS_PER_LOAD + kr, kc * 8);
     }
     if (v_role) {
-      const __amdgpu_buffer_rsrc_t rsV = tile_rows(Vb, g.vs[0], vs2b, k0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (VEC)
-          rl[r] = __builtin_amdgcn_raw_buffer_load_b128(rsV, vV, r * vs2b, 0);
-        else
-          rl[r] = element_row(Vb, g.vs[0], es_v, k0 + kq * 4 + r, db * 8);
-      }
+      for (int r = 0; r < 4; ++r) rl[r] = element_row(Vb, g.vs[0], es_v, k0 + kq * 4 + r, db * 8);
     }
   };
   auto store_tile = [&](int kt) {
@@ -248,20 +602,16 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll 1
     for (int key = kt * BN; key < min(Sk, kt * BN + BN); ++key) {
       int64_t es = es_v;
-      if (!VEC) asm volatile("" : "+s"(es));  // (the addresses of a row are not kept over the loop)
+      asm volatile("" : "+s"(es));  // (the addresses of a row are not kept over the loop)
 #pragma unroll
       for (int i = 0; i < G::DBLK; ++i) {
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int d = i * 32 + r4 * 8 + half * 4;  // acc_row(4 r4, lane)
           uint16_t x[4] = {0, 0, 0, 0};
-          if (VEC) {
-            if (d < D) *(u32x2*)x = *(const u32x2*)(Vb + key * g.vs[0] + d);
-          } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (d + u < D) x[u] = Vb[key * g.vs[0] + (d + u) * es];
-          }
+          for (int u = 0; u < 4; ++u)
+            if (d + u < D) x[u] = Vb[key * g.vs[0] + (d + u) * es];
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             if ((x[u] & 0x7fffu) >= inf_bits<T> && key <= last) o_acc[i][4 * r4 + u] += elem<T>::to_float(x[u]);
@@ -399,13 +749,9 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
         const int ot = orow / g.group;
         const float* sp = stage + lr * ST + (e & 15) * 4;
         uint16_t* O = (uint16_t*)g.o + (q_begin + ot) * g.os[0] + (head * g.group + (orow - ot * g.group)) * g.os[1];
-        if (VEC) {
-          *(u32x2*)(O + d0) = u32x2{pack2<T>(sp[0], sp[1]), pack2<T>(sp[2], sp[3])};
-        } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (d0 + u < D) O[(d0 + u) * g.os[2]] = elem<T>::from_float(sp[u]);
-        }
+        for (int u = 0; u < 4; ++u)
+          if (d0 + u < D) O[(d0 + u) * g.os[2]] = elem<T>::from_float(sp[u]);
       }
     }
     wave_lds_order();
@@ -427,11 +773,11 @@ static int prompt_launch(PromptArgs g, hipStream_t stream) {
   g.units = unit_count(g.map);
   if (g.units * g.kv_heads > 0x7fffffffLL) return NT_ERR_INVALID;
   const dim3 grid((unsigned)(g.units * g.kv_heads)), block(pa::NW * 64);
-#define NT_PROMPT(DM)                                                                      \
-  if (vec)                                                                                 \
-    hipLaunchKernelGGL((prompt_attention_kernel<T, DM, true>), grid, block, 0, stream, g); \
-  else                                                                                     \
-    hipLaunchKernelGGL((prompt_attention_kernel<T, DM, false>), grid, block, 0, stream, g);
+#define NT_PROMPT(DM)                                                             \
+  if (vec)                                                                        \
+    hipLaunchKernelGGL((prompt_stream_kernel<T, DM>), grid, block, 0, stream, g); \
+  else                                                                            \
+    hipLaunchKernelGGL((prompt_elements_kernel<T, DM>), grid, block, 0, stream, g);
   if (g.dim <= 64) {
     NT_PROMPT(64)
   } else {
