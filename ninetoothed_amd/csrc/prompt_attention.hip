@@ -109,7 +109,7 @@ struct PromptBlock {
   int64_t q_begin, k_begin;
   int head, r0, rows, Sq, Sk;  // rows: of the sequence; 0: nothing to do
 };
-__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
+__device__ __forceinline__ PromptBlock find_block(const PromptArgs& g) {
   using namespace pa;
   PromptBlock p{};
   // Ids go to the 8 XCDs round-robin, each with its own L2: where the heads divide by 8, an XCD
@@ -180,6 +180,14 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
   p.r0 = __builtin_amdgcn_readfirstlane(__shfl(block, who, 64)) * BM;
   sequence(__builtin_amdgcn_readfirstlane(who));
   return p;
+}
+
+// The same, in scalar registers.
+__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
+  PromptBlock p = find_block(g);
+  auto one = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto two = [&](int64_t x) { return (int64_t)(uint32_t)one((int)x) | (int64_t)one((int)(x >> 32)) << 32; };
+  return {two(p.q_begin), two(p.k_begin), one(p.head), one(p.r0), one(p.rows), one(p.Sq), one(p.Sk)};
 }
 
 // Per row i of a sequence (a token and a head of its group) over the keys j it may see:
@@ -341,18 +349,6 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
     for (int r = 0; r < 16; ++r) o_acc[i][r] = 0.f;
 
-  auto scores = [&](int stage) {
-    const char* base = lds + stage * TILE;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
-#pragma unroll
-    for (int dd = 0; dd < DSUB; ++dd)
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        s[kb] = mfma_traits<T>::mma(*(const frag*)(base + k_rd[dd] + kb * (32 * ROW)), qf[dd], s[kb]);
-  };
   auto v_frag = [&](const char* base, int t, int i) {
     typedef short v4i16 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4i16* lds_v4;
@@ -362,32 +358,72 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
   bool odd = false;  // a tile that this wave masks holds an infinite or NaN v
-  auto values = [&](int kt, int stage) {
-    const char* base = lds + stage * TILE;
-    if (g.causal && kt >= full_w) {
-      uint32_t most = 0;
+  auto look_for_odd = [&](int stage) {
+    uint32_t most = 0;
 #pragma unroll 4
-      for (int i = 0; i < TILE / 1024; ++i) {
-        const u32x4 x = *(const u32x4*)(base + STAGES * TILE + i * 1024 + lane * 16);
+    for (int i = 0; i < TILE / 1024; ++i) {
+      const u32x4 x = *(const u32x4*)(lds + (STAGES + stage) * TILE + i * 1024 + lane * 16);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) most = max(most, max(x[w] & 0x7fffu, (x[w] >> 16) & 0x7fffu));
-      }
-      odd |= __builtin_amdgcn_ballot_w64(most >= inf_bits<T>) != 0;
+      for (int w = 0; w < 4; ++w) most = max(most, max(x[w] & 0x7fffu, (x[w] >> 16) & 0x7fffu));
     }
-#pragma unroll
-    for (int t = 0; t < BN / 16; ++t)
-#pragma unroll
-      for (int i = 0; i < DBLK; ++i)
-        o_acc[i] = mfma_traits<T>::mma(__builtin_bit_cast(frag, v_frag(base, t, i)), pf[t], o_acc[i]);
+    odd |= __builtin_amdgcn_ballot_w64(most >= inf_bits<T>) != 0;
   };
-  auto weights = [&](int kt) {
+  // O^T += V^T P^T of the tile in stage `vs` and S^T = K Q^T of that in stage `ks`: one line of
+  // products, each fragment read several products ahead of its own.
+  auto products = [&](auto with_v, auto with_k, int vs, int ks) {
+    constexpr bool WV = decltype(with_v)::value, WK = decltype(with_k)::value;
+    constexpr int NV = BN / 16 * DBLK, NK = 2 * DSUB;
+    const char *vbase = lds + vs * TILE, *kbase = lds + ks * TILE;
+    if constexpr (WV) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        o_acc[n % DBLK] = mfma_traits<T>::mma(__builtin_bit_cast(frag, v_frag(vbase, n / DBLK, n % DBLK)), pf[n / DBLK],
+                                              o_acc[n % DBLK]);
+    }
+    if constexpr (WK) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+        s[n & 1] = mfma_traits<T>::mma(*(const frag*)(kbase + k_rd[n >> 1] + (n & 1) * (32 * ROW)), qf[n >> 1], s[n & 1]);
+    }
+    constexpr int MFMA = 0x8, READ = 0x100, AHEAD_V = 6, AHEAD_K = 8;  // (a V fragment is two reads)
+    if constexpr (WV) {
+      __builtin_amdgcn_sched_group_barrier(READ, 2 * AHEAD_V, 0);
+      static_for<0, NV - AHEAD_V>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(READ, 2, 0);
+      });
+      if constexpr (WK) {
+        static_for<0, AHEAD_V>([](auto i) {
+          __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(READ, decltype(i)::value < 2 ? 2 : 1, 0);
+        });
+      } else {
+        __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD_V, 0);
+      }
+    } else {
+      __builtin_amdgcn_sched_group_barrier(READ, AHEAD_K, 0);
+    }
+    if constexpr (WK) {
+      static_for<0, NK - AHEAD_K>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(READ, 1, 0);
+      });
+      __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD_K, 0);
+    }
+  };
+  auto weights = [&](auto first, int kt) {
+    constexpr bool FIRST = decltype(first)::value;
     if (kt >= full_w) {
+      const int room = min(last, Sk - 1) - kt * BN - half * 4;  // (acc_row)
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = kt * BN + kb * 32 + acc_row(r, lane);
-          if (key >= Sk || key > last) s[kb][r] = -INFINITY;
+          if (kb * 32 + (r >> 2) * 8 + (r & 3) > room) s[kb][r] = -INFINITY;
         }
     }
     float mx = max3(s[0][0], s[0][1], s[0][2]);
@@ -395,9 +431,11 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     for (int e = 3; e < 31; e += 2) mx = max3(mx, s[e >> 4][e & 15], s[(e + 1) >> 4][(e + 1) & 15]);
     mx = max_halves(fmaxf(mx, s[1][15]));
     const float over = __builtin_fmaf(mx, c, -m);
-    const bool grow = (kt == 0 && mx != -INFINITY) || over > RESCALE_LOG2;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float delta = grow ? over : 0.f, alpha = kt == 0 ? 1.f : __builtin_amdgcn_exp2f(-delta);
+    const bool grow = over > RESCALE_LOG2;
+    if constexpr (FIRST) {
+      m = mx == -INFINITY ? 0.f : over;
+    } else if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float delta = grow ? over : 0.f, alpha = __builtin_amdgcn_exp2f(-delta);
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < DBLK; ++i)
@@ -428,31 +466,59 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   };
 
   const bool second = wave >= NW / 2;
-  wait_loads<0>();
-  end_half();
-  if (second) end_half();
-  for (int t = 0, at = 0; t <= nkt; ++t) {  // at: t % 3, the stage of tile t
-    const int next = at == 2 ? 0 : at + 1, before = at == 0 ? 2 : at - 1;
-    // (the stages filled now were read for the last time two halves ago)
-    if (second) {
-      issue_k(t + 2, before);
-      issue_v(t + 1, next);
-    }
+  // Step t: products of tile t's scores and tile t - 1's values in its first half, tile t's weights in
+  // the second.  The stages filled in it were read for the last time two halves before.
+  int stage = 0;  // t % 3
+  auto next = [&]() { return stage == 2 ? 0 : stage + 1; };
+  auto before = [&]() { return stage == 0 ? 2 : stage - 1; };
+  auto fill = [&](int t) {
+    issue_k(t + 2, before());
+    issue_v(t + 1, next());
+  };
+  auto begin = [&](int t) {
+    if (second) fill(t);
     __builtin_amdgcn_s_setprio(1);
-    if (t > 0 && t - 1 < nkt_w) values(t - 1, before);
-    if (t < nkt_w) scores(at);
+  };
+  auto middle = [&](int t) {
     __builtin_amdgcn_s_setprio(0);
     if (second) wait_loads<2 * LPW>();
     end_half();
-    if (t == nkt) break;
-    if (!second) {
-      issue_k(t + 2, before);
-      issue_v(t + 1, next);
-    }
-    if (t < nkt_w) weights(t);
+    if (!second && t < nkt) fill(t);
+  };
+  auto end = [&]() {
     if (!second) wait_loads<2 * LPW>();
     end_half();
-    at = next;
+    stage = next();
+  };
+  wait_loads<0>();
+  end_half();
+  if (second) end_half();
+  int t = 0;
+  if (nkt_w > 0) {
+    begin(0);
+    products(std::false_type{}, std::true_type{}, 0, 0);
+    middle(0);
+    weights(std::true_type{}, 0);
+    end();
+    for (t = 1; t < nkt_w; ++t) {
+      if (g.causal && t > full_w) look_for_odd(before());
+      begin(t);
+      products(std::true_type{}, std::true_type{}, before(), stage);
+      middle(t);
+      weights(std::false_type{}, t);
+      end();
+    }
+    if (g.causal && t > full_w) look_for_odd(before());
+    begin(t);
+    products(std::true_type{}, std::false_type{}, before(), 0);
+    middle(t);
+    if (t < nkt) end();
+    ++t;
+  }
+  for (; t <= nkt; ++t) {  // what the workgroup's other waves still need
+    begin(t);
+    middle(t);
+    if (t < nkt) end();
   }
   if (!second) end_half();
 
