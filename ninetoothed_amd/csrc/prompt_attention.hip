@@ -12,6 +12,7 @@ constexpr int NW = 8;              // waves per workgroup, two per SIMD
 constexpr int BM = NW * 32;        // query rows per workgroup
 constexpr int BN = 64;             // keys per tile
 constexpr float RESCALE_LOG2 = 8.0f;
+constexpr float MOST_SUM = 4096.0f;  // of a lane's 32 weights of a tile, each of which fp16 then holds
 // V^T rows: 64 keys + 8 pad.  Within each 16-key slice the keys lie in the order in which a
 // lane's P^T slots take them (0-3, 8-11 | 4-7, 12-15), so that a fragment is 16 contiguous bytes.
 constexpr int VT_STRIDE = BN + 8;
@@ -199,8 +200,9 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
 // one row, its max and sum take no LDS, and P^T goes from the score registers to the second product
 // as it is.
 //   - Scores stay unscaled in fp32 until exp2(s scale - m): q is not rounded a second time.
-//   - m is raised only where a tile's max passes it by 2^8 (o and l are rescaled then): p stays
-//     within 2^8 and keeps its relative precision; o / l is the same.
+//   - m is the max of a row's first tile, raised only where a later tile's weights grow past what
+//     MOST_SUM (or RESCALE_LOG2) allows (o and l are rescaled then): p keeps its relative precision, and
+//     o / l is the same.  Most tiles so take no max.
 //   - p is rounded to the operands' type for the product; its row sums are of the rounded p.
 //   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
 //     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: rows of a
@@ -303,18 +305,26 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     vk[u] = kc * 8 < D ? key * ks2b + kc * 16 : 0x7fffffff;  // (elements past D: past the buffer's end, zeros)
     vv[u] = vc * 8 < D ? key * vs2b + vc * 16 : 0x7fffffff;
   }
-  // A tile's rows as a buffer that ends with the sequence: keys past it read as zeros.
-  auto issue = [&](const char* base, int64_t stride2b, const int (&off)[LPW], int t, uint32_t to) {
-    const int n = t < nkt ? min(Sk - t * BN, BN) : 0;
-    const u32x4 rs = buffer_of(base + (n > 0 ? (int64_t)t * BN * stride2b : 0), n > 0 ? (n - 1) * (int)stride2b + D * 2 : 0);
+  // The next tile of K or V: its rows as a buffer that ends with the sequence, so that keys past it
+  // read as zeros.
+  struct Stream {
+    const char* at;
+    int left;  // keys from there on
+  };
+  Stream ks{Kb, nkt * BN < Sk ? nkt * BN : Sk}, vs{Vb, ks.left};
+  auto issue = [&](Stream& x, int stride2b, const int (&off)[LPW], uint32_t to) {
+    const int n = min(x.left, BN);
+    const u32x4 rs = buffer_of(x.at, n > 0 ? (n - 1) * stride2b + D * 2 : 0);
 #pragma unroll
     for (int u = 0; u < LPW; ++u) buffer_to_lds(rs, lds_at + to + (wave * LPW + u) * 1024, off[u], 0);
+    x.at += (int64_t)stride2b * BN;
+    x.left -= BN;
   };
-  auto issue_k = [&](int t, int stage) { issue(Kb, ks2b, vk, t, stage * TILE); };
-  auto issue_v = [&](int t, int stage) { issue(Vb, vs2b, vv, t, (STAGES + stage) * TILE); };
-  issue_k(0, 0);
-  issue_k(1, 1);
-  issue_v(0, 0);
+  auto issue_k = [&](int stage) { issue(ks, ks2b, vk, stage * TILE); };
+  auto issue_v = [&](int stage) { issue(vs, vs2b, vv, (STAGES + stage) * TILE); };
+  issue_k(0);
+  issue_k(1);
+  issue_v(0);
 
   const float c = fabsf(g.scale_log2);
   const uint32_t flip = g.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes to q's signs)
@@ -426,34 +436,46 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
           if (kb * 32 + (r >> 2) * 8 + (r & 3) > room) s[kb][r] = -INFINITY;
         }
     }
-    float mx = max3(s[0][0], s[0][1], s[0][2]);
+    // exp2(s c - m), rounded, and the row sum of this lane's half of the keys.
+    auto exponentials = [&]() {
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 3; e < 31; e += 2) mx = max3(mx, s[e >> 4][e & 15], s[(e + 1) >> 4][(e + 1) & 15]);
-    mx = max_halves(fmaxf(mx, s[1][15]));
-    const float over = __builtin_fmaf(mx, c, -m);
-    const bool grow = over > RESCALE_LOG2;
-    if constexpr (FIRST) {
-      m = mx == -INFINITY ? 0.f : over;
-    } else if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float delta = grow ? over : 0.f, alpha = __builtin_amdgcn_exp2f(-delta);
-      l *= alpha;
+      for (int t = 0; t < BN / 16; ++t) {
+        u32x4 w;
 #pragma unroll
-      for (int i = 0; i < DBLK; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o_acc[i][r] *= alpha;
-      m += delta;
-    }
-#pragma unroll
-    for (int t = 0; t < BN / 16; ++t) {
-      u32x4 w;
-#pragma unroll
-      for (int sl = 0; sl < 4; ++sl) {
-        const int e = 8 * (t & 1) + 2 * sl;
-        w[sl] = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][e], c, -m)),
-                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][e + 1], c, -m)));
-        l = add2<T>(w[sl], l);
+        for (int sl = 0; sl < 4; ++sl) {
+          const int e = 8 * (t & 1) + 2 * sl;
+          w[sl] = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][e], c, -m)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][e + 1], c, -m)));
+          sum[sl & 1] = add2<T>(w[sl], sum[sl & 1]);
+        }
+        pf[t] = __builtin_bit_cast(frag, w);
       }
-      pf[t] = __builtin_bit_cast(frag, w);
+      return sum[0] + sum[1];
+    };
+    auto largest = [&]() {
+      float mx = max3(s[0][0], s[0][1], s[0][2]);
+#pragma unroll
+      for (int e = 3; e < 31; e += 2) mx = max3(mx, s[e >> 4][e & 15], s[(e + 1) >> 4][(e + 1) & 15]);
+      return max_halves(fmaxf(mx, s[1][15]));
+    };
+    if constexpr (FIRST) {
+      const float mx = largest();
+      m = mx == -INFINITY ? 0.f : mx * c;
+      l = exponentials();
+    } else {
+      float sum = exponentials();
+      if (__builtin_amdgcn_ballot_w64(!(sum <= MOST_SUM))) {
+        const float over = fmaxf(__builtin_fmaf(largest(), c, -m), 0.f), alpha = __builtin_amdgcn_exp2f(-over);
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < DBLK; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o_acc[i][r] *= alpha;
+        m += over;
+        sum = exponentials();
+      }
+      l += sum;
     }
   };
   // No access to LDS and no product moves over the end of a half.
@@ -471,19 +493,19 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   int stage = 0;  // t % 3
   auto next = [&]() { return stage == 2 ? 0 : stage + 1; };
   auto before = [&]() { return stage == 0 ? 2 : stage - 1; };
-  auto fill = [&](int t) {
-    issue_k(t + 2, before());
-    issue_v(t + 1, next());
+  auto fill = [&]() {  // (tiles past the end read as zeros: every fill counts the same loads)
+    issue_k(before());
+    issue_v(next());
   };
-  auto begin = [&](int t) {
-    if (second) fill(t);
+  auto begin = [&]() {
+    if (second) fill();
     __builtin_amdgcn_s_setprio(1);
   };
   auto middle = [&](int t) {
     __builtin_amdgcn_s_setprio(0);
     if (second) wait_loads<2 * LPW>();
     end_half();
-    if (!second && t < nkt) fill(t);
+    if (!second && t < nkt) fill();
   };
   auto end = [&]() {
     if (!second) wait_loads<2 * LPW>();
@@ -495,28 +517,28 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   if (second) end_half();
   int t = 0;
   if (nkt_w > 0) {
-    begin(0);
+    begin();
     products(std::false_type{}, std::true_type{}, 0, 0);
     middle(0);
     weights(std::true_type{}, 0);
     end();
     for (t = 1; t < nkt_w; ++t) {
       if (g.causal && t > full_w) look_for_odd(before());
-      begin(t);
+      begin();
       products(std::true_type{}, std::true_type{}, before(), stage);
       middle(t);
       weights(std::false_type{}, t);
       end();
     }
     if (g.causal && t > full_w) look_for_odd(before());
-    begin(t);
+    begin();
     products(std::true_type{}, std::false_type{}, before(), 0);
     middle(t);
     if (t < nkt) end();
     ++t;
   }
   for (; t <= nkt; ++t) {  // what the workgroup's other waves still need
-    begin(t);
+    begin();
     middle(t);
     if (t < nkt) end();
   }
