@@ -255,10 +255,8 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
       *(u32x2*)(O + d0 + i) = u32x2{pa::pack2<T>(o[i] * inv, o[i + 1] * inv), pa::pack2<T>(o[i + 2] * inv, o[i + 3] * inv)};
 }
 
-// Unit element strides and 16-byte aligned rows.  K and V stream by direct loads into three LDS stages
-// of 64 keys each.  The two waves of a SIMD work half a tile apart, kept there by a barrier for each half:
-// while one has the matrix core (the products of a tile's scores and of the tile before with V), the
-// other turns its scores into weights.  A load is issued two halves before the barrier that ends it.
+// Unit element strides and 16-byte aligned rows.  K and V stream by direct loads into four LDS stages
+// of 64 keys each, two tiles under way while two are worked on.
 // LDS: K [key][DM] in 16-byte chunks XORed by key, so that the 16 keys of a fragment read fall on 16
 // distinct bank groups; V [key][DM] in 64-byte chunks XORed by key, for the 4 keys of a transposing read.
 template <typename T, int DM>
@@ -267,7 +265,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   using namespace pa;
   typedef typename mfma_traits<T>::frag frag;
   constexpr int DSUB = DM / 16, DBLK = DM / 32, ROW = DM * 2, CHUNKS = ROW / 16, TILE = BN * ROW;
-  constexpr int STAGES = 3, LPW = TILE / 1024 / NW, KEYS = 1024 / ROW;  // loads a wave and operand, keys of each
+  constexpr int STAGES = 4, LPW = TILE / 1024 / NW, KEYS = 1024 / ROW;  // loads a wave and operand, keys of each
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGES * TILE];  // K's stages, then V's
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -324,7 +322,9 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   auto issue_v = [&](int stage) { issue(vs, vs2b, vv, (STAGES + stage) * TILE); };
   issue_k(0);
   issue_k(1);
+  issue_k(2);
   issue_v(0);
+  issue_v(1);
 
   const float c = fabsf(g.scale_log2);
   const uint32_t flip = g.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes to q's signs)
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   };
   // O^T += V^T P^T of the tile in stage `vs` and S^T = K Q^T of that in stage `ks`: one line of
   // products, each fragment read several products ahead of its own.
-  auto products = [&](auto with_v, auto with_k, int vs, int ks) {
+  auto products = [&](auto with_v, auto with_k, int vs, int ks) __attribute__((always_inline)) {
     constexpr bool WV = decltype(with_v)::value, WK = decltype(with_k)::value;
     constexpr int NV = BN / 16 * DBLK, NK = 2 * DSUB;
     const char *vbase = lds + vs * TILE, *kbase = lds + ks * TILE;
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD_K, 0);
     }
   };
-  auto weights = [&](auto first, int kt) {
+  auto weights = [&](auto first, int kt) __attribute__((always_inline)) {
     constexpr bool FIRST = decltype(first)::value;
     if (kt >= full_w) {
       const int room = min(last, Sk - 1) - kt * BN - half * 4;  // (acc_row)
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
         }
     }
     // exp2(s c - m), rounded, and the row sum of this lane's half of the keys.
-    auto exponentials = [&]() {
+    auto exponentials = [&]() __attribute__((always_inline)) {
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < BN / 16; ++t) {
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       }
       return sum[0] + sum[1];
     };
-    auto largest = [&]() {
+    auto largest = [&]() __attribute__((always_inline)) {
       float mx = max3(s[0][0], s[0][1], s[0][2]);
 #pragma unroll
       for (int e = 3; e < 31; e += 2) mx = max3(mx, s[e >> 4][e & 15], s[(e + 1) >> 4][(e + 1) & 15]);
@@ -478,8 +478,8 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       l += sum;
     }
   };
-  // No access to LDS and no product moves over the end of a half.
-  auto end_half = [&]() {
+  // No access to LDS and no product moves over it.
+  auto end_steps = [&]() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -487,62 +487,60 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  const bool second = wave >= NW / 2;
-  // Step t: products of tile t's scores and tile t - 1's values in its first half, tile t's weights in
-  // the second.  The stages filled in it were read for the last time two halves before.
-  int stage = 0;  // t % 3
-  auto next = [&]() { return stage == 2 ? 0 : stage + 1; };
-  auto before = [&]() { return stage == 0 ? 2 : stage - 1; };
-  auto fill = [&]() {  // (tiles past the end read as zeros: every fill counts the same loads)
-    issue_k(before());
-    issue_v(next());
+  // Step t takes the products of tile t's scores and of tile t - 1's values, then tile t's weights.  A
+  // barrier ends every second step only, and products go before weights, so that the waves of a SIMD
+  // drift apart and one's products meet the other's weights.  In step t's middle the loads are issued of
+  // what step t + 2 needs, into stages that neither it nor the step after it reads.
+  auto fill = [&](int t) {
+    issue_k((t + 2) & 3);
+    issue_v((t + 1) & 3);
   };
-  auto begin = [&]() {
-    if (second) fill();
+  auto step = [&](int t) __attribute__((always_inline)) {
+    if (g.causal && t > full_w) look_for_odd((t - 1) & 3);
     __builtin_amdgcn_s_setprio(1);
-  };
-  auto middle = [&](int t) {
+    products(std::true_type{}, std::true_type{}, (t - 1) & 3, t & 3);
     __builtin_amdgcn_s_setprio(0);
-    if (second) wait_loads<2 * LPW>();
-    end_half();
-    if (!second && t < nkt) fill();
+    fill(t);
+    weights(std::false_type{}, t);
   };
-  auto end = [&]() {
-    if (!second) wait_loads<2 * LPW>();
-    end_half();
-    stage = next();
+  auto last_values = [&](int t) __attribute__((always_inline)) {
+    if (g.causal && t > full_w) look_for_odd((t - 1) & 3);
+    products(std::true_type{}, std::false_type{}, (t - 1) & 3, 0);
+    fill(t);
   };
-  wait_loads<0>();
-  end_half();
-  if (second) end_half();
-  int t = 0;
+  auto end_pair = [&]() {
+    wait_loads<0>();
+    end_steps();
+  };
+  wait_loads<4 * LPW>();  // K's first tile
+  end_steps();
   if (nkt_w > 0) {
-    begin();
     products(std::false_type{}, std::true_type{}, 0, 0);
-    middle(0);
     weights(std::true_type{}, 0);
-    end();
-    for (t = 1; t < nkt_w; ++t) {
-      if (g.causal && t > full_w) look_for_odd(before());
-      begin();
-      products(std::true_type{}, std::true_type{}, before(), stage);
-      middle(t);
-      weights(std::false_type{}, t);
-      end();
+  }
+  end_pair();
+  int t = 1;
+  for (; t + 1 < nkt_w; t += 2) {
+    step(t);
+    step(t + 1);
+    end_pair();
+  }
+  if (t <= nkt_w) {
+    if (t < nkt_w) {
+      step(t);
+      last_values(t + 1);
+    } else {
+      last_values(t);
+      fill(t + 1);
     }
-    if (g.causal && t > full_w) look_for_odd(before());
-    begin();
-    products(std::true_type{}, std::false_type{}, before(), 0);
-    middle(t);
-    if (t < nkt) end();
-    ++t;
+    end_pair();
+    t += 2;
   }
-  for (; t <= nkt; ++t) {  // what the workgroup's other waves still need
-    begin();
-    middle(t);
-    if (t < nkt) end();
+  for (; t <= nkt; t += 2) {  // what the workgroup's other waves still need
+    fill(t);
+    fill(t + 1);
+    end_pair();
   }
-  if (!second) end_half();
 
   uint16_t* O = (uint16_t*)g.o + (blk.q_begin + tok) * g.os[0] + qhead * g.os[1];
   if (odd) {
