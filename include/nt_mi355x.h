@@ -443,12 +443,16 @@ int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, cons
  * of i's sequence, with `causal` those with j <= i + (its keys - its queries).  Head h of q reads head
  * h / (heads / kv_heads) of k and v.  A query that sees no key gives zeros.  dtype F16 or BF16 (all
  * tensors), dim <= 128, any strides (unit element strides, strides of multiples of 8 and 16-byte
- * aligned tensors take vector loads). */
+ * aligned tensors take vector loads).  With few rows over many keys the keys are split over workgroups,
+ * whose states (fp32) pass through `workspace` (16-byte aligned, nt_prompt_attention_workspace_size
+ * bytes; 0: none wanted); with none or too little they are not split.  It holds nothing between calls. */
+int64_t nt_prompt_attention_workspace_size(int64_t q_tokens, int64_t k_tokens, int64_t sequences, int64_t heads,
+                                           int64_t kv_heads, int64_t dim);
 int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                         const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides, int dtype,
                         const int32_t* q_starts, const int32_t* k_starts, int64_t q_tokens, int64_t k_tokens,
                         int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, float scale, int causal,
-                        hipStream_t stream);
+                        hipStream_t stream, void* workspace, int64_t workspace_bytes);
 
 /* Attention of one query a sequence ([sequences, heads, dim]) over the first lengths[b] keys (at most
  * page_size * table_width) of its pages: as above, not causal, with the cache's layouts and types;

@@ -100,7 +100,8 @@ _SIGNATURES = {
     "nt_rotary": (_P, _I64P, _P, _I64P, _I, _P, _I64, _I, _P, _I64, _I64, _I64, _I64, _I, _I, _F, _P),
     "nt_cache_append": (_P, _I64P, _P, _I64P, _I, _P, _I64P, _P, _I64P, _I, _P, _P, _P, _I64, _P, _P, _P) + (_I64,) * 8
                        + (_I, _F, _P),
-    "nt_prompt_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P) + (_I64,) * 6 + (_F, _I, _P),
+    "nt_prompt_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P) + (_I64,) * 6 + (_F, _I, _P, _P, _I64),
+    "nt_prompt_attention_workspace_size": (_I64,) * 6,
     "nt_cache_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P, _P, _I64P, _I, _P, _I64, _P) + (_I64,) * 7
                           + (_F, _P, _P, _I64),
     "nt_cache_attention_workspace_size": (_I64,) * 6 + (_I,),
@@ -112,6 +113,7 @@ _SIGNATURES = {
 }
 _RESTYPES = {"nt_conv2d_workspace_size": ctypes.c_int64, "nt_attention_workspace_size": ctypes.c_int64,
              "nt_gemm_workspace_size": ctypes.c_int64, "nt_cache_attention_workspace_size": ctypes.c_int64,
+             "nt_prompt_attention_workspace_size": ctypes.c_int64,
              "nt_rtc_free": None}
 
 _lock = threading.Lock()

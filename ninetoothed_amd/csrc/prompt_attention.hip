@@ -9,8 +9,9 @@ namespace nt {
 namespace pa {
 
 constexpr int NW = 8;              // waves per workgroup, two per SIMD
-constexpr int BM = NW * 32;        // query rows per workgroup
+constexpr int BM = NW * 32;        // query rows per workgroup (the kernel for few rows: half of both)
 constexpr int BN = 64;             // keys per tile
+constexpr int FEW_BLOCKS = 512;   // of 256 rows: below that many the kernel of 128 rows runs
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr float MOST_SUM = 4096.0f;  // of a lane's 32 weights of a tile, each of which fp16 then holds
 // V^T rows: 64 keys + 8 pad.  Within each 16-key slice the keys lie in the order in which a
@@ -100,6 +101,11 @@ struct PromptArgs {
   int64_t k_tokens, units;
   int kv_heads, group, dim, causal;
   float scale_log2;  // softmax scale * log2(e)
+  // Keys of a block of rows over several workgroups: their partial states in the workspace, for each
+  // split and row (token, head of q): O [dim] and (max, sum).
+  int splits;
+  int64_t rows;  // of q, all tokens and heads
+  float *part_o, *part_ml;
 };
 
 // The block of rows a workgroup takes: longest first.  Up to 64 sequences: a lane for each, which
@@ -109,14 +115,17 @@ struct PromptArgs {
 struct PromptBlock {
   int64_t q_begin, k_begin;
   int head, r0, rows, Sq, Sk;  // rows: of the sequence; 0: nothing to do
+  int split;
 };
 __device__ __forceinline__ PromptBlock find_block(const PromptArgs& g) {
   using namespace pa;
   PromptBlock p{};
   // Ids go to the 8 XCDs round-robin, each with its own L2: where the heads divide by 8, an XCD
   // keeps to the K and V of heads of its own.
+  const int BM = g.map.per;
   p.head = (int)(blockIdx.x % g.kv_heads);
-  const int64_t id = blockIdx.x / g.kv_heads;
+  const int64_t nth = blockIdx.x / g.kv_heads, id = g.splits == 1 ? nth : nth / g.splits;
+  p.split = g.splits == 1 ? 0 : (int)(nth - id * g.splits);
   auto k_clamp = [&](int64_t s) { return s < 0 ? 0 : s > g.k_tokens ? g.k_tokens : s; };
   auto sequence = [&](int b) {
     p.q_begin = clamped_start(g.map, b);
@@ -188,7 +197,7 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
   PromptBlock p = find_block(g);
   auto one = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   auto two = [&](int64_t x) { return (int64_t)(uint32_t)one((int)x) | (int64_t)one((int)(x >> 32)) << 32; };
-  return {two(p.q_begin), two(p.k_begin), one(p.head), one(p.r0), one(p.rows), one(p.Sq), one(p.Sk)};
+  return {two(p.q_begin), two(p.k_begin), one(p.head), one(p.r0), one(p.rows), one(p.Sq), one(p.Sk), one(p.split)};
 }
 
 // Per row i of a sequence (a token and a head of its group) over the keys j it may see:
@@ -207,13 +216,33 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
 //   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
 //     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: rows of a
 //     tile that is masked and holds one are taken key by key, each over the keys that it sees.
+// What a row's state ends as: the output, or a split's partial state.
+template <typename T>
+struct PromptRow {
+  uint16_t* o;      // the output's row, or
+  float *part, *ml;  // the partial state's
+  __device__ __forceinline__ PromptRow(const PromptArgs& g, const PromptBlock& blk, int tok, int qhead) {
+    o = (uint16_t*)g.o + (blk.q_begin + tok) * g.os[0] + qhead * g.os[1];
+    const int64_t row = blk.split * g.rows + (blk.q_begin + tok) * (int64_t)(g.kv_heads * g.group) + qhead;
+    part = g.part_o + row * g.dim;
+    ml = g.part_ml + row * 2;
+  }
+  // Four neighbouring elements from d on: x times f (1 / sum, or 1).
+  __device__ __forceinline__ void store(bool whole, int d, float f, float x0, float x1, float x2, float x3) const {
+    if (whole)
+      *(u32x2*)(o + d) = u32x2{pa::pack2<T>(x0 * f, x1 * f), pa::pack2<T>(x2 * f, x3 * f)};
+    else
+      *(floatx4*)(part + d) = floatx4{x0, x1, x2, x3};
+  }
+};
+
 // A wave's 32 rows, one to a lane and its other half, which share its elements: the same sums key by key
-// over the `keys` first keys, those up to each row's `last`.  For rows whose masked keys hold
+// over the keys [from, to), those up to each row's `last`.  For rows whose masked keys hold
 // infinities or NaN; slow.
 template <typename T, int DM>
-__device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char* K, const char* V, uint16_t* O,
-                                                   int64_t ks2b, int64_t vs2b, int keys, int last, bool valid, int D,
-                                                   float scale_log2) {
+__device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char* K, const char* V, PromptRow<T> out,
+                                                   int64_t ks2b, int64_t vs2b, int from, int to, int last, bool valid,
+                                                   int D, float scale_log2, bool whole) {
   constexpr int N = DM / 2;  // elements of a lane
   const int d0 = ((threadIdx.x >> 5) & 1) * N;
   float o[N], m = -INFINITY, l = 0.f;
@@ -225,7 +254,7 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
     q[i] = valid && d0 + i * 8 < D ? *(const u32x4*)(Q + d0 + i * 8) : u32x4{0u, 0u, 0u, 0u};
   auto value = [](const u32x4& x, int e) { return elem<T>::to_float((uint16_t)(x[e >> 1] >> ((e & 1) * 16))); };
 #pragma unroll 1
-  for (int key = 0; key < keys; ++key) {
+  for (int key = from; key < to; ++key) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < N / 8; ++i) {
@@ -248,24 +277,28 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
         if (seen) o[i * 8 + e] = __builtin_fmaf(p, value(v, e), o[i * 8 + e] * alpha);
     }
   }
+  if (!valid) return;
   const float inv = l != 0.f ? 1.0f / l : 0.f;
 #pragma unroll
   for (int i = 0; i < N; i += 4)
-    if (valid && d0 + i < D)
-      *(u32x2*)(O + d0 + i) = u32x2{pa::pack2<T>(o[i] * inv, o[i + 1] * inv), pa::pack2<T>(o[i + 2] * inv, o[i + 3] * inv)};
+    if (d0 + i < D) out.store(whole, d0 + i, inv, o[i], o[i + 1], o[i + 2], o[i + 3]);
+  if (!whole && d0 == 0) *(float2*)out.ml = float2{m, l};
 }
 
-// Unit element strides and 16-byte aligned rows.  K and V stream by direct loads into four LDS stages
-// of 64 keys each, two tiles under way while two are worked on.
+// Unit element strides and 16-byte aligned rows.  K and V stream by direct loads into LDS stages of 64
+// keys each: four of them, two tiles under way while two are worked on, or with NW = 4 (for few rows) two,
+// one under way beside one, so that two workgroups share a CU.
 // LDS: K [key][DM] in 16-byte chunks XORed by key, so that the 16 keys of a fragment read fall on 16
 // distinct bank groups; V [key][DM] in 64-byte chunks XORed by key, for the 4 keys of a transposing read.
-template <typename T, int DM>
-__global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_stream_kernel(
-    PromptArgs g) {
+template <typename T, int DM, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DM == 64 ? 4 : 2, DM == 64 ? 4 : 2))) void
+prompt_stream_kernel(PromptArgs g) {
   using namespace pa;
+  constexpr int BM = NW * 32;
   typedef typename mfma_traits<T>::frag frag;
   constexpr int DSUB = DM / 16, DBLK = DM / 32, ROW = DM * 2, CHUNKS = ROW / 16, TILE = BN * ROW;
-  constexpr int STAGES = 4, LPW = TILE / 1024 / NW, KEYS = 1024 / ROW;  // loads a wave and operand, keys of each
+  constexpr int STAGES = NW == 8 ? 4 : 2, STEPS = STAGES / 2;  // STEPS: from barrier to barrier
+  constexpr int LPW = TILE / 1024 / NW, KEYS = 1024 / ROW;     // loads a wave and operand, keys of each
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGES * TILE];  // K's stages, then V's
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -288,6 +321,13 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     full_w = begin_w < 0 ? 0 : min(full_w, (begin_w + 1) / BN);
   }
   if (rw >= rows) nkt_w = 0;
+  // This split's tiles: t0 to nkt, for this wave to nkt_w.  (Below, tiles count from t0 on.)
+  const int t0 = g.splits == 1 ? 0 : (int)((int64_t)nkt * blk.split / g.splits);
+  if (g.splits > 1) nkt = (int)((int64_t)nkt * (blk.split + 1) / g.splits);
+  const int key0 = t0 * BN;
+  nkt -= t0;
+  nkt_w = max(0, min(nkt_w - t0, nkt));
+  full_w -= t0;
 
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const char* Kb = (const char*)((const uint16_t*)g.k + blk.k_begin * g.ks[0] + head * g.ks[1]);
@@ -309,7 +349,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     const char* at;
     int left;  // keys from there on
   };
-  Stream ks{Kb, nkt * BN < Sk ? nkt * BN : Sk}, vs{Vb, ks.left};
+  Stream ks{Kb + (int64_t)key0 * ks2b, min(Sk - key0, nkt * BN)}, vs{Vb + (int64_t)key0 * vs2b, ks.left};
   auto issue = [&](Stream& x, int stride2b, const int (&off)[LPW], uint32_t to) {
     const int n = min(x.left, BN);
     const u32x4 rs = buffer_of(x.at, n > 0 ? (n - 1) * stride2b + D * 2 : 0);
@@ -322,9 +362,9 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   auto issue_v = [&](int stage) { issue(vs, vs2b, vv, (STAGES + stage) * TILE); };
   issue_k(0);
   issue_k(1);
-  issue_k(2);
+  if (STEPS == 2) issue_k(2 % STAGES);
   issue_v(0);
-  issue_v(1);
+  if (STEPS == 2) issue_v(1);
 
   const float c = fabsf(g.scale_log2);
   const uint32_t flip = g.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes to q's signs)
@@ -428,7 +468,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   auto weights = [&](auto first, int kt) __attribute__((always_inline)) {
     constexpr bool FIRST = decltype(first)::value;
     if (kt >= full_w) {
-      const int room = min(last, Sk - 1) - kt * BN - half * 4;  // (acc_row)
+      const int room = min(last, Sk - 1) - key0 - kt * BN - half * 4;  // (acc_row)
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -488,65 +528,67 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   };
 
   // Step t takes the products of tile t's scores and of tile t - 1's values, then tile t's weights.  A
-  // barrier ends every second step only, and products go before weights, so that the waves of a SIMD
+  // barrier ends every STEPS of them, and products go before weights, so that the waves of a SIMD
   // drift apart and one's products meet the other's weights.  In step t's middle the loads are issued of
-  // what step t + 2 needs, into stages that neither it nor the step after it reads.
+  // what step t + STEPS needs, into stages that no step before the barrier reads.
+  constexpr int MASK = STAGES - 1;
   auto fill = [&](int t) {
-    issue_k((t + 2) & 3);
-    issue_v((t + 1) & 3);
+    issue_k((t + STEPS) & MASK);
+    issue_v((t + STEPS - 1) & MASK);
   };
   auto step = [&](int t) __attribute__((always_inline)) {
-    if (g.causal && t > full_w) look_for_odd((t - 1) & 3);
+    if (g.causal && t > full_w) look_for_odd((t - 1) & MASK);
     __builtin_amdgcn_s_setprio(1);
-    products(std::true_type{}, std::true_type{}, (t - 1) & 3, t & 3);
+    products(std::true_type{}, std::true_type{}, (t - 1) & MASK, t & MASK);
     __builtin_amdgcn_s_setprio(0);
     fill(t);
     weights(std::false_type{}, t);
   };
   auto last_values = [&](int t) __attribute__((always_inline)) {
-    if (g.causal && t > full_w) look_for_odd((t - 1) & 3);
-    products(std::true_type{}, std::false_type{}, (t - 1) & 3, 0);
+    if (g.causal && t > full_w) look_for_odd((t - 1) & MASK);
+    products(std::true_type{}, std::false_type{}, (t - 1) & MASK, 0);
     fill(t);
   };
-  auto end_pair = [&]() {
+  auto end = [&]() {
     wait_loads<0>();
     end_steps();
   };
-  wait_loads<4 * LPW>();  // K's first tile
+  wait_loads<(STAGES - 1) * LPW>();  // K's first tile
   end_steps();
   if (nkt_w > 0) {
     products(std::false_type{}, std::true_type{}, 0, 0);
     weights(std::true_type{}, 0);
   }
-  end_pair();
+  end();
   int t = 1;
-  for (; t + 1 < nkt_w; t += 2) {
+  for (; t + STEPS - 1 < nkt_w; t += STEPS) {
     step(t);
-    step(t + 1);
-    end_pair();
+    if (STEPS == 2) step(t + 1);
+    end();
   }
   if (t <= nkt_w) {
-    if (t < nkt_w) {
+    if (STEPS == 2 && t < nkt_w) {
       step(t);
       last_values(t + 1);
     } else {
       last_values(t);
-      fill(t + 1);
+      if (STEPS == 2) fill(t + 1);
     }
-    end_pair();
-    t += 2;
+    end();
+    t += STEPS;
   }
-  for (; t <= nkt; t += 2) {  // what the workgroup's other waves still need
+  for (; t <= nkt; t += STEPS) {  // what the workgroup's other waves still need
     fill(t);
-    fill(t + 1);
-    end_pair();
+    if (STEPS == 2) fill(t + 1);
+    end();
   }
 
-  uint16_t* O = (uint16_t*)g.o + (blk.q_begin + tok) * g.os[0] + qhead * g.os[1];
+  const PromptRow<T> out(g, blk, tok, qhead);
+  const bool whole = g.splits == 1;
   if (odd) {
     const uint16_t* Q = (const uint16_t*)g.q + (blk.q_begin + tok) * g.qs[0] + qhead * g.qs[1];
-    prompt_rows_by_key<T, DM>(Q, Kb, Vb, O, ks2b, vs2b, min(Sk, nkt_w * BN), row < rows ? last : -1, row < rows, D,
-                              g.scale_log2);
+    prompt_rows_by_key<T, DM>(Q, Kb, Vb, out, ks2b, vs2b, key0, min(Sk, key0 + nkt_w * BN), row < rows ? last : -1,
+                              row < rows, D, g.scale_log2, whole);
     return;
   }
   l += other_half(l);
@@ -558,10 +600,34 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       for (int r4 = 0; r4 < 4; ++r4) {
         const int d = i * 32 + r4 * 8 + half * 4;
         if (d < D)
-          *(u32x2*)(O + d) = u32x2{pack2<T>(o_acc[i][4 * r4] * inv, o_acc[i][4 * r4 + 1] * inv),
-                                   pack2<T>(o_acc[i][4 * r4 + 2] * inv, o_acc[i][4 * r4 + 3] * inv)};
+          out.store(whole, d, inv, o_acc[i][4 * r4], o_acc[i][4 * r4 + 1], o_acc[i][4 * r4 + 2], o_acc[i][4 * r4 + 3]);
       }
+    if (!whole && half == 0) *(float2*)out.ml = float2{l != 0.f ? m : -INFINITY, l};
   }
+}
+
+// Joins the splits of a row: a wave for each, a lane for every 64th element.
+template <typename T>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs g) {
+  const int lane = threadIdx.x & 63, heads = g.kv_heads * g.group;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), token = row / heads;
+  // (rows before the first sequence or behind the last have no states)
+  if (row >= g.rows || token < clamped_start(g.map, 0) || token >= clamped_start(g.map, g.map.sequences)) return;
+  float mm = -INFINITY;
+  for (int s = 0; s < g.splits; ++s) mm = fmaxf(mm, g.part_ml[(s * g.rows + row) * 2]);
+  float sum = 0.f, o[2] = {0.f, 0.f};
+  for (int s = 0; s < g.splits; ++s) {
+    const float2 ml = *(const float2*)(g.part_ml + (s * g.rows + row) * 2);
+    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
+    sum += ml.y * f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (u * 64 + lane < g.dim) o[u] += g.part_o[(s * g.rows + row) * g.dim + u * 64 + lane] * f;
+  }
+  uint16_t* O = (uint16_t*)g.o + token * g.os[0] + (row - token * heads) * g.os[1];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (u * 64 + lane < g.dim) O[u * 64 + lane] = elem<T>::from_float(sum != 0.f ? o[u] / sum : 0.f);
 }
 
 // Any strides, element by element: keys and values through registers into two LDS stages of 64 keys,
@@ -844,32 +910,62 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   }
 }
 
-template <typename T>
-static int prompt_launch(PromptArgs g, hipStream_t stream) {
+static bool prompt_vectors(const PromptArgs& g) {
   auto rows_ok = [&](const void* p, const int64_t* s) {
     return s[2] == 1 && s[0] >= 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && (uintptr_t)p % 16 == 0;
   };
   // A tile's keys are addressed with 32-bit buffer offsets.
   auto span_ok = [&](const int64_t* s) { return 2 * pa::BN * s[0] * 2 < 0x7fffffffLL; };
-  const bool vec = g.dim % 8 == 0 && rows_ok(g.q, g.qs) && rows_ok(g.k, g.ks) && rows_ok(g.v, g.vs) &&
-                   rows_ok(g.o, g.os) && span_ok(g.ks) && span_ok(g.vs);
+  return g.dim % 8 == 0 && rows_ok(g.q, g.qs) && rows_ok(g.k, g.ks) && rows_ok(g.v, g.vs) && rows_ok(g.o, g.os) &&
+         span_ok(g.ks) && span_ok(g.vs);
+}
+
+// The rows of a workgroup, and over how many its keys are split.
+struct PromptPlan {
+  int per, splits;
+};
+static PromptPlan prompt_plan(int64_t q_tokens, int64_t k_tokens, int64_t sequences, int64_t kv_heads, int64_t group) {
+  UnitMap map{nullptr, q_tokens, (int)sequences, (int)group, pa::BM, 1};
+  PromptPlan p{pa::BM, 1};
+  if (unit_count(map) * kv_heads < pa::FEW_BLOCKS) p.per = map.per = pa::BM / 2;
+  const int64_t blocks = unit_count(map) * kv_heads, tiles = k_tokens / std::max<int64_t>(1, sequences) / pa::BN;
+  if (p.per < pa::BM) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, tiles / 4, 16}));
+  return p;
+}
+
+template <typename T>
+static int prompt_launch(PromptArgs g, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  const bool vec = prompt_vectors(g);
+  PromptPlan plan{pa::BM, 1};
+  if (vec) plan = prompt_plan(g.map.tokens, g.k_tokens, g.map.sequences, g.kv_heads, g.group);
+  g.rows = g.map.tokens * g.kv_heads * g.group;
+  if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < g.rows * plan.splits * (g.dim + 2) * 4))
+    plan.splits = 1;
+  g.splits = plan.splits;
+  g.part_o = (float*)workspace;
+  g.part_ml = plan.splits > 1 ? g.part_o + g.rows * plan.splits * g.dim : nullptr;
   g.map.rows = g.group;
-  g.map.per = pa::BM;
+  g.map.per = plan.per;
   g.map.extra = 1;
   g.units = unit_count(g.map);
-  if (g.units * g.kv_heads > 0x7fffffffLL) return NT_ERR_INVALID;
-  const dim3 grid((unsigned)(g.units * g.kv_heads)), block(pa::NW * 64);
-#define NT_PROMPT(DM)                                                             \
-  if (vec)                                                                        \
-    hipLaunchKernelGGL((prompt_stream_kernel<T, DM>), grid, block, 0, stream, g); \
-  else                                                                            \
-    hipLaunchKernelGGL((prompt_elements_kernel<T, DM>), grid, block, 0, stream, g);
+  const int64_t blocks = g.units * g.kv_heads * plan.splits;
+  if (blocks > 0x7fffffffLL) return NT_ERR_INVALID;
+  const dim3 grid((unsigned)blocks), block(plan.per * 2);
+#define NT_PROMPT(DM)                                                                \
+  if (!vec)                                                                          \
+    hipLaunchKernelGGL((prompt_elements_kernel<T, DM>), grid, block, 0, stream, g);  \
+  else if (plan.per == pa::BM)                                                       \
+    hipLaunchKernelGGL((prompt_stream_kernel<T, DM, 8>), grid, block, 0, stream, g); \
+  else                                                                               \
+    hipLaunchKernelGGL((prompt_stream_kernel<T, DM, 4>), grid, block, 0, stream, g);
   if (g.dim <= 64) {
     NT_PROMPT(64)
   } else {
     NT_PROMPT(128)
   }
 #undef NT_PROMPT
+  if (plan.splits > 1)
+    hipLaunchKernelGGL((prompt_join_kernel<T>), dim3((unsigned)cdiv(g.rows, 4)), dim3(256), 0, stream, g);
   return launch_status();
 }
 
@@ -879,7 +975,8 @@ extern "C" int nt_prompt_attention(const void* q, const int64_t* q_strides, cons
                                    const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
                                    int dtype, const int32_t* q_starts, const int32_t* k_starts, int64_t q_tokens,
                                    int64_t k_tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
-                                   float scale, int causal, hipStream_t stream) {
+                                   float scale, int causal, hipStream_t stream, void* workspace,
+                                   int64_t workspace_bytes) {
   if (q_tokens < 0 || k_tokens < 0 || sequences < 0 || heads < 0 || kv_heads < 0 || dim < 0 || dim > 128 ||
       (dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || k_tokens > 0x7fffff00LL || sequences > (1 << 30))
     return NT_ERR_INVALID;
@@ -908,7 +1005,17 @@ extern "C" int nt_prompt_attention(const void* q, const int64_t* q_strides, cons
   g.dim = (int)dim;
   g.causal = causal != 0;
   g.scale_log2 = scale * 1.44269504088896340736f;
-  return dtype == NT_DTYPE_F16 ? nt::prompt_launch<nt::f16_t>(g, stream) : nt::prompt_launch<nt::bf16_t>(g, stream);
+  return dtype == NT_DTYPE_F16 ? nt::prompt_launch<nt::f16_t>(g, workspace, workspace_bytes, stream)
+                               : nt::prompt_launch<nt::bf16_t>(g, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t nt_prompt_attention_workspace_size(int64_t q_tokens, int64_t k_tokens, int64_t sequences,
+                                                      int64_t heads, int64_t kv_heads, int64_t dim) {
+  if (q_tokens <= 0 || k_tokens < 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 ||
+      dim > 128)
+    return 0;
+  const int splits = nt::prompt_plan(q_tokens, k_tokens, sequences, kv_heads, heads / kv_heads).splits;
+  return splits > 1 ? q_tokens * heads * splits * (dim + 2) * 4 : 0;
 }
 
 extern "C" int nt_prompt_attention_packed(const int64_t* packed) {
@@ -934,6 +1041,8 @@ extern "C" int nt_prompt_attention_packed(const int64_t* packed) {
   float scale = p.f();
   int causal = p.i();
   hipStream_t stream = (hipStream_t)p.ptr<void>();
+  void* workspace = p.ptr<void>();
+  int64_t workspace_bytes = p.i64();
   return nt_prompt_attention(q, qs, k, ks, v, vs, o, os, dtype, q_starts, k_starts, q_tokens, k_tokens, sequences,
-                             heads, kv_heads, dim, scale, causal, stream);
+                             heads, kv_heads, dim, scale, causal, stream, workspace, workspace_bytes);
 }

@@ -882,17 +882,19 @@ def bind_prompt_attention(q, k, v, out, q_starts, k_starts, causal=True, scale=N
     (one tensor may serve as both where they agree).  ``causal``: query i sees the keys up to
     i + (keys - queries), so that the last query sees them all.  ``scale`` defaults to
     dim ** -0.5.  Scores, softmax and sums are in fp32, the weights rounded to the inputs' type for the
-    product with v.  A query without keys gives zeros; rows behind the last sequence are left alone."""
+    product with v.  A query without keys gives zeros; rows behind the last sequence are left alone.
+    A call of few rows over many keys takes a workspace from torch's allocator, and goes without where
+    that has none."""
     code = check_prompt_attention(q, k, v, out, q_starts, k_starts, causal, scale)
     device = _check_device(q, k, v, out, q_starts, k_starts)
-    dim = q.shape[2]
+    sizes = (q.shape[0], k.shape[0], q_starts.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2])
+    nbytes = int(_lib.load().nt_prompt_attention_workspace_size(*sizes))
     launch = _bind_packed("nt_prompt_attention_packed", device, (
         _POINTER, q.stride(), _POINTER, k.stride(), _POINTER, v.stride(), _POINTER, out.stride(), code, _POINTER,
-        _POINTER, q.shape[0], k.shape[0], q_starts.shape[0] - 1, q.shape[1], k.shape[1], dim,
-        float(dim ** -0.5 if scale is None else scale), bool(causal), _STREAM))
+        _POINTER, *sizes, float(q.shape[2] ** -0.5 if scale is None else scale), bool(causal), _STREAM, _POINTER, nbytes))
 
     def call(q, k, v, out, q_starts, k_starts):
-        launch((q, k, v, out, q_starts, k_starts))
+        launch((q, k, v, out, q_starts, k_starts, _workspace(nbytes, device) if nbytes else None))
 
     return call
 

@@ -163,7 +163,8 @@ def _append(lib, dtype=1, cache=1, k=P, scale=P, tokens=4, seqs=2, heads=2, dim=
 
 
 def _prompt(lib, dtype=1, q=P, tokens=4, keys=4, seqs=2, heads=2, kv=2, dim=64):
-    return lib.nt_prompt_attention(q, S3, P, S3, P, S3, P, S3, dtype, P, P, tokens, keys, seqs, heads, kv, dim, 1.0, 1, None)
+    return lib.nt_prompt_attention(q, S3, P, S3, P, S3, P, S3, dtype, P, P, tokens, keys, seqs, heads, kv, dim, 1.0, 1, None,
+                                   None, 0)
 
 
 def _step(lib, dtype=1, cache=1, q=P, scale=P, seqs=2, heads=2, kv=2, dim=64, pages=5, page=16, width=2, ws=None, nbytes=0,
@@ -196,6 +197,10 @@ def test_entry_points_reject_before_they_launch():
 
 
 def test_workspace_size():
+    size = _lib.load().nt_prompt_attention_workspace_size
+    assert size(100000, 100000, 4, 32, 8, 128) == 0  # rows enough for every workgroup
+    assert size(0, 100, 1, 8, 8, 64) == 0 and size(10, 100, 1, 8, 3, 64) == 0
+    assert size(100, 50000, 1, 8, 8, 64) > 0
     size = _lib.load().nt_cache_attention_workspace_size
     for cache in (_lib.DTYPE_F16, _lib.DTYPE_E4M3):
         assert size(4, 8, 8, 128, 16, 8, cache) == 0  # at most one block of keys a sequence
