@@ -107,12 +107,7 @@ __device__ __forceinline__ int line_blocks(int keys) { return max(1, (keys + ca:
 // not in use before the last barrier.
 __device__ __forceinline__ void line_scan(int n, int* sums, int& before, int& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int upto = n;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int other = __shfl_up(upto, off, 64);
-    if (lane >= off) upto += other;
-  }
+  const int upto = wave_scan(n);
   if (lane == 63) sums[wave] = upto;
   __syncthreads();
   before = upto - n;

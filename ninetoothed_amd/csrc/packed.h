@@ -49,6 +49,19 @@ __device__ __forceinline__ int find_sequence(const UnitMap& u, int64_t id) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// The sum of x over a wave's lanes up to each, and over all of them.  Row shifts and broadcasts take
+// a few cycles each where a shuffle passes through LDS.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15, into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31, into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
 // cos and sin of position * frequency, times `magnitude`.  The angle is reduced to a part of a
 // turn in 64 bits (a position of a million times a frequency of 1 leaves 2^-4 of a turn to 32
 // bits), its cosine and sine are taken in 32.

@@ -11,6 +11,7 @@ namespace pa {
 constexpr int NW = 8;              // waves per workgroup, two per SIMD
 constexpr int BM = NW * 32;        // query rows per workgroup (the kernel for few rows: half of both)
 constexpr int BN = 64;             // keys per tile
+constexpr int MOST_SPLITS = 16;   // of a block's keys
 constexpr int FEW_BLOCKS = 512;   // of 256 rows: below that many the kernel of 128 rows runs
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr float MOST_SUM = 4096.0f;  // of a lane's 32 weights of a tile, each of which fp16 then holds
@@ -159,36 +160,32 @@ __device__ __forceinline__ PromptBlock find_block(const PromptArgs& g) {
     const int64_t from = ((int64_t)(n - 1) * BN - offset) * g.group;  // the first row that needs them
     return from <= 0 ? blocks : from >= rows ? 0 : blocks - (int)(from / BM);
   };
-  auto sum = [&](int x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-    return x;
-  };
+  const PromptBlock mine = p;
   p.rows = 0;
-  if (id >= sum(blocks)) return p;
-  int lo = 0, hi = tiles;  // of the wanted block: lo <= its tiles <= hi
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) hi = max(hi, __shfl_xor(hi, off, 64));
+  if (id >= wave_total(blocks)) return p;
+  // Of the wanted block: lo <= its tiles <= hi.  (The longest sequence's tiles: by halving too.)
+  int lo = 0, hi = 0x7fffffff >> 6;
+  while (hi >> 1 && !__builtin_amdgcn_ballot_w64(tiles > hi >> 1)) hi >>= 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (sum(at_least(mid)) > id)
+    if (wave_total(at_least(mid)) > id)
       lo = mid;
     else
       hi = mid - 1;
   }
-  const int more = at_least(lo + 1), here = at_least(lo) - more;
-  int upto = here;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int other = __shfl_up(upto, off, 64);
-    if (lane >= off) upto += other;
-  }
-  const int rank = (int)id - sum(more);  // among the blocks of as many tiles
+  const int more = at_least(lo + 1), here = at_least(lo) - more, upto = wave_scan(here);
+  const int rank = (int)id - wave_total(more);  // among the blocks of as many tiles
   const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rank));
   // (a sequence's blocks grow in tiles: those of exactly `lo` end before its last `more`)
   const int block = blocks - more - (upto - rank);
-  p.r0 = __builtin_amdgcn_readfirstlane(__shfl(block, who, 64)) * BM;
-  sequence(__builtin_amdgcn_readfirstlane(who));
+  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, who); };
+  auto of64 = [&](int64_t x) { return (int64_t)(uint32_t)of((int)x) | (int64_t)of((int)(x >> 32)) << 32; };
+  p.q_begin = of64(mine.q_begin);
+  p.k_begin = of64(mine.k_begin);
+  p.Sq = of(mine.Sq);
+  p.Sk = of(mine.Sk);
+  p.rows = of(rows);
+  p.r0 = of(block) * BM;
   return p;
 }
 
@@ -606,28 +603,39 @@ prompt_stream_kernel(PromptArgs g) {
   }
 }
 
-// Joins the splits of a row: a wave for each, a lane for every 64th element.
+// Joins the splits of a row: a wave for each, a lane for two elements.
 template <typename T>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs g) {
+  using namespace pa;
   const int lane = threadIdx.x & 63, heads = g.kv_heads * g.group;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), token = row / heads;
   // (rows before the first sequence or behind the last have no states)
   if (row >= g.rows || token < clamped_start(g.map, 0) || token >= clamped_start(g.map, g.map.sequences)) return;
-  float mm = -INFINITY;
-  for (int s = 0; s < g.splits; ++s) mm = fmaxf(mm, g.part_ml[(s * g.rows + row) * 2]);
-  float sum = 0.f, o[2] = {0.f, 0.f};
-  for (int s = 0; s < g.splits; ++s) {
-    const float2 ml = *(const float2*)(g.part_ml + (s * g.rows + row) * 2);
-    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
-    sum += ml.y * f;
+  float2 ml[MOST_SPLITS], x[MOST_SPLITS];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (u * 64 + lane < g.dim) o[u] += g.part_o[(s * g.rows + row) * g.dim + u * 64 + lane] * f;
+  for (int s = 0; s < MOST_SPLITS; ++s) {
+    if (s < g.splits) {
+      ml[s] = *(const float2*)(g.part_ml + (s * g.rows + row) * 2);
+      if (2 * lane < g.dim) x[s] = *(const float2*)(g.part_o + (s * g.rows + row) * g.dim + 2 * lane);
+    }
   }
-  uint16_t* O = (uint16_t*)g.o + token * g.os[0] + (row - token * heads) * g.os[1];
+  float mm = -INFINITY, sum = 0.f, o[2] = {0.f, 0.f};
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (u * 64 + lane < g.dim) O[u * 64 + lane] = elem<T>::from_float(sum != 0.f ? o[u] / sum : 0.f);
+  for (int s = 0; s < MOST_SPLITS; ++s)
+    if (s < g.splits) mm = fmaxf(mm, ml[s].x);
+#pragma unroll
+  for (int s = 0; s < MOST_SPLITS; ++s) {
+    if (s < g.splits) {
+      const float f = ml[s].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[s].x - mm);
+      sum += ml[s].y * f;
+      o[0] += x[s].x * f;
+      o[1] += x[s].y * f;
+    }
+  }
+  if (2 * lane >= g.dim) return;
+  uint16_t* O = (uint16_t*)g.o + token * g.os[0] + (row - token * heads) * g.os[1];
+  const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+  *(uint32_t*)(O + 2 * lane) = pack2<T>(o[0] * inv, o[1] * inv);
 }
 
 // Any strides, element by element: keys and values through registers into two LDS stages of 64 keys,
@@ -929,7 +937,7 @@ static PromptPlan prompt_plan(int64_t q_tokens, int64_t k_tokens, int64_t sequen
   PromptPlan p{pa::BM, 1};
   if (unit_count(map) * kv_heads < pa::FEW_BLOCKS) p.per = map.per = pa::BM / 2;
   const int64_t blocks = unit_count(map) * kv_heads, tiles = k_tokens / std::max<int64_t>(1, sequences) / pa::BN;
-  if (p.per < pa::BM) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, tiles / 4, 16}));
+  if (p.per < pa::BM) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, tiles / 4, pa::MOST_SPLITS}));
   return p;
 }
 
