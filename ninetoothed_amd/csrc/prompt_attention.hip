@@ -12,7 +12,7 @@ constexpr int NW = 8;              // waves per workgroup, two per SIMD
 constexpr int BM = NW * 32;        // query rows per workgroup (the kernel for few rows: half of both)
 constexpr int BN = 64;             // keys per tile
 constexpr int MOST_SPLITS = 16;   // of a block's keys
-constexpr int FEW_BLOCKS = 512;   // of 256 rows: below that many the kernel of 128 rows runs
+constexpr int FEW_BLOCKS = 512;   // of 256 rows
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr float MOST_SUM = 4096.0f;  // of a lane's 32 weights of a tile, each of which fp16 then holds
 // V^T rows: 64 keys + 8 pad.  Within each 16-key slice the keys lie in the order in which a
@@ -929,15 +929,24 @@ static bool prompt_vectors(const PromptArgs& g) {
 }
 
 // The rows of a workgroup, and over how many its keys are split.
+// 128 rows (two workgroups a CU) where 256 would leave CUs idle, or where sequences are so short that
+// one workgroup a CU mostly starts and ends: us with 128 / 256 rows, causal, bf16, heads of 128, D = 32
+// heads on 8: 1 x 1,024 25.6 / 33.6, 1 x 2,048 52.6 / 59.9, 64 x 256 132 / 183, 32 x 512 156 / 189, 16 x 1,024
+// 208 / 230, but 16 x 2,048 679 / 661, 1 x 16,384 1,896 / 1,821; ungrouped, whose K and V then do not stay
+// in the L2s, 32 x 512 193 / 209, 32 x 1,024 625 / 516.
+// Keys are split while workgroups are few, 16 tiles each at least (the join costs a launch): 512
+// queries over 8,192 keys 85 us, unsplit 146, 64 over 16,384 37 / 294, but over 512 keys in splits of 4
+// tiles 22.7 / 16.8.
 struct PromptPlan {
   int per, splits;
 };
 static PromptPlan prompt_plan(int64_t q_tokens, int64_t k_tokens, int64_t sequences, int64_t kv_heads, int64_t group) {
   UnitMap map{nullptr, q_tokens, (int)sequences, (int)group, pa::BM, 1};
   PromptPlan p{pa::BM, 1};
-  if (unit_count(map) * kv_heads < pa::FEW_BLOCKS) p.per = map.per = pa::BM / 2;
-  const int64_t blocks = unit_count(map) * kv_heads, tiles = k_tokens / std::max<int64_t>(1, sequences) / pa::BN;
-  if (p.per < pa::BM) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, tiles / 4, pa::MOST_SPLITS}));
+  const int64_t tiles = k_tokens / std::max<int64_t>(1, sequences) / pa::BN, blocks = unit_count(map) * kv_heads;
+  if (blocks >= pa::FEW_BLOCKS && tiles > (group >= 4 ? 16 : 8)) return p;
+  p.per = map.per = pa::BM / 2;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / (unit_count(map) * kv_heads), tiles / 16, pa::MOST_SPLITS}));
   return p;
 }
 
