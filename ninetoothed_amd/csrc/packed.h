@@ -118,5 +118,26 @@ template <typename S, int N>
 struct alignas(sizeof(S) * N) Vec {
   S e[N];
 };
+// Stores them; `past`: past the caches, as what is larger than these does not stay in them (a
+// rotation of 67 MB 35.1 us, with such stores 22.6).
+template <typename S, int N>
+__device__ __forceinline__ void store_vec(S* p, const Vec<S, N>& v, bool past) {
+  if constexpr (sizeof(v) == 16) {
+    if (past) return __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)p);
+  } else if constexpr (sizeof(v) == 8) {
+    if (past) return __builtin_nontemporal_store(__builtin_bit_cast(u32x2, v), (u32x2*)p);
+  }
+  *(Vec<S, N>*)p = v;
+}
+constexpr int64_t PAST_CACHES = 8 << 20;  // bytes written from which stores go past the caches
+
+// n / d for 0 <= n < 2^16 and 0 < d <= 2^15: floor(n ceil(2^32 / d) / 2^32), off by less than n / 2^32.
+struct Divider {
+  uint32_t d, magic;
+  __device__ __forceinline__ int operator()(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, magic); }
+};
+inline Divider divider(int64_t d) {
+  return Divider{(uint32_t)d, (uint32_t)(((1ull << 32) + (uint64_t)d - 1) / (uint64_t)d)};
+}
 
 }  // namespace nt

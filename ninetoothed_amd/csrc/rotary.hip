@@ -17,8 +17,9 @@ struct RotaryArgs {
   int heads, dim, pairs, heads_per_wave;
   int long_positions, interleaved, inverse;
   float magnitude;
-  int units, per_head;     // of a head: vectors of pairs, and those plus vectors that are copied
-  uint32_t per_head_magic;  // ceil(2^32 / per_head), for per_head above 1
+  int units;         // vectors of pairs of a head
+  Divider per_head;  // those and the vectors that are copied
+  bool past_caches;
 };
 
 constexpr int ROTARY_PAIRS = 256;  // dim <= 512
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
   float2* turn = turn_all[wave];
   const int head0 = blockIdx.y * g.heads_per_wave;
   const int nheads = min(g.heads - head0, g.heads_per_wave);
-  const int items = nheads * g.per_head;
+  const int items = nheads * (int)g.per_head.d;
   const S* x = (const S*)g.x + token * g.xs[0] + head0 * g.xs[1];
   S* out = (S*)g.out + token * g.os[0] + head0 * g.os[1];
   const int second = g.interleaved ? N : g.pairs;  // where an item's second vector starts
@@ -59,8 +60,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
     for (int i = 0; i < U; ++i) {
       const int item = base + i * 64 + lane;
       if (item >= items) break;
-      head[i] = g.per_head == 1 ? item : (int)__umulhi((uint32_t)item, g.per_head_magic);
-      const int unit = item - head[i] * g.per_head;
+      head[i] = g.per_head(item);
+      const int unit = item - head[i] * (int)g.per_head.d;
       turned[i] = unit < g.units;
       first[i] = turned[i] ? (g.interleaved ? 2 * N * unit : N * unit) : 2 * g.pairs + (unit - g.units) * N;
       const S* row = x + head[i] * g.xs[1];
@@ -111,8 +112,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
         }
       }
       if (UNIT) {
-        *(Vec<S, N>*)(row + first[i]) = a[i];
-        if (turned[i]) *(Vec<S, N>*)(row + first[i] + second) = b[i];
+        store_vec(row + first[i], a[i], g.past_caches);
+        if (turned[i]) store_vec(row + first[i] + second, b[i], g.past_caches);
       } else {
         row[first[i] * g.os[2]] = a[i].e[0];
         if (turned[i]) row[(first[i] + second) * g.os[2]] = b[i].e[0];
@@ -135,13 +136,14 @@ static int rotary_launch(RotaryArgs g, hipStream_t stream) {
   };
   const int n = fits(full) ? full : fits(full / 2) ? full / 2 : 1;
   g.units = g.pairs / n;
-  g.per_head = g.units + (g.dim - 2 * g.pairs) / n;
-  g.per_head_magic = (uint32_t)(((1ull << 32) + g.per_head - 1) / g.per_head);
+  const int per_head = g.units + (g.dim - 2 * g.pairs) / n;
+  g.per_head = divider(per_head);
+  g.past_caches = g.tokens * g.heads * g.dim * bytes >= PAST_CACHES;
   // A wave takes all of a token's heads where tokens alone fill the chip, else fewer of them.
   const int64_t want = std::max<int64_t>(1, 4096 / std::max<int64_t>(1, g.tokens));
-  int64_t splits = std::min<int64_t>({want, (int64_t)g.heads, std::max<int64_t>(1, (int64_t)g.heads * g.per_head / 64)});
-  // (an item number stays below 2^16, so that the multiplied division is exact)
-  splits = std::max<int64_t>(splits, cdiv((int64_t)g.heads * g.per_head, 32768));
+  int64_t splits = std::min<int64_t>({want, (int64_t)g.heads, std::max<int64_t>(1, (int64_t)g.heads * per_head / 64)});
+  // (an item number stays below 2^16, for the division)
+  splits = std::max<int64_t>(splits, cdiv((int64_t)g.heads * per_head, 32768));
   splits = std::min<int64_t>(splits, g.heads);
   g.heads_per_wave = (int)cdiv(g.heads, splits);
   const int64_t blocks = cdiv(g.tokens, 4), parts = cdiv(g.heads, g.heads_per_wave);
@@ -167,6 +169,8 @@ struct AppendArgs {
   int64_t table_stride, pages;
   int heads, dim, pairs, page_size, table_width, heads_per_block, interleaved;
   float magnitude;
+  Divider per_row, per_token;  // items of a row, and of a token's heads of one workgroup
+  bool past_caches;
 };
 
 // The tokens [first, first + count) of the packed tensors that a unit takes, at the positions
@@ -181,11 +185,12 @@ __device__ __forceinline__ AppendUnit append_unit(const AppendArgs& g, int64_t i
   u.sequence = find_sequence(g.map, id);
   const int64_t begin = clamped_start(g.map, u.sequence), end = clamped_start(g.map, u.sequence + 1);
   const int64_t cached = g.lengths[u.sequence], block = g.map.per;
-  const int64_t which = cached / block + (id - first_unit(g.map, u.sequence));  // of the sequence's blocks of positions
+  const int64_t nth = id - first_unit(g.map, u.sequence);
+  const int64_t which = (uint32_t)cached / (uint32_t)block + nth;  // of the sequence's blocks of positions
   const int64_t from = max(cached, which * block), to = min(cached + (end - begin), (which + 1) * block);
   u.position = (uint32_t)from;
   u.first = begin + (from - cached);
-  u.count = cached < 0 || id < first_unit(g.map, u.sequence) || to <= from ? 0 : (int)(to - from);
+  u.count = cached < 0 || nth < 0 || to <= from ? 0 : (int)(to - from);
   return u;
 }
 // The page of a position, or -1 where the table or the cache has none.
@@ -195,56 +200,6 @@ __device__ __forceinline__ int64_t page_of(const AppendArgs& g, int sequence, ui
   const int64_t page = g.tables[sequence * g.table_stride + n];
   return page < 0 || page >= g.pages ? -1 : page;
 }
-
-// One row's item: 2 N elements, N pairs to turn or 2 N neighbours to copy.
-template <typename T, int N>
-struct AppendItem {
-  int d0, d1;  // where its two vectors of N start
-  int pair;    // its first pair, or -1
-};
-template <typename T, int N>
-__device__ __forceinline__ AppendItem<T, N> append_item(int unit, int pairs, int interleaved) {
-  const bool turned = unit * N < pairs;
-  const int d0 = turned && !interleaved ? unit * N : 2 * N * unit;
-  return {d0, turned && !interleaved ? d0 + pairs : d0 + N, turned ? unit * N : -1};
-}
-template <typename T, int N, bool UNIT>
-__device__ __forceinline__ void append_load(const typename elem<T>::storage* row, int64_t es, const AppendItem<T, N>& it,
-                                            const float2* turn, int interleaved, float (&y)[2 * N]) {
-  typedef typename elem<T>::storage S;
-  Vec<S, N> a, b;
-  if (UNIT) {
-    a = *(const Vec<S, N>*)(row + it.d0);
-    b = *(const Vec<S, N>*)(row + it.d1);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      a.e[e] = row[(it.d0 + e) * es];
-      b.e[e] = row[(it.d1 + e) * es];
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    y[e] = elem<T>::to_float(a.e[e]);
-    y[N + e] = elem<T>::to_float(b.e[e]);
-  }
-  if (it.pair < 0) return;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float2 cs = turn[it.pair + e];
-    // (a register array is indexed by constants only: both layouts are written out)
-    if (interleaved) {
-      const float p = y[2 * e], q = y[2 * e + 1];
-      y[2 * e] = p * cs.x - q * cs.y;
-      y[2 * e + 1] = q * cs.x + p * cs.y;
-    } else {
-      const float p = y[e], q = y[N + e];
-      y[e] = p * cs.x - q * cs.y;
-      y[N + e] = q * cs.x + p * cs.y;
-    }
-  }
-}
-
 // The angles of a unit's tokens: turn[token * pairs + pair].
 __device__ __forceinline__ void append_turns(const AppendArgs& g, const AppendUnit& u, float2* turn) {
   for (int i = threadIdx.x; i < u.count * g.pairs; i += 256) {
@@ -253,57 +208,131 @@ __device__ __forceinline__ void append_turns(const AppendArgs& g, const AppendUn
   }
 }
 
-// Keys (turned by position) and values into pages of their own 16-bit type.  Bound by HBM: each
-// element read and written once.  A workgroup takes up to `per` positions of one sequence and some
-// heads of k or of v: the angles are then taken once for those heads.
+// One row's item: 2 N elements, N pairs to turn or 2 N neighbours to copy, as they lie in memory.
 template <typename T, int N, bool UNIT>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
+struct AppendItem {
   typedef typename elem<T>::storage S;
-  extern __shared__ float2 turn[];
-  const AppendUnit u = append_unit(g, blockIdx.x);
-  if (u.count == 0) return;
-  const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
-  const int nheads = min(g.heads - head0, g.heads_per_block);
-  const int pairs = which == 0 ? g.pairs : 0;
-  if (pairs) {
-    append_turns(g, u, turn);
-    __syncthreads();
+  Vec<S, N> a, b;
+  int d0, d1;  // where its two vectors of N start
+  int pair;    // its first pair, or -1
+  __device__ __forceinline__ AppendItem() {}
+  __device__ __forceinline__ AppendItem(int unit, int pairs, int interleaved) {
+    const bool turned = unit * N < pairs;
+    d0 = turned && !interleaved ? unit * N : 2 * N * unit;
+    d1 = turned && !interleaved ? d0 + pairs : d0 + N;
+    pair = turned ? unit * N : -1;
   }
-  const int per_row = g.dim / (2 * N), per_token = per_row * nheads, items = u.count * per_token;
-  const S* x = (const S*)g.x[which] + u.first * g.xs[which][0] + head0 * g.xs[which][1];
-  S* cache = (S*)g.cache[which] + head0 * g.cs[which][2];
-  for (int i = threadIdx.x; i < items; i += 256) {
-    const int t = i / per_token, r = i - t * per_token, h = r / per_row;
-    const AppendItem<T, N> it = append_item<T, N>(r - h * per_row, pairs, g.interleaved);
-    const uint32_t position = u.position + t;
-    const int64_t page = page_of(g, u.sequence, position);
-    float y[2 * N];
-    append_load<T, N, UNIT>(x + t * g.xs[which][0] + h * g.xs[which][1], g.xs[which][2], it, turn + t * g.pairs,
-                            g.interleaved, y);
-    if (page < 0) continue;
-    S* row = cache + page * g.cs[which][0] + (int64_t)(position % (uint32_t)g.page_size) * g.cs[which][1] + h * g.cs[which][2];
-    Vec<S, N> a, b;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      a.e[e] = elem<T>::from_float(y[e]);
-      b.e[e] = elem<T>::from_float(y[N + e]);
-    }
+  __device__ __forceinline__ void load(const S* row, int64_t es) {
     if (UNIT) {
-      *(Vec<S, N>*)(row + it.d0) = a;
-      *(Vec<S, N>*)(row + it.d1) = b;
+      a = *(const Vec<S, N>*)(row + d0);
+      b = *(const Vec<S, N>*)(row + d1);
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        row[it.d0 + e] = a.e[e];
-        row[it.d1 + e] = b.e[e];
+        a.e[e] = row[(d0 + e) * es];
+        b.e[e] = row[(d1 + e) * es];
+      }
+    }
+  }
+  // Its elements in fp32, turned.  `turn`: of its token.
+  __device__ __forceinline__ void values(const float2* turn, int interleaved, float (&y)[2 * N]) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      y[e] = elem<T>::to_float(a.e[e]);
+      y[N + e] = elem<T>::to_float(b.e[e]);
+    }
+    if (pair < 0) return;
+    // (a register array is indexed by constants only: both layouts are written out)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float2 cs = turn[pair + e];
+      if (interleaved) {
+        const float p = y[2 * e], q = y[2 * e + 1];
+        y[2 * e] = p * cs.x - q * cs.y;
+        y[2 * e + 1] = q * cs.x + p * cs.y;
+      } else {
+        const float p = y[e], q = y[N + e];
+        y[e] = p * cs.x - q * cs.y;
+        y[N + e] = q * cs.x + p * cs.y;
+      }
+    }
+  }
+};
+
+// Keys (turned by position) and values into pages of their own 16-bit type.  Bound by HBM: each
+// element read and written once.  A workgroup takes up to `per` positions of one sequence and some
+// heads of k or of v: the angles and the places in the cache are then found once for those heads.
+// The loads of U items a lane are in flight together, the first of them before the angles.
+constexpr int APPEND_TOKENS = 64;
+template <typename T, int N, bool UNIT>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
+  typedef typename elem<T>::storage S;
+  typedef AppendItem<T, N, UNIT> Item;
+  constexpr int U = N == 1 ? 2 : 4;
+  extern __shared__ float2 turn[];
+  __shared__ int64_t row_at[APPEND_TOKENS];  // of a token in the cache, or -1
+  const AppendUnit u = append_unit(g, blockIdx.x);
+  if (u.count == 0) return;
+  const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
+  const int pairs = which == 0 ? g.pairs : 0;
+  const int items = u.count * (int)g.per_token.d;
+  const S* x = (const S*)g.x[which] + u.first * g.xs[which][0];
+  S* cache = (S*)g.cache[which];
+  Item it[U];
+  int token[U], head[U];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int n = base + i * 256 + threadIdx.x;
+      if (n >= items) break;
+      token[i] = g.per_token(n);
+      const int r = n - token[i] * (int)g.per_token.d, h = g.per_row(r);
+      head[i] = head0 + h;
+      it[i] = Item(r - h * (int)g.per_row.d, pairs, g.interleaved);
+      if (head[i] < g.heads) it[i].load(x + token[i] * g.xs[which][0] + head[i] * g.xs[which][1], g.xs[which][2]);
+    }
+  };
+  load(0);
+  if ((int)threadIdx.x < u.count) {
+    const uint32_t position = u.position + threadIdx.x;
+    const int64_t page = page_of(g, u.sequence, position);
+    row_at[threadIdx.x] =
+        page < 0 ? -1 : page * g.cs[which][0] + (int64_t)(position % (uint32_t)g.page_size) * g.cs[which][1];
+  }
+  if (pairs) append_turns(g, u, turn);
+  __syncthreads();
+  for (int base = 0; base < items; base += 256 * U) {
+    if (base) load(base);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (base + i * 256 + (int)threadIdx.x >= items) break;
+      if (head[i] >= g.heads || row_at[token[i]] < 0) continue;
+      float y[2 * N];
+      it[i].values(turn + token[i] * pairs, g.interleaved, y);
+      S* row = cache + row_at[token[i]] + head[i] * g.cs[which][2];
+      Vec<S, N> a, b;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        a.e[e] = elem<T>::from_float(y[e]);
+        b.e[e] = elem<T>::from_float(y[N + e]);
+      }
+      if (UNIT) {
+        store_vec(row + it[i].d0, a, g.past_caches);
+        store_vec(row + it[i].d1, b, g.past_caches);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          row[it[i].d0 + e] = a.e[e];
+          row[it[i].d1 + e] = b.e[e];
+        }
       }
     }
   }
 }
 
-// e4m3 from fp32, to nearest even; |x| <= 448 but for NaN, which stays one.
-__device__ __forceinline__ uint8_t e4m3_of(float x) {
-  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false);
+// Four e4m3 from fp32, to nearest even; |x| <= 448 but for NaN, which stays one.
+__device__ __forceinline__ uint32_t e4m3_of(float x0, float x1, float x2, float x3) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false), true);
 }
 // The exponent of the least power of two that 448 times is at least x (x finite, not negative):
 // x = m 2^e with m in [0.5, 1), and 448 = 0.875 * 2^9.  Held in the range in which a scale's
@@ -321,15 +350,15 @@ __device__ __forceinline__ int fitting_exponent(float x) {
 // the page already holds is divided exactly.  A scale is taken afresh when a page is begun (its slot 0
 // is among the new tokens); else it only grows.  Infinities and NaN are stored as NaN, which is
 // all that e4m3 has of them, and do not count for the scale.
-// A workgroup takes the new tokens of one page and some heads of k or of v: per head the values
-// are turned and held in registers (HOLD items a lane, the rest is turned again), their largest
-// found, then stored.
-template <typename T, int N, bool UNIT>
+// A workgroup takes the new tokens of one page and some heads of k or of v: per head their values
+// are loaded once, HOLD items a lane (what is more is loaded again), turned for their largest
+// magnitude and again to be stored.
+template <typename T, int N, bool UNIT, int HOLD>
 __global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
   typedef typename elem<T>::storage S;
-  constexpr int HOLD = N == 8 ? 4 : 8;
+  typedef AppendItem<T, N, UNIT> Item;
   extern __shared__ float2 turn[];
-  __shared__ float largest[2][4];
+  __shared__ uint32_t largest[2][4];
   const AppendUnit u = append_unit(g, blockIdx.x);
   if (u.count == 0) return;
   const int64_t page = page_of(g, u.sequence, u.position);
@@ -337,49 +366,79 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
   const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
   const int nheads = min(g.heads - head0, g.heads_per_block);
   const int pairs = which == 0 ? g.pairs : 0;
+  const int slot0 = (int)(u.position % (uint32_t)g.page_size);
+  const int per_row = (int)g.per_row.d, items = u.count * per_row;
+  const S* x = (const S*)g.x[which] + u.first * g.xs[which][0] + head0 * g.xs[which][1];
+  Item held[HOLD];
+  int token[HOLD];
+  auto item = [&](int i, int& t) {
+    t = g.per_row(i);
+    return Item(i - t * per_row, pairs, g.interleaved);
+  };
+  auto load = [&](int h) {
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k) {
+      const int i = k * 256 + threadIdx.x;
+      if (i >= items) break;
+      held[k] = item(i, token[k]);
+      held[k].load(x + token[k] * g.xs[which][0] + h * g.xs[which][1], g.xs[which][2]);
+    }
+  };
+  load(0);
   if (pairs) {
     append_turns(g, u, turn);
     __syncthreads();
   }
-  const int slot0 = (int)(u.position % (uint32_t)g.page_size);
-  const int per_row = g.dim / (2 * N), items = u.count * per_row;
   for (int h = 0; h < nheads; ++h) {
-    const S* x = (const S*)g.x[which] + u.first * g.xs[which][0] + (head0 + h) * g.xs[which][1];
+    const S* xh = x + h * g.xs[which][1];
     uint8_t* cache = (uint8_t*)g.cache[which] + page * g.cs[which][0] + (head0 + h) * g.cs[which][2];
     float* scale_at = g.scale[which] + page * g.heads + head0 + h;
-    const float old = *scale_at;
-    float held[HOLD][2 * N];
-    float most = 0.f;
-    auto load = [&](int i, float (&y)[2 * N]) {
-      const int t = i / per_row;
-      append_load<T, N, UNIT>(x + t * g.xs[which][0], g.xs[which][2], append_item<T, N>(i - t * per_row, pairs, g.interleaved),
-                              turn + t * g.pairs, g.interleaved, y);
-    };
-    auto look = [&](const float (&y)[2 * N]) {
+    const float old = slot0 ? *scale_at : 0.f;
+    // f(values) for each of this lane's items.
+    auto each = [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 2 * N; ++e) {
-        const float m = fabsf(y[e]);
-        most = m < INFINITY ? fmaxf(most, m) : most;
+      for (int k = 0; k < HOLD; ++k) {
+        if (k * 256 + (int)threadIdx.x >= items) break;
+        float y[2 * N];
+        held[k].values(turn + token[k] * pairs, g.interleaved, y);
+        f(held[k], token[k], y);
+      }
+      for (int i = HOLD * 256 + threadIdx.x; i < items; i += 256) {
+        int t;
+        Item it = item(i, t);
+        it.load(xh + t * g.xs[which][0], g.xs[which][2]);
+        float y[2 * N];
+        it.values(turn + t * pairs, g.interleaved, y);
+        f(it, t, y);
       }
     };
+    // The largest magnitude's bits, in their order as integers: infinities and NaN come last.
+    uint32_t most = 0;
+    each([&](const Item&, int, const float (&y)[2 * N]) {
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) {
-      const int i = k * 256 + threadIdx.x;
-      if (i < items) {
-        load(i, held[k]);
-        look(held[k]);
-      }
+      for (int e = 0; e < 2 * N; ++e) most = max(most, __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu);
+    });
+    auto over_all = [&](uint32_t x, uint32_t (&lds)[4]) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, off, 64));
+      if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+      __syncthreads();  // (also: every lane has read the old scale)
+      return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+    };
+    most = over_all(most, largest[h & 1]);
+    if (most >= 0x7f800000u) {  // seldom: the largest of the others
+      most = 0;
+      each([&](const Item&, int, const float (&y)[2 * N]) {
+#pragma unroll
+        for (int e = 0; e < 2 * N; ++e) {
+          const uint32_t bits = __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu;
+          most = max(most, bits < 0x7f800000u ? bits : 0u);
+        }
+      });
+      __syncthreads();  // (every lane has read the first answer)
+      most = over_all(most, largest[h & 1]);
     }
-    for (int i = HOLD * 256 + threadIdx.x; i < items; i += 256) {
-      float y[2 * N];
-      load(i, y);
-      look(y);
-    }
-    most = wave_max(most);
-    if ((threadIdx.x & 63) == 0) largest[h & 1][threadIdx.x >> 6] = most;
-    __syncthreads();  // (also: every lane has read the old scale)
-    most = fmaxf(fmaxf(largest[h & 1][0], largest[h & 1][1]), fmaxf(largest[h & 1][2], largest[h & 1][3]));
-    const float fitting = ldexpf(1.0f, fitting_exponent(most));
+    const float fitting = ldexpf(1.0f, fitting_exponent(__builtin_bit_cast(float, most)));
     const float scale = slot0 ? fmaxf(old, fitting) : fitting, inverse = 1.0f / scale;
     if (threadIdx.x == 0) *scale_at = scale;
     if (slot0 && scale != old) {  // what the page held follows its scale
@@ -387,44 +446,39 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
       for (int i = threadIdx.x; i < slot0 * (g.dim / 4); i += 256) {
         const int t = i / (g.dim / 4), d = (i - t * (g.dim / 4)) * 4;
         uint8_t* row = cache + t * g.cs[which][1] + d;
+        float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          row[e] = e4m3_of(__builtin_amdgcn_cvt_f32_fp8((int)row[e], 0) * ratio);
+        for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_cvt_f32_fp8((int)row[e], 0) * ratio;
+        const uint32_t q = e4m3_of(y[0], y[1], y[2], y[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) row[e] = (uint8_t)(q >> (8 * e));
       }
     }
-    auto store = [&](int i, const float (&y)[2 * N]) {
-      const int t = i / per_row;
-      const AppendItem<T, N> it = append_item<T, N>(i - t * per_row, pairs, g.interleaved);
+    each([&](const Item& it, int t, const float (&y)[2 * N]) {
       uint8_t* row = cache + (slot0 + t) * g.cs[which][1];
-      Vec<uint8_t, N> v[2];
+      // (y * 0 is NaN for infinities too)
+      auto q = [&](int e) { return __builtin_fmaf(y[e], inverse, y[e] * 0.f); };
+      if constexpr (UNIT) {
+        Vec<uint32_t, N / 4> v[2];
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float q = y[w * N + e] * inverse;
-          v[w].e[e] = e4m3_of(fabsf(q) < INFINITY ? q : NAN);
-        }
-      if (UNIT) {
-        *(Vec<uint8_t, N>*)(row + it.d0) = v[0];
-        *(Vec<uint8_t, N>*)(row + it.d1) = v[1];
+          for (int e = 0; e < N / 4; ++e) {
+            const int i = w * N + 4 * e;
+            v[w].e[e] = e4m3_of(q(i), q(i + 1), q(i + 2), q(i + 3));
+          }
+        store_vec((uint32_t*)(row + it.d0), v[0], g.past_caches);
+        store_vec((uint32_t*)(row + it.d1), v[1], g.past_caches);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          row[it.d0 + e] = v[0].e[e];
-          row[it.d1 + e] = v[1].e[e];
+          const uint32_t both = e4m3_of(q(e), q(N + e), 0.f, 0.f);
+          row[it.d0 + e] = (uint8_t)both;
+          row[it.d1 + e] = (uint8_t)(both >> 8);
         }
       }
-    };
-#pragma unroll
-    for (int k = 0; k < HOLD; ++k) {
-      const int i = k * 256 + threadIdx.x;
-      if (i < items) store(i, held[k]);
-    }
-    for (int i = HOLD * 256 + threadIdx.x; i < items; i += 256) {
-      float y[2 * N];
-      load(i, y);
-      store(i, y);
-    }
+    });
+    if (h + 1 < nheads) load(h + 1);
   }
 }
 
@@ -440,30 +494,42 @@ static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
   };
   const int n = fits(8) ? 8 : fits(4) ? 4 : 1;
   // A unit is a page of an 8-bit cache, else 64 positions; its angles take at most 64 KiB of LDS.
-  g.map.per = eight ? g.page_size : 64;
+  g.map.per = eight ? g.page_size : APPEND_TOKENS;
   g.map.rows = 1;
   g.map.extra = 2;
   const int64_t units = unit_count(g.map);
   // All heads of a unit share its angles where there are enough units (and k and v) for that.
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.heads, 2048 / std::max<int64_t>(1, units)));
-  g.heads_per_block = (int)cdiv(g.heads, parts);
+  const int64_t per_row = g.dim / (2 * n);
+  g.heads_per_block = (int)std::min<int64_t>(cdiv(g.heads, parts), 65535 / (APPEND_TOKENS * per_row));
   const int64_t y = cdiv(g.heads, g.heads_per_block);
   if (units > 0x7fffffffLL || y > 65535) return NT_ERR_INVALID;
+  g.per_row = divider(per_row);
+  g.per_token = divider(per_row * g.heads_per_block);
+  g.past_caches = 2 * g.map.tokens * g.heads * g.dim * (eight ? 1 : 2) >= PAST_CACHES;
+  const int64_t most_tokens = std::min<int64_t>(g.map.per, g.map.tokens);
   const dim3 grid((unsigned)units, (unsigned)y, 2), block(256);
-  const size_t lds = (size_t)std::min<int64_t>(g.map.per, g.map.tokens) * g.pairs * sizeof(float2);
-#define NT_APPEND(kernel)                                                                  \
-  if (n == 8)                                                                              \
-    hipLaunchKernelGGL((kernel<T, 8, true>), grid, block, lds, stream, g);                 \
-  else if (n == 4)                                                                         \
-    hipLaunchKernelGGL((kernel<T, 4, true>), grid, block, lds, stream, g);                 \
-  else                                                                                     \
-    hipLaunchKernelGGL((kernel<T, 1, false>), grid, block, lds, stream, g);
-  if (eight) {
-    NT_APPEND(append8_kernel)
+  const size_t lds = (size_t)most_tokens * g.pairs * sizeof(float2);
+  if (!eight) {
+    if (n == 8)
+      hipLaunchKernelGGL((append_kernel<T, 8, true>), grid, block, lds, stream, g);
+    else if (n == 4)
+      hipLaunchKernelGGL((append_kernel<T, 4, true>), grid, block, lds, stream, g);
+    else
+      hipLaunchKernelGGL((append_kernel<T, 1, false>), grid, block, lds, stream, g);
+  } else if (n == 8) {
+    const int64_t items = cdiv(most_tokens * per_row, 256);  // of a lane
+    if (items <= 1)
+      hipLaunchKernelGGL((append8_kernel<T, 8, true, 1>), grid, block, lds, stream, g);
+    else if (items <= 2)
+      hipLaunchKernelGGL((append8_kernel<T, 8, true, 2>), grid, block, lds, stream, g);
+    else
+      hipLaunchKernelGGL((append8_kernel<T, 8, true, 4>), grid, block, lds, stream, g);
+  } else if (n == 4) {
+    hipLaunchKernelGGL((append8_kernel<T, 4, true, 4>), grid, block, lds, stream, g);
   } else {
-    NT_APPEND(append_kernel)
+    hipLaunchKernelGGL((append8_kernel<T, 1, false, 4>), grid, block, lds, stream, g);
   }
-#undef NT_APPEND
   return launch_status();
 }
 
