@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
   for (int p = lane; p < g.pairs; p += 64) {
     float2 cs = rotation((double)position, g.freqs[p], g.magnitude);
     if (g.inverse) cs.y = -cs.y;
-    turn[p] = cs;
+    turn[(p % N) * g.units + p / N] = cs;  // (an item's lanes then read neighbours)
   }
   wave_lds_order();
   for (int base = 0; base < items; base += 64 * U) {
@@ -88,14 +88,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
       if (base + i * 64 + lane >= items) break;
       S* row = out + head[i] * g.os[1];
       if (turned[i]) {
-        const int pair = g.interleaved ? first[i] >> 1 : first[i];
+        const float2* at = turn + (g.interleaved ? first[i] >> 1 : first[i]) / N;
         if (g.interleaved && N > 1) {  // a holds the first N / 2 pairs, b the others
 #pragma unroll
           for (int e = 0; e < N; e += 2) {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
               Vec<S, N>& v = w ? b[i] : a[i];
-              const float2 cs = turn[pair + w * (N / 2) + e / 2];
+              const float2 cs = at[(w * (N / 2) + e / 2) * g.units];
               const float p = elem<T>::to_float(v.e[e]), q = elem<T>::to_float(v.e[e + 1 < N ? e + 1 : e]);
               v.e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
               v.e[e + 1 < N ? e + 1 : e] = elem<T>::from_float(q * cs.x + p * cs.y);
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
         } else {
 #pragma unroll
           for (int e = 0; e < N; ++e) {
-            const float2 cs = turn[pair + e];
+            const float2 cs = at[e * g.units];
             const float p = elem<T>::to_float(a[i].e[e]), q = elem<T>::to_float(b[i].e[e]);
             a[i].e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
             b[i].e[e] = elem<T>::from_float(q * cs.x + p * cs.y);
@@ -200,12 +200,49 @@ __device__ __forceinline__ int64_t page_of(const AppendArgs& g, int sequence, ui
   const int64_t page = g.tables[sequence * g.table_stride + n];
   return page < 0 || page >= g.pages ? -1 : page;
 }
-// The angles of a unit's tokens: turn[token * pairs + pair].
+// cos and sin for a unit's tokens: that of pair N unit + e of a token at
+//   turn[token * turn_row<N>(pairs) + e * (pairs / N) + unit],
+// so that the lanes of a row read neighbours, and the rows of a wave do not meet in a bank.
+// They are taken for every eighth token and for eight tokens' steps, and multiplied:
+//   cos(a + b) = cos a cos b - sin a sin b, ...
+// which is a quarter of the angles of 64 tokens, and is off by four roundings of fp32.
+template <int N>
+__host__ __device__ constexpr int turn_row(int pairs) {
+  return pairs + (N == 8 ? 8 : 0);
+}
+template <int N>
 __device__ __forceinline__ void append_turns(const AppendArgs& g, const AppendUnit& u, float2* turn) {
-  for (int i = threadIdx.x; i < u.count * g.pairs; i += 256) {
-    const int t = i / g.pairs;
-    turn[i] = rotation((double)(u.position + t), g.freqs[i - t * g.pairs], g.magnitude);
+  const int pairs = g.pairs, units = pairs / N, row = turn_row<N>(pairs);
+  if (u.count <= 8) {
+    for (int i = threadIdx.x; i < u.count * pairs; i += 256) {
+      const int t = i / pairs, p = i - t * pairs;
+      turn[t * row + (p % N) * units + p / N] = rotation((double)(u.position + t), g.freqs[p], g.magnitude);
+    }
+    __syncthreads();
+    return;
   }
+  float2* steps = turn + u.count * row;  // of 1 to 7 tokens
+  const int anchors = (u.count + 7) / 8;
+  for (int i = threadIdx.x; i < (anchors + 7) * pairs; i += 256) {
+    const int n = i / pairs, p = i - n * pairs, at = (p % N) * units + p / N;
+    if (n < anchors)
+      turn[n * 8 * row + at] = rotation((double)(u.position + n * 8), g.freqs[p], g.magnitude);
+    else
+      steps[(n - anchors) * pairs + at] = rotation((double)(n - anchors + 1), g.freqs[p], 1.0f);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < u.count * pairs; i += 256) {
+    const int t = i / pairs, at = i - t * pairs;
+    if (t % 8 == 0) continue;
+    const float2 a = turn[(t & ~7) * row + at], b = steps[(t % 8 - 1) * pairs + at];
+    turn[t * row + at] = float2{a.x * b.x - a.y * b.y, a.y * b.x + a.x * b.y};
+  }
+  __syncthreads();
+}
+// The LDS they take.
+static size_t turn_bytes(int64_t tokens, int pairs, int n) {
+  const int64_t row = n == 8 ? turn_row<8>(pairs) : pairs;
+  return (size_t)(pairs ? tokens * row + (tokens > 8 ? 7 * pairs : 0) : 0) * sizeof(float2);
 }
 
 // One row's item: 2 N elements, N pairs to turn or 2 N neighbours to copy, as they lie in memory.
@@ -214,13 +251,13 @@ struct AppendItem {
   typedef typename elem<T>::storage S;
   Vec<S, N> a, b;
   int d0, d1;  // where its two vectors of N start
-  int pair;    // its first pair, or -1
+  int unit;    // of N pairs, or -1
   __device__ __forceinline__ AppendItem() {}
-  __device__ __forceinline__ AppendItem(int unit, int pairs, int interleaved) {
-    const bool turned = unit * N < pairs;
-    d0 = turned && !interleaved ? unit * N : 2 * N * unit;
+  __device__ __forceinline__ AppendItem(int nth, int pairs, int interleaved) {
+    const bool turned = nth * N < pairs;
+    d0 = turned && !interleaved ? nth * N : 2 * N * nth;
     d1 = turned && !interleaved ? d0 + pairs : d0 + N;
-    pair = turned ? unit * N : -1;
+    unit = turned ? nth : -1;
   }
   __device__ __forceinline__ void load(const S* row, int64_t es) {
     if (UNIT) {
@@ -234,18 +271,18 @@ struct AppendItem {
       }
     }
   }
-  // Its elements in fp32, turned.  `turn`: of its token.
-  __device__ __forceinline__ void values(const float2* turn, int interleaved, float (&y)[2 * N]) const {
+  // Its elements in fp32, turned.  `turn`: its token's row of `units` times N.
+  __device__ __forceinline__ void values(const float2* turn, int units, int interleaved, float (&y)[2 * N]) const {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       y[e] = elem<T>::to_float(a.e[e]);
       y[N + e] = elem<T>::to_float(b.e[e]);
     }
-    if (pair < 0) return;
+    if (unit < 0) return;
     // (a register array is indexed by constants only: both layouts are written out)
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float2 cs = turn[pair + e];
+      const float2 cs = turn[e * units + unit];
       if (interleaved) {
         const float p = y[2 * e], q = y[2 * e + 1];
         y[2 * e] = p * cs.x - q * cs.y;
@@ -299,8 +336,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
     row_at[threadIdx.x] =
         page < 0 ? -1 : page * g.cs[which][0] + (int64_t)(position % (uint32_t)g.page_size) * g.cs[which][1];
   }
-  if (pairs) append_turns(g, u, turn);
-  __syncthreads();
+  if (pairs)
+    append_turns<N>(g, u, turn);
+  else
+    __syncthreads();
   for (int base = 0; base < items; base += 256 * U) {
     if (base) load(base);
 #pragma unroll
@@ -308,7 +347,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
       if (base + i * 256 + (int)threadIdx.x >= items) break;
       if (head[i] >= g.heads || row_at[token[i]] < 0) continue;
       float y[2 * N];
-      it[i].values(turn + token[i] * pairs, g.interleaved, y);
+      it[i].values(turn + token[i] * turn_row<N>(pairs), pairs / N, g.interleaved, y);
       S* row = cache + row_at[token[i]] + head[i] * g.cs[which][2];
       Vec<S, N> a, b;
 #pragma unroll
@@ -351,18 +390,16 @@ __device__ __forceinline__ int fitting_exponent(float x) {
 // is among the new tokens); else it only grows.  Infinities and NaN are stored as NaN, which is
 // all that e4m3 has of them, and do not count for the scale.
 // A workgroup takes the new tokens of one page and some heads of k or of v: per head their values
-// are loaded once, HOLD items a lane (what is more is loaded again), turned for their largest
-// magnitude and again to be stored.
+// are loaded, turned and held, HOLD items a lane (what is more is loaded and turned again), their largest
+// magnitude found, and stored.
 template <typename T, int N, bool UNIT, int HOLD>
-__global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
+__global__ __launch_bounds__(256, N == 8 && HOLD == 4 ? 2 : 3) void append8_kernel(AppendArgs g) {
   typedef typename elem<T>::storage S;
   typedef AppendItem<T, N, UNIT> Item;
   extern __shared__ float2 turn[];
-  __shared__ uint32_t largest[2][4];
+  __shared__ float largest[2][4];
   const AppendUnit u = append_unit(g, blockIdx.x);
   if (u.count == 0) return;
-  const int64_t page = page_of(g, u.sequence, u.position);
-  if (page < 0) return;
   const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
   const int nheads = min(g.heads - head0, g.heads_per_block);
   const int pairs = which == 0 ? g.pairs : 0;
@@ -375,70 +412,74 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
     t = g.per_row(i);
     return Item(i - t * per_row, pairs, g.interleaved);
   };
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k) held[k] = item(min(k * 256 + (int)threadIdx.x, items - 1), token[k]);
   auto load = [&](int h) {
 #pragma unroll
     for (int k = 0; k < HOLD; ++k) {
-      const int i = k * 256 + threadIdx.x;
-      if (i >= items) break;
-      held[k] = item(i, token[k]);
+      if (k * 256 + (int)threadIdx.x >= items) break;
       held[k].load(x + token[k] * g.xs[which][0] + h * g.xs[which][1], g.xs[which][2]);
     }
   };
   load(0);
-  if (pairs) {
-    append_turns(g, u, turn);
-    __syncthreads();
-  }
+  const int64_t page = page_of(g, u.sequence, u.position);
+  if (page < 0) return;
+  if (pairs) append_turns<N>(g, u, turn);
   for (int h = 0; h < nheads; ++h) {
     const S* xh = x + h * g.xs[which][1];
     uint8_t* cache = (uint8_t*)g.cache[which] + page * g.cs[which][0] + (head0 + h) * g.cs[which][2];
     float* scale_at = g.scale[which] + page * g.heads + head0 + h;
     const float old = slot0 ? *scale_at : 0.f;
+    float y[HOLD][2 * N];
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k)
+      if (k * 256 + (int)threadIdx.x < items)
+        held[k].values(turn + token[k] * turn_row<N>(pairs), pairs / N, g.interleaved, y[k]);
+    if (h + 1 < nheads) load(h + 1);  // (under way while this head's are stored)
     // f(values) for each of this lane's items.
     auto each = [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
       for (int k = 0; k < HOLD; ++k) {
         if (k * 256 + (int)threadIdx.x >= items) break;
-        float y[2 * N];
-        held[k].values(turn + token[k] * pairs, g.interleaved, y);
-        f(held[k], token[k], y);
+        f(held[k], token[k], y[k]);
       }
       for (int i = HOLD * 256 + threadIdx.x; i < items; i += 256) {
         int t;
         Item it = item(i, t);
         it.load(xh + t * g.xs[which][0], g.xs[which][2]);
-        float y[2 * N];
-        it.values(turn + t * pairs, g.interleaved, y);
-        f(it, t, y);
+        float z[2 * N];
+        it.values(turn + t * turn_row<N>(pairs), pairs / N, g.interleaved, z);
+        f(it, t, z);
       }
     };
-    // The largest magnitude's bits, in their order as integers: infinities and NaN come last.
-    uint32_t most = 0;
-    each([&](const Item&, int, const float (&y)[2 * N]) {
-#pragma unroll
-      for (int e = 0; e < 2 * N; ++e) most = max(most, __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu);
-    });
-    auto over_all = [&](uint32_t x, uint32_t (&lds)[4]) {
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, off, 64));
+    auto over_all = [&](float x, float (&lds)[4]) {
+      x = wave_max(x);
       if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
       __syncthreads();  // (also: every lane has read the old scale)
-      return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+      return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
     };
-    most = over_all(most, largest[h & 1]);
-    if (most >= 0x7f800000u) {  // seldom: the largest of the others
-      most = 0;
+    float most = 0.f;
+    bool odd = false;
+    each([&](const Item&, int, const float (&y)[2 * N]) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        most = fmaxf(most, fmaxf(fabsf(y[e]), fabsf(y[N + e])));
+        odd |= !(fabsf(y[e]) + fabsf(y[N + e]) < INFINITY);
+      }
+    });
+    // (an infinity or NaN of any lane, told by one: the max of the others is looked for again)
+    most = over_all(__builtin_amdgcn_ballot_w64(odd) ? INFINITY : most, largest[h & 1]);
+    odd = most == INFINITY;
+    if (odd) {
+      most = 0.f;
       each([&](const Item&, int, const float (&y)[2 * N]) {
 #pragma unroll
-        for (int e = 0; e < 2 * N; ++e) {
-          const uint32_t bits = __builtin_bit_cast(uint32_t, y[e]) & 0x7fffffffu;
-          most = max(most, bits < 0x7f800000u ? bits : 0u);
-        }
+        for (int e = 0; e < 2 * N; ++e) most = fabsf(y[e]) < INFINITY ? fmaxf(most, fabsf(y[e])) : most;
       });
       __syncthreads();  // (every lane has read the first answer)
       most = over_all(most, largest[h & 1]);
     }
-    const float fitting = ldexpf(1.0f, fitting_exponent(__builtin_bit_cast(float, most)));
+    const float fitting = ldexpf(1.0f, fitting_exponent(most));
     const float scale = slot0 ? fmaxf(old, fitting) : fitting, inverse = 1.0f / scale;
     if (threadIdx.x == 0) *scale_at = scale;
     if (slot0 && scale != old) {  // what the page held follows its scale
@@ -446,18 +487,23 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
       for (int i = threadIdx.x; i < slot0 * (g.dim / 4); i += 256) {
         const int t = i / (g.dim / 4), d = (i - t * (g.dim / 4)) * 4;
         uint8_t* row = cache + t * g.cs[which][1] + d;
-        float y[4];
+        float z[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_cvt_f32_fp8((int)row[e], 0) * ratio;
-        const uint32_t q = e4m3_of(y[0], y[1], y[2], y[3]);
+        for (int e = 0; e < 4; ++e) z[e] = __builtin_amdgcn_cvt_f32_fp8((int)row[e], 0) * ratio;
+        const uint32_t q = e4m3_of(z[0], z[1], z[2], z[3]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) row[e] = (uint8_t)(q >> (8 * e));
       }
     }
     each([&](const Item& it, int t, const float (&y)[2 * N]) {
       uint8_t* row = cache + (slot0 + t) * g.cs[which][1];
-      // (y * 0 is NaN for infinities too)
-      auto q = [&](int e) { return __builtin_fmaf(y[e], inverse, y[e] * 0.f); };
+      float q[2 * N];
+#pragma unroll
+      for (int e = 0; e < 2 * N; ++e) q[e] = y[e] * inverse;
+      if (odd) {
+#pragma unroll
+        for (int e = 0; e < 2 * N; ++e) q[e] = fabsf(q[e]) < INFINITY ? q[e] : NAN;
+      }
       if constexpr (UNIT) {
         Vec<uint32_t, N / 4> v[2];
 #pragma unroll
@@ -465,20 +511,19 @@ __global__ __launch_bounds__(256) void append8_kernel(AppendArgs g) {
 #pragma unroll
           for (int e = 0; e < N / 4; ++e) {
             const int i = w * N + 4 * e;
-            v[w].e[e] = e4m3_of(q(i), q(i + 1), q(i + 2), q(i + 3));
+            v[w].e[e] = e4m3_of(q[i], q[i + 1], q[i + 2], q[i + 3]);
           }
         store_vec((uint32_t*)(row + it.d0), v[0], g.past_caches);
         store_vec((uint32_t*)(row + it.d1), v[1], g.past_caches);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const uint32_t both = e4m3_of(q(e), q(N + e), 0.f, 0.f);
+          const uint32_t both = e4m3_of(q[e], q[N + e], 0.f, 0.f);
           row[it.d0 + e] = (uint8_t)both;
           row[it.d1 + e] = (uint8_t)(both >> 8);
         }
       }
     });
-    if (h + 1 < nheads) load(h + 1);
   }
 }
 
@@ -493,13 +538,13 @@ static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
     return ok;
   };
   const int n = fits(8) ? 8 : fits(4) ? 4 : 1;
-  // A unit is a page of an 8-bit cache, else 64 positions; its angles take at most 64 KiB of LDS.
+  // A unit is a page of an 8-bit cache, else 64 positions; its angles take at most 76 KiB of LDS.
   g.map.per = eight ? g.page_size : APPEND_TOKENS;
   g.map.rows = 1;
   g.map.extra = 2;
   const int64_t units = unit_count(g.map);
   // All heads of a unit share its angles where there are enough units (and k and v) for that.
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.heads, 2048 / std::max<int64_t>(1, units)));
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.heads, 768 / std::max<int64_t>(1, units)));
   const int64_t per_row = g.dim / (2 * n);
   g.heads_per_block = (int)std::min<int64_t>(cdiv(g.heads, parts), 65535 / (APPEND_TOKENS * per_row));
   const int64_t y = cdiv(g.heads, g.heads_per_block);
@@ -509,7 +554,7 @@ static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
   g.past_caches = 2 * g.map.tokens * g.heads * g.dim * (eight ? 1 : 2) >= PAST_CACHES;
   const int64_t most_tokens = std::min<int64_t>(g.map.per, g.map.tokens);
   const dim3 grid((unsigned)units, (unsigned)y, 2), block(256);
-  const size_t lds = (size_t)most_tokens * g.pairs * sizeof(float2);
+  const size_t lds = turn_bytes(most_tokens, g.pairs, n);
   if (!eight) {
     if (n == 8)
       hipLaunchKernelGGL((append_kernel<T, 8, true>), grid, block, lds, stream, g);
