@@ -19,7 +19,6 @@ struct RotaryArgs {
   float magnitude;
   int units;         // vectors of pairs of a head
   Divider per_head;  // those and the vectors that are copied
-  bool past_caches;
 };
 
 constexpr int ROTARY_PAIRS = 256;  // dim <= 512
@@ -29,13 +28,13 @@ constexpr int ROTARY_PAIRS = 256;  // dim <= 512
 // (inverse: the angle negated, which is the transpose and so the gradient).
 // Bound by HBM: x read and y written once.  A wave takes one token and some of its heads; its
 // lanes compute one angle each and pass cos and sin through LDS, so the angles cost a token, not
-// a head, and every lane then loads two 16-byte vectors (a and b of N pairs) for a rotation.
-// The loads of U items are in flight together, the first of them before the angles.
+// a head, and every lane then loads two 16-byte vectors (a and b of N pairs) for a rotation.  One
+// such item a lane at a time: four in flight together are no faster (8,192 tokens of 32 x 128 bf16 22.5 us
+// either way), as 16 waves a CU are.
 // UNIT: unit element strides and N-element aligned rows; else one pair at a time by strides.
-template <typename T, int N, bool UNIT>
+template <typename T, int N, bool UNIT, bool PAST>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
   typedef typename elem<T>::storage S;
-  constexpr int U = N > 1 ? 4 : 2;
   __shared__ float2 turn_all[4][ROTARY_PAIRS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t token = (int64_t)blockIdx.x * 4 + wave;
@@ -52,72 +51,60 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
   S* out = (S*)g.out + token * g.os[0] + head0 * g.os[1];
   const int second = g.interleaved ? N : g.pairs;  // where an item's second vector starts
 
-  Vec<S, N> a[U], b[U];
-  int head[U], first[U];
-  bool turned[U];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int item = base + i * 64 + lane;
-      if (item >= items) break;
-      head[i] = g.per_head(item);
-      const int unit = item - head[i] * (int)g.per_head.d;
-      turned[i] = unit < g.units;
-      first[i] = turned[i] ? (g.interleaved ? 2 * N * unit : N * unit) : 2 * g.pairs + (unit - g.units) * N;
-      const S* row = x + head[i] * g.xs[1];
-      if (UNIT) {
-        a[i] = *(const Vec<S, N>*)(row + first[i]);
-        if (turned[i]) b[i] = *(const Vec<S, N>*)(row + first[i] + second);
-      } else {
-        a[i].e[0] = row[first[i] * g.xs[2]];
-        if (turned[i]) b[i].e[0] = row[(first[i] + second) * g.xs[2]];
-      }
+  Vec<S, N> a, b;
+  int head, first, unit;
+  auto load = [&](int item) {
+    head = g.per_head(item);
+    unit = item - head * (int)g.per_head.d;
+    first = unit >= g.units ? 2 * g.pairs + (unit - g.units) * N : g.interleaved ? 2 * N * unit : N * unit;
+    const S* row = x + head * g.xs[1];
+    if (UNIT) {
+      a = *(const Vec<S, N>*)(row + first);
+      if (unit < g.units) b = *(const Vec<S, N>*)(row + first + second);
+    } else {
+      a.e[0] = row[first * g.xs[2]];
+      if (unit < g.units) b.e[0] = row[(first + second) * g.xs[2]];
     }
   };
-  load(0);
+  if (lane < items) load(lane);
   for (int p = lane; p < g.pairs; p += 64) {
     float2 cs = rotation((double)position, g.freqs[p], g.magnitude);
     if (g.inverse) cs.y = -cs.y;
     turn[(p % N) * g.units + p / N] = cs;  // (an item's lanes then read neighbours)
   }
   wave_lds_order();
-  for (int base = 0; base < items; base += 64 * U) {
-    if (base) load(base);
+  for (int item = lane; item < items; item += 64) {
+    if (item != lane) load(item);
+    if (unit < g.units) {
+      if (g.interleaved && N > 1) {  // a holds the first N / 2 pairs, b the others
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (base + i * 64 + lane >= items) break;
-      S* row = out + head[i] * g.os[1];
-      if (turned[i]) {
-        const float2* at = turn + (g.interleaved ? first[i] >> 1 : first[i]) / N;
-        if (g.interleaved && N > 1) {  // a holds the first N / 2 pairs, b the others
+        for (int e = 0; e < N; e += 2) {
 #pragma unroll
-          for (int e = 0; e < N; e += 2) {
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              Vec<S, N>& v = w ? b[i] : a[i];
-              const float2 cs = at[(w * (N / 2) + e / 2) * g.units];
-              const float p = elem<T>::to_float(v.e[e]), q = elem<T>::to_float(v.e[e + 1 < N ? e + 1 : e]);
-              v.e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
-              v.e[e + 1 < N ? e + 1 : e] = elem<T>::from_float(q * cs.x + p * cs.y);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float2 cs = at[e * g.units];
-            const float p = elem<T>::to_float(a[i].e[e]), q = elem<T>::to_float(b[i].e[e]);
-            a[i].e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
-            b[i].e[e] = elem<T>::from_float(q * cs.x + p * cs.y);
+          for (int w = 0; w < 2; ++w) {
+            Vec<S, N>& v = w ? b : a;
+            const float2 cs = turn[(w * (N / 2) + e / 2) * g.units + unit];
+            const float p = elem<T>::to_float(v.e[e]), q = elem<T>::to_float(v.e[e + 1 < N ? e + 1 : e]);
+            v.e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
+            v.e[e + 1 < N ? e + 1 : e] = elem<T>::from_float(q * cs.x + p * cs.y);
           }
         }
-      }
-      if (UNIT) {
-        store_vec(row + first[i], a[i], g.past_caches);
-        if (turned[i]) store_vec(row + first[i] + second, b[i], g.past_caches);
       } else {
-        row[first[i] * g.os[2]] = a[i].e[0];
-        if (turned[i]) row[(first[i] + second) * g.os[2]] = b[i].e[0];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float2 cs = turn[e * g.units + unit];
+          const float p = elem<T>::to_float(a.e[e]), q = elem<T>::to_float(b.e[e]);
+          a.e[e] = elem<T>::from_float(p * cs.x - q * cs.y);
+          b.e[e] = elem<T>::from_float(q * cs.x + p * cs.y);
+        }
       }
+    }
+    S* row = out + head * g.os[1];
+    if (UNIT) {
+      store_vec(row + first, a, PAST);
+      if (unit < g.units) store_vec(row + first + second, b, PAST);
+    } else {
+      row[first * g.os[2]] = a.e[0];
+      if (unit < g.units) row[(first + second) * g.os[2]] = b.e[0];
     }
   }
 }
@@ -138,7 +125,7 @@ static int rotary_launch(RotaryArgs g, hipStream_t stream) {
   g.units = g.pairs / n;
   const int per_head = g.units + (g.dim - 2 * g.pairs) / n;
   g.per_head = divider(per_head);
-  g.past_caches = g.tokens * g.heads * g.dim * bytes >= PAST_CACHES;
+  const bool past = g.tokens * g.heads * g.dim * bytes >= PAST_CACHES;
   // A wave takes all of a token's heads where tokens alone fill the chip, else fewer of them.
   const int64_t want = std::max<int64_t>(1, 4096 / std::max<int64_t>(1, g.tokens));
   int64_t splits = std::min<int64_t>({want, (int64_t)g.heads, std::max<int64_t>(1, (int64_t)g.heads * per_head / 64)});
@@ -149,12 +136,14 @@ static int rotary_launch(RotaryArgs g, hipStream_t stream) {
   const int64_t blocks = cdiv(g.tokens, 4), parts = cdiv(g.heads, g.heads_per_wave);
   if (blocks > 0x7fffffffLL || parts > 65535) return NT_ERR_INVALID;
   const dim3 grid((unsigned)blocks, (unsigned)parts), block(256);
-  if (n == full)
-    hipLaunchKernelGGL((rotary_kernel<T, full, true>), grid, block, 0, stream, g);
+  if (n == full && past)
+    hipLaunchKernelGGL((rotary_kernel<T, full, true, true>), grid, block, 0, stream, g);
+  else if (n == full)
+    hipLaunchKernelGGL((rotary_kernel<T, full, true, false>), grid, block, 0, stream, g);
   else if (n == full / 2)
-    hipLaunchKernelGGL((rotary_kernel<T, full / 2, true>), grid, block, 0, stream, g);
+    hipLaunchKernelGGL((rotary_kernel<T, full / 2, true, false>), grid, block, 0, stream, g);
   else
-    hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, block, 0, stream, g);
+    hipLaunchKernelGGL((rotary_kernel<T, 1, false, false>), grid, block, 0, stream, g);
   return launch_status();
 }
 
@@ -170,7 +159,6 @@ struct AppendArgs {
   int heads, dim, pairs, page_size, table_width, heads_per_block, interleaved;
   float magnitude;
   Divider per_row, per_token;  // items of a row, and of a token's heads of one workgroup
-  bool past_caches;
 };
 
 // The tokens [first, first + count) of the packed tensors that a unit takes, at the positions
@@ -301,11 +289,11 @@ struct AppendItem {
 // heads of k or of v: the angles and the places in the cache are then found once for those heads.
 // The loads of U items a lane are in flight together, the first of them before the angles.
 constexpr int APPEND_TOKENS = 64;
-template <typename T, int N, bool UNIT>
+template <typename T, int N, bool UNIT, bool PAST>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
   typedef typename elem<T>::storage S;
   typedef AppendItem<T, N, UNIT> Item;
-  constexpr int U = N == 1 ? 2 : 4;
+  constexpr int U = 2;
   extern __shared__ float2 turn[];
   __shared__ int64_t row_at[APPEND_TOKENS];  // of a token in the cache, or -1
   const AppendUnit u = append_unit(g, blockIdx.x);
@@ -356,8 +344,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
         b.e[e] = elem<T>::from_float(y[N + e]);
       }
       if (UNIT) {
-        store_vec(row + it[i].d0, a, g.past_caches);
-        store_vec(row + it[i].d1, b, g.past_caches);
+        store_vec(row + it[i].d0, a, PAST);
+        store_vec(row + it[i].d1, b, PAST);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -513,8 +501,8 @@ __global__ __launch_bounds__(256, N == 8 && HOLD == 4 ? 2 : 3) void append8_kern
             const int i = w * N + 4 * e;
             v[w].e[e] = e4m3_of(q[i], q[i + 1], q[i + 2], q[i + 3]);
           }
-        store_vec((uint32_t*)(row + it.d0), v[0], g.past_caches);
-        store_vec((uint32_t*)(row + it.d1), v[1], g.past_caches);
+        *(Vec<uint32_t, N / 4>*)(row + it.d0) = v[0];
+        *(Vec<uint32_t, N / 4>*)(row + it.d1) = v[1];
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -543,7 +531,9 @@ static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
   g.map.rows = 1;
   g.map.extra = 2;
   const int64_t units = unit_count(g.map);
-  // All heads of a unit share its angles where there are enough units (and k and v) for that.
+  // All heads of a unit share its angles where there are enough units (and k and v) for that: 768 workgroups
+  // a tensor (us at 512 / 768 / 1,024 / 2,048 / 4,096: 17,637 tokens in 8 bits 36.1 / 34.3 / 41.8 / 45 / 52,
+  // 4,636 of 32 x 64 in 16 bits 19.3 / 19.0 / 22.5 / 23.8 / 32).
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.heads, 768 / std::max<int64_t>(1, units)));
   const int64_t per_row = g.dim / (2 * n);
   g.heads_per_block = (int)std::min<int64_t>(cdiv(g.heads, parts), 65535 / (APPEND_TOKENS * per_row));
@@ -551,30 +541,34 @@ static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
   if (units > 0x7fffffffLL || y > 65535) return NT_ERR_INVALID;
   g.per_row = divider(per_row);
   g.per_token = divider(per_row * g.heads_per_block);
-  g.past_caches = 2 * g.map.tokens * g.heads * g.dim * (eight ? 1 : 2) >= PAST_CACHES;
+  const bool past = 4 * g.map.tokens * g.heads * g.dim >= PAST_CACHES;
   const int64_t most_tokens = std::min<int64_t>(g.map.per, g.map.tokens);
   const dim3 grid((unsigned)units, (unsigned)y, 2), block(256);
   const size_t lds = turn_bytes(most_tokens, g.pairs, n);
+#define NT_APPEND(...) hipLaunchKernelGGL((__VA_ARGS__), grid, block, lds, stream, g)
   if (!eight) {
-    if (n == 8)
-      hipLaunchKernelGGL((append_kernel<T, 8, true>), grid, block, lds, stream, g);
+    if (n == 8 && past)
+      NT_APPEND(append_kernel<T, 8, true, true>);
+    else if (n == 8)
+      NT_APPEND(append_kernel<T, 8, true, false>);
     else if (n == 4)
-      hipLaunchKernelGGL((append_kernel<T, 4, true>), grid, block, lds, stream, g);
+      NT_APPEND(append_kernel<T, 4, true, false>);
     else
-      hipLaunchKernelGGL((append_kernel<T, 1, false>), grid, block, lds, stream, g);
+      NT_APPEND(append_kernel<T, 1, false, false>);
   } else if (n == 8) {
     const int64_t items = cdiv(most_tokens * per_row, 256);  // of a lane
     if (items <= 1)
-      hipLaunchKernelGGL((append8_kernel<T, 8, true, 1>), grid, block, lds, stream, g);
+      NT_APPEND(append8_kernel<T, 8, true, 1>);
     else if (items <= 2)
-      hipLaunchKernelGGL((append8_kernel<T, 8, true, 2>), grid, block, lds, stream, g);
+      NT_APPEND(append8_kernel<T, 8, true, 2>);
     else
-      hipLaunchKernelGGL((append8_kernel<T, 8, true, 4>), grid, block, lds, stream, g);
+      NT_APPEND(append8_kernel<T, 8, true, 4>);
   } else if (n == 4) {
-    hipLaunchKernelGGL((append8_kernel<T, 4, true, 4>), grid, block, lds, stream, g);
+    NT_APPEND(append8_kernel<T, 4, true, 4>);
   } else {
-    hipLaunchKernelGGL((append8_kernel<T, 1, false, 4>), grid, block, lds, stream, g);
+    NT_APPEND(append8_kernel<T, 1, false, 4>);
   }
+#undef NT_APPEND
   return launch_status();
 }
 
