@@ -198,7 +198,11 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = g.dim;
 
-  const int h = blockIdx.x % g.kv_heads, part = blockIdx.x / g.kv_heads;
+  // Two heads' rows of 64 bytes share a line of the L2: neighbours go to one XCD (ids go to the 8 of them in
+  // turn), the two eight ids apart; 16 x 4,000 keys of 16 x 64 so take 43 us instead of 52.
+  int wg = blockIdx.x;
+  if (G::ROW == 64 && (wg | 15) < (int)gridDim.x) wg = (wg & ~15) | (wg & 7) << 1 | (wg >> 3 & 1);
+  const int h = wg % g.kv_heads, part = wg / g.kv_heads;
   int share = 0;
   const LinePlace place = line_place(g, -1, line_lds, [&](int length) {
     share = (length + g.parts - 1) / g.parts;
@@ -214,11 +218,14 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
   const uint32_t ring_w = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring + wave * G::RING;
   const char* ring_p = ring + wave * G::RING;
   const int kst = (int)(g.ks[1] * ES), vst = (int)(g.vs[1] * ES);
-  int kv_key[G::LOADS], kv_byte[G::LOADS];
+  const uint32_t page_k = (uint32_t)(g.ks[0] * ES), page_v = (uint32_t)(g.vs[0] * ES);  // (SIXTEENS: 32 bits)
+  int kv_key[G::LOADS], kv_byte[G::LOADS], k_off[G::LOADS], v_off[G::LOADS];
 #pragma unroll
   for (int u = 0; u < G::LOADS; ++u) {
     kv_key[u] = u * G::KEYS + lane / G::CHUNKS;
     kv_byte[u] = ((lane % G::CHUNKS) ^ G::swizzle(kv_key[u])) * 16;
+    k_off[u] = kv_byte[u] < D * ES ? (kv_key[u] & 15) * kst + kv_byte[u] : 0x7fffffff;
+    v_off[u] = kv_byte[u] < D * ES ? (kv_key[u] & 15) * vst + kv_byte[u] : 0x7fffffff;
   }
   auto k_frag = [&](int stage, int kb, int u) {
     const int key = kb * 16 + col, chunk = u * 4 + quad;
@@ -251,19 +258,17 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
       vs = fmaxf(vs, LEAST_SCALE);
       return Scales{ks * g.scale_log2, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
     };
-    auto page_number = [&](int sixteen) {  // of 16 keys; -1: none
-      const int n = g.page_shift >= 0 ? sixteen >> g.page_shift : sixteen / (g.page_size >> 4);
-      const int32_t page = n < g.table_width ? table[n] : -1;
-      return page >= 0 && page < g.pages ? page : -1;
-    };
-    // SIXTEENS: the pages of the tiles that come next (looked up ahead), and the scales of those
-    // under way.
+    // SIXTEENS: the pages of the tile that comes next (looked up ahead), and of those under way their
+    // scales and what a page adds to its exponents: nothing, or where there is none minus infinity.
     int next_page[2];
-    float k_sc[G::STAGES][2], v_sc[G::STAGES][2];
-    bool real[G::STAGES][2];
+    float k_sc[G::STAGES][2], v_sc[G::STAGES][2], add[G::STAGES][2];
     auto look = [&](int j) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) next_page[kb] = j < nt ? page_number(2 * (t0 + j * NW) + kb) : -1;
+      for (int kb = 0; kb < 2; ++kb) {
+        const int sixteen = 2 * (t0 + j * NW) + kb;
+        const int n = g.page_shift >= 0 ? sixteen >> g.page_shift : sixteen / (g.page_size >> 4);
+        next_page[kb] = j < nt && n < g.table_width ? table[n] : -1;
+      }
     };
     auto issue = [&](int j, int stage) {
       const int k0 = (t0 + j * NW) * BN;
@@ -272,28 +277,27 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
         u32x4 rk[2], rv[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const int first = k0 + kb * 16, n = min(16, len - first);
-          const bool ok = next_page[kb] >= 0 && n > 0;
-          const int64_t page = ok ? next_page[kb] : 0;
-          const int slot = first - (g.page_shift >= 0 ? (first >> (g.page_shift + 4)) << (g.page_shift + 4)
-                                                      : first / g.page_size * g.page_size);
+          const int first = k0 + kb * 16;
+          const bool ok = (uint32_t)next_page[kb] < (uint32_t)g.pages;  // (SIXTEENS: 32 bits)
+          const uint32_t page = ok ? next_page[kb] : 0;
+          const int slot = g.page_shift >= 0 ? first & (g.page_size - 1) : first % g.page_size;
           // (a buffer ends with the last key: what lies past it, or in no page, reads as zeros)
-          rk[kb] = buffer_of(kbase + (page * g.ks[0] + slot * g.ks[1]) * ES, ok ? (n - 1) * kst + D * ES : 0);
-          rv[kb] = buffer_of(vbase + (page * g.vs[0] + slot * g.vs[1]) * ES, ok ? (n - 1) * vst + D * ES : 0);
-          real[stage][kb] = ok;
+          const int n = ok ? min(16, len - first) : 0;
+          rk[kb] = buffer_of(kbase + ((uint64_t)page * page_k + (uint32_t)(slot * kst)), n > 0 ? (n - 1) * kst + D * ES : 0);
+          rv[kb] = buffer_of(vbase + ((uint64_t)page * page_v + (uint32_t)(slot * vst)), n > 0 ? (n - 1) * vst + D * ES : 0);
+          add[stage][kb] = ok ? 0.f : -INFINITY;
           if (EIGHT) {
-            k_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.k_scale)[page * g.kv_heads + h];
-            v_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.v_scale)[page * g.kv_heads + h];
+            const float ks = ((ScalarFloats)(uintptr_t)g.k_scale)[page * (uint32_t)g.kv_heads + h];
+            k_sc[stage][kb] = ok ? ks : 0.f;
+            v_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.v_scale)[page * (uint32_t)g.kv_heads + h];
           }
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int u = 0; u < G::LOADS; ++u) {
-            const int kb = u * G::KEYS / 16, st = w ? vst : kst;
-            const int off = kv_byte[u] < D * ES ? (kv_key[u] - kb * 16) * st + kv_byte[u] : 0x7fffffff;
-            buffer_to_lds(w ? rv[kb] : rk[kb], to + w * G::TILE + u * 1024, off, 0);
-          }
+          for (int u = 0; u < G::LOADS; ++u)
+            buffer_to_lds(w ? rv[u * G::KEYS / 16] : rk[u * G::KEYS / 16], to + w * G::TILE + u * 1024,
+                          w ? v_off[u] : k_off[u], 0);
         look(j + 1);
       } else {
         // Lane i looks up key i % 32; then each lane takes what its loads need.  (Keys past the end
@@ -348,6 +352,10 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
         qf[s] = __builtin_bit_cast(typename MQ::frag, w);
       }
     }
+    // The queries are there from here on: in the loop the compiler would wait for them at every tile, and so
+    // for the loads that it does not count.
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) asm volatile("" : "+v"(qf[s]));
     floatx4 acc[DL];
 #pragma unroll
     for (int c = 0; c < DL; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -377,37 +385,34 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
       }
       float y[8], rv[8];
       Scales sc[2];
-      if (SIXTEENS && EIGHT) {
+      if (SIXTEENS) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          sc[kb] = real[stage][kb] ? scales(k_sc[stage][kb], v_sc[stage][kb]) : Scales{0.f, 0.f, 1.0f};
+        for (int kb = 0; kb < 2; ++kb) {
+          sc[kb] = EIGHT ? scales(k_sc[stage][kb], v_sc[stage][kb]) : Scales{g.scale_log2, 0.f, 1.0f};
+          sc[kb].lv += add[stage][kb];
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int kb = e >> 2, key = kb * 16 + quad * 4 + (e & 3);
         if (SIXTEENS) {
-          y[e] = EIGHT ? __builtin_fmaf(s[kb][e & 3], sc[kb].kf, sc[kb].lv) : s[kb][e & 3] * g.scale_log2;
-          rv[e] = EIGHT ? sc[kb].rv : 1.0f;
+          y[e] = __builtin_fmaf(s[kb][e & 3], sc[kb].kf, sc[kb].lv);
+          rv[e] = sc[kb].rv;
         } else {
-          y[e] = __builtin_fmaf(s[kb][e & 3], key_scale[wave][stage][0][key & (NKEYS - 1)],
-                                key_scale[wave][stage][1][key & (NKEYS - 1)]);
+          const float lv = key_scale[wave][stage][1][key & (NKEYS - 1)];
+          y[e] = __builtin_fmaf(s[kb][e & 3], key_scale[wave][stage][0][key & (NKEYS - 1)], lv);
+          y[e] = lv == -INFINITY ? -INFINITY : y[e];
           rv[e] = key_scale[wave][stage][2][key & (NKEYS - 1)];
         }
       }
-      const bool cut = k0 + BN > len || (SIXTEENS && !(real[stage][0] && real[stage][1]));
-      if (cut) {
+      if (k0 + BN > len) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (k0 + (e >> 2) * 16 + quad * 4 + (e & 3) >= len || (SIXTEENS && !real[stage][e >> 2])) y[e] = -INFINITY;
+          if (k0 + (e >> 2) * 16 + quad * 4 + (e & 3) >= len) y[e] = -INFINITY;
       }
-      if (!SIXTEENS) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (key_scale[wave][stage][1][((e >> 2) * 16 + quad * 4 + (e & 3)) & (NKEYS - 1)] == -INFINITY) y[e] = -INFINITY;
-      }
-      float mx = y[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, y[e]);
+      float mx = max3(y[0], y[1], y[2]);
+      mx = max3(mx, y[3], y[4]);
+      mx = max3(mx, y[5], fmaxf(y[6], y[7]));
       if (__builtin_amdgcn_ballot_w64(mx > m + RESCALE_LOG2)) {
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -502,7 +507,7 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
     }
     __syncthreads();
     const bool whole = blk0 == 0 && blk1 == nblk;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (at == begin ? 0 : 1);
+    const int64_t slot = 2 * (int64_t)wg + (at == begin ? 0 : 1);
     for (int e = tid; e < rows * DM; e += NW * 64) {
       const int r = e / DM, d = e % DM;
       float mm = merge_ml[0][0][r];
@@ -652,7 +657,10 @@ static int64_t cache_parts(int64_t kv_heads, int64_t blocks, bool eight, bool wi
 template <typename T, bool EIGHT, int DM>
 static void cache_launch(const CacheArgs& g, int64_t join_grid, hipStream_t stream) {
   const dim3 grid((unsigned)(g.parts * g.kv_heads)), block(ca::NW * 64);
-  if (g.page_size % 16 == 0)
+  // (in whole sixteens a page's place and its slots are reckoned in 32 bits)
+  const int64_t es = EIGHT ? 1 : 2;
+  auto small = [&](const int64_t* s) { return s[0] >= 0 && s[0] * es <= 0xffffffffLL && s[1] * es * g.page_size <= 0x7fffffffLL; };
+  if (g.page_size % 16 == 0 && small(g.ks) && small(g.vs) && g.pages <= 0x7fffffffLL && g.pages * g.kv_heads <= 0x7fffffffLL)
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, true>), grid, block, 0, stream, g);
   else
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, false>), grid, block, 0, stream, g);

@@ -84,6 +84,12 @@ struct Packed {
   P* ptr() { return (P*)(uintptr_t)*v++; }
 };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // Buffer resource of `bytes` bytes from `base` on (uniform: in scalar registers): reads past its
 // end give zeros.
 __device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {

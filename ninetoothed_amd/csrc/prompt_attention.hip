@@ -47,11 +47,6 @@ constexpr uint32_t inf_bits = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
 template <typename T>
 constexpr uint32_t one_bits = std::is_same<T, f16_t>::value ? 0x3c00u : 0x3f80u;
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
 // x of lane l ^ 32, and the larger of the two.  (v_permlane32_swap of two copies of x leaves the
 // low half's values in the first and the high half's in the second, in both halves; the VALU
 // write of its operands needs wait states before it.)
