@@ -682,7 +682,8 @@ static int64_t cache_plan(int64_t sequences, int64_t heads, int64_t kv_heads, in
 extern "C" int64_t nt_cache_attention_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
                                                      int64_t page_size, int64_t table_width, int cache_dtype) {
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim > 128 || page_size <= 0 ||
-      table_width <= 0)
+      table_width <= 0 || sequences > (1 << 24) || heads > (1 << 20) || page_size > 0x7fffff00LL ||
+      table_width > 0x7fffff00LL)
     return 0;
   int64_t parts;
   return 4 * cache_plan(sequences, heads, kv_heads, dim, page_size, table_width, cache_dtype, parts);
@@ -702,7 +703,7 @@ extern "C" int nt_cache_attention(const void* q, const int64_t* q_strides, const
       table_width > 0x7fffff00LL || page_size * table_width > 0x7fffff00LL)
     return NT_ERR_INVALID;
   if ((dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || (!eight && cache_dtype != dtype)) return NT_ERR_INVALID;
-  if (sequences * heads * dim == 0) return 0;
+  if (!sequences || !heads || !dim) return 0;
   if (kv_heads == 0 || heads % kv_heads) return NT_ERR_INVALID;
   if (pages == 0) table_width = 0;  // no keys: every output is zero
   if (!q || !o || !q_strides || !k_strides || !v_strides || !o_strides || !lengths) return NT_ERR_INVALID;

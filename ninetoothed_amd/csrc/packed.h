@@ -6,8 +6,6 @@
 
 namespace nt {
 
-constexpr float E4M3_MAX = 448.0f;
-
 // Work over packed sequences is dealt out in units of `per` rows (a row: a token, or a token's
 // share of a group of heads) that no two sequences share.  How many there are is known on the
 // device only, so sequence b's units get the numbers from first_unit(b) on, with
@@ -134,7 +132,7 @@ __device__ __forceinline__ void store_vec(S* p, const Vec<S, N>& v, bool past) {
 }
 // Bytes written from which 16-byte stores go past the caches (us without / with: a rotation of 67 MB
 // 34.5 / 22.6, of 13 MB 10.2 / 8.4, an append of 38 MB 21.0 / 19.0; 8-byte stores gain nothing).
-constexpr int64_t PAST_CACHES = 8 << 20;  // bytes written from which stores go past the caches
+constexpr int64_t PAST_CACHES = 8 << 20;
 
 // n / d for 0 <= n < 2^16 and 0 < d <= 2^15: floor(n ceil(2^32 / d) / 2^32), off by less than n / 2^32.
 struct Divider {

@@ -192,22 +192,6 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& g) {
   return {two(p.q_begin), two(p.k_begin), one(p.head), one(p.r0), one(p.rows), one(p.Sq), one(p.Sk), one(p.split)};
 }
 
-// Per row i of a sequence (a token and a head of its group) over the keys j it may see:
-//   s_ij = scale q_i . k_j,  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i);
-// causal: j <= i + (keys - queries).  A row that sees no key gives zeros.
-// MFMA-bound: 4 dim flops a head and visible pair.  A workgroup takes 256 rows, a group's heads
-// side by side for each token, so that short sequences fill its rows and share K and V; eight waves
-// of 32 rows, two a SIMD.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: a lane holds
-// one row, its max and sum take no LDS, and P^T goes from the score registers to the second product
-// as it is.
-//   - Scores stay unscaled in fp32 until exp2(s scale - m): q is not rounded a second time.
-//   - m is the max of a row's first tile, raised only where a later tile's weights grow past what
-//     MOST_SUM (or RESCALE_LOG2) allows (o and l are rescaled then): p keeps its relative precision, and
-//     o / l is the same.  Most tiles so take no max.
-//   - p is rounded to the operands' type for the product; its row sums are of the rounded p.
-//   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
-//     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: rows of a
-//     tile that is masked and holds one are taken key by key, each over the keys that it sees.
 // What a row's state ends as: the output, or a split's partial state.
 template <typename T>
 struct PromptRow {
@@ -277,9 +261,25 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
   if (!whole && d0 == 0) *(float2*)out.ml = float2{m, l};
 }
 
-// Unit element strides and 16-byte aligned rows.  K and V stream by direct loads into LDS stages of 64
-// keys each: four of them, two tiles under way while two are worked on, or with NW = 4 (for few rows) two,
-// one under way beside one, so that two workgroups share a CU.
+// Per row i of a sequence (a token and a head of its group) over the keys j it may see:
+//   s_ij = scale q_i . k_j,  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i);
+// causal: j <= i + (keys - queries).  A row that sees no key gives zeros.
+// MFMA-bound: 4 dim flops a head and visible pair.  A workgroup takes 256 rows, a group's heads
+// side by side for each token, so that short sequences fill its rows and share K and V; eight waves
+// of 32 rows, two a SIMD.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: a lane holds
+// one row, its max and sum take no LDS, and P^T goes from the score registers to the second product
+// as it is.
+//   - Scores stay unscaled in fp32 until exp2(s scale - m): q is not rounded a second time.
+//   - m is the max of a row's first tile, raised only where a later tile's weights grow past what
+//     MOST_SUM (or RESCALE_LOG2) allows (o and l are rescaled then): p keeps its relative precision, and
+//     o / l is the same.  Most tiles so take no max.
+//   - p is rounded to the operands' type for the product; its row sums are of the rounded p.
+//   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
+//     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: rows of a
+//     tile that is masked and holds one are taken key by key, each over the keys that it sees.
+// This kernel: unit element strides and 16-byte aligned rows.  K and V stream by direct loads into LDS
+// stages of 64 keys each: four of them, two tiles under way while two are worked on, or with NW = 4 (for
+// few rows) two, one under way beside one, so that two workgroups share a CU.
 // LDS: K [key][DM] in 16-byte chunks XORed by key, so that the 16 keys of a fragment read fall on 16
 // distinct bank groups; V [key][DM] in 64-byte chunks XORed by key, for the 4 keys of a transposing read.
 template <typename T, int DM, int NW>
@@ -358,7 +358,7 @@ prompt_stream_kernel(PromptArgs g) {
   issue_v(0);
   if (STEPS == 2) issue_v(1);
 
-  const float c = fabsf(g.scale_log2);
+  const float c = fmaxf(fabsf(g.scale_log2), 1.2e-38f);  // (of a scale of 0 times minus infinity would be NaN)
   const uint32_t flip = g.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes to q's signs)
   frag qf[DSUB];
   {
@@ -990,9 +990,10 @@ extern "C" int nt_prompt_attention(const void* q, const int64_t* q_strides, cons
                                    float scale, int causal, hipStream_t stream, void* workspace,
                                    int64_t workspace_bytes) {
   if (q_tokens < 0 || k_tokens < 0 || sequences < 0 || heads < 0 || kv_heads < 0 || dim < 0 || dim > 128 ||
-      (dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || k_tokens > 0x7fffff00LL || sequences > (1 << 30))
+      (dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || k_tokens > 0x7fffff00LL || q_tokens > 0x7fffff00LL ||
+      heads > (1 << 20) || sequences > (1 << 30))
     return NT_ERR_INVALID;
-  if (q_tokens * sequences * heads * dim == 0) return 0;
+  if (!q_tokens || !sequences || !heads || !dim) return 0;
   if (kv_heads == 0 || heads % kv_heads || q_tokens * (heads / kv_heads) > 0x7fffff00LL) return NT_ERR_INVALID;
   if (!q || !o || !q_strides || !o_strides || !q_starts || !k_starts || !k_strides || !v_strides) return NT_ERR_INVALID;
   if (k_tokens > 0 && (!k || !v)) return NT_ERR_INVALID;
@@ -1024,7 +1025,7 @@ extern "C" int nt_prompt_attention(const void* q, const int64_t* q_strides, cons
 extern "C" int64_t nt_prompt_attention_workspace_size(int64_t q_tokens, int64_t k_tokens, int64_t sequences,
                                                       int64_t heads, int64_t kv_heads, int64_t dim) {
   if (q_tokens <= 0 || k_tokens < 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 ||
-      dim > 128)
+      dim > 128 || q_tokens > 0x7fffff00LL || heads > (1 << 20) || sequences > (1 << 30))
     return 0;
   const int splits = nt::prompt_plan(q_tokens, k_tokens, sequences, kv_heads, heads / kv_heads).splits;
   return splits > 1 ? q_tokens * heads * splits * (dim + 2) * 4 : 0;

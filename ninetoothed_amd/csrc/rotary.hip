@@ -578,10 +578,10 @@ extern "C" int nt_rotary(const void* x, const int64_t* x_strides, void* out, con
                          const void* positions, int64_t position_stride, int position_bits, const double* freqs,
                          int64_t tokens, int64_t heads, int64_t dim, int64_t pairs, int interleaved, int inverse,
                          float magnitude, hipStream_t stream) {
-  if (tokens < 0 || heads < 0 || dim < 0 || pairs < 0 || dim > 2 * nt::ROTARY_PAIRS || 2 * pairs > dim ||
-      heads > (1 << 20) || !nt::valid_dtype(dtype) || (position_bits != 32 && position_bits != 64))
+  if (tokens < 0 || tokens > (1LL << 33) || heads < 0 || dim < 0 || pairs < 0 || dim > 2 * nt::ROTARY_PAIRS ||
+      2 * pairs > dim || heads > (1 << 20) || !nt::valid_dtype(dtype) || (position_bits != 32 && position_bits != 64))
     return NT_ERR_INVALID;
-  if (tokens * heads * dim == 0) return 0;
+  if (tokens == 0 || heads == 0 || dim == 0) return 0;
   if (!x || !out || !x_strides || !out_strides || !positions || (pairs && !freqs)) return NT_ERR_INVALID;
   nt::RotaryArgs g{};
   g.x = x;
@@ -619,7 +619,7 @@ extern "C" int nt_cache_append(const void* k, const int64_t* k_strides, const vo
       page_size > (eight ? 128 : (1 << 30)) || table_width > (1 << 30))
     return NT_ERR_INVALID;
   if ((dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || (!eight && cache_dtype != dtype)) return NT_ERR_INVALID;
-  if (tokens * sequences * heads * dim * pages * table_width == 0) return 0;
+  if (!tokens || !sequences || !heads || !dim || !pages || !table_width) return 0;
   if (!k || !v || !k_strides || !v_strides || !k_cache || !v_cache || !kc_strides || !vc_strides || !tables || !lengths ||
       !starts || (pairs && !freqs) || (eight && (!k_scale || !v_scale)))
     return NT_ERR_INVALID;

@@ -563,6 +563,7 @@ def attention(q, k, v, o, causal=False, q_scale=LOG2E, config=0):
 # metadata, as a Handle does, so a serving loop may call it directly.
 _POINTER, _STREAM = object(), object()
 _bound_launchers = {}
+_PLAIN_OPTIONS = frozenset((bool, int, float, type(None)))
 _MAX_BOUND = 4096  # (prompts come in ever new lengths: the launchers are dropped when there are so many)
 
 
@@ -615,7 +616,7 @@ def _bind_packed(name, device, arguments):
 def _launch_bound(bind, tensors, options):
     """Launch ``bind(*tensors, *options)`` on ``tensors``, bound once per metadata and options."""
     key = None
-    if _fastkey is not None:
+    if _fastkey is not None and _PLAIN_OPTIONS.issuperset(map(type, options)):
         try:
             given = _fastkey.key(tuple([t for t in tensors if t is not None]))
             if given is not None:
@@ -624,7 +625,7 @@ def _launch_bound(bind, tensors, options):
                 if launch is not None:
                     launch(*tensors)
                     return
-        except TypeError:  # an unhashable option: the checks report it
+        except TypeError:  # not a tensor: the checks report it
             key = None
     launch = bind(*tensors, *options)
     launch(*tensors)
@@ -819,7 +820,8 @@ def bind_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=N
     number it has in the cache already; the caller counts on), which is slot position % page_size of
     page tables[b, position // page_size].  k is rotated by its position on the way (``freqs`` None:
     not at all), as :func:`bind_rotary` rotates.  Tokens past a table's width or of a page number the
-    cache does not have are not stored; a page may be written for one sequence only.
+    cache does not have are not stored; a page may be written for one sequence only, and the two caches
+    must not overlap.
 
     Caches of ``torch.float8_e4m3fn`` hold x / scale with a scale for each page and head (k_scale,
     v_scale [pages, heads], fp32): the least power of two that fits the page's largest value to 448,
@@ -863,8 +865,8 @@ def check_prompt_attention(q, k, v, out, q_starts, k_starts, causal=True, scale=
     if k.shape[2] != q.shape[2] or not 0 < q.shape[2] <= 128:
         raise ValueError("prompt_attention head dims must be one and <= 128")
     _check_heads(q.shape[1], k.shape[1])
-    if q.shape[0] * (q.shape[1] // k.shape[1]) > 0x7FFFFF00 or k.shape[0] > 0x7FFFFF00:
-        raise ValueError("prompt_attention takes less than 2^31 rows")
+    if q.shape[0] * (q.shape[1] // k.shape[1]) > 0x7FFFFF00 or k.shape[0] > 0x7FFFFF00 or q.shape[1] > 1 << 20:
+        raise ValueError("prompt_attention takes less than 2^31 rows, of at most 2^20 heads")
     _check_starts(q_starts, "q_starts")
     _check_starts(k_starts, "k_starts", q_starts.shape[0] - 1)
     _check_written(out, "out")
@@ -883,8 +885,8 @@ def bind_prompt_attention(q, k, v, out, q_starts, k_starts, causal=True, scale=N
     i + (keys - queries), so that the last query sees them all.  ``scale`` defaults to
     dim ** -0.5.  Scores, softmax and sums are in fp32, the weights rounded to the inputs' type for the
     product with v.  A query without keys gives zeros; rows behind the last sequence are left alone.
-    A call of few rows over many keys takes a workspace from torch's allocator, and goes without where
-    that has none."""
+    ``out`` must not overlap the inputs.  A call of few rows over many keys takes a workspace from torch's
+    allocator, and goes without where that has none."""
     code = check_prompt_attention(q, k, v, out, q_starts, k_starts, causal, scale)
     device = _check_device(q, k, v, out, q_starts, k_starts)
     sizes = (q.shape[0], k.shape[0], q_starts.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2])
@@ -938,7 +940,8 @@ def bind_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=None
     times their scales (any that are not negative).  Scores, softmax and sums are in fp32; the weights are
     rounded to the cache's type (to fp16 for 8-bit caches) for the product with v.  Lengths past a table's
     pages are cut, page numbers the cache does not have hold no keys, and without keys the output is zero.
-    A call takes a workspace for keys that are split over workgroups from torch's allocator."""
+    ``out`` must not overlap the inputs.  A call takes a workspace for keys that are split over
+    workgroups from torch's allocator."""
     cache_code = check_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale, v_scale, scale)
     device = _check_device(q, k_cache, v_cache, tables, lengths, out, k_scale, v_scale)
     import torch

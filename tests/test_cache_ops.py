@@ -194,6 +194,11 @@ def test_entry_points_reject_before_they_launch():
     assert _step(lib, seqs=0, q=None) == 0
     for name in ("rotary", "cache_append", "prompt_attention", "cache_attention"):
         assert getattr(lib, f"nt_{name}_packed")(None) == INVALID
+    # sizes whose product passes 64 bits are no empty call (2^16 tokens of 2^8 sequences, ..., 2^64 in all)
+    big = dict(tokens=1 << 16, seqs=1 << 8, heads=1 << 3, dim=1 << 7, pages=1 << 20, width=1 << 10, k=None)
+    assert _append(lib, **big) == INVALID
+    assert _prompt(lib, tokens=1 << 30, seqs=1 << 20, heads=1 << 8, kv=1 << 8, dim=1 << 6, q=None) == INVALID
+    assert _rotary(lib, tokens=1 << 33, heads=1 << 20, dim=1 << 9, x=None) == INVALID
 
 
 def test_workspace_size():

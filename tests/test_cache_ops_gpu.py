@@ -17,7 +17,7 @@ import math
 import pytest
 import torch
 
-from ninetoothed_amd import kernels
+from ninetoothed_amd import _lib, kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -246,6 +246,7 @@ def run_append(lengths, cached, page, heads, dim, part, dtype, cache, layout="sl
     ([1] * 70, [7 * i for i in range(70)], 16, 2, 64, 64),
     ([1, 0, 300, 17, 0, 64, 1], [5, 9, 0, 130, 0, 64, 63], 64, 4, 128, 128),
     ([130, 257], [3, 0], 128, 3, 128, 64),
+    ([300], [70], 128, 2, 128, 128),
     ([33, 5, 12], [0, 31, 17], 5, 2, 80, 40),
     ([3, 4, 9], [0, 2, 1], 1, 2, 48, 22),
     ([40, 700], [0, 100], 24, 8, 96, 96),
@@ -259,6 +260,62 @@ def test_append(lengths, cached, page, heads, dim, part, dtype, cache):
 @pytest.mark.parametrize("layout", ("heads", "joint"))
 def test_append_layouts(layout, cache):
     run_append([50, 1, 90], [0, 40, 11], 32, 4, 64, 64, BF16, cache, layout=layout, fused=True)
+
+
+@pytest.mark.parametrize("cache", (BF16, E4M3))
+def test_append_many_sequences(cache):
+    g = torch.Generator().manual_seed(7)
+    lengths, cached = (torch.randint(0, 90, (150,), generator=g).tolist() for _ in range(2))
+    run_append(lengths, cached, 32, 2, 64, 64, BF16, cache)
+
+
+@pytest.mark.parametrize("cache", (BF16, E4M3))
+def test_append_pages_past_32_bits(cache):
+    # pages whose slots lie past 2^32 elements, in a cache of 2^33 and in one with pages far apart
+    page, heads, dim, far = 64, 8, 128, 1 << 31
+    for pages, stride in ((1 << 17, page * heads * dim), (5, far)):
+        kc, vc = (torch.empty((pages - 1) * stride + page * heads * dim, dtype=cache, device=DEV).as_strided(
+            (pages, page, heads, dim), (stride, heads * dim, dim, 1)) for _ in range(2))
+        used = [pages - 1, 1, pages - 2, pages // 2]
+        tables, lengths, cached = i32([used[:2], used[2:]]), [100, 20], [5, 60]
+        few = i32([[3, 1], [2, 0]])
+        near = caches((4, page, heads, dim), cache)
+        for c, n in zip((kc, vc), near):
+            for i, p in enumerate((used[3], 1, used[2], used[0])):
+                c[p].copy_(n[i])
+        k, v = randn(120, heads, dim, dtype=BF16), randn(120, heads, dim, dtype=BF16, seed=1)
+        scales = [[None] * 2] * 2
+        if cache == E4M3:
+            scales = [[torch.full((n, heads), 2.0**-6, device=DEV) for _ in range(2)] for n in (pages, 4)]
+        starts, freqs = starts_of(lengths), kernels.rotary_frequencies(dim)
+        kernels.cache_append(k, v, kc, vc, tables, i32(cached), starts, *scales[0], freqs=freqs)
+        kernels.cache_append(k, v, *near, few, i32(cached), starts, *scales[1], freqs=freqs)
+        for c, n in zip((kc, vc), near):
+            for i, p in enumerate((used[3], 1, used[2], used[0])):
+                assert torch.equal(c[p].contiguous().view(torch.uint8), n[i].view(torch.uint8)), (pages, i)
+        # and read again from there
+        q, total = randn(2, 16, dim, dtype=BF16), i32([105, 80])
+        got = kernels.cache_attention(q, kc, vc, tables, total, torch.empty_like(q), *scales[0])
+        want = kernels.cache_attention(q, *near, few, total, torch.empty_like(q), *scales[1])
+        assert torch.equal(got, want) and want.isfinite().all()
+
+
+def test_rows_past_32_bits():
+    # tokens far apart: the last ones' rows lie past 2^32 elements
+    n, heads, dim, stride = 70, 2, 64, 1 << 26
+    far = [torch.empty((n - 1) * stride + heads * dim, dtype=BF16, device=DEV).as_strided((n, heads, dim), (stride, dim, 1))
+           for _ in range(2)]
+    x, y = randn(n, heads, dim, dtype=BF16), randn(n, heads, dim, dtype=BF16, seed=1)
+    far[0].copy_(x)
+    positions, freqs, starts = torch.arange(n, device=DEV), kernels.rotary_frequencies(dim), i32([0, 3, n])
+    want, size = turned(x, positions, freqs, False)
+    kernels.rotary(far[0], positions, freqs, far[1])
+    close(far[1].contiguous(), want, rotary_tol(want, size, BF16))
+    far[1].copy_(y)
+    out = kernels.prompt_attention(x, far[0], far[1], torch.empty_like(x), starts, starts)
+    check_prompt(x, x, y, out, [3, n - 3], [3, n - 3], True)
+    kernels.prompt_attention(far[0], x, y, far[1], starts, starts)
+    check_prompt(x, x, y, far[1].contiguous(), [3, n - 3], [3, n - 3], True)
 
 
 def test_append_large_pages_of_16_bits():
@@ -365,9 +422,55 @@ def test_prompt_attention_over_other_keys(dtype, causal):
     run_prompt([10, 5, 100, 70, 8, 1, 33], [200, 5, 40, 1, 0, 500, 34], 4, 2, 128, dtype, causal)
 
 
+def test_prompt_attention_scales():
+    # (of 0: every key counts alike; negative: the least score wins)
+    for scale in (0.0, -0.2, 3.0):
+        run_prompt([100, 70], [100, 130], 4, 2, 64, BF16, True, scale=scale)
+        run_prompt([40], [40], 2, 2, 30, F16, True, scale=scale)
+
+
 def test_prompt_attention_long():
     run_prompt([2049], [2049], 2, 1, 128, BF16, True)
     run_prompt([700, 1500], [2500, 1500], 2, 2, 64, F16, True, scale=0.3)
+
+
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("dtype,dim", ((F16, 64), (BF16, 128), (BF16, 72)))
+def test_prompt_attention_split_keys(dtype, dim, causal):
+    # few rows over many keys: workgroups that each take some of the keys, and join their states
+    def edit(q, k, v):
+        v[4190, 0, 5], v[4199, 1, 9], v[3000, 1, 1] = float("inf"), float("nan"), float("-inf")
+        v[5000, 0, 0] = float("inf")
+        k[4150, 1] = float("nan")
+
+    queries, keys = [40, 3, 0, 70], [4200, 3600, 900, 30]
+    assert _lib.load().nt_prompt_attention_workspace_size(115, 8732, 4, 4, 2, dim) > 0
+    run_prompt(queries, keys, 4, 2, dim, dtype, causal)
+    run_prompt(queries, keys, 4, 2, dim, dtype, causal, edit=edit, scale=-0.1)
+
+
+def test_prompt_attention_split_keys_captured():
+    # two graphs on two streams, each with its own workspace, beside the eager call
+    queries, keys = [40, 3, 70], [4200, 2600, 300]
+    q, k, v = randn(113, 4, 64, dtype=BF16), randn(7100, 2, 64, dtype=BF16, seed=1), randn(7100, 2, 64, dtype=BF16, seed=2)
+    starts, k_starts = starts_of(queries), starts_of(keys)
+    assert _lib.load().nt_prompt_attention_workspace_size(113, 7100, 3, 4, 2, 64) > 0
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(2):
+        outs.append(torch.empty_like(q))
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            kernels.prompt_attention(q, k, v, outs[-1], starts, k_starts)
+    for i in range(4):
+        q.copy_(randn(113, 4, 64, dtype=BF16, seed=10 + i))
+        want = kernels.prompt_attention(q, k, v, torch.empty_like(q), starts, k_starts)
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+    check_prompt(q, k, v, want, queries, keys, True)
 
 
 def test_prompt_attention_many_sequences():
@@ -417,7 +520,8 @@ def test_prompt_attention_strides():
 
 
 # ------------------------------------------------------------------------------- cache attention
-def run_step(lengths, heads, kv_heads, dim, page, dtype, cache, layout="slots", edit=None, width=None, seed=0):
+def run_step(lengths, heads, kv_heads, dim, page, dtype, cache, layout="slots", edit=None, width=None, seed=0,
+             scale=None):
     tables, pages = paged([max(n, 0) for n in lengths], page)
     if width:
         tables = torch.cat([tables, tables.new_full((tables.shape[0], width - tables.shape[1]), -5)], 1)
@@ -436,9 +540,9 @@ def run_step(lengths, heads, kv_heads, dim, page, dtype, cache, layout="slots", 
     if edit:
         edit(q, kc, vc, tables)
     out = torch.full_like(q, float("nan"))
-    got = kernels.cache_attention(q, kc, vc, tables, i32(lengths), out, k_scale=ks, v_scale=vs)
+    got = kernels.cache_attention(q, kc, vc, tables, i32(lengths), out, k_scale=ks, v_scale=vs, scale=scale)
     assert got is out
-    group, scale = heads // kv_heads, dim**-0.5
+    group, scale = heads // kv_heads, dim**-0.5 if scale is None else scale
     weight_type = F16 if cache == E4M3 else dtype
     for b, n in enumerate(lengths):
         n = min(max(n, 0), tables.shape[1] * page)
@@ -474,6 +578,24 @@ def test_cache_attention_split_keys(page, cache):
     # one long sequence over all workgroups; long and short ones beside each other; a table with room
     run_step([40001], 4, 1, 128, page, F16, cache)
     run_step([9000, 5, 0, 3000, 1, 129], 8, 2, 64, page, F16, cache, width=700)
+
+
+@pytest.mark.parametrize("cache", (BF16, E4M3))
+def test_cache_attention_scales(cache):
+    for scale in (0.0, -0.1, 1.5):
+        run_step([100, 70, 300], 4, 2, 64, 16, BF16, cache, scale=scale)
+        run_step([100, 70, 300], 4, 2, 64, 10, BF16, cache, scale=scale)
+
+
+@pytest.mark.parametrize("cache", (F16, E4M3))
+def test_cache_attention_missing_odd_pages(cache):
+    # pages of no whole sixteens: a missing one reaches no output, though the first page is NaN
+    def edit(q, kc, vc, tables):
+        kc[0], vc[0] = float("nan"), float("nan")
+        tables[tables == 0] = -1
+        tables[0, 1], tables[1, 0] = -7, 1 << 30
+
+    run_step([100, 20, 300], 4, 2, 64, 24, F16, cache, edit=edit)
 
 
 def test_cache_attention_many_sequences():
