@@ -929,19 +929,30 @@ static bool prompt_vectors(const PromptArgs& g) {
 // heads on 8: 1 x 1,024 25.6 / 33.6, 1 x 2,048 52.6 / 59.9, 64 x 256 132 / 183, 32 x 512 156 / 189, 16 x 1,024
 // 208 / 230, but 16 x 2,048 679 / 661, 1 x 16,384 1,896 / 1,821; ungrouped, whose K and V then do not stay
 // in the L2s, 32 x 512 193 / 209, 32 x 1,024 625 / 516.
-// Keys are split while workgroups are few, 16 tiles each at least (the join costs a launch): 512
-// queries over 8,192 keys 85 us, unsplit 146, 64 over 16,384 37 / 294, but over 512 keys in splits of 4
-// tiles 22.7 / 16.8.
+// Keys are split while workgroups are few, in as many parts as this estimate finds shortest: a tile takes a
+// workgroup 0.7 us, or 0.98 beside another one on its CU, and the join 3 us and 125 ns for each MB of
+// partial states.  us unsplit / split, heads of 128, 32 on 8: 1 query over 4,000 keys 59 / 14.6 (in 16),
+// 128 over 2,000 40.8 / 21.6 (6), 512 over 8,192 146 / 87 (3); where it leaves the keys whole, and two parts
+// would cost: 512 over 512 17.3 / 23.1, 768 over 768 22.1 / 30.4.
 struct PromptPlan {
   int per, splits;
 };
-static PromptPlan prompt_plan(int64_t q_tokens, int64_t k_tokens, int64_t sequences, int64_t kv_heads, int64_t group) {
+static PromptPlan prompt_plan(int64_t q_tokens, int64_t k_tokens, int64_t sequences, int64_t kv_heads, int64_t group,
+                              int64_t dim) {
   UnitMap map{nullptr, q_tokens, (int)sequences, (int)group, pa::BM, 1};
   PromptPlan p{pa::BM, 1};
   const int64_t tiles = k_tokens / std::max<int64_t>(1, sequences) / pa::BN, blocks = unit_count(map) * kv_heads;
   if (blocks >= pa::FEW_BLOCKS && tiles > (group >= 4 ? 16 : 8)) return p;
   p.per = map.per = pa::BM / 2;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / (unit_count(map) * kv_heads), tiles / 16, pa::MOST_SPLITS}));
+  const int64_t workgroups = unit_count(map) * kv_heads, most = std::min<int64_t>(512 / workgroups, pa::MOST_SPLITS);
+  const double state_ns = 0.125e-3 * 8 * (double)q_tokens * kv_heads * group * (dim + 2);  // (written and read)
+  double least = 0;
+  for (int64_t s = 1; s <= most; ++s) {
+    const double ns = cdiv(tiles, s) * (workgroups * s > 256 ? 980.0 : 700.0) + (s > 1 ? 3000.0 + s * state_ns : 0.0);
+    if (s > 1 && ns >= least) continue;
+    least = ns;
+    p.splits = (int)s;
+  }
   return p;
 }
 
@@ -949,7 +960,7 @@ template <typename T>
 static int prompt_launch(PromptArgs g, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const bool vec = prompt_vectors(g);
   PromptPlan plan{pa::BM, 1};
-  if (vec) plan = prompt_plan(g.map.tokens, g.k_tokens, g.map.sequences, g.kv_heads, g.group);
+  if (vec) plan = prompt_plan(g.map.tokens, g.k_tokens, g.map.sequences, g.kv_heads, g.group, g.dim);
   g.rows = g.map.tokens * g.kv_heads * g.group;
   if (plan.splits > 1 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < g.rows * plan.splits * (g.dim + 2) * 4))
     plan.splits = 1;
@@ -1027,7 +1038,7 @@ extern "C" int64_t nt_prompt_attention_workspace_size(int64_t q_tokens, int64_t 
   if (q_tokens <= 0 || k_tokens < 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 ||
       dim > 128 || q_tokens > 0x7fffff00LL || heads > (1 << 20) || sequences > (1 << 30))
     return 0;
-  const int splits = nt::prompt_plan(q_tokens, k_tokens, sequences, kv_heads, heads / kv_heads).splits;
+  const int splits = nt::prompt_plan(q_tokens, k_tokens, sequences, kv_heads, heads / kv_heads, dim).splits;
   return splits > 1 ? q_tokens * heads * splits * (dim + 2) * 4 : 0;
 }
 
