@@ -68,8 +68,12 @@ struct Geo {
   static constexpr int ROW = DM * ES, CHUNKS = ROW / 16, TILE = BN * ROW, STAGE = 2 * TILE;
   static constexpr int LOADS = TILE / 1024, KEYS = BN / LOADS;  // of k or v, and the keys of each
   static constexpr int STAGES = 2, RING = STAGES * STAGE;
-  static constexpr int OROW = DM + 4, MERGE = BQ * OROW * 4;  // a wave's state, for the merge
-  static constexpr int LDS = NW * (RING > MERGE ? RING : MERGE);
+  static constexpr int LDS = NW * RING;
+  // A wave's state for the merge, in its second stage: 16-byte chunks XORed by row, as the writes go by rows.
+  static_assert(BQ * DM * 4 <= STAGE, "a state has a stage");
+  __device__ __forceinline__ static int merge_at(int wave, int row, int d) {
+    return (wave * RING + STAGE) / 4 + row * DM + ((((d >> 2) ^ row) & (DM / 4 - 1)) << 2 | (d & 3));
+  }
   __device__ __forceinline__ static int swizzle(int key) {
     return ROW == 256 ? key & 15 : ROW == 128 ? (key >> 1) & 7 : (key >> 2) & 3;
   }
@@ -189,6 +193,10 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
   constexpr int KL = DM * ES / 64;               // 16-byte reads of a key a lane
   constexpr int DL = DM / 16, VW = DL * ES / 4;  // elements of v a lane, and their words
   constexpr int NKEYS = SIXTEENS ? 1 : BN;
+  // The next sequence's first keys are sent for before a sequence's states are merged: us with / without, of 256
+  // sequences of 100 keys on 8 heads of 128, 16 bits 37.8 / 44.0 (one workgroup a CU); 8 bits 23.3 / 21.4 (two
+  // hide it from each other).
+  constexpr bool AHEAD = !EIGHT;
   __shared__ __attribute__((aligned(1024))) char ring[G::LDS];
   __shared__ float merge_ml[NW][2][BQ];
   __shared__ int line_lds[8];
@@ -237,119 +245,127 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
                                (((byte >> 4) ^ G::swizzle(key)) * 16) + (byte & 15));
   };
 
-  while (at < stop) {
-    const int nblk = line_blocks(len), inside = at - seq0, rb = g.row_blocks == 1 ? 0 : inside / nblk, blk0 = inside - rb * nblk;
-    const int blk1 = min(nblk, blk0 + (stop - at));
-    const int rows = min(BQ, g.group - rb * BQ);
-    const int head0 = h * g.group + rb * BQ;
+  // A piece of the stretch: blocks [blk0, blk1) of a sequence and of a block of its rows.
+  int nblk, blk0, blk1, rows, head0, t0, nt;  // nt: this wave's tiles, t0 + j NW
+  ScalarInts table;
+  const char* kbase = (const char*)g.k + h * g.ks[2] * ES;
+  const char* vbase = (const char*)g.v + h * g.vs[2] * ES;
 
-    const ScalarInts table = (ScalarInts)(uintptr_t)(g.tables + b * g.table_stride);
-    const char* kbase = (const char*)g.k + h * g.ks[2] * ES;
-    const char* vbase = (const char*)g.v + h * g.vs[2] * ES;
-    const int tiles = (len + BN - 1) / BN;
-    const int t0 = blk0 * NW + wave, t_end = min(blk1 * NW, tiles);
-    const int nt = t0 < t_end ? (t_end - t0 + NW - 1) / NW : 0;  // this wave's tiles: t0 + j NW
-
-    // The scales of a page's head; as a factor of scores, and what v's adds to exponents and sums.
-    struct Scales {
-      float kf, lv, rv;
-    };
-    auto scales = [&](float ks, float vs) {
-      vs = fmaxf(vs, LEAST_SCALE);
-      return Scales{ks * g.scale_log2, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
-    };
-    // SIXTEENS: the pages of the tile that comes next (looked up ahead), and of those under way their
-    // scales and what a page adds to its exponents: nothing, or where there is none minus infinity.
-    int next_page[2];
-    float k_sc[G::STAGES][2], v_sc[G::STAGES][2], add[G::STAGES][2];
-    auto look = [&](int j) {
+  // The scales of a page's head; as a factor of scores, and what v's adds to exponents and sums.
+  struct Scales {
+    float kf, lv, rv;
+  };
+  auto scales = [&](float ks, float vs) {
+    vs = fmaxf(vs, LEAST_SCALE);
+    return Scales{ks * g.scale_log2, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+  };
+  // SIXTEENS: the pages of the tile that comes next (looked up ahead), and of those under way their
+  // scales and what a page adds to its exponents: nothing, or where there is none minus infinity.
+  int next_page[2];
+  float k_sc[G::STAGES][2], v_sc[G::STAGES][2], add[G::STAGES][2];
+  auto look = [&](int j) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int sixteen = 2 * (t0 + j * NW) + kb;
+      const int n = g.page_shift >= 0 ? sixteen >> g.page_shift : sixteen / (g.page_size >> 4);
+      next_page[kb] = j < nt && n < g.table_width ? table[n] : -1;
+    }
+  };
+  auto issue = [&](int j, int stage) {
+    const int k0 = (t0 + j * NW) * BN;
+    const uint32_t to = ring_w + (uint32_t)(stage * G::STAGE);
+    if (SIXTEENS) {
+      u32x4 rk[2], rv[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const int sixteen = 2 * (t0 + j * NW) + kb;
-        const int n = g.page_shift >= 0 ? sixteen >> g.page_shift : sixteen / (g.page_size >> 4);
-        next_page[kb] = j < nt && n < g.table_width ? table[n] : -1;
-      }
-    };
-    auto issue = [&](int j, int stage) {
-      const int k0 = (t0 + j * NW) * BN;
-      const uint32_t to = ring_w + (uint32_t)(stage * G::STAGE);
-      if (SIXTEENS) {
-        u32x4 rk[2], rv[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const int first = k0 + kb * 16;
-          const bool ok = (uint32_t)next_page[kb] < (uint32_t)g.pages;  // (SIXTEENS: 32 bits)
-          const uint32_t page = ok ? next_page[kb] : 0;
-          const int slot = g.page_shift >= 0 ? first & (g.page_size - 1) : first % g.page_size;
-          // (a buffer ends with the last key: what lies past it, or in no page, reads as zeros)
-          const int n = ok ? min(16, len - first) : 0;
-          rk[kb] = buffer_of(kbase + ((uint64_t)page * page_k + (uint32_t)(slot * kst)), n > 0 ? (n - 1) * kst + D * ES : 0);
-          rv[kb] = buffer_of(vbase + ((uint64_t)page * page_v + (uint32_t)(slot * vst)), n > 0 ? (n - 1) * vst + D * ES : 0);
-          add[stage][kb] = ok ? 0.f : -INFINITY;
-          if (EIGHT) {
-            const float ks = ((ScalarFloats)(uintptr_t)g.k_scale)[page * (uint32_t)g.kv_heads + h];
-            k_sc[stage][kb] = ok ? ks : 0.f;
-            v_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.v_scale)[page * (uint32_t)g.kv_heads + h];
-          }
+        const int first = k0 + kb * 16;
+        const bool ok = (uint32_t)next_page[kb] < (uint32_t)g.pages;  // (SIXTEENS: 32 bits)
+        const uint32_t page = ok ? next_page[kb] : 0;
+        const int slot = g.page_shift >= 0 ? first & (g.page_size - 1) : first % g.page_size;
+        // (a buffer ends with the last key: what lies past it, or in no page, reads as zeros)
+        const int n = ok ? min(16, len - first) : 0;
+        rk[kb] = buffer_of(kbase + ((uint64_t)page * page_k + (uint32_t)(slot * kst)), n > 0 ? (n - 1) * kst + D * ES : 0);
+        rv[kb] = buffer_of(vbase + ((uint64_t)page * page_v + (uint32_t)(slot * vst)), n > 0 ? (n - 1) * vst + D * ES : 0);
+        add[stage][kb] = ok ? 0.f : -INFINITY;
+        if (EIGHT) {
+          const float ks = ((ScalarFloats)(uintptr_t)g.k_scale)[page * (uint32_t)g.kv_heads + h];
+          k_sc[stage][kb] = ok ? ks : 0.f;
+          v_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.v_scale)[page * (uint32_t)g.kv_heads + h];
         }
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-          for (int u = 0; u < G::LOADS; ++u)
-            buffer_to_lds(w ? rv[u * G::KEYS / 16] : rk[u * G::KEYS / 16], to + w * G::TILE + u * 1024,
-                          w ? v_off[u] : k_off[u], 0);
-        look(j + 1);
-      } else {
-        // Lane i looks up key i % 32; then each lane takes what its loads need.  (Keys past the end
-        // repeat the last one.)
-        const int key = min(k0 + (lane & 31), len - 1), n = key / g.page_size;
-        const int32_t found = g.tables[b * g.table_stride + n];
-        const bool ok = found >= 0 && found < g.pages;
-        const int64_t page = ok ? found : 0;
-        const int slot = key - n * g.page_size;
-        if (lane < 32) {
-          key_at[wave][0][lane & (NKEYS - 1)] = (page * g.ks[0] + slot * g.ks[1]) * ES;
-          key_at[wave][1][lane & (NKEYS - 1)] = (page * g.vs[0] + slot * g.vs[1]) * ES;
-          Scales x{g.scale_log2, 0.f, 1.0f};
-          if (EIGHT && ok) x = scales(g.k_scale[page * g.kv_heads + h], g.v_scale[page * g.kv_heads + h]);
-          key_scale[wave][stage][0][lane & (NKEYS - 1)] = x.kf;
-          key_scale[wave][stage][1][lane & (NKEYS - 1)] = ok ? x.lv : -INFINITY;  // (a key of no page)
-          key_scale[wave][stage][2][lane & (NKEYS - 1)] = x.rv;
-        }
-        wave_lds_order();
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-          for (int u = 0; u < G::LOADS; ++u)
-            global_to_lds((w ? vbase : kbase) + key_at[wave][w][kv_key[u] & (NKEYS - 1)] +
-                              (kv_byte[u] < D * ES ? kv_byte[u] : 0),
-                          to + w * G::TILE + u * 1024);
-        wave_lds_order();
       }
-    };
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int u = 0; u < G::LOADS; ++u)
+          buffer_to_lds(w ? rv[u * G::KEYS / 16] : rk[u * G::KEYS / 16], to + w * G::TILE + u * 1024,
+                        w ? v_off[u] : k_off[u], 0);
+      look(j + 1);
+    } else {
+      // Lane i looks up key i % 32; then each lane takes what its loads need.  (Keys past the end
+      // repeat the last one.)
+      const int key = min(k0 + (lane & 31), len - 1), n = key / g.page_size;
+      const int32_t found = g.tables[b * g.table_stride + n];
+      const bool ok = found >= 0 && found < g.pages;
+      const int64_t page = ok ? found : 0;
+      const int slot = key - n * g.page_size;
+      if (lane < 32) {
+        key_at[wave][0][lane & (NKEYS - 1)] = (page * g.ks[0] + slot * g.ks[1]) * ES;
+        key_at[wave][1][lane & (NKEYS - 1)] = (page * g.vs[0] + slot * g.vs[1]) * ES;
+        Scales x{g.scale_log2, 0.f, 1.0f};
+        if (EIGHT && ok) x = scales(g.k_scale[page * g.kv_heads + h], g.v_scale[page * g.kv_heads + h]);
+        key_scale[wave][stage][0][lane & (NKEYS - 1)] = x.kf;
+        key_scale[wave][stage][1][lane & (NKEYS - 1)] = ok ? x.lv : -INFINITY;  // (a key of no page)
+        key_scale[wave][stage][2][lane & (NKEYS - 1)] = x.rv;
+      }
+      wave_lds_order();
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int u = 0; u < G::LOADS; ++u)
+          global_to_lds((w ? vbase : kbase) + key_at[wave][w][kv_key[u] & (NKEYS - 1)] +
+                            (kv_byte[u] < D * ES ? kv_byte[u] : 0),
+                        to + w * G::TILE + u * 1024);
+      wave_lds_order();
+    }
+  };
+  // Finds the piece that begins at `at` and sends for the wave's first tile.
+  auto begin_piece = [&]() __attribute__((always_inline)) {
+    nblk = line_blocks(len);
+    const int inside = at - seq0, rb = g.row_blocks == 1 ? 0 : inside / nblk;
+    blk0 = inside - rb * nblk;
+    blk1 = min(nblk, blk0 + (stop - at));
+    rows = min(BQ, g.group - rb * BQ);
+    head0 = h * g.group + rb * BQ;
+    table = (ScalarInts)(uintptr_t)(g.tables + b * g.table_stride);
+    t0 = blk0 * NW + wave;
+    const int t_end = min(blk1 * NW, (len + BN - 1) / BN);
+    nt = t0 < t_end ? (t_end - t0 + NW - 1) / NW : 0;
     if (SIXTEENS) look(0);
-#pragma unroll
-    for (int j = 0; j < G::STAGES; ++j)
-      if (j < nt) issue(j, j);
-
+    if (nt > 0) issue(0, 0);
+  };
+  if (AHEAD) begin_piece();
+  while (true) {
+    if (!AHEAD) begin_piece();
+    if (nt > 1) issue(1, 1);
+    const int next_keys = line_keys(g, min(b + 1, g.sequences - 1));
     typename MQ::frag qf[STEPS];
-    {
-      const uint16_t* Q = (const uint16_t*)g.q + b * g.qs[0] + (head0 + col) * g.qs[1];
+    // (D: whole 16s)
+    auto q_at = [&](int s) { return EIGHT ? (s >> 1) * 64 + quad * 16 + (s & 1) * 8 : s * 32 + quad * 8; };
+    const uint16_t* Q = (const uint16_t*)g.q + b * g.qs[0] + (head0 + col) * g.qs[1];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = __builtin_bit_cast(typename MQ::frag, u32x4{0u, 0u, 0u, 0u});
+    if (g.q_vectors) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (col < rows && q_at(s) < D) qf[s] = *(const typename MQ::frag*)(Q + q_at(s));
+    } else if (col < rows) {
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        const int d = EIGHT ? (s >> 1) * 64 + quad * 16 + (s & 1) * 8 : s * 32 + quad * 8;  // (D: whole 16s)
-        u32x4 w = {0u, 0u, 0u, 0u};
-        if (col < rows && d < D) {
-          if (g.q_vectors) {
-            w = *(const u32x4*)(Q + d);
-          } else {
-            uint16_t x[8];
+        if (q_at(s) >= D) continue;
+        uint16_t x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = Q[(d + e) * g.qs[2]];
-            w = *(const u32x4*)x;
-          }
-        }
-        qf[s] = __builtin_bit_cast(typename MQ::frag, w);
+        for (int e = 0; e < 8; ++e) x[e] = Q[(q_at(s) + e) * g.qs[2]];
+        qf[s] = __builtin_bit_cast(typename MQ::frag, *(const u32x4*)x);
       }
     }
     // The queries are there from here on: in the loop the compiler would wait for them at every tile, and so
@@ -490,25 +506,35 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
       if (j + 1 < nt) compute(j + 1, 1);
     }
 
-    // The waves' states through LDS, then the output, or a partial state where the keys go on in
-    // another workgroup's stretch.
+    // The waves' states through LDS, where the next piece's first tiles are already on their way; then
+    // the output, or a partial state where the keys go on in another workgroup's stretch.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    __syncthreads();  // other waves may still read their stages, which the states cover
     float* merge_o = (float*)ring;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < DL; ++c)
-        merge_o[wave * (G::MERGE / 4) + col * G::OROW + (quad * 4 + r) * DL + c] = acc[c][r];
+      for (int c = 0; c < DL; ++c) merge_o[G::merge_at(wave, col, (quad * 4 + r) * DL + c)] = acc[c][r];
     if (quad == 0) {
       merge_ml[wave][0][col] = m;
       merge_ml[wave][1][col] = l;
     }
-    __syncthreads();
     const bool whole = blk0 == 0 && blk1 == nblk;
     const int64_t slot = 2 * (int64_t)wg + (at == begin ? 0 : 1);
-    for (int e = tid; e < rows * DM; e += NW * 64) {
+    const int out_rows = rows;
+    uint16_t* out = (uint16_t*)g.o + b * g.os[0] + head0 * g.os[1];
+    at += blk1 - blk0;
+    const bool more = at < stop;
+    if (more) {
+      if (at - seq0 == nblk * g.row_blocks) {
+        seq0 = at;
+        len = __builtin_amdgcn_readfirstlane(next_keys);
+        ++b;
+      }
+      if (AHEAD) begin_piece();
+    }
+    __syncthreads();
+    for (int e = tid; e < out_rows * DM; e += NW * 64) {
       const int r = e / DM, d = e % DM;
       float mm = merge_ml[0][0][r];
 #pragma unroll
@@ -518,12 +544,10 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
       for (int w = 0; w < NW; ++w) {
         const float mw = merge_ml[w][0][r], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
         sum += merge_ml[w][1][r] * f;
-        o += merge_o[w * (G::MERGE / 4) + r * G::OROW + d] * f;
+        o += merge_o[G::merge_at(w, r, d)] * f;
       }
       if (whole) {
-        if (d < D)
-          ((uint16_t*)g.o)[b * g.os[0] + (head0 + r) * g.os[1] + d * g.os[2]] =
-              elem<T>::from_float(sum == 0.f ? 0.f : o / sum);
+        if (d < D) out[r * g.os[1] + d * g.os[2]] = elem<T>::from_float(sum == 0.f ? 0.f : o / sum);
       } else {
         g.part_o[(slot * BQ + r) * DM + d] = o;
         if (d == 0) {
@@ -532,12 +556,8 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
         }
       }
     }
-    __syncthreads();
-    at += blk1 - blk0;
-    if (at - seq0 == nblk * g.row_blocks && at < stop) {
-      seq0 = at;
-      len = line_keys(g, ++b);
-    }
+    if (!more) return;
+    __syncthreads();  // the states have been read: the second stages are free again
   }
 }
 
