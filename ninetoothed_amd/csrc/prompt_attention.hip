@@ -931,9 +931,9 @@ static bool prompt_vectors(const PromptArgs& g) {
 // in the L2s, 32 x 512 193 / 209, 32 x 1,024 625 / 516.
 // Keys are split while workgroups are few, in as many parts as this estimate finds shortest: a tile takes a
 // workgroup 0.7 us, or 0.98 beside another one on its CU, and the join 3 us and 125 ns for each MB of
-// partial states.  us unsplit / split, heads of 128, 32 on 8: 1 query over 4,000 keys 59 / 14.6 (in 16),
-// 128 over 2,000 40.8 / 21.6 (6), 512 over 8,192 146 / 87 (3); where it leaves the keys whole, and two parts
-// would cost: 512 over 512 17.3 / 23.1, 768 over 768 22.1 / 30.4.
+// partial states; whole keys are kept where that gains less than 5 %.  us unsplit / split, heads of 128, 32
+// on 8: 1 query over 4,000 keys 59 / 14.6 (in 16), 128 over 2,000 40.8 / 21.6 (6), 512 over 8,192 146 / 87 (3);
+// where it leaves the keys whole, and two parts would cost: 512 over 512 17.3 / 23.1, 768 over 768 22.1 / 30.4.
 struct PromptPlan {
   int per, splits;
 };
@@ -944,11 +944,18 @@ static PromptPlan prompt_plan(int64_t q_tokens, int64_t k_tokens, int64_t sequen
   const int64_t tiles = k_tokens / std::max<int64_t>(1, sequences) / pa::BN, blocks = unit_count(map) * kv_heads;
   if (blocks >= pa::FEW_BLOCKS && tiles > (group >= 4 ? 16 : 8)) return p;
   p.per = map.per = pa::BM / 2;
-  const int64_t workgroups = unit_count(map) * kv_heads, most = std::min<int64_t>(512 / workgroups, pa::MOST_SPLITS);
+  // At most two workgroups a CU.  (unit_count bounds them: a unit a sequence fewer where lengths are whole
+  // multiples.  What then passes 512 waits for a whole turn in heads of 128, which fill a CU with two; in
+  // heads of 64 four fit: 2 x 700 over 5,000, 16 heads, with that unit counted / not 78.9 / 97.8 us, of 64
+  // 59.3 / 59.1, and 2 x 512 over 4,012 41.7 / 39.2.)
+  const int64_t workgroups = unit_count(map) * kv_heads;
+  const int64_t whole = std::max(q_tokens * group / map.per, sequences) * kv_heads;
+  const int64_t most = std::min<int64_t>(512 / (dim <= 64 ? whole : workgroups), pa::MOST_SPLITS);
   const double state_ns = 0.125e-3 * 8 * (double)q_tokens * kv_heads * group * (dim + 2);  // (written and read)
   double least = 0;
   for (int64_t s = 1; s <= most; ++s) {
-    const double ns = cdiv(tiles, s) * (workgroups * s > 256 ? 980.0 : 700.0) + (s > 1 ? 3000.0 + s * state_ns : 0.0);
+    const double ns = s == 1 ? 0.95 * 700.0 * tiles
+                             : cdiv(tiles, s) * (workgroups * s > 256 ? 980.0 : 700.0) + 3000.0 + s * state_ns;
     if (s > 1 && ns >= least) continue;
     least = ns;
     p.splits = (int)s;
