@@ -431,7 +431,8 @@ int nt_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t*
  * stored is x / scale, with scale the least power of two (from 2^-64 on) for which 448 scale is
  * at least the page's largest finite value.  A page whose slot 0 is among the new tokens takes a
  * scale afresh; else the scale only grows, and what the page held before the new slots is divided to match.
- * Infinities are stored as NaN.  dim a multiple of 4 up to 128; pages of 8 bits up to 128 slots. */
+ * Infinities are stored as NaN.  dim a multiple of 4 up to 128; pages of 8 bits up to 128 slots.
+ * The two caches must not overlap; at most 65535 heads and 2^31 - 1 tokens. */
 int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
                     void* k_cache, const int64_t* kc_strides, void* v_cache, const int64_t* vc_strides,
                     int cache_dtype, float* k_scale, float* v_scale, const int32_t* tables, int64_t table_stride,
@@ -445,7 +446,9 @@ int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, cons
  * tensors), dim <= 128, any strides (unit element strides, strides of multiples of 8 and 16-byte
  * aligned tensors take vector loads).  With few rows over many keys the keys are split over workgroups,
  * whose states (fp32) pass through `workspace` (16-byte aligned, nt_prompt_attention_workspace_size
- * bytes; 0: none wanted); with none or too little they are not split.  It holds nothing between calls. */
+ * bytes; 0: none wanted); with none or too little they are not split.  It holds nothing between calls, but
+ * calls that may run at once need one each.  o must not overlap q, k or v.  Less than 2^31 - 255 keys, and
+ * queries times heads / kv_heads; at most 2^20 heads. */
 int64_t nt_prompt_attention_workspace_size(int64_t q_tokens, int64_t k_tokens, int64_t sequences, int64_t heads,
                                            int64_t kv_heads, int64_t dim);
 int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -460,7 +463,8 @@ int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, 
  * as 2^-64).  Keys of a page outside [0, pages) do not count; without keys the output is zero.
  * dim a multiple of 16 up to 128; caches 16-byte aligned, with strides of multiples of 16 bytes.
  * The workspace (16-byte aligned, nt_cache_attention_workspace_size bytes, 0: none needed) holds
- * partial states of sequences whose keys are split over workgroups; nothing between calls. */
+ * partial states of sequences whose keys are split over workgroups; nothing between calls, but calls that
+ * may run at once need one each.  o must not overlap the inputs. */
 int64_t nt_cache_attention_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
                                           int64_t page_size, int64_t table_width, int cache_dtype);
 int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,

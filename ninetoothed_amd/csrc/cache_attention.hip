@@ -175,6 +175,9 @@ __device__ __forceinline__ LinePlace line_place(const CacheArgs& g, int which, i
 // of its own (loads that bypass the registers, no barrier in the loop), so that 8 KiB (8 bits) or 16 a
 // wave are under way while it computes.  P^T goes from the scores' registers to the second product as it
 // is, and V, read eight keys by DM / 16 neighbouring elements a lane, is transposed by byte permutes.
+// 28 heads on 4 of 128, two sequences of 95,000 keys in fp16: 79 us, 4.9 TB/s; 32 on 8, 128 sequences of 100
+// to 9,000 keys in e4m3: 238 us, 4.9 TB/s, as a large copy; 8 of 4,000: 23 us, 2.8 TB/s, of which 9 are two
+// launches, the first loads and the join.
 // 8 bits: e4m3 widens exactly, so k's scale multiplies the score and v's enters the weight:
 //   w_ij = exp2(s_ij + log2 vs_j - M_i),  o_i = sum_j w_ij vq_j / sum_j w_ij / vs_j,
 // with M the running max of the exponents: w stays within 2^8 for any scales, is rounded to fp16
@@ -506,7 +509,7 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
       if (j + 1 < nt) compute(j + 1, 1);
     }
 
-    // The waves' states through LDS, where the next piece's first tiles are already on their way; then
+    // The waves' states through LDS (the second stages: AHEAD fills the first ones meanwhile); then
     // the output, or a partial state where the keys go on in another workgroup's stretch.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);

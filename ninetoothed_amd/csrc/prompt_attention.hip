@@ -264,7 +264,9 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
 // Per row i of a sequence (a token and a head of its group) over the keys j it may see:
 //   s_ij = scale q_i . k_j,  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i);
 // causal: j <= i + (keys - queries).  A row that sees no key gives zeros.
-// MFMA-bound: 4 dim flops a head and visible pair.  A workgroup takes 256 rows, a group's heads
+// MFMA-bound: 4 dim flops a head and visible pair, and beside it the softmax's VALU work, which an MFMA
+// keeps waiting half of its time (bf16, 32 heads: 4 x 4,096 full 1,106 TFLOP/s in heads of 128, 1,028 in
+// heads of 64; causal, on 8 heads, 1 x 16,384 1,200, 4 x 4,096 1,034).  A workgroup takes 256 rows, a group's heads
 // side by side for each token, so that short sequences fill its rows and share K and V; eight waves
 // of 32 rows, two a SIMD.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: a lane holds
 // one row, its max and sum take no LDS, and P^T goes from the score registers to the second product
