@@ -166,6 +166,15 @@ __device__ __forceinline__ LinePlace line_place(const CacheArgs& g, int which, i
   return p;
 }
 
+// A workgroup's number, of which the head comes first.  Two heads' rows of 64 bytes share a line of the L2:
+// neighbours go to one XCD (ids go to the 8 of them in turn), the two eight ids apart; 16 x 4,000 keys of
+// 16 x 64 so take 43 us instead of 52.
+template <bool EIGHT, int DM>
+__device__ __forceinline__ int cache_workgroup() {
+  const int id = blockIdx.x;
+  return EIGHT && DM == 64 && (id | 15) < (int)gridDim.x ? (id & ~15) | (id & 7) << 1 | (id >> 3 & 1) : id;
+}
+
 // Per sequence and head of k and v, for the heads of q that share it (rows i):
 //   s_ij = scale q_i . (kq_j ks_j),  o_i = sum_j p_ij (vq_j vs_j) / sum_j p_ij,  p_ij = exp(s_ij - m_i)
 // over its cached keys; an empty sequence gives zeros.
@@ -209,10 +218,7 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = g.dim;
 
-  // Two heads' rows of 64 bytes share a line of the L2: neighbours go to one XCD (ids go to the 8 of them in
-  // turn), the two eight ids apart; 16 x 4,000 keys of 16 x 64 so take 43 us instead of 52.
-  int wg = blockIdx.x;
-  if (G::ROW == 64 && (wg | 15) < (int)gridDim.x) wg = (wg & ~15) | (wg & 7) << 1 | (wg >> 3 & 1);
+  const int wg = cache_workgroup<EIGHT, DM>();
   const int h = wg % g.kv_heads, part = wg / g.kv_heads;
   int share = 0;
   const LinePlace place = line_place(g, -1, line_lds, [&](int length) {
@@ -567,7 +573,7 @@ __global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs 
 // Joins the partial states of a sequence's query rows, where its keys were split.  A workgroup takes
 // join_rows of them.  Many states: row by row, the weight of each state first, a lane for each, then
 // groups of lanes that each sum some of the outputs, 16 bytes a lane.  Few: a group of lanes a row.
-template <typename T, int DM>
+template <typename T, bool EIGHT, int DM>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs g) {
   using namespace ca;
   constexpr int LANES = DM / 4, GROUPS = 256 / LANES, FEW = 8;
@@ -576,12 +582,12 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs g) {
   __shared__ float4 part[GROUPS][LANES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunks = (min(g.group, BQ) + g.join_rows - 1) / g.join_rows;
-  int id = blockIdx.x;
+  int id = cache_workgroup<EIGHT, DM>();
+  const int h = id % g.kv_heads;  // (first: on the XCD whose L2 the head's states were written to)
+  id /= g.kv_heads;
   const int chunk = id % chunks;
   id /= chunks;
-  const int rb = id % g.row_blocks;
-  id /= g.row_blocks;
-  const int h = id % g.kv_heads, b = id / g.kv_heads;
+  const int rb = id % g.row_blocks, b = id / g.row_blocks;
   const LinePlace place = line_place(g, b, line_lds, [](int) { return 0; });
   const int share = (place.length + g.parts - 1) / g.parts, nblk = line_blocks(place.keys);
   const int from = place.before + rb * nblk, to = from + nblk;
@@ -688,7 +694,7 @@ static void cache_launch(const CacheArgs& g, int64_t join_grid, hipStream_t stre
   else
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, false>), grid, block, 0, stream, g);
   if (join_grid)
-    hipLaunchKernelGGL((cache_join_kernel<T, DM>), dim3((unsigned)join_grid), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((cache_join_kernel<T, EIGHT, DM>), dim3((unsigned)join_grid), dim3(256), 0, stream, g);
 }
 
 }  // namespace nt
