@@ -95,7 +95,7 @@ struct PromptArgs {
   UnitMap map;                         // of q's rows: tokens * group
   const int32_t* k_starts;
   int64_t k_tokens, units;
-  int kv_heads, group, dim, causal;
+  int kv_heads, group, dim, causal, by_sequence;
   float scale_log2;  // softmax scale * log2(e)
   // Keys of a block of rows over several workgroups: their partial states in the workspace, for each
   // split and row (token, head of q): O [dim] and (max, sum).
@@ -104,10 +104,10 @@ struct PromptArgs {
   float *part_o, *part_ml;
 };
 
-// The block of rows a workgroup takes: longest first.  Up to 64 sequences: a lane for each, which
-// counts its blocks of at least so many key tiles; the number of tiles of the wanted block is found by
-// bisection, so the last workgroups of a launch are its shortest.  More sequences: from the last
-// block to the first.
+// The block of rows a workgroup takes.  By sequence: from the last block to the first.  Else (up to 64
+// sequences) longest first: a lane for each sequence, which counts its blocks of at least so many key tiles;
+// the number of tiles of the wanted block is found by bisection, so the last workgroups of a launch are its
+// shortest.
 struct PromptBlock {
   int64_t q_begin, k_begin;
   int head, r0, rows, Sq, Sk;  // rows: of the sequence; 0: nothing to do
@@ -130,7 +130,7 @@ __device__ __forceinline__ PromptBlock find_block(const PromptArgs& g) {
     p.Sk = (int)max((int64_t)0, k_clamp(g.k_starts[b + 1]) - p.k_begin);
     p.rows = p.Sq * g.group;
   };
-  if (g.map.sequences > 64) {
+  if (g.by_sequence) {
     const int64_t unit = g.units - 1 - id;
     const int b = find_sequence(g.map, unit);
     sequence(b);
@@ -988,6 +988,14 @@ static int prompt_launch(PromptArgs g, void* workspace, int64_t workspace_bytes,
   g.units = unit_count(g.map);
   const int64_t blocks = g.units * g.kv_heads * plan.splits;
   if (blocks > 0x7fffffffLL) return NT_ERR_INVALID;
+  // Longest blocks first of all sequences, or one sequence after another, whose K and V then stay in the L2s, but
+  // whose last blocks leave more CUs idle: with more sequences than the first can take, or four turns of
+  // workgroups (and 32 sequences in heads of 64).  us longest first / by sequence, causal, heads of 128, 32 on
+  // 8: 64 x 1,024 918 / 773, 64 x 256 131 / 120; ungrouped 1,037 / 870, 160 / 151, 8 x 2,048 358 / 330; heads of
+  // 64, 32 on 8: 64 x 1,024 441 / 408, 64 x 256 60 / 53, but 8 x 2,048 167 / 175, 4 x 4,096 296 / 316, and 16
+  // heads, 2.3 turns, 90 / 105.
+  const bool turns = blocks * plan.per / 32 >= 4 * 256 * (g.dim <= 64 ? 16 : 8);
+  g.by_sequence = g.map.sequences > 64 || (turns && (g.dim > 64 || g.map.sequences >= 32));
   const dim3 grid((unsigned)blocks), block(plan.per * 2);
 #define NT_PROMPT(DM)                                                                \
   if (!vec)                                                                          \

@@ -489,6 +489,27 @@ def test_prompt_attention_many_sequences():
     assert out.isfinite().all()
 
 
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("group", (1, 4))
+def test_prompt_attention_many_turns(group, dim):
+    # more workgroups than the card holds several times over, of sequences of very different lengths
+    g = torch.Generator().manual_seed(1)
+    lengths = torch.randint(0, 1600, (40,), generator=g).tolist()
+    heads = 32
+    q = randn(sum(lengths) + 3, heads, dim, dtype=BF16)
+    k, v = (randn(sum(lengths) + 3, heads // group, dim, dtype=BF16, seed=i) for i in (1, 2))
+    out = torch.full_like(q, float("nan"))
+    starts = starts_of(lengths)
+    kernels.prompt_attention(q, k, v, out, starts, starts)
+    assert out[:sum(lengths)].isfinite().all() and out[sum(lengths):].isnan().all()
+    for i in range(0, 40, 3):
+        a, n = int(starts[i]), lengths[i]
+        for h in (i % heads, heads - 1):
+            o, size = attended(q[a:a + n, h], k[a:a + n, h // group], v[a:a + n, h // group], dim**-0.5,
+                               torch.arange(n, device=DEV))
+            close(out[a:a + n, h], o, attention_tol(o, size, BF16, n, 5.0), f"sequence {i} of {n}, head {h}")
+
+
 @pytest.mark.parametrize("dim", (64, 128, 72))
 @pytest.mark.parametrize("dtype", (F16, BF16))
 def test_prompt_attention_masked_infinities(dtype, dim):
