@@ -11,7 +11,7 @@ namespace ca {
 constexpr int NW = 4;        // waves per workgroup
 constexpr int BN = 32;       // keys a wave takes at a time
 constexpr int BLOCK = NW * BN;
-constexpr int MOST_PARTS = 768;  // workgroups of a head
+constexpr int MOST_PARTS = 1024;  // workgroups of a head
 constexpr int BQ = 16;       // query rows: heads that share a head of k and v
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr float LEAST_SCALE = 0x1p-64f;  // a smaller v scale (or none) counts as this one
@@ -194,7 +194,7 @@ __device__ __forceinline__ int cache_workgroup() {
 // SIXTEENS: pages are whole multiples of 16 keys, so that a load's keys lie in one page and its
 // address and scale are uniform; else each key's page is looked up.
 template <typename T, bool EIGHT, int DM, bool SIXTEENS>
-__global__ __launch_bounds__(ca::NW * 64) void cache_attention_kernel(CacheArgs g) {
+__global__ __launch_bounds__(ca::NW * 64, EIGHT && DM == 64 ? 4 : 1) void cache_attention_kernel(CacheArgs g) {
   using namespace ca;
   typedef typename std::conditional<EIGHT, f16_t, T>::type P;  // the type of V^T P^T
   typedef mma16<T> MQ;
@@ -677,9 +677,10 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs g) {
 
 // Workgroups a head: all heads' together as many as the CUs' LDS holds at once, or fewer where the
 // longest possible sequences have fewer blocks; partial states only where a sequence can have
-// more than one.
+// more than one.  (Four a CU of 8 bits in heads of 64, whose registers are held to 128 for that, us against
+// three: 128 x 1,000 keys of 8 heads 36.9 / 43.0, 16 x 4,000 of 16 41.8 / 43.7, 2 x 60,000 of 2 18.4 / 17.5.)
 static int64_t cache_parts(int64_t kv_heads, int64_t blocks, bool eight, bool wide) {
-  const int64_t a_cu = eight ? (wide ? 2 : 3) : (wide ? 1 : 2);
+  const int64_t a_cu = eight ? (wide ? 2 : 4) : (wide ? 1 : 2);
   return std::max<int64_t>(1, std::min<int64_t>({256 * a_cu / kv_heads, blocks, (int64_t)ca::MOST_PARTS}));
 }
 
