@@ -933,10 +933,11 @@ static bool prompt_vectors(const PromptArgs& g) {
 
 // The rows of a workgroup, and over how many its keys are split.
 // 128 rows (two workgroups a CU) where 256 would leave CUs idle, or where sequences are so short that
-// one workgroup a CU mostly starts and ends: us with 128 / 256 rows, causal, bf16, heads of 128, D = 32
-// heads on 8: 1 x 1,024 25.6 / 33.6, 1 x 2,048 52.6 / 59.9, 64 x 256 132 / 183, 32 x 512 156 / 189, 16 x 1,024
-// 208 / 230, but 16 x 2,048 679 / 661, 1 x 16,384 1,896 / 1,821; ungrouped, whose K and V then do not stay
-// in the L2s, 32 x 512 193 / 209, 32 x 1,024 625 / 516.
+// one workgroup a CU mostly starts and ends: us with 128 / 256 rows, causal, bf16, heads of 128, 32 on 8:
+// 1 x 1,024 25.6 / 33.6, 1 x 2,048 52.6 / 59.9, 64 x 256 119 / 139, 32 x 512 145 / 162, 16 x 1,024 198 / 208, but
+// 1 x 16,384 1,944 / 1,869; ungrouped 32 x 512 172 / 183, 16 x 1,024 225 / 228, 9 of 100 to 2,500 149 / 155, but
+// 4 x 4,096 558 / 552; 16 heads of 64, 64 x 1,024 226 / 236, 12 x 800 34.4 / 40.1, but 4 x 4,096 158 / 153, and
+// 60 x 150 over 700 62 / 52, whose rows one workgroup of 256 holds.
 // Keys are split while workgroups are few, in as many parts as this estimate finds shortest: a tile takes a
 // workgroup 0.7 us, or 0.98 beside another one on its CU, and the join 3 us and 125 ns for each MB of
 // partial states; whole keys are kept where that gains less than 5 %.  us unsplit / split, heads of 128, 32
@@ -950,7 +951,8 @@ static PromptPlan prompt_plan(int64_t q_tokens, int64_t k_tokens, int64_t sequen
   UnitMap map{nullptr, q_tokens, (int)sequences, (int)group, pa::BM, 1};
   PromptPlan p{pa::BM, 1};
   const int64_t tiles = k_tokens / std::max<int64_t>(1, sequences) / pa::BN, blocks = unit_count(map) * kv_heads;
-  if (blocks >= pa::FEW_BLOCKS && tiles > (group >= 4 ? 16 : 8)) return p;
+  const bool one_block = q_tokens * group <= pa::BM * sequences;  // of 256 rows a sequence
+  if (blocks >= pa::FEW_BLOCKS && tiles > (one_block ? 8 : 16)) return p;
   p.per = map.per = pa::BM / 2;
   // At most two workgroups a CU.  (unit_count bounds them: a unit a sequence fewer where lengths are whole
   // multiples.  What then passes 512 waits for a whole turn in heads of 128, which fill a CU with two; in
