@@ -430,7 +430,8 @@ int nt_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t*
  * cache_dtype is dtype (F16 or BF16), or NT_DTYPE_E4M3 with k_scale, v_scale [pages, heads] (contiguous):
  * stored is x / scale, with scale the least power of two (from 2^-64 on) for which 448 scale is
  * at least the page's largest finite value.  A page whose slot 0 is among the new tokens takes a
- * scale afresh; else the scale only grows, and what the page held before the new slots is divided to match.
+ * scale afresh; else the scale only grows, and all that the page holds in other slots is divided to match, behind
+ * the new ones too, so that it keeps its value.
  * Infinities are stored as NaN.  dim a multiple of 4 up to 128; pages of 8 bits up to 128 slots.
  * The two caches must not overlap; at most 65535 heads and 2^31 - 1 tokens. */
 int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,

@@ -474,17 +474,28 @@ __global__ __launch_bounds__(256, N == 8 && HOLD == 4 ? 2 : 3) void append8_kern
     const float fitting = ldexpf(1.0f, fitting_exponent(most));
     const float scale = slot0 ? fmaxf(old, fitting) : fitting, inverse = 1.0f / scale;
     if (threadIdx.x == 0) *scale_at = scale;
-    if (slot0 && scale != old) {  // what the page held follows its scale
+    if (slot0 && scale != old) {  // what the page held follows its scale, before the new slots and behind them
       const float ratio = old * inverse;
-      for (int i = threadIdx.x; i < slot0 * (g.dim / 4); i += 256) {
-        const int t = i / (g.dim / 4), d = (i - t * (g.dim / 4)) * 4;
+      const int quarter = g.dim / 4, begin = slot0 * quarter, end = begin + u.count * quarter;
+      for (int i = threadIdx.x; i < g.page_size * quarter; i += 256) {
+        if (i >= begin && i < end) continue;
+        const int t = i / quarter, d = (i - t * quarter) * 4;
         uint8_t* row = cache + t * g.cs[which][1] + d;
-        float z[4];
+        uint32_t q = 0;
+        if constexpr (UNIT) {
+          q = *(const uint32_t*)row;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = __builtin_amdgcn_cvt_f32_fp8((int)row[e], 0) * ratio;
-        const uint32_t q = e4m3_of(z[0], z[1], z[2], z[3]);
+          for (int e = 0; e < 4; ++e) q |= (uint32_t)row[e] << (8 * e);
+        }
+        q = e4m3_of(__builtin_amdgcn_cvt_f32_fp8((int)q, 0) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)q, 1) * ratio,
+                    __builtin_amdgcn_cvt_f32_fp8((int)q, 2) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)q, 3) * ratio);
+        if constexpr (UNIT) {
+          *(uint32_t*)row = q;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) row[e] = (uint8_t)(q >> (8 * e));
+          for (int e = 0; e < 4; ++e) row[e] = (uint8_t)(q >> (8 * e));
+        }
       }
     }
     each([&](const Item& it, int t, const float (&y)[2 * N]) {

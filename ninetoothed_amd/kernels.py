@@ -825,7 +825,7 @@ def bind_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=N
 
     Caches of ``torch.float8_e4m3fn`` hold x / scale with a scale for each page and head (k_scale,
     v_scale [pages, heads], fp32): the least power of two that fits the page's largest value to 448,
-    taken afresh when the page's slot 0 is written, and growing (the slots before the new ones then
+    taken afresh when the page's slot 0 is written, and growing (the page's other slots then
     follow) when a later token needs it.  Infinities are stored as NaN."""
     cache_code = check_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs,
                                     interleaved, magnitude)
