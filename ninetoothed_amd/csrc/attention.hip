@@ -751,8 +751,9 @@ constexpr int VREG = STAGES * STAGE;       // V stages follow the K stages
 constexpr int LDS_BYTES = 2 * VREG;        // 128 KiB
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 // 16 bytes per lane from buffer `rs` at voffset + soffset into LDS at lds_addr + 16 * lane.
+// (The load reads M0, one wait state after it was written: the compiler counts none in inline assembly.)
 __device__ __forceinline__ void load_lds16(u32x4 rs, uint32_t lds_addr, int voffset, int soffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voffset), "s"(rs),
                  "s"(__builtin_amdgcn_readfirstlane(soffset))

@@ -456,8 +456,9 @@ __device__ __forceinline__ u32x4 rsrc(const void* base, uint32_t bytes) {
   return u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, bytes, 0x00020000u};
 }
 // 16 bytes per lane from buffer `rs` at voffset + soffset into LDS at lds_addr + 16 * lane.
+// (The load reads M0, one wait state after it was written: the compiler counts none in inline assembly.)
 __device__ __forceinline__ void load_lds16(u32x4 rs, uint32_t lds_addr, int voffset, int soffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds_addr), "v"(voffset), "s"(rs), "s"(soffset)
                : "memory", "m0");

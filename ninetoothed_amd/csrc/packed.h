@@ -97,16 +97,17 @@ __device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
                (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
 }
 // 16 bytes a lane, from buffer `rs` at offset + soffset or from an address of each lane's own, into
-// LDS at lds_addr + 16 * lane.  Nothing waits for them but wait_loads.
+// LDS at lds_addr + 16 * lane.  Nothing waits for them but wait_loads.  (The load reads M0, one wait state
+// after it was written: the compiler counts none in inline assembly.)
 __device__ __forceinline__ void buffer_to_lds(u32x4 rs, uint32_t lds_addr, int offset, int soffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(offset), "s"(rs),
                  "s"(__builtin_amdgcn_readfirstlane(soffset))
                : "memory", "m0");
 }
 __device__ __forceinline__ void global_to_lds(const void* p, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(p)
                : "memory", "m0");
