@@ -885,10 +885,13 @@ __global__ __launch_bounds__(ap::NW * 64) __attribute__((amdgpu_waves_per_eu(1, 
   const int npair = (nkt + 1) / 2;  // tile pairs of the workgroup
   auto issue = [&](int tp) {        // tile pair tp into stage tp % 4
     const uint32_t st = lds0 + (uint32_t)((tp & 3) * ap::STAGE) + (uint32_t)(4 * wave * 1024);
+    int ko = __builtin_amdgcn_readfirstlane(tp * kstep), vo = __builtin_amdgcn_readfirstlane(tp * vstep);
+    // (a load reads a scalar five wait states after a vector instruction wrote it, which tp's may be)
+    asm volatile("s_nop 4" : "+s"(ko), "+s"(vo));
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      ap::load_lds16(rsK, st + u * 1024, vk[u], tp * kstep);
-      ap::load_lds16(rsV, st + ap::VREG + u * 1024, vv[u], tp * vstep);
+      ap::load_lds16(rsK, st + u * 1024, vk[u], ko);
+      ap::load_lds16(rsV, st + ap::VREG + u * 1024, vv[u], vo);
     }
   };
   issue(0);

@@ -131,3 +131,17 @@ def test_a_load_into_lds_comes_a_wait_state_after_its_address(kernels):
     bad = violations(into_lds, lambda m, ops: {"m0"} if m.startswith("s_") and ops and ops[0] == "m0" else set(),
                      lambda m: 1, lambda m, ops: {"m0"} if "lds" in ops or "load_lds" in m else set())
     assert not bad, (len(bad), bad[:3])
+
+
+def test_a_load_comes_five_wait_states_after_a_vector_instruction_wrote_its_scalars(kernels):
+    # v_readfirstlane and comparisons write scalar registers that a memory instruction reads five wait states later.
+    def written(m, ops):
+        return {r for r in registers(ops[0]) if r[0] == "s" or r == "vcc"} if m.startswith("v_") and ops else set()
+
+    def read(m, ops):
+        if not m.startswith(("buffer_", "global_", "flat_", "scratch_")):
+            return set()
+        return {r for op in ops for r in registers(op)}
+
+    bad = violations(kernels, written, lambda m: 5, read)
+    assert not bad, (len(bad), bad[:3])
