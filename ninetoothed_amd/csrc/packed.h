@@ -82,6 +82,7 @@ struct Packed {
   P* ptr() { return (P*)(uintptr_t)*v++; }
 };
 
+// (Not of what a matrix instruction has just written: the compiler waits for those, but not in inline assembly.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));

@@ -488,10 +488,12 @@ prompt_stream_kernel(PromptArgs g) {
       return sum[0] + sum[1];
     };
     auto largest = [&]() __attribute__((always_inline)) {
-      float mx = max3(s[0][0], s[0][1], s[0][2]);
+      // (The first maximum is the compiler's, of both products: it waits until they are there, which it would not
+      // for inline assembly.)
+      float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-      for (int e = 3; e < 31; e += 2) mx = max3(mx, s[e >> 4][e & 15], s[(e + 1) >> 4][(e + 1) & 15]);
-      return max_halves(fmaxf(mx, s[1][15]));
+      for (int e = 1; e < 16; ++e) mx = max3(mx, s[0][e], s[1][e]);
+      return max_halves(mx);
     };
     if constexpr (FIRST) {
       const float mx = largest();
