@@ -298,8 +298,9 @@ __global__ __launch_bounds__(ca::NW * 64, EIGHT && DM == 64 ? 4 : 1) void cache_
         add[stage][kb] = ok ? 0.f : -INFINITY;
         if (EIGHT) {
           const float ks = ((ScalarFloats)(uintptr_t)g.k_scale)[page * (uint32_t)g.kv_heads + h];
-          k_sc[stage][kb] = ok ? ks : 0.f;
-          v_sc[stage][kb] = ((ScalarFloats)(uintptr_t)g.v_scale)[page * (uint32_t)g.kv_heads + h];
+          const float vs = ((ScalarFloats)(uintptr_t)g.v_scale)[page * (uint32_t)g.kv_heads + h];
+          k_sc[stage][kb] = ok ? ks : 0.f;  // (of no page: not those of page 0, which may be infinite)
+          v_sc[stage][kb] = ok ? vs : 1.f;
         }
       }
 #pragma unroll
