@@ -14,6 +14,7 @@ constexpr int BN = 64;             // keys per tile
 constexpr int MOST_SPLITS = 16;   // of a block's keys
 constexpr int FEW_BLOCKS = 512;   // of 256 rows
 constexpr float RESCALE_LOG2 = 8.0f;
+constexpr float UNSET = -3.0e38f;    // the max of no key, or of keys that all score -infinity: any other key grows it
 constexpr float MOST_SUM = 4096.0f;  // of a lane's 32 weights of a tile, each of which fp16 then holds
 // V^T rows: 64 keys + 8 pad.  Within each 16-key slice the keys lie in the order in which a
 // lane's P^T slots take them (0-3, 8-11 | 4-7, 12-15), so that a fragment is 16 contiguous bytes.
@@ -272,9 +273,9 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
 // one row, its max and sum take no LDS, and P^T goes from the score registers to the second product
 // as it is.
 //   - Scores stay unscaled in fp32 until exp2(s scale - m): q is not rounded a second time.
-//   - m is the max of a row's first tile, raised only where a later tile's weights grow past what
-//     MOST_SUM (or RESCALE_LOG2) allows (o and l are rescaled then): p keeps its relative precision, and
-//     o / l is the same.  Most tiles so take no max.
+//   - m is the max of a row's first tile (UNSET where that is minus infinity), raised only where a later tile's
+//     weights grow past what MOST_SUM (or RESCALE_LOG2) allows (o and l are rescaled then): p keeps its relative
+//     precision, and o / l is the same.  Most tiles so take no max.
 //   - p is rounded to the operands' type for the product; its row sums are of the rounded p.
 //   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
 //     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: rows of a
@@ -387,7 +388,7 @@ prompt_stream_kernel(PromptArgs g) {
 
   floatx16 o_acc[DBLK], s[2];
   frag pf[BN / 16];
-  float m = 0.f, l = 0.f;  // m: the first tile sets it to its max; l: of this lane's half of the keys
+  float m = UNSET, l = 0.f;  // m: the first tile sets it to its max; l: of this lane's half of the keys
 #pragma unroll
   for (int i = 0; i < DBLK; ++i)
 #pragma unroll
@@ -497,18 +498,18 @@ prompt_stream_kernel(PromptArgs g) {
     };
     if constexpr (FIRST) {
       const float mx = largest();
-      m = mx == -INFINITY ? 0.f : mx * c;
+      m = fmaxf(mx * c, UNSET);
       l = exponentials();
     } else {
       float sum = exponentials();
       if (__builtin_amdgcn_ballot_w64(!(sum <= MOST_SUM))) {
-        const float over = fmaxf(__builtin_fmaf(largest(), c, -m), 0.f), alpha = __builtin_amdgcn_exp2f(-over);
+        const float grown = fmaxf(largest() * c, m), alpha = __builtin_amdgcn_exp2f(m - grown);
         l *= alpha;
 #pragma unroll
         for (int i = 0; i < DBLK; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o_acc[i][r] *= alpha;
-        m += over;
+        m = grown;
         sum = exponentials();
       }
       l += sum;
@@ -785,7 +786,7 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       }
     }
   };
-  float m = 0.f;  // the first tile sets it to its max
+  float m = 0.f;  // the first tile with a key that counts sets it to its max
 #pragma unroll
   for (int r = 0; r < 16; ++r) l_acc[r] = 0.f;
 #pragma unroll
@@ -848,9 +849,10 @@ __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const bool grow = (kt == 0 && mx != -INFINITY) || mx > RESCALE_LOG2;
+    const bool first = l_acc[0] == 0.f;  // (no key counted yet: the row's max weight is 1 where it was taken)
+    const bool grow = (first && mx != -INFINITY) || mx > RESCALE_LOG2;
     if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float delta = grow ? mx : 0.f, alpha = kt == 0 ? 1.f : __builtin_amdgcn_exp2f(-delta);
+      const float delta = grow ? mx : 0.f, alpha = first ? 1.f : __builtin_amdgcn_exp2f(-delta);
 #pragma unroll
       for (int r = 0; r < 16; ++r) l_acc[r] *= alpha;
 #pragma unroll
