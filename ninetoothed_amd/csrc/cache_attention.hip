@@ -92,7 +92,7 @@ struct CacheArgs {
   const int32_t *tables, *lengths;
   int64_t table_stride, pages;
   int sequences, kv_heads, group, dim, page_size, table_width, row_blocks, parts;
-  int q_vectors, join_rows;
+  int q_vectors, join_rows, first_join;  // (workgroup of this launch)
   int page_shift;  // page_size = 16 << page_shift, or -1
   float scale_log2;
   float *part_o, *part_ml;  // partial states, two a workgroup: [slot][row][DM], [slot][row][2]
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs g) {
   __shared__ float4 part[GROUPS][LANES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunks = (min(g.group, BQ) + g.join_rows - 1) / g.join_rows;
-  int id = cache_workgroup<EIGHT, DM>();
+  int id = g.first_join + cache_workgroup<EIGHT, DM>();
   const int h = id % g.kv_heads;  // (first: on the XCD whose L2 the head's states were written to)
   id /= g.kv_heads;
   const int chunk = id % chunks;
@@ -686,7 +686,7 @@ static int64_t cache_parts(int64_t kv_heads, int64_t blocks, bool eight, bool wi
 }
 
 template <typename T, bool EIGHT, int DM>
-static void cache_launch(const CacheArgs& g, int64_t join_grid, hipStream_t stream) {
+static void cache_launch(CacheArgs g, int64_t join_grid, hipStream_t stream) {
   const dim3 grid((unsigned)(g.parts * g.kv_heads)), block(ca::NW * 64);
   // (in whole sixteens a page's place and its slots are reckoned in 32 bits)
   const int64_t es = EIGHT ? 1 : 2;
@@ -695,8 +695,10 @@ static void cache_launch(const CacheArgs& g, int64_t join_grid, hipStream_t stre
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, true>), grid, block, 0, stream, g);
   else
     hipLaunchKernelGGL((cache_attention_kernel<T, EIGHT, DM, false>), grid, block, 0, stream, g);
-  if (join_grid)
-    hipLaunchKernelGGL((cache_join_kernel<T, EIGHT, DM>), dim3((unsigned)join_grid), dim3(256), 0, stream, g);
+  in_launches(join_grid, 256, [&](int64_t first, unsigned count) {
+    g.first_join = (int)first;
+    hipLaunchKernelGGL((cache_join_kernel<T, EIGHT, DM>), dim3(count), dim3(256), 0, stream, g);
+  });
 }
 
 }  // namespace nt

@@ -119,6 +119,15 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
+// f(first, count) for the workgroups of a grid, launch by launch: one takes less than 2^32 threads (a larger grid
+// wraps around and leaves the rest out, with no error).
+template <typename F>
+inline void in_launches(int64_t workgroups, int threads, F&& f) {
+  const int64_t most = (1LL << 31) / threads;
+  for (int64_t first = 0; first < workgroups; first += most)
+    f(first, (unsigned)(workgroups - first < most ? workgroups - first : most));
+}
+
 // N neighbouring elements as they lie in memory.
 template <typename S, int N>
 struct alignas(sizeof(S) * N) Vec {

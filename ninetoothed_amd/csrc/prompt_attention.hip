@@ -96,6 +96,7 @@ struct PromptArgs {
   UnitMap map;                         // of q's rows: tokens * group
   const int32_t* k_starts;
   int64_t k_tokens, units;
+  int first_block;  // of this launch
   int kv_heads, group, dim, causal, by_sequence;
   float scale_log2;  // softmax scale * log2(e)
   // Keys of a block of rows over several workgroups: their partial states in the workspace, for each
@@ -120,8 +121,9 @@ __device__ __forceinline__ PromptBlock find_block(const PromptArgs& g) {
   // Ids go to the 8 XCDs round-robin, each with its own L2: where the heads divide by 8, an XCD
   // keeps to the K and V of heads of its own.
   const int BM = g.map.per;
-  p.head = (int)(blockIdx.x % g.kv_heads);
-  const int64_t nth = blockIdx.x / g.kv_heads, id = g.splits == 1 ? nth : nth / g.splits;
+  const uint32_t wg = g.first_block + blockIdx.x;
+  p.head = (int)(wg % g.kv_heads);
+  const int64_t nth = wg / g.kv_heads, id = g.splits == 1 ? nth : nth / g.splits;
   p.split = g.splits == 1 ? 0 : (int)(nth - id * g.splits);
   auto k_clamp = [&](int64_t s) { return s < 0 ? 0 : s > g.k_tokens ? g.k_tokens : s; };
   auto sequence = [&](int b) {
@@ -1002,7 +1004,6 @@ static int prompt_launch(PromptArgs g, void* workspace, int64_t workspace_bytes,
   // heads, 2.3 turns, 90 / 105.
   const bool turns = blocks * plan.per / 32 >= 4 * 256 * (g.dim <= 64 ? 16 : 8);
   g.by_sequence = g.map.sequences > 64 || (turns && (g.dim > 64 || g.map.sequences >= 32));
-  const dim3 grid((unsigned)blocks), block(plan.per * 2);
 #define NT_PROMPT(DM)                                                                \
   if (!vec)                                                                          \
     hipLaunchKernelGGL((prompt_elements_kernel<T, DM>), grid, block, 0, stream, g);  \
@@ -1010,11 +1011,15 @@ static int prompt_launch(PromptArgs g, void* workspace, int64_t workspace_bytes,
     hipLaunchKernelGGL((prompt_stream_kernel<T, DM, 8>), grid, block, 0, stream, g); \
   else                                                                               \
     hipLaunchKernelGGL((prompt_stream_kernel<T, DM, 4>), grid, block, 0, stream, g);
-  if (g.dim <= 64) {
-    NT_PROMPT(64)
-  } else {
-    NT_PROMPT(128)
-  }
+  in_launches(blocks, plan.per * 2, [&](int64_t first, unsigned count) {
+    const dim3 grid(count), block(plan.per * 2);
+    g.first_block = (int)first;
+    if (g.dim <= 64) {
+      NT_PROMPT(64)
+    } else {
+      NT_PROMPT(128)
+    }
+  });
 #undef NT_PROMPT
   const int64_t head_rows = g.map.tokens * g.group;
   if (plan.splits > 1 && g.dim <= 64)

@@ -13,7 +13,7 @@ struct RotaryArgs {
   const void* positions;
   int64_t position_stride;
   const double* freqs;
-  int64_t tokens;
+  int64_t tokens, first_block;  // (of this launch: of four tokens)
   int heads, dim, pairs, heads_per_wave;
   int long_positions, interleaved, inverse;
   float magnitude;
@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs g) {
   typedef typename elem<T>::storage S;
   __shared__ float2 turn_all[4][ROTARY_PAIRS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t token = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t token = (g.first_block + blockIdx.x) * 4 + wave;
   if (token >= g.tokens) return;
   const int64_t at = token * g.position_stride;
   const int64_t position =
@@ -136,15 +136,18 @@ static int rotary_launch(RotaryArgs g, hipStream_t stream) {
   g.heads_per_wave = (int)cdiv(g.heads, splits);
   const int64_t blocks = cdiv(g.tokens, 4), parts = cdiv(g.heads, g.heads_per_wave);
   if (blocks > 0x7fffffffLL || parts > 65535) return NT_ERR_INVALID;
-  const dim3 grid((unsigned)blocks, (unsigned)parts), block(256);
-  if (n == full && past)
-    hipLaunchKernelGGL((rotary_kernel<T, full, true, true>), grid, block, 0, stream, g);
-  else if (n == full)
-    hipLaunchKernelGGL((rotary_kernel<T, full, true, false>), grid, block, 0, stream, g);
-  else if (n == full / 2)
-    hipLaunchKernelGGL((rotary_kernel<T, full / 2, true, false>), grid, block, 0, stream, g);
-  else
-    hipLaunchKernelGGL((rotary_kernel<T, 1, false, false>), grid, block, 0, stream, g);
+  in_launches(blocks, 256, [&](int64_t first, unsigned count) {
+    const dim3 grid(count, (unsigned)parts), block(256);
+    g.first_block = first;
+    if (n == full && past)
+      hipLaunchKernelGGL((rotary_kernel<T, full, true, true>), grid, block, 0, stream, g);
+    else if (n == full)
+      hipLaunchKernelGGL((rotary_kernel<T, full, true, false>), grid, block, 0, stream, g);
+    else if (n == full / 2)
+      hipLaunchKernelGGL((rotary_kernel<T, full / 2, true, false>), grid, block, 0, stream, g);
+    else
+      hipLaunchKernelGGL((rotary_kernel<T, 1, false, false>), grid, block, 0, stream, g);
+  });
   return launch_status();
 }
 
@@ -156,7 +159,7 @@ struct AppendArgs {
   const int32_t *tables, *lengths;
   const double* freqs;
   UnitMap map;
-  int64_t table_stride, pages;
+  int64_t table_stride, pages, first_unit;  // (of this launch)
   int heads, dim, pairs, page_size, table_width, heads_per_block, interleaved;
   float magnitude;
   Divider per_row, per_token;  // items of a row, and of a token's heads of one workgroup
@@ -298,7 +301,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs g) {
   constexpr int U = 2;
   extern __shared__ float2 turn[];
   __shared__ int64_t row_at[APPEND_TOKENS];  // of a token in the cache, or -1
-  const AppendUnit u = append_unit(g, blockIdx.x);
+  const AppendUnit u = append_unit(g, g.first_unit + blockIdx.x);
   if (u.count == 0) return;
   const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
   const int pairs = which == 0 ? g.pairs : 0;
@@ -390,7 +393,7 @@ __global__ __launch_bounds__(256, N == 8 && HOLD == 4 ? 2 : 3) void append8_kern
   typedef AppendItem<T, N, UNIT> Item;
   extern __shared__ float2 turn[];
   __shared__ float largest[2][4];
-  const AppendUnit u = append_unit(g, blockIdx.x);
+  const AppendUnit u = append_unit(g, g.first_unit + blockIdx.x);
   if (u.count == 0) return;
   const int which = blockIdx.z, head0 = blockIdx.y * g.heads_per_block;
   const int nheads = min(g.heads - head0, g.heads_per_block);
@@ -558,31 +561,34 @@ static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
   g.per_token = divider(per_row * g.heads_per_block);
   const bool past = 4 * g.map.tokens * g.heads * g.dim >= PAST_CACHES;
   const int64_t most_tokens = std::min<int64_t>(g.map.per, g.map.tokens);
-  const dim3 grid((unsigned)units, (unsigned)y, 2), block(256);
   const size_t lds = turn_bytes(most_tokens, g.pairs, n);
 #define NT_APPEND(...) hipLaunchKernelGGL((__VA_ARGS__), grid, block, lds, stream, g)
-  if (!eight) {
-    if (n == 8 && past)
-      NT_APPEND(append_kernel<T, 8, true, true>);
-    else if (n == 8)
-      NT_APPEND(append_kernel<T, 8, true, false>);
-    else if (n == 4)
-      NT_APPEND(append_kernel<T, 4, true, false>);
-    else
-      NT_APPEND(append_kernel<T, 1, false, false>);
-  } else if (n == 8) {
-    const int64_t items = cdiv(most_tokens * per_row, 256);  // of a lane
-    if (items <= 1)
-      NT_APPEND(append8_kernel<T, 8, true, 1>);
-    else if (items <= 2)
-      NT_APPEND(append8_kernel<T, 8, true, 2>);
-    else
-      NT_APPEND(append8_kernel<T, 8, true, 4>);
-  } else if (n == 4) {
-    NT_APPEND(append8_kernel<T, 4, true, 4>);
-  } else {
-    NT_APPEND(append8_kernel<T, 1, false, 4>);
-  }
+  in_launches(units, 256, [&](int64_t first, unsigned count) {
+    const dim3 grid(count, (unsigned)y, 2), block(256);
+    g.first_unit = first;
+    if (!eight) {
+      if (n == 8 && past)
+        NT_APPEND(append_kernel<T, 8, true, true>);
+      else if (n == 8)
+        NT_APPEND(append_kernel<T, 8, true, false>);
+      else if (n == 4)
+        NT_APPEND(append_kernel<T, 4, true, false>);
+      else
+        NT_APPEND(append_kernel<T, 1, false, false>);
+    } else if (n == 8) {
+      const int64_t items = cdiv(most_tokens * per_row, 256);  // of a lane
+      if (items <= 1)
+        NT_APPEND(append8_kernel<T, 8, true, 1>);
+      else if (items <= 2)
+        NT_APPEND(append8_kernel<T, 8, true, 2>);
+      else
+        NT_APPEND(append8_kernel<T, 8, true, 4>);
+    } else if (n == 4) {
+      NT_APPEND(append8_kernel<T, 4, true, 4>);
+    } else {
+      NT_APPEND(append8_kernel<T, 1, false, 4>);
+    }
+  });
 #undef NT_APPEND
   return launch_status();
 }

@@ -7,7 +7,8 @@ import torch
 
 from ninetoothed_amd import kernels
 
-from test_cache_ops_gpu import BF16, DEV, E4M3, F16, attended, attention_tol, caches, close, i32, randn, starts_of
+from test_cache_ops_gpu import (BF16, DEV, E4M3, F16, attended, attention_tol, caches, close, i32, randn, rotary_tol,
+                                starts_of, turned)
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,74 @@ def test_keys_of_no_weight_come_first(dim, dtype, causal):
             # less than 2^-10, and the weights and their sum by as much)
             close(out[a:a + n, h], o, attention_tol(o, size, dtype, n, 5.0) + 2.0**-9 * size, f"{n} keys, head {h}")
     assert (out[starts[2]:] == 0).all()  # (nothing but keys of no weight)
+
+
+def test_rotary_of_more_tokens_than_one_launch_takes():
+    # 2^32 threads and more: a grid of 2^24 workgroups of 256 takes 2^26 tokens
+    tokens = (1 << 26) + 1027
+    x = torch.empty(tokens, 1, 2, dtype=BF16, device=DEV)
+    x[..., 0], x[..., 1] = 1.0, 0.5
+    positions = torch.arange(tokens, dtype=torch.int32, device=DEV)
+    freqs = torch.full((1,), 0.001, dtype=torch.float64, device=DEV)
+    out = kernels.rotary(x, positions, freqs, torch.zeros_like(x))
+    for part in (slice(0, 5000), slice((1 << 26) - 5000, tokens)):
+        want, size = turned(x[part], positions[part], freqs, False)
+        close(out[part], want, rotary_tol(want, size, BF16))
+    assert (out != 0).any(-1).all()
+
+
+def test_append_of_more_sequences_than_one_launch_takes():
+    # 2^23 sequences have 2^24 workgroups kept for them; one token each, of which eight have a page
+    tokens, dim = (1 << 23) + 77, 16
+    kc, vc = (torch.zeros(8, 4, 1, dim, dtype=F16, device=DEV) for _ in range(2))
+    tables = torch.full((tokens, 1), -1, dtype=torch.int32, device=DEV)
+    tables[:4, 0], tables[-4:, 0] = torch.arange(4, device=DEV), torch.arange(4, 8, device=DEV)
+    starts = torch.arange(tokens + 1, dtype=torch.int32, device=DEV)
+    k = torch.arange(tokens, device=DEV).remainder(1009).to(F16)[:, None, None].expand(tokens, 1, dim)
+    kernels.cache_append(k, -k, kc, vc, tables, torch.zeros_like(tables[:, 0]), starts)
+    used = torch.cat([k[:4], k[-4:]])
+    assert torch.equal(kc[:, 0], used) and torch.equal(vc[:, 0], -used) and (kc[:, 1:] == 0).all()
+
+
+def test_append_of_more_pages_than_one_launch_takes():
+    # pages of one slot: a workgroup each
+    tokens, dim = (1 << 24) + 1027, 16
+    kc, vc = (torch.zeros(tokens, 1, 1, dim, dtype=E4M3, device=DEV) for _ in range(2))
+    ks, vs = (torch.zeros(tokens, 1, device=DEV) for _ in range(2))
+    tables = torch.arange(tokens, dtype=torch.int32, device=DEV)[None]
+    k = torch.exp2(torch.arange(tokens, device=DEV).remainder(13).float()).to(F16)[:, None, None].expand(tokens, 1, dim)
+    kernels.cache_append(k, -k, kc, vc, tables, i32([0]), i32([0, tokens]), k_scale=ks, v_scale=vs)
+    for c, s, sign in ((kc, ks, 1), (vc, vs, -1)):
+        for a in range(0, tokens, 1 << 22):
+            at = slice(a, a + (1 << 22))
+            assert torch.equal(c[at, 0].float() * s[at][:, :, None] * sign, k[at].float())
+
+
+def test_prompts_of_more_sequences_than_one_launch_takes():
+    # one token each, so that each query's output is its value; 16 heads of 2^20 sequences are 2^24 workgroups
+    sequences, heads, dim = (1 << 20) + 77, 16, 8
+    v = (torch.arange(sequences * heads, device=DEV).remainder(2003).to(F16)).view(sequences, heads, 1).expand(-1, -1, dim)
+    v = v.contiguous()
+    q = torch.ones(sequences, heads, dim, dtype=F16, device=DEV)
+    starts = torch.arange(sequences + 1, dtype=torch.int32, device=DEV)
+    out = kernels.prompt_attention(q, q, v, torch.full_like(q, math.nan), starts, starts)
+    assert torch.equal(out, v)
+
+
+def test_joins_of_more_states_than_one_launch_takes():
+    # 32,768 sequences of 512 heads: 2^24 workgroups; sequence 16,416 is split between two workgroups a head
+    sequences, heads, dim, page = (1 << 15) + 64, 512, 16, 16
+    few = 16
+    q = randn(few, heads, dim, dtype=F16)
+    kc, vc = caches((9, page, heads, dim), E4M3)
+    ks, vs = (torch.full((9, heads), 2.0**-7, device=DEV) for _ in range(2))
+    tables = torch.arange(9, dtype=torch.int32, device=DEV)[None]
+    want = kernels.cache_attention(q, kc, vc, tables.expand(few, 9), i32([144] * few), torch.empty_like(q), ks, vs)
+    lengths = torch.full((sequences,), 144, dtype=torch.int32, device=DEV)
+    lengths[0] = 100  # (one block of 128 keys, the others two)
+    many = q.repeat(sequences // few, 1, 1)
+    out = kernels.cache_attention(many, kc, vc, tables.expand(sequences, 9), lengths, torch.full_like(many, math.nan), ks, vs)
+    # either is off by its rounding and that of its weights, 2^-11 each, and by 2^-12 for its scores, of at most 3.5
+    tol = 2 * (want.abs().double() * 2.0**-11 + 3.5 * (2.0**-11 + 2.0**-12 + 144 * 2.0**-25))
+    err = (out.view(-1, few, heads, dim) - want).double().abs().view(sequences, heads, dim)[1:]
+    assert (err <= tol.repeat(sequences // few, 1, 1)[1:]).all() and out[0].isfinite().all()
