@@ -738,8 +738,8 @@ def rotary(x, positions, freqs, out, interleaved=False, inverse=False, magnitude
     return out
 
 
-def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, heads, dim):
-    """The element-type code of a pair of caches for tokens of ``dtype``."""
+def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, heads, dim, multiple):
+    """The element-type code of a pair of caches for tokens of ``dtype`` and heads of a ``multiple`` of elements."""
     import torch
 
     if dtype not in (torch.float16, torch.bfloat16):
@@ -754,8 +754,8 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, heads, dim):
     eight = k_cache.dtype == torch.float8_e4m3fn
     if not eight and k_cache.dtype != dtype:
         raise TypeError(f"caches must be {dtype} or torch.float8_e4m3fn")
-    if dim % 16 or not 0 < dim <= 128:
-        raise ValueError("a cache's head dim must be a multiple of 16 up to 128")
+    if dim % multiple or not 0 < dim <= 128:
+        raise ValueError(f"a cache's head dim must be a multiple of {multiple} up to 128")
     if page_size < 1 or (eight and page_size > 128):
         raise ValueError("pages must have at least one slot, and at most 128 in 8 bits")
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
@@ -799,7 +799,7 @@ def check_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=
     tokens, heads, dim = k.shape
     if tokens > 0x7FFFFFFF or heads > 65535:
         raise ValueError("cache_append takes less than 2^31 tokens of at most 65535 heads")
-    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, heads, dim)
+    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, heads, dim, 4)
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _check_written(t, name)
     _check_tables(tables, lengths)
@@ -814,7 +814,8 @@ def bind_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=N
                       interleaved=False, magnitude=1.0):
     """launch(k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs): the packed
     tokens' k, v [tokens, heads, dim] into the sequences' pages of the caches [pages, page_size, heads,
-    dim] (or any permutation of such storage that leaves elements side by side).
+    dim] (or any permutation of such storage that leaves elements side by side); dim is a multiple of 4 up to 128
+    (:func:`bind_cache_attention` reads those of 16).
 
     Sequence b's tokens are rows starts[b] to starts[b + 1]; the first goes to position lengths[b] (the
     number it has in the cache already; the caller counts on), which is slot position % page_size of
@@ -913,7 +914,7 @@ def check_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=Non
         raise TypeError("cache_attention q and out must share one dtype")
     if k_cache.dim() != 4:
         raise ValueError("caches must be [pages, page_size, heads, dim] tensors")
-    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, k_cache.shape[2], q.shape[2])
+    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, k_cache.shape[2], q.shape[2], 16)
     _check_heads(q.shape[1], k_cache.shape[2])
     _check_tables(tables, lengths)
     if tables.shape[0] != q.shape[0]:

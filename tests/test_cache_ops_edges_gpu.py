@@ -8,7 +8,7 @@ import torch
 from ninetoothed_amd import kernels
 
 from test_cache_ops_gpu import (BF16, DEV, E4M3, F16, attended, attention_tol, caches, close, i32, randn, rotary_tol,
-                                starts_of, turned)
+                                run_append, starts_of, turned)
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,9 @@ def test_joins_of_more_states_than_one_launch_takes():
     tol = 2 * (want.abs().double() * 2.0**-11 + 3.5 * (2.0**-11 + 2.0**-12 + 144 * 2.0**-25))
     err = (out.view(-1, few, heads, dim) - want).double().abs().view(sequences, heads, dim)[1:]
     assert (err <= tol.repeat(sequences // few, 1, 1)[1:]).all() and out[0].isfinite().all()
+
+
+@pytest.mark.parametrize("cache", (F16, E4M3))
+@pytest.mark.parametrize("dim,part", ((4, 4), (4, 2), (20, 16), (36, 36), (124, 2)))
+def test_append_of_heads_of_whole_fours(dim, part, cache):
+    run_append([33, 1, 70], [5, 31, 40], 32, 3, dim, part, F16, cache, interleaved=dim == 36)
