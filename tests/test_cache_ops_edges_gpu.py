@@ -7,8 +7,8 @@ import torch
 
 from ninetoothed_amd import kernels
 
-from test_cache_ops_gpu import (BF16, DEV, E4M3, F16, attended, attention_tol, caches, close, i32, randn, rotary_tol,
-                                run_append, starts_of, turned)
+from test_cache_ops_gpu import (BF16, DEV, E4M3, F16, attended, attention_tol, caches, check_append, close, i32, paged,
+                                randn, rotary_tol, run_append, starts_of, turned)
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +131,39 @@ def test_joins_of_more_states_than_one_launch_takes():
 @pytest.mark.parametrize("dim,part", ((4, 4), (4, 2), (20, 16), (36, 36), (124, 2)))
 def test_append_of_heads_of_whole_fours(dim, part, cache):
     run_append([33, 1, 70], [5, 31, 40], 32, 3, dim, part, F16, cache, interleaved=dim == 36)
+
+
+@pytest.mark.parametrize("cache", (F16, E4M3))
+@pytest.mark.parametrize("lengths,cached,page,heads,dim,part", (
+    ([200, 128], [70, 0], 128, 2, 80, 40),  # 8-byte vectors, more of a page's items than its lanes hold
+    ([40, 5, 1], [9, 17, 40], 32, 2, 48, 22),  # element by element, into pages that were begun
+    ([90, 300], [31, 100], 128, 2, 128, 128),  # 16-byte vectors, four items a lane
+))
+def test_append_of_every_width(lengths, cached, page, heads, dim, part, cache):
+    for dtype in (F16, BF16) if cache == E4M3 else (cache,):
+        run_append(lengths, cached, page, heads, dim, part, dtype, cache, interleaved=part == 22)
+
+
+@pytest.mark.parametrize("cache", (BF16, E4M3))
+@pytest.mark.parametrize("which", ("elements", "tokens", "caches"))
+def test_append_of_strided_and_unaligned_tensors(which, cache):
+    # k and v every other element of a wider tensor, or one element behind 16 bytes; caches one element behind them
+    lengths, cached, page, heads, dim = [100, 1, 60], [33, 15, 0], 64, 3, 64
+    tables, pages = paged([n + c for n, c in zip(lengths, cached)], page)
+    total = sum(lengths)
+    kc, vc = caches((pages, page, heads, dim), cache)
+    if which == "elements":
+        k, v = (randn(total, heads, 2 * dim, dtype=BF16, seed=i)[..., ::2] for i in (1, 2))
+    elif which == "tokens":
+        k, v = (randn(total * heads * dim + 1, dtype=BF16, seed=i)[1:].view(total, heads, dim) for i in (1, 2))
+    else:
+        k, v = (randn(total, heads, dim, dtype=BF16, seed=i) for i in (1, 2))
+        for i, c in enumerate((kc, vc)):
+            moved = torch.zeros(c.numel() + 1, dtype=cache, device=DEV)[1:].view(c.shape)
+            moved.copy_(c)
+            kc, vc = (moved, vc) if i == 0 else (kc, moved)
+    ks, vs = (torch.full((pages, heads), 2.0**-12, device=DEV) for _ in range(2)) if cache == E4M3 else (None, None)
+    freqs = kernels.rotary_frequencies(dim)
+    before = [None if t is None else t.clone() for t in (kc, vc, ks, vs)]
+    kernels.cache_append(k, v, kc, vc, tables, i32(cached), starts_of(lengths), k_scale=ks, v_scale=vs, freqs=freqs)
+    check_append(k, v, kc, vc, ks, vs, before, tables, cached, lengths, page, freqs, False)
