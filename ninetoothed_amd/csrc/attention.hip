@@ -1574,7 +1574,7 @@ static int attention_launch(const void* q, const int64_t* qs, const void* k, con
     int splits = config == 0 && !causal ? attention_splits(B * H, Sq, Sk) : 1;
     if (splits > 1 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < attention_workspace(B * H, Sq, Sk, D, splits)))
       splits = 1;
-    if (qblocks * B * H * splits > 0x7fffffffLL) return NT_ERR_INVALID;
+    if (!grid_fits(qblocks * B * H * splits, ak::NW * 64)) return NT_ERR_INVALID;
     g.q_blocks = (int)qblocks;
     g.splits = splits;
     g.part_o = (float*)workspace;
@@ -1603,7 +1603,7 @@ static int attention_launch(const void* q, const int64_t* qs, const void* k, con
   static_assert(ap::BM == NW * 32, "both fast kernels take 256 queries per workgroup");
   const int64_t bm = pipe || fast ? NW * 32 : AT_BM;
   const int64_t qblocks = cdiv(Sq, bm);
-  if (qblocks * B * H > 0x7fffffffLL) return NT_ERR_INVALID;
+  if (!grid_fits(qblocks * B * H, pipe || fast ? NW * 64 : AT_THREADS)) return NT_ERR_INVALID;
   g.q_blocks = (int)qblocks;
   const dim3 grid((unsigned)(qblocks * B * H)), blk(AT_THREADS);
   if (pipe) {
@@ -1793,7 +1793,7 @@ static int attention_f32_launch(const void* q, const int64_t* qs, const void* k,
   // Four waves splitting the keys of each query block when there are fewer than 512 blocks.
   const int64_t lpq = D <= 64 ? 1 : 2;
   const int64_t qblocks = cdiv(Sq, 64 / lpq);
-  if (qblocks * B * H > 0x7fffffffLL) return NT_ERR_INVALID;
+  if (!grid_fits(qblocks * B * H, 64)) return NT_ERR_INVALID;
   g.q_blocks = (int)qblocks;
   const bool split = qblocks * B * H < 512;
   const dim3 grid((unsigned)(qblocks * B * H));

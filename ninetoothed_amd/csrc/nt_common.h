@@ -104,6 +104,9 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 __host__ __device__ __forceinline__ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Whether one launch takes a grid: one of 2^32 threads or more wraps around and leaves the rest out, with no error.
+inline bool grid_fits(int64_t workgroups, int64_t threads) { return workgroups < (1LL << 32) / threads; }
+
 // Lanes of one wave exchanging data through LDS (a lane reads what other lanes wrote): the
 // hardware executes a wave's LDS instructions in program order, but the compiler may move
 // one lane's load above a store whose address it can prove differs for that lane, which

@@ -447,6 +447,23 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_any_kernel(const typename 
   }
 }
 
+// More segments than any kernel's one launch takes (1,024 lanes each) go out in pieces: f(x, y, rows, cols) on
+// some rows, or on some segments of one.
+template <typename F>
+static int softmax_pieces(const void* x, int64_t x_row, int64_t x_col, void* y, int64_t y_row, int64_t y_col,
+                          int64_t rows, int64_t cols, int64_t block, F&& f) {  // (strides in bytes)
+  const int64_t segs_per_row = cdiv(cols, block), segs = rows * segs_per_row;
+  const int64_t parts = cdiv(segs, (1LL << 32) / 1024 / 2);
+  const int64_t some_rows = cdiv(rows, parts), some_cols = rows > 1 ? cols : cdiv(segs_per_row, parts) * block;
+  for (int64_t r = 0; r < rows; r += some_rows)
+    for (int64_t c = 0; c < cols; c += some_cols) {
+      const int status = f((const char*)x + r * x_row + c * x_col, (char*)y + r * y_row + c * y_col,
+                           std::min(some_rows, rows - r), std::min(some_cols, cols - c));
+      if (status) return status;
+    }
+  return 0;
+}
+
 template <typename Ti, typename To>
 static void softmax_any_launch(const void* x, int64_t xs, int64_t xcs, void* y, int64_t ys, int64_t ycs, int64_t cols,
                                int64_t block, int64_t segs_per_row, int64_t segs, hipStream_t stream) {
@@ -476,6 +493,11 @@ static int softmax_launch(const void* x, int64_t xs, int64_t xcs, void* y, int64
   const int64_t segs_per_row = cdiv(cols, block);
   const int64_t segs = rows * segs_per_row;
   if (segs > 0x7fffffffLL) return NT_ERR_INVALID;
+  if (!grid_fits(segs, 1024))
+    return softmax_pieces(x, xs * sizeof(S), xcs * sizeof(S), y, ys * sizeof(S), ycs * sizeof(S), rows, cols, block,
+                          [&](const void* x, void* y, int64_t rows, int64_t cols) {
+                            return softmax_launch<T>(x, xs, xcs, y, ys, ycs, rows, cols, block, stream, config);
+                          });
   const bool unit = cols <= 1 || (xcs == 1 && ycs == 1);
   if (config == 6 || (config == 0 && !unit)) {
     softmax_any_launch<T, T>(x, xs, xcs, y, ys, ycs, cols, block, segs_per_row, segs, stream);
@@ -609,6 +631,13 @@ static int softmax_cast_to(const void* x, int64_t xs, int64_t xcs, void* y, int 
   const int64_t segs_per_row = cdiv(cols, block);
   const int64_t segs = rows * segs_per_row;
   if (segs > 0x7fffffffLL) return NT_ERR_INVALID;
+  if (!grid_fits(segs, SM_THREADS)) {
+    const int64_t xb = sizeof(typename elem<Ti>::storage), yb = y_dtype == NT_DTYPE_F32 ? 4 : 2;
+    return softmax_pieces(x, xs * xb, xcs * xb, y, ys * yb, ycs * yb, rows, cols, block,
+                          [&](const void* x, void* y, int64_t rows, int64_t cols) {
+                            return softmax_cast_to<Ti>(x, xs, xcs, y, y_dtype, ys, ycs, rows, cols, block, stream);
+                          });
+  }
   if (y_dtype == NT_DTYPE_F32)
     softmax_any_launch<Ti, float>(x, xs, xcs, y, ys, ycs, cols, block, segs_per_row, segs, stream);
   else if (y_dtype == NT_DTYPE_F16)
