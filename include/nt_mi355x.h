@@ -353,7 +353,8 @@ int nt_conv2d_noalloc_bf16(const void* x, const int64_t* x_strides, const void* 
  * whose q pre-scale is the constant 1.44269504089 and whose causal mask is
  * q_pos >= k_pos.  Tensors are [B, H, S, D] with arbitrary strides; D <= 128.
  * With no keys (Sk == 0) every output is zero, as torch's scaled_dot_product_attention
- * gives; q, k and v are then not read and may be null.
+ * gives; q, k and v are then not read and may be null.  A call whose query blocks (of 32 to 256 queries)
+ * pass the 2^32 threads of one launch is refused.
  * ------------------------------------------------------------------------- */
 int nt_attention_f16(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                      const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
@@ -423,15 +424,17 @@ int nt_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t*
               int64_t tokens, int64_t heads, int64_t dim, int64_t pairs, int interleaved, int inverse,
               float magnitude, hipStream_t stream);
 
-/* New tokens' k (rotated as above by their position) and v into a paged cache.  Token i of sequence
- * b gets position lengths[b] + i: slot position % page_size of page tables[b][position / page_size].
+/* New tokens' k (rotated as above by their position, where cosine and sine of tokens side by side may be products of
+ * two rotations in fp32) and v into a paged cache.  Token i of sequence b gets position lengths[b] + i: slot
+ * position % page_size of page tables[b][position / page_size].
  * A token past its table's width, or of a page outside [0, pages), is not stored.  Two sequences
  * may share pages, but no page into which this call writes for both.
  * cache_dtype is dtype (F16 or BF16), or NT_DTYPE_E4M3 with k_scale, v_scale [pages, heads] (contiguous):
  * stored is x / scale, with scale the least power of two (from 2^-64 on) for which 448 scale is
  * at least the page's largest finite value.  A page whose slot 0 is among the new tokens takes a
  * scale afresh; else the scale only grows, and all that the page holds in other slots is divided to match, behind
- * the new ones too, so that it keeps its value.
+ * the new ones too, so that it keeps its value but for a rounding by 2^-10 of the new scale where less than 2^-6
+ * of it is left.
  * Infinities are stored as NaN.  dim a multiple of 4 up to 128; pages of 8 bits up to 128 slots.
  * The two caches must not overlap; at most 65535 heads and 2^31 - 1 tokens. */
 int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
@@ -449,7 +452,8 @@ int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, cons
  * whose states (fp32) pass through `workspace` (16-byte aligned, nt_prompt_attention_workspace_size
  * bytes; 0: none wanted); with none or too little they are not split.  It holds nothing between calls, but
  * calls that may run at once need one each.  o must not overlap q, k or v.  Less than 2^31 - 255 keys, and
- * queries times heads / kv_heads; at most 2^20 heads. */
+ * queries times heads / kv_heads; at most 2^20 heads.  Weights and their sum are rounded to dtype for the product
+ * with v. */
 int64_t nt_prompt_attention_workspace_size(int64_t q_tokens, int64_t k_tokens, int64_t sequences, int64_t heads,
                                            int64_t kv_heads, int64_t dim);
 int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -462,7 +466,8 @@ int nt_prompt_attention(const void* q, const int64_t* q_strides, const void* k, 
  * page_size * table_width) of its pages: as above, not causal, with the cache's layouts and types;
  * E4M3 values count times their page's and head's scale (not negative; a v scale below 2^-64 counts
  * as 2^-64).  Keys of a page outside [0, pages) do not count; without keys the output is zero.
- * dim a multiple of 16 up to 128; caches 16-byte aligned, with strides of multiples of 16 bytes.
+ * dim a multiple of 16 up to 128; caches 16-byte aligned, with strides of multiples of 16 bytes.  Weights are
+ * rounded to the cache's type (8 bits: F16) for the product with v.
  * The workspace (16-byte aligned, nt_cache_attention_workspace_size bytes, 0: none needed) holds
  * partial states of sequences whose keys are split over workgroups; nothing between calls, but calls that
  * may run at once need one each.  o must not overlap the inputs. */

@@ -178,19 +178,22 @@ __device__ __forceinline__ int cache_workgroup() {
 // Per sequence and head of k and v, for the heads of q that share it (rows i):
 //   s_ij = scale q_i . (kq_j ks_j),  o_i = sum_j p_ij (vq_j vs_j) / sum_j p_ij,  p_ij = exp(s_ij - m_i)
 // over its cached keys; an empty sequence gives zeros.
-// HBM-bound: each cached element is read once, 4 group flops for each.  The rows of a group are
-// the columns of 16 x 16 x 32 products, so that MHA to MQA read the cache once: S^T = K Q^T, with
-// keys as the rows, and O^T += V^T P^T.  Every wave streams 32 keys at a time through two LDS stages
+// HBM-bound: each cached element is read once for up to 16 heads that share it, 4 group flops for each.  The
+// rows of a group are the columns of 16 x 16 x 32 products: S^T = K Q^T, with keys as the rows, and O^T += V^T P^T.
+// More heads take the line once for each 16 (32 sequences of 4,000 keys on one head, 16 / 32 / 48 heads of q:
+// bf16 23.6 / 32.0 / 42.1 us, 8 bits 19.7 / 23.0 / 32.3).  Every wave streams 32 keys at a time through two LDS stages
 // of its own (loads that bypass the registers, no barrier in the loop), so that 8 KiB (8 bits) or 16 a
 // wave are under way while it computes.  P^T goes from the scores' registers to the second product as it
 // is, and V, read eight keys by DM / 16 neighbouring elements a lane, is transposed by byte permutes.
 // 28 heads on 4 of 128, two sequences of 95,000 keys in fp16: 79 us, 4.9 TB/s; 32 on 8, 128 sequences of 100
 // to 9,000 keys in e4m3: 238 us, 4.9 TB/s, as a large copy; 8 of 4,000: 23 us, 2.8 TB/s, of which 9 are two
-// launches, the first loads and the join.
+// launches, the first loads and the join.  Short sequences are a tile a wave and a merge: 256 of 100 / 250 / 300 keys,
+// 32 heads on 8, bf16 38 / 70 / 73 us (1.8 / 1.3 / 1.1 times the bytes' time), 8 bits 21.5 / 43 / 51 (2.0 / 1.6 / 1.6).
 // 8 bits: e4m3 widens exactly, so k's scale multiplies the score and v's enters the weight:
 //   w_ij = exp2(s_ij + log2 vs_j - M_i),  o_i = sum_j w_ij vq_j / sum_j w_ij / vs_j,
 // with M the running max of the exponents: w stays within 2^8 for any scales, is rounded to fp16
-// (11 bits, also for bf16 queries) for the product with v, and its sum stays in fp32.
+// (11 bits, also for bf16 queries; below 2^-14 fewer, by 2^-25 at most) for the product with v, and its sum stays in
+// fp32.
 // SIXTEENS: pages are whole multiples of 16 keys, so that a load's keys lie in one page and its
 // address and scale are uniform; else each key's page is looked up.
 template <typename T, bool EIGHT, int DM, bool SIXTEENS>

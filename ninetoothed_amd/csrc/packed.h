@@ -133,7 +133,7 @@ template <typename S, int N>
 struct alignas(sizeof(S) * N) Vec {
   S e[N];
 };
-// Stores them; `past`: past the caches, as what is larger than these does not stay in them.
+// Stores them; `past`: past the caches (PAST_CACHES).
 template <typename S, int N>
 __device__ __forceinline__ void store_vec(S* p, const Vec<S, N>& v, bool past) {
   if constexpr (sizeof(v) == 16) {
@@ -141,8 +141,12 @@ __device__ __forceinline__ void store_vec(S* p, const Vec<S, N>& v, bool past) {
   }
   *(Vec<S, N>*)p = v;
 }
-// Bytes written from which 16-byte stores go past the caches (us without / with: a rotation of 67 MB
-// 34.5 / 22.6, of 13 MB 10.2 / 8.4, an append of 38 MB 21.0 / 19.0; 8-byte stores gain nothing).
+// Bytes written from which 16-byte stores go past the caches: they return sooner, and a call that reads the output
+// next may find less of it there.  us without / with, 32 heads of 128 on 8, bf16: a rotation of 8 / 17 / 34 / 67 / 134 MB
+// 6.3 / 5.3, 8.1 / 6.3, 14.5 / 11.7, 24.8 / 22.9, 47.7 / 42.5, and with the prompt attention over it 21.7 / 20.1,
+// 30.9 / 27.4, 46.8 / 47.5, 76.0 / 79.5, 170.5 / 166.1 (in place 75.4 / 74.5 at 67 MB); an append of 8 / 17 / 34 / 67 MB
+// 12.4 / 10.9, 16.6 / 14.7, 30.2 / 28.8, 39.8 / 40.6, and with a decode step over it 23.1 / 20.8, 27.8 / 26.6,
+// 46.4 / 45.0, 64.2 / 67.2.  8-byte stores gain nothing.
 constexpr int64_t PAST_CACHES = 8 << 20;
 
 // n / d for 0 <= n < 2^16 and 0 < d <= 2^15: floor(n ceil(2^32 / d) / 2^32), off by less than n / 2^32.

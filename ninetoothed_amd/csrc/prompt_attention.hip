@@ -267,8 +267,8 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
 // Per row i of a sequence (a token and a head of its group) over the keys j it may see:
 //   s_ij = scale q_i . k_j,  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i);
 // causal: j <= i + (keys - queries).  A row that sees no key gives zeros.
-// MFMA-bound: 4 dim flops a head and visible pair, and beside it the softmax's VALU work, which an MFMA
-// keeps waiting half of its time (bf16, 32 heads: 4 x 4,096 full 1,106 TFLOP/s in heads of 128, 1,028 in
+// MFMA-bound: 4 dim flops a head and visible pair, and beside it the softmax's VALU work, which hardly runs at the
+// same time (three prompts of 3,000 to 8,000: MFMAs take 53 % of the cycles, VALU instructions 41 %; bf16, 32 heads: 4 x 4,096 full 1,106 TFLOP/s in heads of 128, 1,028 in
 // heads of 64; causal, on 8 heads, 1 x 16,384 1,200, 4 x 4,096 1,034).  A workgroup takes 256 rows, a group's heads
 // side by side for each token, so that short sequences fill its rows and share K and V; eight waves
 // of 32 rows, two a SIMD.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: a lane holds
@@ -278,7 +278,8 @@ __device__ __forceinline__ void prompt_rows_by_key(const uint16_t* Q, const char
 //   - m is the max of a row's first tile (UNSET where that is minus infinity), raised only where a later tile's
 //     weights grow past what MOST_SUM (or RESCALE_LOG2) allows (o and l are rescaled then): p keeps its relative
 //     precision, and o / l is the same.  Most tiles so take no max.
-//   - p is rounded to the operands' type for the product; its row sums are of the rounded p.
+//   - p is rounded to the operands' type for the product (in fp16 by 2^-25 at most where it is small); its row sums
+//     are of the rounded p.
 //   - Keys past a sequence's end read as zeros (another sequence's rows lie there).  A causally
 //     masked key meets p = 0, which an infinite or NaN v would still turn into NaN: rows of a
 //     tile that is masked and holds one are taken key by key, each over the keys that it sees.
@@ -647,7 +648,8 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs g) {
 }
 
 // Any strides, element by element: keys and values through registers into two LDS stages of 64 keys,
-// waves 0-3 fetching K and 4-7 V, transposed in registers on the way.  (Here a tile that any row of the
+// waves 0-3 fetching K and 4-7 V, transposed in registers on the way (8 x 1,024, 32 heads on 8, causal, bf16, one
+// element off 16 bytes: heads of 128 789 us, of 64 198, where the streaming kernel takes 121 and 57; heads of 100 748).  (Here a tile that any row of the
 // workgroup masks gets its infinities and NaN taken out as it is stored.)
 template <typename T, int DM>
 __global__ __launch_bounds__(pa::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_elements_kernel(

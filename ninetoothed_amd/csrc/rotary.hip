@@ -197,7 +197,8 @@ __device__ __forceinline__ int64_t page_of(const AppendArgs& g, int sequence, ui
 // so that the lanes of a row read neighbours, and the rows of a wave do not meet in a bank.
 // They are taken for every eighth token and for eight tokens' steps, and multiplied:
 //   cos(a + b) = cos a cos b - sin a sin b, ...
-// which is a quarter of the angles of 64 tokens, and is off by four roundings of fp32.
+// which is a quarter of the angles of 64 tokens, and is off by four roundings of fp32 (so the last bit of a turned
+// key may differ from what rotary_kernel stores, and with the number of tokens of a unit).
 template <int N>
 __host__ __device__ constexpr int turn_row(int pairs) {
   return pairs + (N == 8 ? 8 : 0);
@@ -379,14 +380,16 @@ __device__ __forceinline__ int fitting_exponent(float x) {
 // The same into pages of e4m3 with a scale for each page and head.  The scale is a power of two,
 // the least that fits the page's largest value: the values of an 8-bit float lose nothing by that
 // (but for one binade of subnormals), and where a later token makes a page's scale grow, what
-// the page already holds is divided exactly.  A scale is taken afresh when a page is begun (its slot 0
+// the page already holds is divided by a power of two: exactly down to 2^-6 of the new scale, below which e4m3 is
+// subnormal, and rounded by 2^-10 of the new scale at most there, each time.  A scale is taken afresh when a page is begun (its slot 0
 // is among the new tokens); else it only grows.  Infinities and NaN are stored as NaN, which is
 // all that e4m3 has of them, and do not count for the scale.
 // A workgroup takes the new tokens of one page and some heads of k or of v: per head their values
 // are loaded, turned and held, HOLD items a lane (what is more is loaded and turned again), their largest
 // magnitude found, and stored.  Bound by what a page's head costs in series: load, largest, a barrier,
 // store; the next head's loads are under way meanwhile.  17,637 tokens of 8 x 128 bf16 in pages of 64, 108 MB
-// read and written: 32.8 us, 3.3 TB/s; 64 single tokens 7.1 us, of which a launch is 4.
+// read and written: 32.8 us, 3.3 TB/s (fp16, whose two items a lane spill ten registers at three workgroups a CU:
+// 42.4); 64 single tokens 7.1 us, of which a launch is 4.
 template <typename T, int N, bool UNIT, int HOLD>
 __global__ __launch_bounds__(256, N == 8 && HOLD == 4 ? 2 : 3) void append8_kernel(AppendArgs g) {
   typedef typename elem<T>::storage S;
@@ -551,7 +554,9 @@ static int append_launch(AppendArgs g, bool eight, hipStream_t stream) {
   const int64_t units = unit_count(g.map);
   // All heads of a unit share its angles where there are enough units (and k and v) for that: 768 workgroups
   // a tensor (us at 512 / 768 / 1,024 / 2,048 / 4,096: 17,637 tokens in 8 bits 36.1 / 34.3 / 41.8 / 45 / 52,
-  // 4,636 of 32 x 64 in 16 bits 19.3 / 19.0 / 22.5 / 23.8 / 32).
+  // 4,636 of 32 x 64 in 16 bits 19.3 / 19.0 / 22.5 / 23.8 / 32).  Heads then fall unevenly at some lengths, which
+  // costs little: 10,000 / 12,000 / 14,000 / 15,000 / 16,000 / 17,600 / 20,000 tokens of 8 heads in pages of 64 take
+  // 23.5 / 24.9 / 27.4 / 29.8 / 29.5 / 32.4 / 35.6 us.
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.heads, 768 / std::max<int64_t>(1, units)));
   const int64_t per_row = g.dim / (2 * n);
   g.heads_per_block = (int)std::min<int64_t>(cdiv(g.heads, parts), 65535 / (APPEND_TOKENS * per_row));

@@ -820,14 +820,15 @@ def bind_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=N
     Sequence b's tokens are rows starts[b] to starts[b + 1]; the first goes to position lengths[b] (the
     number it has in the cache already; the caller counts on), which is slot position % page_size of
     page tables[b, position // page_size].  k is rotated by its position on the way (``freqs`` None:
-    not at all), as :func:`bind_rotary` rotates.  Tokens past a table's width or of a page number the
+    not at all), as :func:`bind_rotary` rotates, but for the last bit where several tokens' angles are
+    multiplied out of one's.  Tokens past a table's width or of a page number the
     cache does not have are not stored; a page may be written for one sequence only, and the two caches
     must not overlap.
 
     Caches of ``torch.float8_e4m3fn`` hold x / scale with a scale for each page and head (k_scale,
     v_scale [pages, heads], fp32): the least power of two that fits the page's largest value to 448,
-    taken afresh when the page's slot 0 is written, and growing (the page's other slots then
-    follow) when a later token needs it.  Infinities are stored as NaN."""
+    taken afresh when the page's slot 0 is written, and growing when a later token needs it (the page's other
+    slots then follow, rounded once more, by 2^-10 of the new scale at most, where less than 2^-6 of it is left).  Infinities are stored as NaN."""
     cache_code = check_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs,
                                     interleaved, magnitude)
     device = _check_device(k, v, k_cache, v_cache, tables, lengths, starts, k_scale, v_scale, freqs)
