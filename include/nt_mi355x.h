@@ -428,7 +428,7 @@ int nt_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t*
  * two rotations in fp32) and v into a paged cache.  Token i of sequence b gets position lengths[b] + i: slot
  * position % page_size of page tables[b][position / page_size].
  * A token past its table's width, or of a page outside [0, pages), is not stored.  Two sequences
- * may share pages, but no page into which this call writes for both.
+ * may share pages, but no page into which this call writes for both, or in two places of one table.
  * cache_dtype is dtype (F16 or BF16), or NT_DTYPE_E4M3 with k_scale, v_scale [pages, heads] (contiguous):
  * stored is x / scale, with scale the least power of two (from 2^-64 on) for which 448 scale is
  * at least the page's largest finite value.  A page whose slot 0 is among the new tokens takes a
@@ -436,7 +436,7 @@ int nt_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t*
  * the new ones too, so that it keeps its value but for a rounding by 2^-10 of the new scale where less than 2^-6
  * of it is left.
  * Infinities are stored as NaN.  dim a multiple of 4 up to 128; pages of 8 bits up to 128 slots.
- * The two caches must not overlap; at most 65535 heads and 2^31 - 1 tokens. */
+ * The two caches and the two scales must not overlap; at most 65535 heads and 2^31 - 1 tokens. */
 int nt_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int dtype,
                     void* k_cache, const int64_t* kc_strides, void* v_cache, const int64_t* vc_strides,
                     int cache_dtype, float* k_scale, float* v_scale, const int32_t* tables, int64_t table_stride,

@@ -822,8 +822,8 @@ def bind_cache_append(k, v, k_cache, v_cache, tables, lengths, starts, k_scale=N
     page tables[b, position // page_size].  k is rotated by its position on the way (``freqs`` None:
     not at all), as :func:`bind_rotary` rotates, but for the last bit where several tokens' angles are
     multiplied out of one's.  Tokens past a table's width or of a page number the
-    cache does not have are not stored; a page may be written for one sequence only, and the two caches
-    must not overlap.
+    cache does not have are not stored; a page may be written for one sequence only, in one place of its
+    table, and the two caches, or scales, must not overlap.
 
     Caches of ``torch.float8_e4m3fn`` hold x / scale with a scale for each page and head (k_scale,
     v_scale [pages, heads], fp32): the least power of two that fits the page's largest value to 448,
