@@ -49,8 +49,8 @@ class Kernel:
         self.name, self.code, self.labels = name, [], {}
 
     def behind(self, i, states):
-        """(instruction, wait states since i, walk) of what may be issued less than ``states`` wait states behind
-        instruction i, on every path; ``walk.send(True)`` ends that path."""
+        """Yields (mnemonic, operands, wait states since i) of what may be issued less than ``states`` wait states behind
+        instruction i, path by path; a true value sent back ends the path."""
         todo, seen = [(i + 1, 0)], set()
         while todo:
             j, passed = todo.pop()
