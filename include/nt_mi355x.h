@@ -480,12 +480,67 @@ int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_ca
                        int64_t kv_heads, int64_t dim, int64_t pages, int64_t page_size, int64_t table_width,
                        float scale, hipStream_t stream, void* workspace, int64_t workspace_bytes);
 
+/* Attention of a chunk of new tokens of each sequence, which are in the cache already, over its pages: q and o packed
+ * [tokens, heads, dim], sequence b's rows starts[b] to starts[b + 1]; it has lengths[b] keys (at most page_size *
+ * table_width), the new tokens' own last.  With `causal` query i sees the keys j <= i + (keys - queries), else all.
+ * Otherwise as nt_cache_attention: layouts, types, scales and pages that the cache does not have.  A query that
+ * sees no key gives zeros; rows behind the last sequence are left alone.  dim a multiple of 16 up to 128; caches 16-byte
+ * aligned, with strides of multiples of 16 bytes.  Weights are rounded to the cache's type (8 bits: F16); their sum is
+ * of the rounded ones in 16 bits, of the others in 8, where a v scale below 2^-64 counts as 0.  Less than 2^31 - 255 tokens times heads / kv_heads.  The workspace (16-byte aligned,
+ * nt_chunk_attention_workspace_size bytes, 0: none needed) holds partial states of rows whose keys are split over
+ * workgroups; nothing between calls, but calls that may run at once need one each.  o must not overlap the inputs. */
+int64_t nt_chunk_attention_workspace_size(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads,
+                                          int64_t dim, int64_t page_size, int64_t table_width, int cache_dtype);
+int nt_chunk_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,
+                       const void* v_cache, const int64_t* v_strides, int cache_dtype, const float* k_scale,
+                       const float* v_scale, void* o, const int64_t* o_strides, int dtype, const int32_t* tables,
+                       int64_t table_stride, const int32_t* lengths, const int32_t* starts, int64_t tokens,
+                       int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages,
+                       int64_t page_size, int64_t table_width, float scale, int causal, hipStream_t stream,
+                       void* workspace, int64_t workspace_bytes);
+
+/* Pages of a cache copied to others: the first counts[i] slots (null: all) of page sources[i] of both caches to page
+ * destinations[i], and with 8 bits the page's scales.  A pair with a page outside [0, pages) or of one page twice is
+ * passed over.  No page may be the destination of two pairs, or of one and the source of another.  Caches as those of
+ * nt_cache_append, of any slots and heads; strides of any size. */
+int nt_cache_copy(void* k_cache, const int64_t* k_strides, void* v_cache, const int64_t* v_strides, int cache_dtype,
+                  float* k_scale, float* v_scale, const int32_t* sources, const int32_t* destinations,
+                  const int32_t* counts, int64_t pairs, int64_t pages, int64_t page_size, int64_t heads, int64_t dim,
+                  hipStream_t stream);
+
+/* What a layer runs beside its attention.
+ *
+ * Root-mean-square norm of rows: s = x + residual (null: x), y = s / sqrt(mean(s^2) + eps) * weight, all in fp32; total =
+ * s rounded (written where there is a residual; it may lie on x or residual exactly), out = y rounded, or for out_dtype
+ * E4M3 y / scale with scale = the largest finite |y| / 448 (2^-64 at least) of a row, or with `group` (32, 64 or 128) of
+ * each so many elements: scale is [rows] or [rows, dim / group], side by side.  Infinite y are stored as NaN.  dtype F32,
+ * F16 or BF16 (x, weight, residual, total; out too where it is not E4M3).  Strides are those of (row, element).
+ * dim <= 65536.  out may lie on x exactly. */
+int nt_rms_norm(const void* x, const int64_t* x_strides, const void* weight, int64_t weight_stride,
+                const void* residual, const int64_t* residual_strides, void* total, const int64_t* total_strides,
+                void* out, const int64_t* out_strides, float* scale, int64_t group, int dtype, int out_dtype,
+                int64_t rows, int64_t dim, float eps, hipStream_t stream);
+
+/* out [rows, n] = c + x [rows, k] W^T, W[n][k] = scales[n][k / group] * (q[n][k] - zeros[n][k / group]) with q of 4
+ * bits, two to a byte of weight [n, k / 2] (element 2 i in the lower half of byte i); zeros null: 8, c null: 0.
+ * x, scales, zeros, c and out are of dtype F16 or BF16.  Strides are those of (row, element), in elements (weight:
+ * bytes).  group a multiple of 32 that divides k.  Sums in fp32, rounded once.  A row of x that holds an infinity
+ * gives NaN.  out may lie on c exactly, and must not overlap the others. */
+int nt_linear_4bit(const void* x, const int64_t* x_strides, const void* weight, const int64_t* weight_strides,
+                   const void* scales, const int64_t* scale_strides, const void* zeros, const int64_t* zero_strides,
+                   const void* c, const int64_t* c_strides, void* out, const int64_t* out_strides, int dtype,
+                   int64_t rows, int64_t n, int64_t k, int64_t group, hipStream_t stream);
+
 /* The same with their arguments in one array, in order: an int64 for each (pointers as their address,
- * a float as its bits), an array of strides as its three values. */
+ * a float as its bits), an array of strides as its values. */
 int nt_rotary_packed(const int64_t* v);
 int nt_cache_append_packed(const int64_t* v);
 int nt_prompt_attention_packed(const int64_t* v);
 int nt_cache_attention_packed(const int64_t* v);
+int nt_chunk_attention_packed(const int64_t* v);
+int nt_cache_copy_packed(const int64_t* v);
+int nt_rms_norm_packed(const int64_t* v);
+int nt_linear_4bit_packed(const int64_t* v);
 
 /* ---------------------------------------------------------------------------
  * Generic kernels for programs that match none of the families above.  They replace

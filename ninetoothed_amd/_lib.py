@@ -105,7 +105,14 @@ _SIGNATURES = {
     "nt_cache_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P, _P, _I64P, _I, _P, _I64, _P) + (_I64,) * 7
                           + (_F, _P, _P, _I64),
     "nt_cache_attention_workspace_size": (_I64,) * 6 + (_I,),
-    **{f"nt_{op}_packed": (_I64P,) for op in ("rotary", "cache_append", "prompt_attention", "cache_attention")},
+    "nt_rms_norm": (_P, _I64P, _P, _I64, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64, _I, _I, _I64, _I64, _F, _P),
+    "nt_linear_4bit": (_P, _I64P) * 6 + (_I,) + (_I64,) * 4 + (_P,),
+    "nt_cache_copy": (_P, _I64P, _P, _I64P, _I, _P, _P, _P, _P, _P) + (_I64,) * 5 + (_P,),
+    "nt_chunk_attention": (_P, _I64P, _P, _I64P, _P, _I64P, _I, _P, _P, _P, _I64P, _I, _P, _I64, _P, _P) + (_I64,) * 8
+                          + (_F, _I, _P, _P, _I64),
+    "nt_chunk_attention_workspace_size": (_I64,) * 7 + (_I,),
+    **{f"nt_{op}_packed": (_I64P,) for op in ("rotary", "cache_append", "prompt_attention", "cache_attention", "rms_norm",
+                                              "linear_4bit", "cache_copy", "chunk_attention")},
     "nt_rtc_compile": (ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_P), _I64P, ctypes.c_char_p, _I64),
     "nt_rtc_free": (_P,),
     "nt_rtc_load": (_P, ctypes.c_char_p, ctypes.POINTER(_P)),
@@ -113,7 +120,7 @@ _SIGNATURES = {
 }
 _RESTYPES = {"nt_conv2d_workspace_size": ctypes.c_int64, "nt_attention_workspace_size": ctypes.c_int64,
              "nt_gemm_workspace_size": ctypes.c_int64, "nt_cache_attention_workspace_size": ctypes.c_int64,
-             "nt_prompt_attention_workspace_size": ctypes.c_int64,
+             "nt_prompt_attention_workspace_size": ctypes.c_int64, "nt_chunk_attention_workspace_size": ctypes.c_int64,
              "nt_rtc_free": None}
 
 _lock = threading.Lock()

@@ -1,0 +1,341 @@
+// Products with weights of 4 bits and a scale (and zero point) for each group of a row's elements.
+#include "packed.h"
+#include "mfma_core.h"
+
+#include <algorithm>
+
+namespace nt {
+
+struct Linear4Args {
+  const void *x, *scales, *zeros, *c;
+  const uint8_t* weight;
+  void* out;
+  int64_t xs[2], ws[2], ss[2], zs[2], cs[2], os[2];  // row, element (weight: bytes)
+  int64_t rows, n, k, first;                         // (of this launch's workgroups)
+  int group;
+};
+
+namespace l4 {
+
+constexpr int WAVES = 8;
+constexpr int STEP = 128;  // elements of k a wave takes at a time: 16 bytes of weights a lane
+
+template <typename T>
+struct mma16;
+template <>
+struct mma16<f16_t> {
+  typedef half8 frag;
+  __device__ __forceinline__ static floatx4 mma(frag a, frag b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  // 16 + q: 1.0 2^4 with q in the mantissa's upper four bits
+  static constexpr uint32_t BASE = 0x4c004c00u, MASK = 0x03c003c0u, ONES = 0x3c003c00u;
+  static constexpr int AT = 6;
+};
+template <>
+struct mma16<bf16_t> {
+  typedef bf16x8 frag;
+  __device__ __forceinline__ static floatx4 mma(frag a, frag b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static constexpr uint32_t BASE = 0x41804180u, MASK = 0x00780078u, ONES = 0x3f803f80u;
+  static constexpr int AT = 3;
+};
+
+// The eight values q of a dword as 16 + q, exactly, in the order (0, 4), (1, 5), (2, 6), (3, 7) of pairs: a
+// shift, a mask and an or for two.
+template <typename T>
+__device__ __forceinline__ u32x4 wide8(uint32_t w) {
+  constexpr int AT = mma16<T>::AT;
+  u32x4 r;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t v = 4 * p <= AT ? w << (AT - 4 * p) : w >> (4 * p - AT);
+    r[p] = (v & mma16<T>::MASK) | mma16<T>::BASE;
+  }
+  return r;
+}
+// Eight neighbouring elements in that order.
+__device__ __forceinline__ u32x4 paired(u32x4 x) {
+  return u32x4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
+               __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
+}
+// Dword d of quad i's lanes to dword i of quad d's (a quad: 16 lanes).
+__device__ __forceinline__ u32x4 across_quads(u32x4 w) {
+  auto swap16 = [](uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+  };
+  auto swap32 = [](uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+  };
+  uint32_t a = w[0], b = w[1], c = w[2], d = w[3];
+  swap16(a, b);
+  swap16(c, d);
+  swap32(a, c);
+  swap32(b, d);
+  return u32x4{a, b, c, d};
+}
+
+}  // namespace l4
+
+// out = c + x W^T with w[n][k] = scale[n][k / group] (q[n][k] - zero[n][k / group]), q in 0 to 15, two to a byte (the
+// lower four bits first).  Sums in fp32, rounded once:
+//   out[m][n] = c[m][n] + sum_g scale[n][g] (sum_k x[m][k] (16 + q[n][k]) - (16 + zero[n][g]) sum_k x[m][k]),
+// where 16 + q is made from the bits, exact in either type, and the sums of x are a product with ones.
+// Bound by HBM for few rows: the weights are read once, 16 bytes a lane, by waves that share 16 NB columns and take
+// turns of 128 elements of k; x comes from the L2 for each of those workgroups.  A wave's 16 x 16 x 32 products take
+// 32 neighbouring elements of k, which lie in one group, so a turn's four dwords go across the quads first.
+// MB: blocks of 16 rows; SUB: products of a turn that share a group.
+template <typename T, int MB, int NB, int SUB>
+__global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) {
+  using namespace l4;
+  typedef mma16<T> M;
+  typedef typename M::frag frag;
+  constexpr int ROWS = MB * 16, COLS = NB * 16;
+  __shared__ float sums[WAVES][ROWS][COLS + 1];
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t m_tiles = (g.rows + ROWS - 1) / ROWS, id = g.first + blockIdx.x;
+  const int64_t m0 = id % m_tiles * ROWS, n0 = id / m_tiles * COLS;
+  const int k = (int)g.k, steps = (k + STEP - 1) / STEP;
+
+  const uint8_t* W[NB];
+  const uint16_t *S[NB], *Z[NB], *X[MB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int64_t n = min(n0 + j * 16 + col, g.n - 1);  // (columns past the end repeat the last)
+    W[j] = g.weight + n * g.ws[0] + quad * 16;
+    S[j] = (const uint16_t*)g.scales + n * g.ss[0];
+    Z[j] = (const uint16_t*)g.zeros + n * g.zs[0];
+  }
+#pragma unroll
+  for (int i = 0; i < MB; ++i) X[i] = (const uint16_t*)g.x + min(m0 + i * 16 + col, g.rows - 1) * g.xs[0] + quad * 8;
+
+  struct Turn {
+    u32x4 w[NB], x[MB][4];
+    uint16_t s[NB][4 / SUB], z[NB][4 / SUB];
+  };
+  auto load = [&](Turn& t, int step) __attribute__((always_inline)) {
+    const int k0 = step * STEP;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      t.w[j] = u32x4{0u, 0u, 0u, 0u};
+      if (k0 + quad * 32 < k) t.w[j] = *(const u32x4*)(W[j] + k0 / 2);
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        t.x[i][p] = u32x4{0u, 0u, 0u, 0u};
+        if (k0 + p * 32 < k) t.x[i][p] = *(const u32x4*)(X[i] + k0 + p * 32);
+      }
+#pragma unroll
+    for (int p = 0; p < 4; p += SUB) {
+      const int64_t group = min(k0 + p * 32, k - 1) / g.group;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        t.s[j][p / SUB] = S[j][group * g.ss[1]];
+        t.z[j][p / SUB] = g.zeros ? Z[j][group * g.zs[1]] : (uint16_t)0;
+      }
+    }
+  };
+  floatx4 acc[MB][NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const frag ones = __builtin_bit_cast(frag, u32x4{M::ONES, M::ONES, M::ONES, M::ONES});
+  auto take = [&](const Turn& t) __attribute__((always_inline)) {
+    u32x4 w[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) w[j] = across_quads(t.w[j]);
+#pragma unroll
+    for (int p0 = 0; p0 < 4; p0 += SUB) {
+      floatx4 part[MB][NB], all[MB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        all[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NB; ++j) part[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int p = p0; p < p0 + SUB; ++p) {
+        frag fw[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) fw[j] = __builtin_bit_cast(frag, wide8<T>(w[j][p]));
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const frag fx = __builtin_bit_cast(frag, paired(t.x[i][p]));
+          all[i] = M::mma(fx, ones, all[i]);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) part[i][j] = M::mma(fx, fw[j], part[i][j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const float s = elem<T>::to_float(t.s[j][p0 / SUB]);
+        const float z = 16.0f + (g.zeros ? elem<T>::to_float(t.z[j][p0 / SUB]) : 8.0f);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[i][j][r] = __builtin_fmaf(s, __builtin_fmaf(-z, all[i][r], part[i][j][r]), acc[i][j][r]);
+      }
+    }
+  };
+  Turn now, next;
+  if (wave < steps) load(now, wave);
+  for (int step = wave; step < steps; step += WAVES) {
+    if (step + WAVES < steps) load(next, step + WAVES);
+    take(now);
+    now = next;
+  }
+  // (row quad * 4 + r, column col of a block)
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sums[wave][i * 16 + quad * 4 + r][j * 16 + col] = acc[i][j][r];
+  __syncthreads();
+  for (int at = tid; at < ROWS * COLS; at += WAVES * 64) {
+    const int m = at / COLS, n = at % COLS;
+    if (m0 + m >= g.rows || n0 + n >= g.n) continue;
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) y += sums[w][m][n];
+    if (g.c) y += elem<T>::to_float(((const uint16_t*)g.c)[(m0 + m) * g.cs[0] + (n0 + n) * g.cs[1]]);
+    ((uint16_t*)g.out)[(m0 + m) * g.os[0] + (n0 + n) * g.os[1]] = elem<T>::from_float(y);
+  }
+}
+
+// The same element by element, for any strides and alignment: a wave a column, ROWS rows at a time, its lanes along k.
+template <typename T, int ROWS>
+__global__ __launch_bounds__(256) void linear4_elements_kernel(Linear4Args g) {
+  const int lane = threadIdx.x & 63;
+  const int64_t m_tiles = (g.rows + ROWS - 1) / ROWS, id = (g.first + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t m0 = id % m_tiles * ROWS, n = id / m_tiles;
+  if (n >= g.n) return;
+  float acc[ROWS] = {};
+  for (int64_t k = 2 * lane; k < g.k; k += 128) {
+    const uint32_t byte = g.weight[n * g.ws[0] + k / 2 * g.ws[1]];
+    const int64_t group = k / g.group;  // (an even number of elements)
+    const float s = elem<T>::to_float(((const uint16_t*)g.scales)[n * g.ss[0] + group * g.ss[1]]);
+    const float z = g.zeros ? elem<T>::to_float(((const uint16_t*)g.zeros)[n * g.zs[0] + group * g.zs[1]]) : 8.0f;
+    const float w0 = ((float)(byte & 15) - z) * s, w1 = ((float)(byte >> 4) - z) * s;
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+      if (m0 + m >= g.rows) break;
+      const uint16_t* x = (const uint16_t*)g.x + (m0 + m) * g.xs[0];
+      acc[m] = __builtin_fmaf(w0, elem<T>::to_float(x[k * g.xs[1]]), acc[m]);
+      acc[m] = __builtin_fmaf(w1, elem<T>::to_float(x[(k + 1) * g.xs[1]]), acc[m]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) {
+    float y = wave_sum(acc[m]);
+    if (lane != m || m0 + m >= g.rows) continue;
+    if (g.c) y += elem<T>::to_float(((const uint16_t*)g.c)[(m0 + m) * g.cs[0] + n * g.cs[1]]);
+    ((uint16_t*)g.out)[(m0 + m) * g.os[0] + n * g.os[1]] = elem<T>::from_float(y);
+  }
+}
+
+template <typename T, int MB, int NB>
+static void linear4_blocks(Linear4Args g, hipStream_t stream) {
+  const int64_t workgroups = cdiv(g.rows, MB * 16) * cdiv(g.n, NB * 16);
+  in_launches(workgroups, l4::WAVES * 64, [&](int64_t first, unsigned count) {
+    g.first = first;
+    const dim3 grid(count), block(l4::WAVES * 64);
+    if (g.group % 128 == 0)
+      hipLaunchKernelGGL((linear4_kernel<T, MB, NB, 4>), grid, block, 0, stream, g);
+    else if (g.group % 64 == 0)
+      hipLaunchKernelGGL((linear4_kernel<T, MB, NB, 2>), grid, block, 0, stream, g);
+    else
+      hipLaunchKernelGGL((linear4_kernel<T, MB, NB, 1>), grid, block, 0, stream, g);
+  });
+}
+
+template <typename T>
+static int linear4_launch(Linear4Args g, hipStream_t stream) {
+  const bool vec = g.xs[1] == 1 && g.xs[0] % 8 == 0 && (uintptr_t)g.x % 16 == 0 && g.ws[1] == 1 && g.ws[0] % 16 == 0 &&
+                   (uintptr_t)g.weight % 16 == 0;
+  if (!vec) {
+    constexpr int ROWS = 8;
+    in_launches(cdiv(cdiv(g.rows, ROWS) * g.n, 4), 256, [&](int64_t first, unsigned count) {
+      g.first = first;
+      hipLaunchKernelGGL((linear4_elements_kernel<T, ROWS>), dim3(count), dim3(256), 0, stream, g);
+    });
+    return launch_status();
+  }
+  if (g.rows <= 16)
+    linear4_blocks<T, 1, 1>(g, stream);
+  else if (g.rows <= 32)
+    linear4_blocks<T, 2, 1>(g, stream);
+  else
+    linear4_blocks<T, 4, 1>(g, stream);
+  return launch_status();
+}
+
+}  // namespace nt
+
+extern "C" int nt_linear_4bit(const void* x, const int64_t* x_strides, const void* weight, const int64_t* weight_strides,
+                              const void* scales, const int64_t* scale_strides, const void* zeros,
+                              const int64_t* zero_strides, const void* c, const int64_t* c_strides, void* out,
+                              const int64_t* out_strides, int dtype, int64_t rows, int64_t n, int64_t k, int64_t group,
+                              hipStream_t stream) {
+  if (rows < 0 || n < 0 || k < 0 || rows > 0x7fffffffLL || n > 0x7fffffffLL || k > 0x7fffff00LL ||
+      (dtype != NT_DTYPE_F16 && dtype != NT_DTYPE_BF16) || group < 32 || group % 32 || k % group)
+    return NT_ERR_INVALID;
+  if (!rows || !n) return 0;
+  if (!out || !out_strides || (c && !c_strides)) return NT_ERR_INVALID;
+  if (k && (!x || !weight || !scales || !x_strides || !weight_strides || !scale_strides || (zeros && !zero_strides)))
+    return NT_ERR_INVALID;
+  nt::Linear4Args g{};
+  g.x = x;
+  g.weight = (const uint8_t*)weight;
+  g.scales = scales;
+  g.zeros = zeros;
+  g.c = c;
+  g.out = out;
+  for (int i = 0; i < 2; ++i) {
+    g.xs[i] = k ? x_strides[i] : 0;
+    g.ws[i] = k ? weight_strides[i] : 0;
+    g.ss[i] = k ? scale_strides[i] : 0;
+    g.zs[i] = k && zeros ? zero_strides[i] : 0;
+    g.cs[i] = c ? c_strides[i] : 0;
+    g.os[i] = out_strides[i];
+  }
+  g.rows = rows;
+  g.n = n;
+  g.k = k;
+  g.group = (int)group;
+  return dtype == NT_DTYPE_F16 ? nt::linear4_launch<nt::f16_t>(g, stream) : nt::linear4_launch<nt::bf16_t>(g, stream);
+}
+
+extern "C" int nt_linear_4bit_packed(const int64_t* packed) {
+  if (!packed) return NT_ERR_INVALID;
+  nt::Packed p{packed};
+  const void* x = p.ptr<const void>();
+  const int64_t* xs = p.array(2);
+  const void* weight = p.ptr<const void>();
+  const int64_t* ws = p.array(2);
+  const void* scales = p.ptr<const void>();
+  const int64_t* ss = p.array(2);
+  const void* zeros = p.ptr<const void>();
+  const int64_t* zs = p.array(2);
+  const void* c = p.ptr<const void>();
+  const int64_t* cs = p.array(2);
+  void* out = p.ptr<void>();
+  const int64_t* os = p.array(2);
+  int dtype = p.i();
+  int64_t rows = p.i64();
+  int64_t n = p.i64();
+  int64_t k = p.i64();
+  int64_t group = p.i64();
+  hipStream_t stream = (hipStream_t)p.ptr<void>();
+  return nt_linear_4bit(x, xs, weight, ws, scales, ss, zeros, zs, c, cs, out, os, dtype, rows, n, k, group, stream);
+}

@@ -970,3 +970,288 @@ def bind_cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=None
 def cache_attention(q, k_cache, v_cache, tables, lengths, out, k_scale=None, v_scale=None, scale=None):
     _launch_bound(bind_cache_attention, (q, k_cache, v_cache, tables, lengths, out, k_scale, v_scale), (scale,))
     return out
+
+
+def check_chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_scale=None, v_scale=None, causal=True,
+                          scale=None):
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError("chunk_attention expects matching [tokens, heads, dim] tensors")
+    if q.dtype != out.dtype:
+        raise TypeError("chunk_attention q and out must share one dtype")
+    if k_cache.dim() != 4:
+        raise ValueError("caches must be [pages, page_size, heads, dim] tensors")
+    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, k_cache.shape[2], q.shape[2], 16)
+    _check_heads(q.shape[1], k_cache.shape[2])
+    _check_tables(tables, lengths)
+    _check_starts(starts, "starts", tables.shape[0])
+    if q.shape[0] * (q.shape[1] // k_cache.shape[2]) > 0x7FFFFF00 or q.shape[1] > 1 << 20 or tables.shape[0] > 1 << 24:
+        raise ValueError("chunk_attention takes less than 2^31 rows, of at most 2^20 heads and 2^24 sequences")
+    if k_cache.shape[1] * tables.shape[1] > 0x7FFFFF00:
+        raise ValueError("chunk_attention takes less than 2^31 keys a sequence")
+    vector = 16 // k_cache.element_size()
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if any(st % vector for st, size in zip(t.stride()[:3], t.shape) if size > 1):
+            raise ValueError(f"{name} rows must start on 16 bytes")
+    _check_written(out, "out")
+    if scale is not None:
+        float(scale)
+    return cache_code
+
+
+def bind_chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_scale=None, v_scale=None, causal=True,
+                         scale=None):
+    """launch(q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale): attention of each sequence's chunk of
+    new tokens (a piece of a prompt, some drafted tokens, one token), q and out packed [tokens, heads, dim],
+    over its pages, in caches as :func:`bind_cache_append` fills them.
+
+    Sequence b's tokens are rows starts[b] to starts[b + 1]; it has lengths[b] keys in the cache, the new tokens'
+    own last (call :func:`cache_append` first, and count on).  ``causal``: query i sees the keys up to
+    i + (keys - queries), so that the last query sees them all.  heads is a multiple of the caches' heads, ``scale``
+    defaults to dim ** -0.5.  8-bit caches count times their scales (any that are not negative).  Scores, softmax and sums
+    are in fp32; the weights are rounded to the cache's type (to fp16 for 8-bit caches) for the product with v, and for
+    16-bit caches in their sum.  Lengths past a table's pages are cut, page numbers the cache does not have hold no keys, a
+    query without keys gives zeros, and rows behind the last sequence are left alone.  ``out`` must not overlap the
+    inputs.  A call takes a workspace for keys that are split over workgroups from torch's allocator."""
+    cache_code = check_chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale, causal, scale)
+    device = _check_device(q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale)
+    import torch
+
+    tokens, heads, dim = q.shape
+    pages, page_size, kv_heads = k_cache.shape[:3]
+    sequences, width = tables.shape[0], tables.shape[1] if pages else 0
+    nbytes = int(_lib.load().nt_chunk_attention_workspace_size(tokens, sequences, heads, kv_heads, dim, page_size, width,
+                                                               cache_code))
+    # (a size of one may have any stride: the kernels take none for it)
+    strides = [tuple(st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape)) for t in (k_cache, v_cache)]
+    launch = _bind_packed("nt_chunk_attention_packed", device, (
+        _POINTER, q.stride(), _POINTER, strides[0], _POINTER, strides[1], cache_code, _POINTER, _POINTER, _POINTER,
+        out.stride(), _lib.dtype_code(q.dtype), _POINTER, tables.stride(0), _POINTER, _POINTER, tokens, sequences, heads,
+        kv_heads, dim, pages, page_size, width, float(dim ** -0.5 if scale is None else scale), bool(causal), _STREAM,
+        _POINTER, nbytes))
+
+    def call(q, k_cache, v_cache, tables, lengths, starts, out, k_scale=None, v_scale=None):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        launch((q, k_cache, v_cache, k_scale, v_scale, out, tables, lengths, starts, ws))
+
+    return call
+
+
+def chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_scale=None, v_scale=None, causal=True, scale=None):
+    _launch_bound(bind_chunk_attention, (q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale),
+                  (causal, scale))
+    return out
+
+
+def check_cache_copy(k_cache, v_cache, sources, destinations, k_scale=None, v_scale=None, counts=None):
+    import torch
+
+    if k_cache.dim() != 4:
+        raise ValueError("caches must be [pages, page_size, heads, dim] tensors")
+    heads, dim = k_cache.shape[2:]
+    dtype = torch.float16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
+    cache_code = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, heads, dim, 4)
+    if heads > 1 << 20 or k_cache.shape[1] * heads > (1 << 40) // dim:
+        raise ValueError("cache_copy takes pages of at most 2^20 heads and 2^40 elements")
+    if sources.dim() != 1 or sources.shape[0] > 0x7FFFFFFF:
+        raise ValueError("sources must be [pairs], less than 2^31")
+    for t, name in ((sources, "sources"), (destinations, "destinations"), (counts, "counts")):
+        if t is not None:
+            _check_index(t, name, sources.shape, (torch.int32,))
+            _check_contiguous(t, name)
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _check_written(t, name)
+    return cache_code
+
+
+def bind_cache_copy(k_cache, v_cache, sources, destinations, k_scale=None, v_scale=None, counts=None):
+    """launch(k_cache, v_cache, sources, destinations, k_scale, v_scale, counts): page sources[i] of both caches (as
+    :func:`bind_cache_append` fills them) copied to page destinations[i], with the page's scales.
+
+    For sequences that fork (each shares its full pages, and takes a copy of the begun one) or a cache that is
+    compacted (pages from behind go to free ones in front; the caller renumbers its tables).  ``counts`` [pairs]:
+    only the first counts[i] slots; the others keep what they held, though the page's scales are the source's.  A pair
+    with a page number the cache does not have, or of one page twice, is passed over.  No page may be the
+    destination of two pairs, or of one and the source of another.  Several layers' caches in one tensor, seen as
+    [layers * pages, ...], take one call."""
+    cache_code = check_cache_copy(k_cache, v_cache, sources, destinations, k_scale, v_scale, counts)
+    device = _check_device(k_cache, v_cache, sources, destinations, k_scale, v_scale, counts)
+    pages, page_size, heads, dim = k_cache.shape
+    strides = [tuple(st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape)) for t in (k_cache, v_cache)]
+    launch = _bind_packed("nt_cache_copy_packed", device, (
+        _POINTER, strides[0], _POINTER, strides[1], cache_code, _POINTER, _POINTER, _POINTER, _POINTER, _POINTER,
+        sources.shape[0], pages, page_size, heads, dim, _STREAM))
+
+    def call(k_cache, v_cache, sources, destinations, k_scale=None, v_scale=None, counts=None):
+        launch((k_cache, v_cache, k_scale, v_scale, sources, destinations, counts))
+
+    return call
+
+
+def cache_copy(k_cache, v_cache, sources, destinations, k_scale=None, v_scale=None, counts=None):
+    _launch_bound(bind_cache_copy, (k_cache, v_cache, sources, destinations, k_scale, v_scale, counts), ())
+
+
+# --------------------------------------------------- beside a layer's attention
+def check_rms_norm(x, weight, out, residual=None, total=None, scale=None, eps=1e-6):
+    """The group of the output's scales (0: a scale a row, or none)."""
+    import torch
+
+    if x.dim() != 2 or out.shape != x.shape:
+        raise ValueError("rms_norm expects matching [rows, dim] tensors")
+    _lib.dtype_code(x.dtype)
+    rows, dim = x.shape
+    if dim > 65536:
+        raise ValueError("rms_norm rows must have at most 65536 elements")
+    if weight.dtype != x.dtype:
+        raise TypeError("rms_norm x and weight must share one dtype")
+    if tuple(weight.shape) != (dim,):
+        raise ValueError(f"weight must have shape {(dim,)}, not {tuple(weight.shape)}")
+    if residual is None:
+        if total is not None:
+            raise ValueError("total belongs to a residual")
+    else:
+        for t, name in ((residual, "residual"), (total, "total")):
+            if t is None:
+                continue
+            if t.dtype != x.dtype:
+                raise TypeError(f"rms_norm x and {name} must share one dtype")
+            if t.shape != x.shape:
+                raise ValueError(f"{name} must have shape {tuple(x.shape)}, not {tuple(t.shape)}")
+        _check_written(residual if total is None else total, "residual" if total is None else "total")
+    _check_written(out, "out")
+    float(eps)
+    if out.dtype != torch.float8_e4m3fn:
+        if out.dtype != x.dtype:
+            raise TypeError(f"rms_norm out must be {x.dtype} or torch.float8_e4m3fn")
+        if scale is not None:
+            raise ValueError("scale belongs to an 8-bit out")
+        return 0
+    if scale is None:
+        raise ValueError("an 8-bit out needs scale")
+    if scale.dtype != torch.float32:
+        raise TypeError("scale must be torch.float32")
+    group = 0
+    if scale.dim() == 2 and scale.shape[0] == rows and scale.shape[1] > 0 and dim % scale.shape[1] == 0:
+        group = dim // scale.shape[1]
+        if group not in (32, 64, 128):
+            raise ValueError("scales are of a row, or of groups of 32, 64 or 128 elements")
+    elif tuple(scale.shape) != (rows,):
+        raise ValueError("scale must be [rows] or [rows, groups]")
+    _check_contiguous(scale, "scale")
+    return group
+
+
+def bind_rms_norm(x, weight, out, residual=None, total=None, scale=None, eps=1e-6):
+    """launch(x, weight, out, residual, total, scale): out = s / sqrt(mean(s^2) + eps) * weight over the rows of
+    s = x + residual [rows, dim], and total = s (in place of residual where ``total`` is None), each
+    rounded once: the norm is of s in fp32, before it is rounded to ``total``.
+
+    x, weight, residual and total share one dtype (fp32, fp16 or bf16), as out does, or out is ``torch.float8_e4m3fn``:
+    then it holds y / scale, with scale [rows], or [rows, dim / group] for groups of 32, 64 or 128 elements, the largest
+    finite |y| of the row or group over 448 (2^-64 at least).  Infinities are stored as NaN there.  Squares
+    and their sum are in fp32, so elements past 2^63 give rows of zeros.  Any strides; up to 65536 elements.
+    ``out`` may be x, and ``total`` x or the residual; else what is written must not overlap anything."""
+    group = check_rms_norm(x, weight, out, residual, total, scale, eps)
+    device = _check_device(x, weight, out, residual, total, scale)
+    rows, dim = x.shape
+    if total is None:
+        total = residual
+    none = (0, 0)
+    out_code = _lib.DTYPE_E4M3 if scale is not None else _lib.dtype_code(out.dtype)
+    launch = _bind_packed("nt_rms_norm_packed", device, (
+        _POINTER, x.stride(), _POINTER, weight.stride(0), _POINTER, none if residual is None else residual.stride(), _POINTER,
+        none if total is None else total.stride(), _POINTER, out.stride(), _POINTER, group, _lib.dtype_code(x.dtype), out_code,
+        rows, dim, float(eps), _STREAM))
+
+    def call(x, weight, out, residual=None, total=None, scale=None):
+        launch((x, weight, residual, residual if total is None else total, out, scale))
+
+    return call
+
+
+def rms_norm(x, weight, out, residual=None, total=None, scale=None, eps=1e-6):
+    _launch_bound(bind_rms_norm, (x, weight, out, residual, total, scale), (eps,))
+    return out
+
+
+def quantize_4bit(w, group=128, symmetric=False):
+    """(weight, scales, zeros) of :func:`linear_4bit` for w [n, k]: each group's values between its smallest and largest
+    (zero among them) on 16 even steps, or with ``symmetric`` steps of a seventh of its largest magnitude around 8
+    (zeros is None then).  Scales and zeros are of w's dtype."""
+    import torch
+
+    if w.dim() != 2 or w.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("quantize_4bit takes [n, k] weights of torch.float16 or torch.bfloat16")
+    n, k = w.shape
+    if group < 32 or group % 32 or k % group:
+        raise ValueError("the group must be a multiple of 32 that divides k")
+    x = w.float().view(n, k // group, group)
+    if symmetric:
+        scales = (x.abs().amax(-1) / 7).to(w.dtype)
+        zeros, shift = None, 8.0
+    else:
+        low, high = x.amin(-1).clamp_max(0), x.amax(-1).clamp_min(0)
+        scales = ((high - low) / 15).to(w.dtype)
+        zeros = torch.where(scales > 0, (-low / scales.float()).round().clamp(0, 15), 0).to(w.dtype)
+        shift = zeros.float()[..., None]
+    step = torch.where(scales > 0, scales.float(), 1.0)[..., None]
+    q = (x / step + shift).round().clamp(0, 15).to(torch.uint8).view(n, k)
+    return q[:, ::2] | q[:, 1::2] << 4, scales, zeros
+
+
+def check_linear_4bit(x, weight, scales, out, zeros=None, c=None):
+    """The group of the weights' scales."""
+    import torch
+
+    if not x.dim() == weight.dim() == scales.dim() == out.dim() == 2:
+        raise ValueError("linear_4bit expects x [rows, k], weight [n, k // 2], scales [n, groups] and out [rows, n]")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("linear_4bit takes torch.float16 or torch.bfloat16")
+    for t, name in ((scales, "scales"), (out, "out"), (zeros, "zeros"), (c, "c")):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"linear_4bit x and {name} must share one dtype")
+    if weight.dtype != torch.uint8:
+        raise TypeError("weight must be torch.uint8, two values to a byte")
+    (rows, k), n = x.shape, weight.shape[0]
+    if weight.shape[1] * 2 != k:
+        raise ValueError(f"weight must be [n, {k // 2}], two values to a byte")
+    groups = scales.shape[1]
+    if scales.shape[0] != n or (k and (groups == 0 or k % groups or k // groups % 32)):
+        raise ValueError("scales must be [n, groups], each of a multiple of 32 elements of k")
+    if zeros is not None and zeros.shape != scales.shape:
+        raise ValueError("zeros must have the shape of scales")
+    for t, name in ((out, "out"), (c, "c")):
+        if t is not None and tuple(t.shape) != (rows, n):
+            raise ValueError(f"{name} must have shape {(rows, n)}, not {tuple(t.shape)}")
+    if max(rows, n, k) > 0x7FFFFF00:
+        raise ValueError("linear_4bit takes sizes of less than 2^31")
+    _check_written(out, "out")
+    return k // groups if k else 32
+
+
+def bind_linear_4bit(x, weight, scales, out, zeros=None, c=None):
+    """launch(x, weight, scales, out, zeros, c): out [rows, n] = c + x [rows, k] @ w.T with
+    w[n, k] = scales[n, k // group] * (q[n, k] - zeros[n, k // group]).
+
+    ``weight`` [n, k // 2] (``torch.uint8``) holds two values q of 0 to 15 a byte, element 2 i in the lower four bits
+    of byte i; the group, k // scales.shape[1], is a multiple of 32.  ``zeros`` of None are 8.  ``c`` (None: nothing) may be
+    a residual or an expanded bias.  All else is of one dtype, fp16 or bf16.  Sums are in fp32 and rounded once; a row
+    of x that holds an infinity gives NaN.  ``out`` may be c, and must not overlap the others.
+    :func:`quantize_4bit` makes the weights."""
+    group = check_linear_4bit(x, weight, scales, out, zeros, c)
+    device = _check_device(x, weight, scales, out, zeros, c)
+    none = (0, 0)
+    launch = _bind_packed("nt_linear_4bit_packed", device, (
+        _POINTER, x.stride(), _POINTER, weight.stride(), _POINTER, scales.stride(), _POINTER,
+        none if zeros is None else zeros.stride(), _POINTER, none if c is None else c.stride(), _POINTER, out.stride(),
+        _lib.dtype_code(x.dtype), x.shape[0], weight.shape[0], x.shape[1], group, _STREAM))
+
+    def call(x, weight, scales, out, zeros=None, c=None):
+        launch((x, weight, scales, zeros, c, out))
+
+    return call
+
+
+def linear_4bit(x, weight, scales, out, zeros=None, c=None):
+    _launch_bound(bind_linear_4bit, (x, weight, scales, out, zeros, c), ())
+    return out
