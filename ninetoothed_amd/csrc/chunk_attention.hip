@@ -13,7 +13,6 @@ using namespace lane_rows;
 constexpr int NW = 8;         // waves per workgroup, two per SIMD
 constexpr int BM = NW * 32;   // rows per workgroup: tokens and heads that share a head of k and v
 constexpr int BN = 64;        // keys per tile
-constexpr int STAGES = 3;     // tiles in LDS: values of the last, keys of this one, the next on its way
 constexpr int OVERHEAD = 2;   // a block's fixed work, in tiles
 constexpr int LEAST = 4;      // tiles of a workgroup
 constexpr int JOIN_ROWS = 16;
@@ -34,14 +33,24 @@ template <typename T>
 __device__ __forceinline__ u32x4 wide8(uint32_t lo, uint32_t hi) {
   return u32x4{of_e4m3<T, false>(lo), of_e4m3<T, true>(lo), of_e4m3<T, false>(hi), of_e4m3<T, true>(hi)};
 }
-// Sixteen e4m3 values with zeros for the NaN.
-__device__ __forceinline__ u32x4 finite16(u32x4 w) {
+// e4m3 values with zeros for the NaN.
+template <typename V>
+__device__ __forceinline__ V finite_bytes(V w) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < (int)(sizeof(V) / 4); ++i)
 #pragma unroll
     for (int b = 0; b < 32; b += 8)
       if (((w[i] >> b) & 0x7fu) == 0x7fu) w[i] &= ~(0xffu << b);
   return w;
+}
+// The bytes at an offset of a buffer of so many bytes (uniform) into registers; zeros past its end.
+template <typename V>
+__device__ __forceinline__ V buffer_load(const void* base, int bytes, int offset) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+  if constexpr (sizeof(V) == 16)
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0));
+  else
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(rs, offset, 0, 0));
 }
 
 }  // namespace ch
@@ -258,6 +267,351 @@ __device__ __forceinline__ void chunk_rows_by_key(const ChunkArgs& g, const int3
   }
 }
 
+// A piece of a workgroup's stretch: tiles [t0, t1) of a block, and what its waves and lanes have of them.
+struct ChunkPiece {
+  int t0, t1, Sk;
+  int full_block;  // tiles before it hold no key that a row of the workgroup does not see
+  int nkt_w, full_w;  // this wave: its tiles' end, and as full_block
+  bool whole, first;  // all of the block's tiles; the block begins in this stretch
+  bool valid;         // this lane's row: is one
+  int tok, qhead, last;  // its token and head, and the last key that it sees
+  int64_t end;  // of the block, on the line
+};
+__device__ __forceinline__ ChunkPiece chunk_piece(const ChunkArgs& g, const ChunkSequence& s, int64_t seq_at, int nth,
+                                                  int64_t begin, int64_t stop, int head, int wave) {
+  using namespace ch;
+  ChunkPiece p;
+  const int64_t block_at = seq_at + chunk_line(s, nth);
+  p.end = seq_at + chunk_line(s, nth + 1);
+  p.first = begin <= block_at;
+  p.whole = p.first && p.end <= stop;
+  const int r0 = nth * BM, rw = r0 + wave * 32, row = rw + (threadIdx.x & 31), offset = s.Sk - s.Sq;
+  p.Sk = s.Sk;
+  int nkt = (int)((uint32_t)(s.Sk + BN - 1) / BN);
+  p.full_block = p.full_w = s.Sk / BN;
+  p.nkt_w = nkt;
+  if (g.causal) {
+    const int end = (min(r0 + BM, s.rows) - 1) / g.group + offset, end_w = (min(rw + 32, s.rows) - 1) / g.group + offset;
+    nkt = end < 0 ? 0 : min(nkt, end / BN + 1);
+    p.nkt_w = end_w < 0 ? 0 : min(nkt, end_w / BN + 1);
+    const int all = r0 / g.group + offset, all_w = rw / g.group + offset;  // every row sees the tiles before it
+    p.full_block = all < 0 ? 0 : min(p.full_block, (all + 1) / BN);
+    p.full_w = all_w < 0 ? 0 : min(p.full_w, (all_w + 1) / BN);
+  }
+  const int64_t keys_at = block_at + (int64_t)OVERHEAD * BN * g.group, tile_line = (int64_t)BN * g.group;
+  auto tile_of = [&](int64_t at) {  // the first tile that begins at a position of the line or behind it
+    return at <= keys_at ? 0 : (int)min((int64_t)nkt, (int64_t)((uint64_t)(at - keys_at + tile_line - 1) / (uint64_t)tile_line));
+  };
+  p.t0 = tile_of(begin);
+  p.t1 = stop >= p.end ? nkt : tile_of(stop);
+  p.nkt_w = rw < s.rows ? min(p.nkt_w, p.t1) : 0;
+  p.valid = row < s.rows;
+  p.tok = row / g.group;
+  p.qhead = head * g.group + (row - p.tok * g.group);
+  p.last = min(g.causal ? p.tok + offset : s.Sk - 1, s.Sk - 1);
+  return p;
+}
+
+// The fragments of a wave's rows of q.
+template <typename T, int DM>
+__device__ __forceinline__ void chunk_queries(const ChunkArgs& g, const ChunkSequence& s, const ChunkPiece& p,
+                                              typename mfma_traits<T>::frag (&qf)[DM / 16]) {
+  const uint32_t flip = g.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes to q's signs)
+  const uint16_t* Q = (const uint16_t*)g.q + (int64_t)(s.begin + p.tok) * g.qs[0] + p.qhead * g.qs[1];
+  const int64_t q_es = stride_here(g.qs[2]);
+  const int q_at = lane_here((threadIdx.x & 32) / 4);
+#pragma unroll
+  for (int dd = 0; dd < DM / 16; ++dd) {
+    const int d = dd * 16 + q_at;
+    u32x4 raw = {0u, 0u, 0u, 0u};
+    if (p.valid && d < g.dim) {
+      if (g.q_vectors) {
+        raw = *(const u32x4*)(Q + d);
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) raw[w] = Q[(d + 2 * w) * q_es] | (uint32_t)Q[(d + 2 * w + 1) * q_es] << 16;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) raw[w] ^= flip;
+    qf[dd] = __builtin_bit_cast(typename mfma_traits<T>::frag, raw);
+  }
+}
+
+// What 16 neighbouring keys share: k's factor of the scores (with the softmax's scale), log2 and reciprocal of v's
+// scale, and whether their page is there (bits).
+struct alignas(16) ChunkFactors {
+  float kf, lv, rv;
+  uint32_t there;
+};
+__device__ __forceinline__ ChunkFactors chunk_factors(float c, float k_scale, float v_scale, bool there) {
+  const float vs = fminf(fmaxf(v_scale, ch::LEAST_SCALE), 3.0e38f);
+  return {there ? fmaxf(c * k_scale, ch::LEAST_FACTOR) : c, there ? __builtin_amdgcn_logf(vs) : 0.f,
+          there ? __builtin_amdgcn_rcpf(vs) : 1.0f, there};
+}
+
+// The state of a wave's rows: a lane has one, and half of its keys.
+template <typename P, int DM>
+struct ChunkState {
+  floatx16 o[DM / 32];
+  typename mfma_traits<P>::frag pf[ch::BN / 16];  // the last tile's weights
+  float m, l;
+  __device__ __forceinline__ void clear() {
+    m = ch::UNSET;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < DM / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  }
+};
+
+// A tile's weights from its scores, and what they add to the sum.  (Register r of block kb: key kb * 32 + r / 4 * 8 +
+// half * 4 + r % 4; 16 neighbouring keys are 8 registers of both halves.)  `hide`: the tile has keys that some row does
+// not see, those past `room` for this lane's.  Scores of 8 bits that are exponents already (EXPONENTS) take
+// reciprocal(r) for each key's v.
+template <typename P, bool EIGHT, bool EXPONENTS, int DM, typename R>
+__device__ __forceinline__ void chunk_weights(ChunkState<P, DM>& x, floatx16 (&sc)[2], const ChunkFactors (&f)[4], R&& reciprocal) {
+  using namespace ch;
+  float add = 0.f;  // of this tile, to l
+  auto exponentials = [&]() __attribute__((always_inline)) {
+    float all = 0.f;
+    add = 0.f;
+#pragma unroll
+    for (int t = 0; t < BN / 16; ++t) {
+      u32x4 w;
+      float sum = 0.f;
+      const float shift = EIGHT && !EXPONENTS ? f[t].lv - x.m : -x.m, kf = EXPONENTS ? 1.0f : f[t].kf;
+#pragma unroll
+      for (int sl = 0; sl < 4; ++sl) {
+        const int e = 8 * (t & 1) + 2 * sl;
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t >> 1][e], kf, shift));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t >> 1][e + 1], kf, shift));
+        w[sl] = pack2<P>(p0, p1);
+        if constexpr (EIGHT) {
+          sum += p0;
+          sum += p1;
+          if constexpr (EXPONENTS) {
+            add = __builtin_fmaf(p0, reciprocal(t >> 1, e), add);
+            add = __builtin_fmaf(p1, reciprocal(t >> 1, e + 1), add);
+          }
+        } else {
+          sum = add2<P>(w[sl], sum);
+        }
+      }
+      x.pf[t] = __builtin_bit_cast(typename mfma_traits<P>::frag, w);
+      all += sum;
+      if constexpr (EIGHT && !EXPONENTS) add = __builtin_fmaf(sum, f[t].rv, add);
+    }
+    if constexpr (!EIGHT) add = all;
+    return all;
+  };
+  const float all = exponentials();
+  if (__builtin_amdgcn_ballot_w64(!(all <= MOST_SUM))) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y = sc[i >> 1][8 * (i & 1)];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) y = fmaxf(y, sc[i >> 1][8 * (i & 1) + r]);
+      mx = fmaxf(mx, EXPONENTS ? y : EIGHT ? __builtin_fmaf(y, f[i].kf, f[i].lv) : y * f[i].kf);
+    }
+    const float grown = fmaxf(max_halves(mx), x.m), alpha = __builtin_amdgcn_exp2f(x.m - grown);
+    x.l *= alpha;
+#pragma unroll
+    for (int i = 0; i < DM / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x.o[i][r] *= alpha;
+    x.m = grown;
+    exponentials();
+  }
+  x.l += add;
+}
+// Minus infinity for the scores of keys past `room` of the tile (less 4 half).
+__device__ __forceinline__ void chunk_hide(floatx16 (&sc)[2], int room) {
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (kb * 32 + (r >> 2) * 8 + (r & 3) > room) sc[kb][r] = -INFINITY;
+}
+
+// The end of a piece: a wave's rows as output, or as a partial state.  `odd`: a tile that the wave masks held an infinite
+// or NaN v.
+template <typename T, typename P, bool EIGHT, int DM>
+__device__ __forceinline__ void chunk_finish(const ChunkArgs& g, const ChunkSequence& s, const ChunkPiece& p,
+                                             const int32_t* table, int head, int wave, bool odd,
+                                             const typename mfma_traits<T>::frag (&qf)[DM / 16], ChunkState<P, DM>& x) {
+  using namespace ch;
+  const int half = (threadIdx.x >> 5) & 1;
+  const float c = fmaxf(fabsf(g.scale_log2), LEAST_FACTOR);
+  const int64_t state = (2 * (int64_t)blockIdx.x + (p.first ? 1 : 0)) * BM + wave * 32 + (threadIdx.x & 31);
+  uint16_t* O = (uint16_t*)g.o + (int64_t)(s.begin + p.tok) * g.os[0] + p.qhead * g.os[1];
+  const int64_t o_es = stride_here(g.os[2]);
+  const int o_at = lane_here(half * 4);
+  // Four neighbouring elements from d on.
+  auto put = [&](int d, float f, float x0, float x1, float x2, float x3) {
+    if (!p.whole) {
+      *(floatx4*)(g.part_o + state * DM + d) = floatx4{x0, x1, x2, x3};
+    } else if (g.o_vectors) {
+      *(u32x2*)(O + d) = u32x2{pack2<T>(x0 * f, x1 * f), pack2<T>(x2 * f, x3 * f)};
+    } else {
+      O[d * o_es] = elem<T>::from_float(x0 * f);
+      O[(d + 1) * o_es] = elem<T>::from_float(x1 * f);
+      O[(d + 2) * o_es] = elem<T>::from_float(x2 * f);
+      O[(d + 3) * o_es] = elem<T>::from_float(x3 * f);
+    }
+  };
+  if (odd) {
+    float o[DM / 2];
+    chunk_rows_by_key<T, EIGHT, DM>(g, table, head, qf, c, p.t0 * BN, min(p.Sk, p.nkt_w * BN), p.valid ? p.last : -1, x.m,
+                                    x.l, o);
+    const float inv = x.l != 0.f ? 1.0f / x.l : 0.f;
+    if (p.valid) {
+#pragma unroll
+      for (int i = 0; i < DM / 2; i += 4) {
+        const int d = i / 8 * 16 + 2 * o_at + i % 8;
+        if (d < g.dim) put(d, inv, o[i], o[i + 1], o[i + 2], o[i + 3]);
+      }
+    }
+  } else {
+    x.l += other_half(x.l);
+    const float inv = x.l != 0.f ? 1.0f / x.l : 0.f;
+    if (p.valid) {
+#pragma unroll
+      for (int i = 0; i < DM / 32; ++i)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int d = i * 32 + r4 * 8 + o_at;
+          if (d < g.dim) put(d, inv, x.o[i][4 * r4], x.o[i][4 * r4 + 1], x.o[i][4 * r4 + 2], x.o[i][4 * r4 + 3]);
+        }
+    }
+  }
+  if (!p.whole && p.valid && half == 0) *(float2*)(g.part_ml + state * 2) = float2{x.l != 0.f ? x.m : -INFINITY, x.l};
+}
+
+// Where a lane reads its fragments in a tile of K, and in one of V through the transposing read.
+// K [key][DM] in 16-byte chunks XORed by key, so that the 16 keys of a fragment read fall on 16 distinct bank
+// groups; V [key][DM] in 64-byte chunks XORed by key, for the 4 keys of a transposing read.
+template <int DM>
+struct ChunkTile {
+  static constexpr int ROW = DM * 2, TILE = ch::BN * ROW;
+  __device__ __forceinline__ static int k_swz(int key) { return DM == 128 ? key & 15 : (key >> 1) & 7; }
+  __device__ __forceinline__ static int v_swz(int key) { return DM == 128 ? key & 3 : (key >> 1) & 1; }
+  // Where chunk c (16 bytes) of a key lies.
+  __device__ __forceinline__ static int k_place(int key, int c) { return key * ROW + (c ^ k_swz(key)) * 16; }
+  __device__ __forceinline__ static int v_place(int key, int c) {
+    return key * ROW + ((((c >> 2) ^ v_swz(key)) << 2) | (c & 3)) * 16;
+  }
+  int k, v;  // of this lane: the first fragment (of the others: XORed)
+  __device__ __forceinline__ ChunkTile() {
+    const int lane = threadIdx.x & 63, row = lane & 31, gq = lane >> 4, r = (lane & 15) >> 2, q = lane & 3;
+    k = k_place(row, lane >> 5);
+    v = (4 * (gq >> 1) + r) * ROW + v_swz(r) * 64 + (16 * (gq & 1) + 4 * q) * 2;
+  }
+  // Elements 16 dd + 8 half on of key 32 kb + lane % 32.
+  __device__ __forceinline__ u32x4 k_frag(const char* tile, int kb, int dd) const {
+    return *(const u32x4*)(tile + kb * 32 * ROW + (k ^ (dd * 32)));
+  }
+  // Element 32 i + lane % 32 of the 16 keys of slice t, in the order of a weight fragment.
+  __device__ __forceinline__ u32x4 v_frag(const char* tile, int t, int i) const {
+    typedef short v4i16 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4i16* lds_v4;
+    const char* p = tile + (v ^ (i * 64)) + t * (16 * ROW);
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)p));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(p + 8 * ROW)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  }
+};
+
+// O^T += V^T P^T of a tile of values and S^T = K Q^T of a tile of keys: one line of products, each fragment read several
+// products ahead of its own.
+template <typename T, typename P, int DM, bool WV, bool WK>
+__device__ __forceinline__ void chunk_products(const ChunkTile<DM>& at, const char* v_tile, const char* k_tile,
+                                               const typename mfma_traits<T>::frag (&qf)[DM / 16], ChunkState<P, DM>& x,
+                                               floatx16 (&sc)[2]) {
+  constexpr int DBLK = DM / 32, DSUB = DM / 16, NV = ch::BN / 16 * DBLK, NK = 2 * DSUB;
+  if constexpr (WV) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+      x.o[n % DBLK] = mfma_traits<P>::mma(__builtin_bit_cast(typename mfma_traits<P>::frag, at.v_frag(v_tile, n / DBLK, n % DBLK)),
+                                          x.pf[n / DBLK], x.o[n % DBLK]);
+  }
+  if constexpr (WK) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[kb][r] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+      sc[n & 1] = mfma_traits<T>::mma(__builtin_bit_cast(typename mfma_traits<T>::frag, at.k_frag(k_tile, n & 1, n >> 1)),
+                                      qf[n >> 1], sc[n & 1]);
+  }
+  constexpr int MFMA = 0x8, READ = 0x100, AHEAD_V = 6, AHEAD_K = 8;  // (a V fragment is two reads)
+  if constexpr (WV) {
+    __builtin_amdgcn_sched_group_barrier(READ, 2 * AHEAD_V, 0);
+    static_for<0, NV - AHEAD_V>([](auto) {
+      __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(READ, 2, 0);
+    });
+    if constexpr (WK) {
+      static_for<0, AHEAD_V>([](auto i) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(READ, decltype(i)::value < 2 ? 2 : 1, 0);
+      });
+    } else {
+      __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD_V, 0);
+    }
+  } else {
+    __builtin_amdgcn_sched_group_barrier(READ, AHEAD_K, 0);
+  }
+  if constexpr (WK) {
+    static_for<0, NK - AHEAD_K>([](auto) {
+      __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(READ, 1, 0);
+    });
+    __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD_K, 0);
+  }
+}
+
+// The stretch of a workgroup, piece by piece: f(sequence, its number, block) for each.
+struct ChunkStretch {
+  int64_t begin, stop, seq_at;
+  int b, nth;
+  ChunkSequence s;
+  bool there;
+  template <int THREADS>
+  __device__ __forceinline__ ChunkStretch(const ChunkArgs& g, ChunkLds<THREADS>& lds, int part) {
+    int64_t share = 0;
+    const ChunkPlace place = chunk_place(g, lds, [&](int64_t length) {
+      share = chunk_share(g, length);
+      return min(part * share, length - 1);  // (a workgroup past the end has nothing to do)
+    });
+    share = scalar64(share);
+    begin = part * share;
+    stop = min(begin + share, place.length);
+    there = begin < stop;
+    if (!there) return;
+    b = place.sequence;
+    seq_at = place.before;
+    s = chunk_sequence(g, b);
+    nth = chunk_block(s, begin - seq_at);
+  }
+  // To the block behind one that ends at `end`; false if that is past the stretch.
+  __device__ __forceinline__ bool next(const ChunkArgs& g, int64_t end) {
+    if (end >= stop) return false;
+    if (++nth == s.blocks) {
+      seq_at += chunk_line(s, s.blocks);
+      do {
+        ++b;
+        s = chunk_sequence(g, b);  // (the line goes on: there is one with rows)
+      } while (s.blocks == 0);
+      nth = 0;
+    }
+    return true;
+  }
+};
+
 // Per row i of a sequence (a new token and a head of its group) over the keys j of its pages that it may see:
 //   s_ij = scale q_i . (kq_j ks_j),  o_i = sum_j p_ij (vq_j vs_j) / sum_j p_ij,  p_ij = exp(s_ij - m_i)
 // causal: j <= i + (keys - queries).  A row that sees no key gives zeros.
@@ -265,120 +619,305 @@ __device__ __forceinline__ void chunk_rows_by_key(const ChunkArgs& g, const int3
 // has few.  A workgroup takes 256 rows, a group's heads side by side for each token; eight waves of 32
 // rows, two a SIMD.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products: a lane holds one row, its max and sum take
 // no LDS, and P^T goes from the score registers to the second product as it is.
-//   - Keys and values pass through registers into LDS stages of 64 keys, so that a key's page is
-//     looked up lane by lane (any page size), 8-bit values are widened once for the eight waves, exactly, and what lies
-//     past a sequence's end or in no page is stored as zeros.
-//   - 8 bits: k's scale multiplies the score and v's enters the weight:
+//   - 8 bits: values are widened once for the eight waves, exactly; k's scale multiplies the score and v's enters the
+//     weight:
 //       w_ij = exp2(s_ij + log2 vs_j - M_i),  o_i = sum_j w_ij vq_j / sum_j w_ij / vs_j,
 //     with M the max of those exponents; w is rounded to fp16 (also for bf16 queries), and as pages' scales may lie
 //     far apart, where fp16 has nothing of some, its sum is of the unrounded ones.
 //   - Scores stay unscaled in fp32 until the exponential.  m is the max of a row's first tile, raised only where a later
 //     tile's weights grow past MOST_SUM (o and l are rescaled then), so most tiles take no max.
 //   - 16 bits: p is rounded to the operands' type for the product; its row sums are of the rounded p.
-//   - A causally masked key meets p = 0, which an infinite or NaN v would still turn into NaN: where a row of
-//     the workgroup masks a tile, those are stored as zeros, and rows of a tile that held one are taken key by
-//     key, each over the keys that it sees.
-// LDS: K [key][DM] in 16-byte chunks XORed by key, so that the 16 keys of a fragment read fall on 16 distinct bank
-// groups; V [key][DM] in 64-byte chunks XORed by key, for the 4 keys of a transposing read.
-// SIXTEENS: pages of 8 bits are whole multiples of 16 keys, whose scales are then the same in 16 scores.
-template <typename T, bool EIGHT, int DM, bool SIXTEENS>
-__global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-chunk_attention_kernel(ChunkArgs g) {
+//   - What lies past a sequence's end or in no page is stored as zeros.  A causally masked key meets p = 0, which an
+//     infinite or NaN v would still turn into NaN: rows of a tile that is masked and holds one are taken key by key, each
+//     over the keys that it sees (8 bits: such values are stored as zeros, and the tile is marked).
+// This kernel: pages of whole multiples of 16 keys, so that the 8 keys of a tile that a wave stages lie in one page, which it
+// looks up by a scalar load.  A step takes tile t's scores and weights and tile t - 1's values; K(t + 3) and V(t + 2) are
+// sent for in it: into LDS (16 bits, four stages), or into registers (8 bits), from where they are widened into LDS (two
+// stages) two steps later.
+template <typename T, bool EIGHT, int DM>
+__global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_pages_kernel(ChunkArgs g) {
   using namespace ch;
   typedef typename std::conditional<EIGHT, f16_t, T>::type P;  // the type of V^T P^T
   typedef typename mfma_traits<T>::frag frag;
-  typedef typename mfma_traits<P>::frag pfrag;
-  constexpr int ES = EIGHT ? 1 : 2, DSUB = DM / 16, DBLK = DM / 32, ROW = DM * 2, TILE = BN * ROW, STAGE = 2 * TILE;
+  typedef ChunkTile<DM> Tile;
+  typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
+  typedef const __attribute__((address_space(4))) float* ScalarFloats;
+  constexpr int ES = EIGHT ? 1 : 2, ROW = Tile::ROW, TILE = Tile::TILE, RING = EIGHT ? 2 : 4, KEYS = BN / NW;
+  constexpr int LOADS = EIGHT ? 1 : KEYS * ROW / 1024;  // of a wave, for K or V
+  constexpr int BYTES = EIGHT ? KEYS * DM / 64 : 16;    // of a lane in each
+  constexpr int PER_KEY = DM * ES / BYTES;              // lanes of a key
+  static_assert(LOADS * 64 * BYTES == KEYS * DM * ES, "a wave's share of a tile");
+  typedef typename std::conditional<BYTES == 16, u32x4, u32x2>::type Held;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * RING * TILE];  // K's stages, then V's
+  __shared__ ChunkLds<NW * 64> place_lds;
+  __shared__ ChunkFactors factors[4][4];  // of tile t in [t % 4], its sixteens
+  __shared__ int odd_tile[RING];          // 8 bits: 1 + the last tile in the stage that held a NaN v
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int D = g.dim, head = blockIdx.x % g.kv_heads;
+  ChunkStretch at(g, place_lds, blockIdx.x / g.kv_heads);
+  if (!at.there) return;
+  const Tile tile;
+  const float c = fmaxf(fabsf(g.scale_log2), LEAST_FACTOR);  // (of a scale of 0 times minus infinity would be NaN)
+  const char* kbase = (const char*)g.k + head * g.ks[2] * ES;
+  const char* vbase = (const char*)g.v + head * g.vs[2] * ES;
+  const int kst = (int)(g.ks[1] * ES), vst = (int)(g.vs[1] * ES);
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  // This lane's bytes of each load, behind the wave's first key; elements past D lie past the buffer's end.
+  int k_off[LOADS], v_off[LOADS];
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) {
+    const int own = u * (64 / PER_KEY) + lane / PER_KEY, key = wave * KEYS + own, p = lane % PER_KEY;
+    const int kc = EIGHT ? p : p ^ Tile::k_swz(key), vc = EIGHT ? p : ((((p >> 2) ^ Tile::v_swz(key)) << 2) | (p & 3));
+    k_off[u] = kc * BYTES < D * ES ? own * kst + kc * BYTES : 0x7fffffff;
+    v_off[u] = vc * BYTES < D * ES ? own * vst + vc * BYTES : 0x7fffffff;
+  }
+  // 8 bits: where this lane's first eight elements lie in a stage (the others of sixteen: XORed by 16).
+  const int own_key = wave * KEYS + lane / PER_KEY, own_chunk = lane % PER_KEY * (BYTES / 8);
+  const int k_to = Tile::k_place(own_key, own_chunk), v_to = RING * TILE + Tile::v_place(own_key, own_chunk);
+  if (EIGHT && tid < RING) odd_tile[tid] = 0;
+
+  while (true) {
+    const ChunkSequence& s = at.s;
+    const ChunkPiece p = chunk_piece(g, s, at.seq_at, at.nth, at.begin, at.stop, head, wave);
+    const int32_t* table = g.tables + at.b * g.table_stride;
+    const ScalarInts pages = (ScalarInts)(uintptr_t)table;
+    // The page of this wave's keys of a tile, or -1.
+    auto look = [&](int t) {
+      const int first = t * BN + wave * KEYS;
+      if (t >= p.t1 || first >= p.Sk) return -1;
+      return (int)pages[g.page_shift >= 0 ? first >> g.page_shift : first / g.page_size];
+    };
+    // The wave's keys of tile t in a page, as a buffer that ends with the last key.
+    struct Buffer {
+      const char* base;
+      int bytes;
+    };
+    auto keys_of = [&](const char* base, int64_t page_stride, int st, int page, int t) {
+      const int first = t * BN + wave * KEYS;
+      const int slot = g.page_shift >= 0 ? first & (g.page_size - 1) : first % g.page_size;
+      const bool ok = (uint32_t)page < (uint64_t)g.pages;
+      const int n = ok ? min(KEYS, p.Sk - first) : 0;
+      return Buffer{base + ((int64_t)(ok ? page : 0) * page_stride * ES + (int64_t)slot * st), n > 0 ? (n - 1) * st + D * ES : 0};
+    };
+    // The pages of tiles t + 4 (looked up), t + 3 and t + 2, and the scales of t + 3's.
+    int page_ahead, page_k, page_v;
+    float ks_k = 1.0f, vs_k = 1.0f, ks_v, vs_v;
+    auto scales = [&](int page) {
+      if constexpr (EIGHT) {
+        if ((uint32_t)page >= (uint64_t)g.pages) return;  // (those of another tile: nothing takes them)
+        const int64_t i = (int64_t)page * g.kv_heads + head;
+        ks_k = ((ScalarFloats)(uintptr_t)g.k_scale)[i];
+        vs_k = ((ScalarFloats)(uintptr_t)g.v_scale)[i];
+      }
+    };
+    // What tile t's keys share, from the wave that has the first of each sixteen.
+    auto share = [&](int t, int page) {
+      const bool there = t * BN + wave * KEYS >= p.Sk || (uint32_t)page < (uint64_t)g.pages;
+      if ((wave & 1) == 0 && lane == 0) factors[t & 3][wave >> 1] = chunk_factors(c, ks_v, vs_v, there);
+    };
+    Held k_held[2], v_held[2];
+    auto send_k = [&](auto set, int t) __attribute__((always_inline)) {
+      const Buffer keys = keys_of(kbase, g.ks[0], kst, page_k, t);
+      if constexpr (EIGHT) {
+        k_held[decltype(set)::value] = buffer_load<Held>(keys.base, keys.bytes, k_off[0]);
+      } else {
+        const u32x4 rs = buffer_of(keys.base, keys.bytes);
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) buffer_to_lds(rs, lds_at + (t & 3) * TILE + (wave * LOADS + u) * 1024, k_off[u], 0);
+      }
+    };
+    auto send_v = [&](auto set, int t) __attribute__((always_inline)) {
+      const Buffer keys = keys_of(vbase, g.vs[0], vst, EIGHT && vs_v < LEAST_SCALE ? -1 : page_v, t);
+      if constexpr (EIGHT) {
+        v_held[decltype(set)::value] = buffer_load<Held>(keys.base, keys.bytes, v_off[0]);
+      } else {
+        const u32x4 rs = buffer_of(keys.base, keys.bytes);
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u)
+          buffer_to_lds(rs, lds_at + (RING + (t & 3)) * TILE + (wave * LOADS + u) * 1024, v_off[u], 0);
+      }
+    };
+    // Tiles t + 3 and t + 2 sent for, and what comes after them looked up.
+    auto send = [&](auto set, int t) __attribute__((always_inline)) {
+      page_v = page_k;
+      ks_v = ks_k;
+      vs_v = vs_k;
+      page_k = page_ahead;
+      page_ahead = look(t + 4);
+      share(t + 2, page_v);
+      send_k(std::integral_constant<int, (decltype(set)::value + 1) & 1>{}, t + 3);
+      send_v(set, t + 2);
+      scales(page_k);
+    };
+    auto widen_k = [&](auto set, int t) __attribute__((always_inline)) {
+      if constexpr (EIGHT) {
+        const Held& x = k_held[decltype(set)::value];
+        *(u32x4*)(lds + (t & 1) * TILE + k_to) = wide8<T>(x[0], x[1]);
+        if constexpr (BYTES == 16) *(u32x4*)(lds + (t & 1) * TILE + (k_to ^ 16)) = wide8<T>(x[2], x[3]);
+      }
+    };
+    auto widen_v = [&](auto set, int t) __attribute__((always_inline)) {
+      if constexpr (EIGHT) {
+        Held x = v_held[decltype(set)::value];
+        if (t >= p.full_block) {
+          bool odd = false;
+#pragma unroll
+          for (int w = 0; w < BYTES / 4; ++w)
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) odd |= ((x[w] >> i) & 0x7fu) == 0x7fu;
+          if (odd) {
+            odd_tile[t & 1] = t + 1;
+            x = finite_bytes(x);
+          }
+        }
+        *(u32x4*)(lds + (t & 1) * TILE + v_to) = wide8<P>(x[0], x[1]);
+        if constexpr (BYTES == 16) *(u32x4*)(lds + (t & 1) * TILE + (v_to ^ 16)) = wide8<P>(x[2], x[3]);
+      }
+    };
+    auto k_tile = [&](int t) { return (const char*)lds + (t & (RING - 1)) * TILE; };
+    auto v_tile = [&](int t) { return (const char*)lds + (RING + (t & (RING - 1))) * TILE; };
+    // No access to LDS moves over it; all but the last two steps' loads into LDS have ended.
+    auto end_step = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!EIGHT) wait_loads<4 * LOADS>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    typedef std::integral_constant<int, 0> Even;
+    typedef std::integral_constant<int, 1> Odd;
+
+    // Tiles t0 to t0 + 2 of K and the first two of V under way (even: t0).
+    page_k = look(p.t0);
+    scales(page_k);
+    page_ahead = look(p.t0 + 1);
+    send_k(Even{}, p.t0);
+    send(Even{}, p.t0 - 2);  // K(t0 + 1), V(t0)
+    frag qf[DM / 16];
+    chunk_queries<T, DM>(g, s, p, qf);
+    widen_k(Even{}, p.t0);
+    send(Odd{}, p.t0 - 1);  // K(t0 + 2), V(t0 + 1)
+    ChunkState<P, DM> x;
+    floatx16 sc[2];
+    x.clear();
+    bool odd = false;
+    if constexpr (!EIGHT) {
+#pragma unroll
+      for (int i = 0; i < DM / 16; ++i) asm volatile("" : "+v"(qf[i]));  // (waits for the queries here, not in the loop)
+    }
+    auto look_for_odd = [&](int t) __attribute__((always_inline)) {
+      if constexpr (EIGHT) {
+        if (t >= p.full_block) odd |= odd_tile[t & 1] == t + 1;
+      } else if (t >= p.full_w) {
+        uint32_t most = 0;
+#pragma unroll 4
+        for (int i = 0; i < TILE / 1024; ++i) {
+          const u32x4 w = *(const u32x4*)(v_tile(t) + i * 1024 + lane * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) most = max(most, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+        }
+        odd |= __builtin_amdgcn_ballot_w64(most >= inf_bits<T>) != 0;
+      }
+    };
+    auto weights = [&](int t) __attribute__((always_inline)) {
+      ChunkFactors f[4];
+      uint32_t there = 1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = factors[t & 3][i];
+        there &= f[i].there;
+        if (!EIGHT) f[i].kf = c;
+      }
+      if (t >= p.full_w) chunk_hide(sc, p.last - t * BN - half * 4);
+      if (!__builtin_amdgcn_readfirstlane(there)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (!f[i].there) sc[i >> 1][8 * (i & 1) + r] = -INFINITY;
+      }
+      chunk_weights<P, EIGHT, false, DM>(x, sc, f, [](int, int) { return 1.0f; });
+    };
+    end_step();
+    auto step = [&](auto set, int t) __attribute__((always_inline)) {
+      constexpr int OTHER = (decltype(set)::value + 1) & 1;
+      if (t < p.nkt_w) {
+        if (t > p.t0) {
+          look_for_odd(t - 1);
+          __builtin_amdgcn_s_setprio(1);
+          chunk_products<T, P, DM, true, true>(tile, v_tile(t - 1), k_tile(t), qf, x, sc);
+          __builtin_amdgcn_s_setprio(0);
+        } else {
+          chunk_products<T, P, DM, false, true>(tile, nullptr, k_tile(t), qf, x, sc);
+        }
+      } else if (t > p.t0 && t == p.nkt_w) {
+        look_for_odd(t - 1);
+        chunk_products<T, P, DM, true, false>(tile, v_tile(t - 1), nullptr, qf, x, sc);
+      }
+      widen_k(std::integral_constant<int, OTHER>{}, t + 1);
+      widen_v(set, t);
+      send(set, t);
+      if (t < p.nkt_w) weights(t);
+      end_step();
+    };
+    for (int t = p.t0; t < p.t1; t += 2) {
+      step(Even{}, t);
+      if (t + 1 < p.t1) step(Odd{}, t + 1);
+    }
+    if (p.t0 < p.t1 && p.nkt_w == p.t1) {
+      look_for_odd(p.t1 - 1);
+      chunk_products<T, P, DM, true, false>(tile, v_tile(p.t1 - 1), nullptr, qf, x, sc);
+    }
+    chunk_finish<T, P, EIGHT, DM>(g, s, p, table, head, wave, odd, qf, x);
+    if (!at.next(g, p.end)) break;
+    // This piece's stages have been read, and what was sent for beyond its end has come.
+    if constexpr (!EIGHT) wait_loads<0>();
+    __syncthreads();
+    if (EIGHT && tid < RING) odd_tile[tid] = 0;
+  }
+  if constexpr (!EIGHT) wait_loads<0>();  // (before the LDS is another workgroup's)
+}
+
+// The same for pages of any number of slots, and strides of any size: a lane finds the page of the keys that it stages, which
+// pass through registers into LDS stages of 64 keys, and 8-bit scales are taken key by key.  Step t takes the values of
+// tile t - 1 and the scores and weights of tile t, stores tile t + 1 and sends for tile t + 2.
+template <typename T, bool EIGHT, int DM>
+__global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_keys_kernel(ChunkArgs g) {
+  using namespace ch;
+  typedef typename std::conditional<EIGHT, f16_t, T>::type P;  // the type of V^T P^T
+  typedef typename mfma_traits<T>::frag frag;
+  typedef ChunkTile<DM> Tile;
+  constexpr int ES = EIGHT ? 1 : 2, TILE = Tile::TILE, STAGES = 3;
   constexpr int CPR = DM * ES / 16, LOADS = 2 * BN * CPR / (NW * 64);  // 16-byte loads of a row, and of a lane
-  constexpr bool SPLIT_ROLES = LOADS == 1;                            // half of the lanes take K, half V
-  __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGES * TILE];  // K's stages, then V's
   __shared__ ChunkLds<NW * 64> place_lds;
   __shared__ int odd_tile[STAGES];  // 1 + the last tile in the stage that held an infinite or NaN v
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int D = g.dim;
-  const int head = blockIdx.x % g.kv_heads, part = blockIdx.x / g.kv_heads;
-  int64_t share = 0;
-  const ChunkPlace place = chunk_place(g, place_lds, [&](int64_t length) {
-    share = chunk_share(g, length);
-    return min(part * share, length - 1);  // (a workgroup past the end has nothing to do)
-  });
-  share = scalar64(share);
-  const int64_t begin = part * share, stop = min(begin + share, place.length);
-  if (begin >= stop) return;
-  int b = place.sequence;
-  int64_t seq_at = place.before;  // the line before sequence b
-  ChunkSequence s = chunk_sequence(g, b);
-  int nth = chunk_block(s, begin - seq_at);  // of its blocks
-
-  // What this lane stages of a tile: load u is 16 bytes of key load_key[u] at chunk load_chunk[u], of K or V.
-  auto k_swz = [](int key) { return DM == 128 ? key & 15 : (key >> 1) & 7; };
-  auto v_swz = [](int key) { return DM == 128 ? key & 3 : (key >> 1) & 1; };
+  const int D = g.dim, head = blockIdx.x % g.kv_heads;
+  ChunkStretch at(g, place_lds, blockIdx.x / g.kv_heads);
+  if (!at.there) return;
+  const Tile tile;
+  const float c = fmaxf(fabsf(g.scale_log2), LEAST_FACTOR);  // (of a scale of 0 times minus infinity would be NaN)
   const char* kbase = (const char*)g.k + head * g.ks[2] * ES;
   const char* vbase = (const char*)g.v + head * g.vs[2] * ES;
-  int load_key[LOADS], to_lds[LOADS];
-  bool load_in[LOADS];
-  int load_byte[LOADS];
-#pragma unroll
-  for (int u = 0; u < LOADS; ++u) {
-    const int at = u * NW * 64 + tid, key = at / CPR % BN, c = at % CPR;
-    const bool is_v = at >= BN * CPR;
-    load_key[u] = key;
-    load_byte[u] = c * 16;
-    load_in[u] = c * 16 < D * ES;
-    const int c16 = EIGHT ? 2 * c : c;  // of 16-bit elements
-    to_lds[u] = key * ROW + (is_v ? TILE + ((((c16 >> 2) ^ v_swz(key)) << 2) | (c16 & 3)) * 16 : (c16 ^ k_swz(key)) * 16);
-  }
-  // 8 bits: the second 8 elements' chunk; a K chunk's place differs in the lowest bit, as V's does.
-  const int row_of = lane & 31;
-  int k_rd[DSUB], v_rd[DBLK];
-#pragma unroll
-  for (int dd = 0; dd < DSUB; ++dd) k_rd[dd] = row_of * ROW + (((2 * dd + half) ^ k_swz(row_of)) * 16);
-  {
-    const int gq = lane >> 4, r = (lane & 15) >> 2, q = lane & 3;
-#pragma unroll
-    for (int i = 0; i < DBLK; ++i)
-      v_rd[i] = TILE + (4 * (gq >> 1) + r) * ROW + ((i ^ v_swz(r)) * 64) + (16 * (gq & 1) + 4 * q) * 2;
-  }
+  // What this lane stages of a tile: 16 bytes a load, at chunk `load % CPR` of key `load / CPR`, of K and then of V.
+  auto load_at = [&](int u) { return u * NW * 64 + tid; };
+  auto is_v = [&](int u) { return load_at(u) >= BN * CPR; };  // (the same in all of a wave's lanes)
   if (tid < STAGES) odd_tile[tid] = 0;
-  const float c = fmaxf(fabsf(g.scale_log2), LEAST_FACTOR);  // (of a scale of 0 times minus infinity would be NaN)
-  const uint32_t flip = g.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes to q's signs)
 
   while (true) {
-    // The piece: tiles [t0, t1) of block nth of sequence b, and whether they are all of its tiles.
-    const int64_t block_at = seq_at + chunk_line(s, nth), block_end = seq_at + chunk_line(s, nth + 1);
-    const int64_t keys_at = block_at + (int64_t)OVERHEAD * BN * g.group, tile_line = (int64_t)BN * g.group;
-    const bool whole = begin <= block_at && block_end <= stop;
-    const int r0 = nth * BM, rows = s.rows;
-    const int Sk = s.Sk, offset = Sk - s.Sq;
-    int nkt = (int)((uint32_t)(Sk + BN - 1) / BN), full_block = Sk / BN;
-    const int rw = r0 + wave * 32;  // first row of this wave
-    int nkt_w = nkt, full_w = Sk / BN;
-    if (g.causal) {
-      const int end = (min(r0 + BM, rows) - 1) / g.group + offset, end_w = (min(rw + 32, rows) - 1) / g.group + offset;
-      nkt = end < 0 ? 0 : min(nkt, end / BN + 1);
-      nkt_w = end_w < 0 ? 0 : min(nkt, end_w / BN + 1);
-      const int all = r0 / g.group + offset, all_w = rw / g.group + offset;  // every row sees the tiles before it
-      full_block = all < 0 ? 0 : min(full_block, (all + 1) / BN);
-      full_w = all_w < 0 ? 0 : min(full_w, (all_w + 1) / BN);
-    }
-    if (rw >= rows) nkt_w = 0;
-    auto tile_of = [&](int64_t p) {  // the first tile that begins at p or behind it
-      return p <= keys_at ? 0 : (int)min((int64_t)nkt, (int64_t)((uint64_t)(p - keys_at + tile_line - 1) / (uint64_t)tile_line));
-    };
-    const int t0 = tile_of(begin), t1 = stop >= block_end ? nkt : tile_of(stop);
-    nkt_w = min(nkt_w, t1);
-    const int row = rw + row_of, tok = row / g.group, qhead = head * g.group + (row - tok * g.group);
-    const bool valid = rw + row_of < rows;
-    const int last = min(g.causal ? tok + offset : Sk - 1, Sk - 1);
-    const int32_t* table = g.tables + b * g.table_stride;
-
-    // Staging.  Lane l of every wave looks up key l of a tile: its page (or -1), and with 8 bits its factors.
-    int page_ahead = -1;  // of the tile after the last one that was looked up
+    const ChunkSequence& s = at.s;
+    const ChunkPiece p = chunk_piece(g, s, at.seq_at, at.nth, at.begin, at.stop, head, wave);
+    const int32_t* table = g.tables + at.b * g.table_stride;
+    // Lane l of every wave looks up key l of a tile: its page (or -1), and with 8 bits its scales.
+    int page_ahead = -1;  // of the tile after the last one that was sent for
     auto page_of = [&](int kt) {
       const int key = kt * BN + lane;
-      if (kt >= t1 || key >= Sk) return -1;
-      return (int)table[g.page_shift >= 0 ? key >> g.page_shift : key / g.page_size];
+      if (kt >= p.t1 || key >= p.Sk) return -1;
+      return (int)table[key / g.page_size];
     };
     struct Keys {
       uint64_t there;   // keys that count
@@ -386,45 +925,35 @@ chunk_attention_kernel(ChunkArgs g) {
     };
     Keys keys_now, keys_next;
     u32x4 held[LOADS];
-    auto load = [&](int kt) __attribute__((always_inline)) {  // of the tile whose pages are page_ahead; then looks up the next
-      Keys found;
+    auto load = [&](int kt) __attribute__((always_inline)) {  // of the tile whose pages are page_ahead
       const bool ok = page_ahead >= 0 && page_ahead < g.pages;
       const int k_page = ok ? page_ahead : -1;
       int v_page = k_page;
-      found.there = __builtin_amdgcn_ballot_w64(ok);
-      found.kf = c;
-      found.lv = 0.f;
-      found.rv = 1.0f;
+      ChunkFactors found{c, 0.f, 1.0f, 0};
       if (EIGHT && ok) {
-        const int64_t at = (int64_t)page_ahead * g.kv_heads + head;
-        const float ks = g.k_scale[at], given = g.v_scale[at], vs = fminf(fmaxf(given, LEAST_SCALE), 3.0e38f);
-        if (given < LEAST_SCALE) v_page = -1;
-        found.kf = fmaxf(c * ks, LEAST_FACTOR);
-        found.lv = __builtin_amdgcn_logf(vs);
-        found.rv = __builtin_amdgcn_rcpf(vs);
+        const int64_t i = (int64_t)page_ahead * g.kv_heads + head;
+        found = chunk_factors(c, g.k_scale[i], g.v_scale[i], true);
+        if (g.v_scale[i] < LEAST_SCALE) v_page = -1;
       }
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) {
-        const bool is_v = SPLIT_ROLES ? tid >= NW * 32 : u >= LOADS / 2;  // (the same in all of a wave's lanes)
-        const int page = __shfl(is_v ? v_page : k_page, load_key[u], 64);
+        const int key = load_at(u) / CPR % BN, byte = load_at(u) % CPR * 16;
+        const int page = __shfl(is_v(u) ? v_page : k_page, key, 64);
         held[u] = u32x4{0u, 0u, 0u, 0u};
-        if (page >= 0 && load_in[u]) {
-          const int key = kt * BN + load_key[u];
-          const int slot = g.page_shift >= 0 ? key & (g.page_size - 1) : key % g.page_size;
-          const int64_t* st = is_v ? g.vs : g.ks;
-          held[u] = *(const u32x4*)((is_v ? vbase : kbase) + (page * st[0] + slot * st[1]) * ES + load_byte[u]);
+        if (page >= 0 && byte < D * ES) {
+          const int slot = (kt * BN + key) % g.page_size;
+          const int64_t page_stride = is_v(u) ? g.vs[0] : g.ks[0], slot_stride = is_v(u) ? g.vs[1] : g.ks[1];
+          held[u] = *(const u32x4*)((is_v(u) ? vbase : kbase) + (page * page_stride + slot * slot_stride) * ES + byte);
         }
       }
       page_ahead = page_of(kt + 1);
-      return found;
+      return Keys{__builtin_amdgcn_ballot_w64(ok), found.kf, found.lv, found.rv};
     };
     auto store = [&](int kt) __attribute__((always_inline)) {
-      char* to = lds + kt % STAGES * STAGE;
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) {
         u32x4 x = held[u];
-        const bool is_v = SPLIT_ROLES ? tid >= NW * 32 : u >= LOADS / 2;
-        if (kt >= full_block && is_v) {
+        if (kt >= p.full_block && is_v(u)) {
           bool odd = false;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -438,93 +967,37 @@ chunk_attention_kernel(ChunkArgs g) {
           if (odd) {
             odd_tile[kt % STAGES] = kt + 1;
             if constexpr (EIGHT)
-              x = finite16(x);
+              x = finite_bytes(x);
             else
               x = finite8<T>(x);
           }
         }
+        const int key = load_at(u) / CPR % BN, chunk = load_at(u) % CPR * (EIGHT ? 2 : 1);
+        const int to = (is_v(u) ? STAGES * TILE + Tile::v_place(key, chunk) : Tile::k_place(key, chunk)) + kt % STAGES * TILE;
         if constexpr (EIGHT) {
-          const u32x4 lo = is_v ? wide8<P>(x[0], x[1]) : wide8<T>(x[0], x[1]);
-          const u32x4 hi = is_v ? wide8<P>(x[2], x[3]) : wide8<T>(x[2], x[3]);
-          *(u32x4*)(to + to_lds[u]) = lo;
-          *(u32x4*)(to + (to_lds[u] ^ 16)) = hi;
+          *(u32x4*)(lds + to) = is_v(u) ? wide8<P>(x[0], x[1]) : wide8<T>(x[0], x[1]);
+          *(u32x4*)(lds + (to ^ 16)) = is_v(u) ? wide8<P>(x[2], x[3]) : wide8<T>(x[2], x[3]);
         } else {
-          *(u32x4*)(to + to_lds[u]) = x;
+          *(u32x4*)(lds + to) = x;
         }
       }
     };
 
-    page_ahead = page_of(t0);
-    if (t0 < t1) keys_now = load(t0);
-    frag qf[DSUB];
-    const uint16_t* Q = (const uint16_t*)g.q + (int64_t)(s.begin + tok) * g.qs[0] + qhead * g.qs[1];
-    const int64_t q_es = stride_here(g.qs[2]);
-    const int q_at = lane_here(half * 8);
-#pragma unroll
-    for (int dd = 0; dd < DSUB; ++dd) {
-      const int d = dd * 16 + q_at;
-      u32x4 raw = {0u, 0u, 0u, 0u};
-      if (valid && d < D) {
-        if (g.q_vectors) {
-          raw = *(const u32x4*)(Q + d);
-        } else {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) raw[w] = Q[(d + 2 * w) * q_es] | (uint32_t)Q[(d + 2 * w + 1) * q_es] << 16;
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) raw[w] ^= flip;
-      qf[dd] = __builtin_bit_cast(frag, raw);
-    }
-
-    floatx16 o_acc[DBLK], sc[2];
-    pfrag pf[BN / 16];
-    float m = UNSET, l = 0.f;  // l: of this lane's half of the keys
+    page_ahead = page_of(p.t0);
+    if (p.t0 < p.t1) keys_now = load(p.t0);
+    frag qf[DM / 16];
+    chunk_queries<T, DM>(g, s, p, qf);
+    ChunkState<P, DM> x;
+    floatx16 sc[2];
+    x.clear();
     bool odd = false;
-#pragma unroll
-    for (int i = 0; i < DBLK; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o_acc[i][r] = 0.f;
-
-    auto v_frag = [&](const char* base, int t, int i) {
-      typedef short v4i16 __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) v4i16* lds_v4;
-      const char* p = base + v_rd[i] + t * (16 * ROW);
-      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)p));
-      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(p + 8 * ROW)));
-      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    auto k_tile = [&](int t) { return (const char*)lds + t % STAGES * TILE; };
+    auto v_tile = [&](int t) { return (const char*)lds + (STAGES + t % STAGES) * TILE; };
+    auto look_for_odd = [&](int t) {
+      if (t >= p.full_block) odd |= odd_tile[t % STAGES] == t + 1;
     };
-    // O^T += V^T P^T of tile kt.
-    auto values = [&](int kt) __attribute__((always_inline)) {
-      const char* base = lds + kt % STAGES * STAGE;
-      if (kt >= full_block) odd |= odd_tile[kt % STAGES] == kt + 1;
-#pragma unroll
-      for (int n = 0; n < BN / 16 * DBLK; ++n)
-        o_acc[n % DBLK] = mfma_traits<P>::mma(__builtin_bit_cast(pfrag, v_frag(base, n / DBLK, n % DBLK)), pf[n / DBLK],
-                                              o_acc[n % DBLK]);
-    };
-    // S^T = K Q^T of tile kt.
-    auto scores = [&](int kt) __attribute__((always_inline)) {
-      const char* base = lds + kt % STAGES * STAGE;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[kb][r] = 0.f;
-#pragma unroll
-      for (int n = 0; n < 2 * DSUB; ++n)
-        sc[n & 1] = mfma_traits<T>::mma(*(const frag*)(base + k_rd[n >> 1] + (n & 1) * (32 * ROW)), qf[n >> 1], sc[n & 1]);
-    };
-    // The tile's weights, and what they add to the sum.  (Register r of block kb: key kb * 32 + r / 4 * 8 + half * 4 +
-    // r % 4; 16 neighbouring keys are 8 registers of both halves.)
-    auto weights = [&](int kt, const Keys& k) __attribute__((always_inline)) {
-      if (kt >= full_w) {
-        const int room = last - kt * BN - half * 4;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (kb * 32 + (r >> 2) * 8 + (r & 3) > room) sc[kb][r] = -INFINITY;
-      }
+    auto weights = [&](int t, const Keys& k) __attribute__((always_inline)) {
+      if (t >= p.full_w) chunk_hide(sc, p.last - t * BN - half * 4);
       if (k.there != ~0ull) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -534,167 +1007,48 @@ chunk_attention_kernel(ChunkArgs g) {
             if (!(there >> ((r >> 2) * 8 + (r & 3)) & 1)) sc[kb][r] = -INFINITY;
         }
       }
-      float kf[4], lv[4], rv[4];
-      if constexpr (EIGHT && SIXTEENS) {
-        auto of = [&](float x, int i) {
-          return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 16 * i));
-        };
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          kf[i] = of(k.kf, i);
-          lv[i] = of(k.lv, i);
-          rv[i] = of(k.rv, i);
-        }
-      } else if constexpr (EIGHT) {
-        // Scales key by key: the scores become exponents, and the weights' reciprocals come in below.
+      auto key_of = [&](int kb, int r) { return kb * 32 + (r >> 2) * 8 + half * 4 + (r & 3); };
+      if constexpr (EIGHT) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = kb * 32 + (r >> 2) * 8 + half * 4 + (r & 3);
-            sc[kb][r] = __builtin_fmaf(sc[kb][r], __shfl(k.kf, key, 64), __shfl(k.lv, key, 64));
-          }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          kf[i] = 1.0f;
-          lv[i] = 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) kf[i] = c;
+          for (int r = 0; r < 16; ++r)
+            sc[kb][r] = __builtin_fmaf(sc[kb][r], __shfl(k.kf, key_of(kb, r), 64), __shfl(k.lv, key_of(kb, r), 64));
       }
-      float add = 0.f;  // of this tile, to l
-      auto exponentials = [&]() __attribute__((always_inline)) {
-        float all = 0.f;
-        add = 0.f;
-#pragma unroll
-        for (int t = 0; t < BN / 16; ++t) {
-          u32x4 w;
-          float sum = 0.f;
-          const float shift = EIGHT ? lv[t] - m : -m;
-#pragma unroll
-          for (int sl = 0; sl < 4; ++sl) {
-            const int e = 8 * (t & 1) + 2 * sl;
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t >> 1][e], kf[t], shift));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t >> 1][e + 1], kf[t], shift));
-            w[sl] = pack2<P>(p0, p1);
-            if constexpr (EIGHT) {
-              sum += p0;
-              sum += p1;
-              if constexpr (!SIXTEENS) {
-                const int key = (t >> 1) * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
-                add = __builtin_fmaf(p0, __shfl(k.rv, key, 64), add);
-                add = __builtin_fmaf(p1, __shfl(k.rv, key + 1, 64), add);
-              }
-            } else {
-              sum = add2<P>(w[sl], sum);
-            }
-          }
-          pf[t] = __builtin_bit_cast(pfrag, w);
-          all += sum;
-          if constexpr (EIGHT && SIXTEENS) add = __builtin_fmaf(sum, rv[t], add);
-        }
-        if constexpr (!EIGHT) add = all;
-        return all;
-      };
-      const float all = exponentials();
-      if (__builtin_amdgcn_ballot_w64(!(all <= MOST_SUM))) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = sc[i >> 1][8 * (i & 1)];
-#pragma unroll
-          for (int r = 1; r < 8; ++r) x = fmaxf(x, sc[i >> 1][8 * (i & 1) + r]);
-          mx = fmaxf(mx, EIGHT ? __builtin_fmaf(x, kf[i], lv[i]) : x * kf[i]);
-        }
-        const float grown = fmaxf(max_halves(mx), m), alpha = __builtin_amdgcn_exp2f(m - grown);
-        l *= alpha;
-#pragma unroll
-        for (int i = 0; i < DBLK; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o_acc[i][r] *= alpha;
-        m = grown;
-        exponentials();
-      }
-      l += add;
+      const ChunkFactors f[4] = {{c, 0.f, 1.0f, 1}, {c, 0.f, 1.0f, 1}, {c, 0.f, 1.0f, 1}, {c, 0.f, 1.0f, 1}};
+      chunk_weights<P, EIGHT, EIGHT, DM>(x, sc, f, [&](int kb, int r) { return __shfl(k.rv, key_of(kb, r), 64); });
     };
-
-    // Step t takes the values of tile t - 1 and the scores of tile t, puts tile t + 1 into its stage (which no step
-    // since the last barrier reads) and sends for tile t + 2, then takes tile t's weights.
-    if (t0 < t1) {
-      store(t0);
-      if (t0 + 1 < t1) keys_next = load(t0 + 1);
+    if (p.t0 < p.t1) {
+      store(p.t0);
+      if (p.t0 + 1 < p.t1) keys_next = load(p.t0 + 1);
     }
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-      if (t < nkt_w) {
-        if (t > t0) values(t - 1);
-        scores(t);
-      } else if (t > t0 && t == nkt_w) {
-        values(t - 1);
+    for (int t = p.t0; t < p.t1; ++t) {
+      if (t < p.nkt_w) {
+        if (t > p.t0) {
+          look_for_odd(t - 1);
+          chunk_products<T, P, DM, true, true>(tile, v_tile(t - 1), k_tile(t), qf, x, sc);
+        } else {
+          chunk_products<T, P, DM, false, true>(tile, nullptr, k_tile(t), qf, x, sc);
+        }
+      } else if (t > p.t0 && t == p.nkt_w) {
+        look_for_odd(t - 1);
+        chunk_products<T, P, DM, true, false>(tile, v_tile(t - 1), nullptr, qf, x, sc);
       }
       Keys keys_then = keys_next;
-      if (t + 1 < t1) store(t + 1);
-      if (t + 2 < t1) keys_then = load(t + 2);
-      if (t < nkt_w) weights(t, keys_now);
+      if (t + 1 < p.t1) store(t + 1);
+      if (t + 2 < p.t1) keys_then = load(t + 2);
+      if (t < p.nkt_w) weights(t, keys_now);
       keys_now = keys_next;
       keys_next = keys_then;
       __syncthreads();
     }
-    if (t0 < t1 && nkt_w == t1) values(t1 - 1);
-
-    l += other_half(l);
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (begin <= block_at ? 1 : 0);
-    const int64_t state = slot * BM + (rw - r0) + row_of;
-    uint16_t* O = (uint16_t*)g.o + (int64_t)(s.begin + tok) * g.os[0] + qhead * g.os[1];
-    const int64_t o_es = stride_here(g.os[2]);
-    const int o_at = lane_here(half * 4);
-    // Four neighbouring elements from d on.
-    auto put = [&](int d, float f, float x0, float x1, float x2, float x3) {
-      if (!whole) {
-        *(floatx4*)(g.part_o + state * DM + d) = floatx4{x0, x1, x2, x3};
-      } else if (g.o_vectors) {
-        *(u32x2*)(O + d) = u32x2{pack2<T>(x0 * f, x1 * f), pack2<T>(x2 * f, x3 * f)};
-      } else {
-        O[d * o_es] = elem<T>::from_float(x0 * f);
-        O[(d + 1) * o_es] = elem<T>::from_float(x1 * f);
-        O[(d + 2) * o_es] = elem<T>::from_float(x2 * f);
-        O[(d + 3) * o_es] = elem<T>::from_float(x3 * f);
-      }
-    };
-    if (odd) {
-      float o[DM / 2];
-      chunk_rows_by_key<T, EIGHT, DM>(g, table, head, qf, c, t0 * BN, min(Sk, nkt_w * BN), valid ? last : -1, m, l, o);
-      const float inv = l != 0.f ? 1.0f / l : 0.f;
-      if (valid) {
-#pragma unroll
-        for (int i = 0; i < DM / 2; i += 4) {
-          const int d = i / 8 * 16 + 2 * o_at + i % 8;
-          if (d < D) put(d, inv, o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
-      }
-    } else if (valid) {
-      const float inv = l != 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-      for (int i = 0; i < DBLK; ++i)
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int d = i * 32 + r4 * 8 + o_at;
-          if (d < D) put(d, inv, o_acc[i][4 * r4], o_acc[i][4 * r4 + 1], o_acc[i][4 * r4 + 2], o_acc[i][4 * r4 + 3]);
-        }
+    if (p.t0 < p.t1 && p.nkt_w == p.t1) {
+      look_for_odd(p.t1 - 1);
+      chunk_products<T, P, DM, true, false>(tile, v_tile(p.t1 - 1), nullptr, qf, x, sc);
     }
-    if (!whole && valid && half == 0) *(float2*)(g.part_ml + state * 2) = float2{l != 0.f ? m : -INFINITY, l};
-
-    // The next piece.
-    if (block_end >= stop) return;
-    if (++nth == s.blocks) {
-      seq_at += chunk_line(s, s.blocks);
-      do {
-        ++b;
-        s = chunk_sequence(g, b);  // (the line goes on: there is one with rows)
-      } while (s.blocks == 0);
-      nth = 0;
-    }
+    chunk_finish<T, P, EIGHT, DM>(g, s, p, table, head, wave, odd, qf, x);
+    if (!at.next(g, p.end)) return;
     __syncthreads();  // this piece's stages have been read
     if (tid < STAGES) odd_tile[tid] = 0;
     __syncthreads();
@@ -775,10 +1129,12 @@ static int64_t chunk_state_bytes(int64_t parts, int64_t kv_heads, int64_t dim) {
 template <typename T, bool EIGHT, int DM>
 static void chunk_launch(const ChunkArgs& g, hipStream_t stream) {
   const dim3 grid((unsigned)(g.parts * g.kv_heads)), block(ch::NW * 64);
-  if (!EIGHT || g.page_size % 16 == 0)
-    hipLaunchKernelGGL((chunk_attention_kernel<T, EIGHT, DM, true>), grid, block, 0, stream, g);
+  // (a wave's eight keys are reckoned in 31 bits)
+  auto small = [&](const int64_t* st) { return st[0] >= 0 && st[1] >= 0 && st[1] <= (1 << 24); };
+  if (g.page_size % 16 == 0 && small(g.ks) && small(g.vs))
+    hipLaunchKernelGGL((chunk_pages_kernel<T, EIGHT, DM>), grid, block, 0, stream, g);
   else
-    hipLaunchKernelGGL((chunk_attention_kernel<T, EIGHT, DM, false>), grid, block, 0, stream, g);
+    hipLaunchKernelGGL((chunk_keys_kernel<T, EIGHT, DM>), grid, block, 0, stream, g);
   if (g.parts > 1)
     hipLaunchKernelGGL((chunk_join_kernel<T, DM>), dim3((unsigned)((g.parts - 1) * g.kv_heads * (ch::BM / ch::JOIN_ROWS))),
                        dim3(256), 0, stream, g);
