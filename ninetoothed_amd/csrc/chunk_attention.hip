@@ -43,15 +43,6 @@ __device__ __forceinline__ V finite_bytes(V w) {
       if (((w[i] >> b) & 0x7fu) == 0x7fu) w[i] &= ~(0xffu << b);
   return w;
 }
-// The bytes at an offset of a buffer of so many bytes (uniform) into registers; zeros past its end.
-template <typename V>
-__device__ __forceinline__ V buffer_load(const void* base, int bytes, int offset) {
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
-  if constexpr (sizeof(V) == 16)
-    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0));
-  else
-    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(rs, offset, 0, 0));
-}
 
 }  // namespace ch
 
@@ -190,8 +181,8 @@ __device__ __forceinline__ int64_t chunk_share(const ChunkArgs& g, int64_t lengt
   return max((length + g.parts - 1) / g.parts, (int64_t)ch::LEAST * ch::BN * g.group);
 }
 
-// A value that the compiler takes for new each time: it would keep what is reckoned from it in registers over the loop
-// of pieces.
+// A value that the compiler takes for new each time: it would keep what is reckoned from it in registers over a loop,
+// and have too few.
 __device__ __forceinline__ int64_t stride_here(int64_t stride) {
   asm volatile("" : "+s"(stride));
   return stride;
@@ -538,14 +529,11 @@ __device__ __forceinline__ void chunk_products(const ChunkTile<DM>& at, const ch
                                           x.pf[n / DBLK], x.o[n % DBLK]);
   }
   if constexpr (WK) {
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sc[kb][r] = 0.f;
+    const floatx16 none = {};
 #pragma unroll
     for (int n = 0; n < NK; ++n)
       sc[n & 1] = mfma_traits<T>::mma(__builtin_bit_cast(typename mfma_traits<T>::frag, at.k_frag(k_tile, n & 1, n >> 1)),
-                                      qf[n >> 1], sc[n & 1]);
+                                      qf[n >> 1], n < 2 ? none : sc[n & 1]);
   }
   constexpr int MFMA = 0x8, READ = 0x100, AHEAD_V = 6, AHEAD_K = 8;  // (a V fragment is two reads)
   if constexpr (WV) {
@@ -631,9 +619,9 @@ struct ChunkStretch {
 //     infinite or NaN v would still turn into NaN: rows of a tile that is masked and holds one are taken key by key, each
 //     over the keys that it sees (8 bits: such values are stored as zeros, and the tile is marked).
 // This kernel: pages of whole multiples of 16 keys, so that the 8 keys of a tile that a wave stages lie in one page, which it
-// looks up by a scalar load.  A step takes tile t's scores and weights and tile t - 1's values; K(t + 3) and V(t + 2) are
-// sent for in it: into LDS (16 bits, four stages), or into registers (8 bits), from where they are widened into LDS (two
-// stages) two steps later.
+// looks up by a scalar load.  A step takes tile t - 1's values and tile t's scores and weights.  K(t + 3) and V(t + 2) are sent
+// for in it, by loads into LDS: four stages; with 8 bits they are raw, and each wave widens its own keys' into two more
+// as they come.
 template <typename T, bool EIGHT, int DM>
 __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_pages_kernel(ChunkArgs g) {
   using namespace ch;
@@ -643,12 +631,10 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
   typedef const __attribute__((address_space(4))) float* ScalarFloats;
   constexpr int ES = EIGHT ? 1 : 2, ROW = Tile::ROW, TILE = Tile::TILE, RING = EIGHT ? 2 : 4, KEYS = BN / NW;
-  constexpr int LOADS = EIGHT ? 1 : KEYS * ROW / 1024;  // of a wave, for K or V
-  constexpr int BYTES = EIGHT ? KEYS * DM / 64 : 16;    // of a lane in each
-  constexpr int PER_KEY = DM * ES / BYTES;              // lanes of a key
-  static_assert(LOADS * 64 * BYTES == KEYS * DM * ES, "a wave's share of a tile");
-  typedef typename std::conditional<BYTES == 16, u32x4, u32x2>::type Held;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * RING * TILE];  // K's stages, then V's
+  constexpr int LOADS = EIGHT ? 1 : KEYS * ROW / 1024;  // of a wave, for K or V: 16 bytes a lane
+  constexpr int PER_KEY = DM * ES / 16;                 // lanes of a key
+  constexpr int RAW = EIGHT ? 2 * RING * TILE : 0, SENT = LOADS * NW * 1024;  // where stages of loads begin, and their size
+  __shared__ __attribute__((aligned(1024))) char lds[RAW + 8 * SENT];  // (wide: K's two, then V's;) K's four, then V's
   __shared__ ChunkLds<NW * 64> place_lds;
   __shared__ ChunkFactors factors[4][4];  // of tile t in [t % 4], its sixteens
   __shared__ int odd_tile[RING];          // 8 bits: 1 + the last tile in the stage that held a NaN v
@@ -669,11 +655,12 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   for (int u = 0; u < LOADS; ++u) {
     const int own = u * (64 / PER_KEY) + lane / PER_KEY, key = wave * KEYS + own, p = lane % PER_KEY;
     const int kc = EIGHT ? p : p ^ Tile::k_swz(key), vc = EIGHT ? p : ((((p >> 2) ^ Tile::v_swz(key)) << 2) | (p & 3));
-    k_off[u] = kc * BYTES < D * ES ? own * kst + kc * BYTES : 0x7fffffff;
-    v_off[u] = vc * BYTES < D * ES ? own * vst + vc * BYTES : 0x7fffffff;
+    k_off[u] = own < KEYS && kc * 16 < D * ES ? own * kst + kc * 16 : 0x7fffffff;
+    v_off[u] = own < KEYS && vc * 16 < D * ES ? own * vst + vc * 16 : 0x7fffffff;
   }
-  // 8 bits: where this lane's first eight elements lie in a stage (the others of sixteen: XORed by 16).
-  const int own_key = wave * KEYS + lane / PER_KEY, own_chunk = lane % PER_KEY * (BYTES / 8);
+  // 8 bits: where this lane's first eight elements lie in a stage (the other eight: XORed by 16).  (In heads of 64 the
+  // upper lanes repeat the lower ones.)
+  const int own_lane = lane & (KEYS * PER_KEY - 1), own_key = wave * KEYS + own_lane / PER_KEY, own_chunk = own_lane % PER_KEY * 2;
   const int k_to = Tile::k_place(own_key, own_chunk), v_to = RING * TILE + Tile::v_place(own_key, own_chunk);
   if (EIGHT && tid < RING) odd_tile[tid] = 0;
 
@@ -689,16 +676,12 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       return (int)pages[g.page_shift >= 0 ? first >> g.page_shift : first / g.page_size];
     };
     // The wave's keys of tile t in a page, as a buffer that ends with the last key.
-    struct Buffer {
-      const char* base;
-      int bytes;
-    };
     auto keys_of = [&](const char* base, int64_t page_stride, int st, int page, int t) {
       const int first = t * BN + wave * KEYS;
       const int slot = g.page_shift >= 0 ? first & (g.page_size - 1) : first % g.page_size;
       const bool ok = (uint32_t)page < (uint64_t)g.pages;
       const int n = ok ? min(KEYS, p.Sk - first) : 0;
-      return Buffer{base + ((int64_t)(ok ? page : 0) * page_stride * ES + (int64_t)slot * st), n > 0 ? (n - 1) * st + D * ES : 0};
+      return buffer_of(base + ((int64_t)(ok ? page : 0) * page_stride * ES + (int64_t)slot * st), n > 0 ? (n - 1) * st + D * ES : 0);
     };
     // The pages of tiles t + 4 (looked up), t + 3 and t + 2, and the scales of t + 3's.
     int page_ahead, page_k, page_v;
@@ -716,64 +699,60 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       const bool there = t * BN + wave * KEYS >= p.Sk || (uint32_t)page < (uint64_t)g.pages;
       if ((wave & 1) == 0 && lane == 0) factors[t & 3][wave >> 1] = chunk_factors(c, ks_v, vs_v, there);
     };
-    Held k_held[2], v_held[2];
-    auto send_k = [&](auto set, int t) __attribute__((always_inline)) {
-      const Buffer keys = keys_of(kbase, g.ks[0], kst, page_k, t);
-      if constexpr (EIGHT) {
-        k_held[decltype(set)::value] = buffer_load<Held>(keys.base, keys.bytes, k_off[0]);
-      } else {
-        const u32x4 rs = buffer_of(keys.base, keys.bytes);
+    auto send_k = [&](int t) __attribute__((always_inline)) {
+      const u32x4 rs = keys_of(kbase, g.ks[0], kst, page_k, t);
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) buffer_to_lds(rs, lds_at + (t & 3) * TILE + (wave * LOADS + u) * 1024, k_off[u], 0);
-      }
+      for (int u = 0; u < LOADS; ++u)
+        buffer_to_lds(rs, lds_at + RAW + (t & 3) * SENT + (wave * LOADS + u) * 1024, k_off[u], 0);
     };
-    auto send_v = [&](auto set, int t) __attribute__((always_inline)) {
-      const Buffer keys = keys_of(vbase, g.vs[0], vst, EIGHT && vs_v < LEAST_SCALE ? -1 : page_v, t);
-      if constexpr (EIGHT) {
-        v_held[decltype(set)::value] = buffer_load<Held>(keys.base, keys.bytes, v_off[0]);
-      } else {
-        const u32x4 rs = buffer_of(keys.base, keys.bytes);
+    auto send_v = [&](int t) __attribute__((always_inline)) {
+      const u32x4 rs = keys_of(vbase, g.vs[0], vst, EIGHT && vs_v < LEAST_SCALE ? -1 : page_v, t);
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u)
-          buffer_to_lds(rs, lds_at + (RING + (t & 3)) * TILE + (wave * LOADS + u) * 1024, v_off[u], 0);
-      }
+      for (int u = 0; u < LOADS; ++u)
+        buffer_to_lds(rs, lds_at + RAW + (4 + (t & 3)) * SENT + (wave * LOADS + u) * 1024, v_off[u], 0);
     };
     // Tiles t + 3 and t + 2 sent for, and what comes after them looked up.
-    auto send = [&](auto set, int t) __attribute__((always_inline)) {
+    auto send = [&](int t) __attribute__((always_inline)) {
       page_v = page_k;
       ks_v = ks_k;
       vs_v = vs_k;
       page_k = page_ahead;
       page_ahead = look(t + 4);
       share(t + 2, page_v);
-      send_k(std::integral_constant<int, (decltype(set)::value + 1) & 1>{}, t + 3);
-      send_v(set, t + 2);
+      send_k(t + 3);
+      send_v(t + 2);
       scales(page_k);
     };
-    auto widen_k = [&](auto set, int t) __attribute__((always_inline)) {
-      if constexpr (EIGHT) {
-        const Held& x = k_held[decltype(set)::value];
-        *(u32x4*)(lds + (t & 1) * TILE + k_to) = wide8<T>(x[0], x[1]);
-        if constexpr (BYTES == 16) *(u32x4*)(lds + (t & 1) * TILE + (k_to ^ 16)) = wide8<T>(x[2], x[3]);
-      }
+    // 8 bits: this wave's keys of a tile, which have come, into its wide stage.
+    auto widen_k = [&](int t) __attribute__((always_inline)) {
+      const u32x4 x = *(const u32x4*)(lds + RAW + (t & 3) * SENT + wave * 1024 + own_lane * 16);
+      *(u32x4*)(lds + (t & 1) * TILE + k_to) = wide8<T>(x[0], x[1]);
+      *(u32x4*)(lds + (t & 1) * TILE + (k_to ^ 16)) = wide8<T>(x[2], x[3]);
     };
-    auto widen_v = [&](auto set, int t) __attribute__((always_inline)) {
-      if constexpr (EIGHT) {
-        Held x = v_held[decltype(set)::value];
-        if (t >= p.full_block) {
-          bool odd = false;
+    auto widen_v = [&](int t) __attribute__((always_inline)) {
+      u32x4 x = *(const u32x4*)(lds + RAW + (4 + (t & 3)) * SENT + wave * 1024 + own_lane * 16);
+      if (t >= p.full_block) {
+        bool odd = false;
 #pragma unroll
-          for (int w = 0; w < BYTES / 4; ++w)
+        for (int w = 0; w < 4; ++w)
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) odd |= ((x[w] >> i) & 0x7fu) == 0x7fu;
-          if (odd) {
-            odd_tile[t & 1] = t + 1;
-            x = finite_bytes(x);
-          }
+          for (int i = 0; i < 32; i += 8) odd |= ((x[w] >> i) & 0x7fu) == 0x7fu;
+        if (odd) {
+          odd_tile[t & 1] = t + 1;
+          x = finite_bytes(x);
         }
-        *(u32x4*)(lds + (t & 1) * TILE + v_to) = wide8<P>(x[0], x[1]);
-        if constexpr (BYTES == 16) *(u32x4*)(lds + (t & 1) * TILE + (v_to ^ 16)) = wide8<P>(x[2], x[3]);
       }
+      *(u32x4*)(lds + (t & 1) * TILE + v_to) = wide8<P>(x[0], x[1]);
+      *(u32x4*)(lds + (t & 1) * TILE + (v_to ^ 16)) = wide8<P>(x[2], x[3]);
+    };
+    // What a step does for the tiles that come.
+    auto go_on = [&](int t) __attribute__((always_inline)) {
+      if constexpr (EIGHT) {
+        wait_loads<2>();  // K(t + 1) and V(t) have come
+        widen_k(t + 1);
+        widen_v(t);
+      }
+      send(t);
     };
     auto k_tile = [&](int t) { return (const char*)lds + (t & (RING - 1)) * TILE; };
     auto v_tile = [&](int t) { return (const char*)lds + (RING + (t & (RING - 1))) * TILE; };
@@ -786,27 +765,26 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
     };
-    typedef std::integral_constant<int, 0> Even;
-    typedef std::integral_constant<int, 1> Odd;
 
-    // Tiles t0 to t0 + 2 of K and the first two of V under way (even: t0).
+    // Tiles t0 to t0 + 2 of K and the first two of V under way.
+    frag qf[DM / 16];
+    chunk_queries<T, DM>(g, s, p, qf);
     page_k = look(p.t0);
     scales(page_k);
     page_ahead = look(p.t0 + 1);
-    send_k(Even{}, p.t0);
-    send(Even{}, p.t0 - 2);  // K(t0 + 1), V(t0)
-    frag qf[DM / 16];
-    chunk_queries<T, DM>(g, s, p, qf);
-    widen_k(Even{}, p.t0);
-    send(Odd{}, p.t0 - 1);  // K(t0 + 2), V(t0 + 1)
+    send_k(p.t0);
+    send(p.t0 - 2);
+    send(p.t0 - 1);
+#pragma unroll
+    for (int i = 0; i < DM / 16; ++i) asm volatile("" : "+v"(qf[i]));  // (waits for the queries here, not in the loop)
+    if constexpr (EIGHT) {
+      wait_loads<4>();  // K(t0) has come
+      widen_k(p.t0);
+    }
     ChunkState<P, DM> x;
     floatx16 sc[2];
     x.clear();
     bool odd = false;
-    if constexpr (!EIGHT) {
-#pragma unroll
-      for (int i = 0; i < DM / 16; ++i) asm volatile("" : "+v"(qf[i]));  // (waits for the queries here, not in the loop)
-    }
     auto look_for_odd = [&](int t) __attribute__((always_inline)) {
       if constexpr (EIGHT) {
         if (t >= p.full_block) odd |= odd_tile[t & 1] == t + 1;
@@ -841,43 +819,41 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       chunk_weights<P, EIGHT, false, DM>(x, sc, f, [](int, int) { return 1.0f; });
     };
     end_step();
-    auto step = [&](auto set, int t) __attribute__((always_inline)) {
-      constexpr int OTHER = (decltype(set)::value + 1) & 1;
-      if (t < p.nkt_w) {
-        if (t > p.t0) {
-          look_for_odd(t - 1);
-          __builtin_amdgcn_s_setprio(1);
-          chunk_products<T, P, DM, true, true>(tile, v_tile(t - 1), k_tile(t), qf, x, sc);
-          __builtin_amdgcn_s_setprio(0);
-        } else {
-          chunk_products<T, P, DM, false, true>(tile, nullptr, k_tile(t), qf, x, sc);
-        }
-      } else if (t > p.t0 && t == p.nkt_w) {
-        look_for_odd(t - 1);
-        chunk_products<T, P, DM, true, false>(tile, v_tile(t - 1), nullptr, qf, x, sc);
-      }
-      widen_k(std::integral_constant<int, OTHER>{}, t + 1);
-      widen_v(set, t);
-      send(set, t);
-      if (t < p.nkt_w) weights(t);
+    int t = p.t0;
+    if (t < p.nkt_w) {
+      chunk_products<T, P, DM, false, true>(tile, nullptr, k_tile(t), qf, x, sc);
+      go_on(t);
+      weights(t);
       end_step();
-    };
-    for (int t = p.t0; t < p.t1; t += 2) {
-      step(Even{}, t);
-      if (t + 1 < p.t1) step(Odd{}, t + 1);
+      for (++t; t < p.nkt_w; ++t) {
+        look_for_odd(t - 1);
+        __builtin_amdgcn_s_setprio(1);
+        chunk_products<T, P, DM, true, true>(tile, v_tile(t - 1), k_tile(t), qf, x, sc);
+        __builtin_amdgcn_s_setprio(0);
+        go_on(t);
+        weights(t);
+        end_step();
+      }
+      look_for_odd(t - 1);
+      chunk_products<T, P, DM, true, false>(tile, v_tile(t - 1), nullptr, qf, x, sc);
+      if (t < p.t1) {
+        go_on(t);
+        end_step();
+        ++t;
+      }
     }
-    if (p.t0 < p.t1 && p.nkt_w == p.t1) {
-      look_for_odd(p.t1 - 1);
-      chunk_products<T, P, DM, true, false>(tile, v_tile(p.t1 - 1), nullptr, qf, x, sc);
+    for (; t < p.t1; ++t) {  // what the workgroup's other waves still need
+      go_on(t);
+      end_step();
     }
     chunk_finish<T, P, EIGHT, DM>(g, s, p, table, head, wave, odd, qf, x);
     if (!at.next(g, p.end)) break;
     // This piece's stages have been read, and what was sent for beyond its end has come.
-    if constexpr (!EIGHT) wait_loads<0>();
+    wait_loads<0>();
     __syncthreads();
     if (EIGHT && tid < RING) odd_tile[tid] = 0;
   }
-  if constexpr (!EIGHT) wait_loads<0>();  // (before the LDS is another workgroup's)
+  wait_loads<0>();  // (before the LDS is another workgroup's)
 }
 
 // The same for pages of any number of slots, and strides of any size: a lane finds the page of the keys that it stages, which
