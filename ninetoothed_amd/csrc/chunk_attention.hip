@@ -637,10 +637,13 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   __shared__ __attribute__((aligned(1024))) char lds[RAW + 8 * SENT];  // (wide: K's two, then V's;) K's four, then V's
   __shared__ ChunkLds<NW * 64> place_lds;
   __shared__ ChunkFactors factors[4][4];  // of tile t in [t % 4], its sixteens
-  __shared__ int odd_tile[RING];          // 8 bits: 1 + the last tile in the stage that held a NaN v
+  __shared__ int odd_tile[RING];          // 8 bits: the mark of the last tile in the stage that held a NaN v
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lead = wave / 4;
   const int D = g.dim, head = blockIdx.x % g.kv_heads;
+  int marked = 0;  // tiles of the pieces before this one
+  if (EIGHT && tid < RING) odd_tile[tid] = 0;
   ChunkStretch at(g, place_lds, blockIdx.x / g.kv_heads);
   if (!at.there) return;
   const Tile tile;
@@ -662,7 +665,6 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   // upper lanes repeat the lower ones.)
   const int own_lane = lane & (KEYS * PER_KEY - 1), own_key = wave * KEYS + own_lane / PER_KEY, own_chunk = own_lane % PER_KEY * 2;
   const int k_to = Tile::k_place(own_key, own_chunk), v_to = RING * TILE + Tile::v_place(own_key, own_chunk);
-  if (EIGHT && tid < RING) odd_tile[tid] = 0;
 
   while (true) {
     const ChunkSequence& s = at.s;
@@ -723,6 +725,7 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       send_v(t + 2);
       scales(page_k);
     };
+    auto mark_of = [&](int t) { return marked + (t - p.t0) + 1; };
     // 8 bits: this wave's keys of a tile, which have come, into its wide stage.
     auto widen_k = [&](int t) __attribute__((always_inline)) {
       const u32x4 x = *(const u32x4*)(lds + RAW + (t & 3) * SENT + wave * 1024 + own_lane * 16);
@@ -738,15 +741,16 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
           for (int i = 0; i < 32; i += 8) odd |= ((x[w] >> i) & 0x7fu) == 0x7fu;
         if (odd) {
-          odd_tile[t & 1] = t + 1;
+          odd_tile[t & 1] = mark_of(t);
           x = finite_bytes(x);
         }
       }
       *(u32x4*)(lds + (t & 1) * TILE + v_to) = wide8<P>(x[0], x[1]);
       *(u32x4*)(lds + (t & 1) * TILE + (v_to ^ 16)) = wide8<P>(x[2], x[3]);
     };
-    // What a step does for the tiles that come.
-    auto go_on = [&](int t) __attribute__((always_inline)) {
+    // What step `now` does for the tiles that come.
+    auto go_on = [&](int now) __attribute__((always_inline)) {
+      const int t = now + lead;
       if constexpr (EIGHT) {
         wait_loads<2>();  // K(t + 1) and V(t) have come
         widen_k(t + 1);
@@ -756,14 +760,18 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     };
     auto k_tile = [&](int t) { return (const char*)lds + (t & (RING - 1)) * TILE; };
     auto v_tile = [&](int t) { return (const char*)lds + (RING + (t & (RING - 1))) * TILE; };
-    // No access to LDS moves over it; all but the last two steps' loads into LDS have ended.
-    auto end_step = [&]() __attribute__((always_inline)) {
+    // No access to LDS moves over a turn; at a step's end all but the last two steps' loads into LDS have ended.
+    auto turn = [&]() __attribute__((always_inline)) {
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (!EIGHT) wait_loads<4 * LOADS>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
+    };
+    auto end_step = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!EIGHT) wait_loads<4 * LOADS>();
+      turn();
     };
 
     // Tiles t0 to t0 + 2 of K and the first two of V under way.
@@ -775,11 +783,16 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     send_k(p.t0);
     send(p.t0 - 2);
     send(p.t0 - 1);
+    if (lead) send(p.t0);
 #pragma unroll
     for (int i = 0; i < DM / 16; ++i) asm volatile("" : "+v"(qf[i]));  // (waits for the queries here, not in the loop)
     if constexpr (EIGHT) {
-      wait_loads<4>();  // K(t0) has come
+      wait_loads<4>();  // K(t0) has come, and in waves that lead K(t0 + 1) and V(t0)
       widen_k(p.t0);
+      if (lead) {
+        widen_k(p.t0 + 1);
+        widen_v(p.t0);
+      }
     }
     ChunkState<P, DM> x;
     floatx16 sc[2];
@@ -787,7 +800,7 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     bool odd = false;
     auto look_for_odd = [&](int t) __attribute__((always_inline)) {
       if constexpr (EIGHT) {
-        if (t >= p.full_block) odd |= odd_tile[t & 1] == t + 1;
+        if (t >= p.full_block) odd |= odd_tile[t & 1] == mark_of(t);
       } else if (t >= p.full_w) {
         uint32_t most = 0;
 #pragma unroll 4
@@ -819,17 +832,18 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       chunk_weights<P, EIGHT, false, DM>(x, sc, f, [](int, int) { return 1.0f; });
     };
     end_step();
+    if (lead) turn();
     int t = p.t0;
     if (t < p.nkt_w) {
       chunk_products<T, P, DM, false, true>(tile, nullptr, k_tile(t), qf, x, sc);
+      turn();
       go_on(t);
       weights(t);
       end_step();
       for (++t; t < p.nkt_w; ++t) {
         look_for_odd(t - 1);
-        __builtin_amdgcn_s_setprio(1);
         chunk_products<T, P, DM, true, true>(tile, v_tile(t - 1), k_tile(t), qf, x, sc);
-        __builtin_amdgcn_s_setprio(0);
+        turn();
         go_on(t);
         weights(t);
         end_step();
@@ -837,21 +851,24 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       look_for_odd(t - 1);
       chunk_products<T, P, DM, true, false>(tile, v_tile(t - 1), nullptr, qf, x, sc);
       if (t < p.t1) {
+        turn();
         go_on(t);
         end_step();
         ++t;
       }
     }
     for (; t < p.t1; ++t) {  // what the workgroup's other waves still need
+      turn();
       go_on(t);
       end_step();
     }
+    if (!lead) turn();
     chunk_finish<T, P, EIGHT, DM>(g, s, p, table, head, wave, odd, qf, x);
     if (!at.next(g, p.end)) break;
     // This piece's stages have been read, and what was sent for beyond its end has come.
     wait_loads<0>();
     __syncthreads();
-    if (EIGHT && tid < RING) odd_tile[tid] = 0;
+    marked += p.t1 - p.t0;
   }
   wait_loads<0>();  // (before the LDS is another workgroup's)
 }
