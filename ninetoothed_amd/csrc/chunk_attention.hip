@@ -628,8 +628,6 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   typedef typename std::conditional<EIGHT, f16_t, T>::type P;  // the type of V^T P^T
   typedef typename mfma_traits<T>::frag frag;
   typedef ChunkTile<DM> Tile;
-  typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
-  typedef const __attribute__((address_space(4))) float* ScalarFloats;
   constexpr int ES = EIGHT ? 1 : 2, ROW = Tile::ROW, TILE = Tile::TILE, RING = EIGHT ? 2 : 4, KEYS = BN / NW;
   constexpr int LOADS = EIGHT ? 1 : KEYS * ROW / 1024;  // of a wave, for K or V: 16 bytes a lane
   constexpr int PER_KEY = DM * ES / 16;                 // lanes of a key
@@ -670,60 +668,58 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     const ChunkSequence& s = at.s;
     const ChunkPiece p = chunk_piece(g, s, at.seq_at, at.nth, at.begin, at.stop, head, wave);
     const int32_t* table = g.tables + at.b * g.table_stride;
-    const ScalarInts pages = (ScalarInts)(uintptr_t)table;
-    // The page of this wave's keys of a tile, or -1.
-    auto look = [&](int t) {
-      const int first = t * BN + wave * KEYS;
-      if (t >= p.t1 || first >= p.Sk) return -1;
-      return (int)pages[g.page_shift >= 0 ? first >> g.page_shift : first / g.page_size];
-    };
-    // The wave's keys of tile t in a page, as a buffer that ends with the last key.
-    auto keys_of = [&](const char* base, int64_t page_stride, int st, int page, int t) {
-      const int first = t * BN + wave * KEYS;
-      const int slot = g.page_shift >= 0 ? first & (g.page_size - 1) : first % g.page_size;
-      const bool ok = (uint32_t)page < (uint64_t)g.pages;
-      const int n = ok ? min(KEYS, p.Sk - first) : 0;
-      return buffer_of(base + ((int64_t)(ok ? page : 0) * page_stride * ES + (int64_t)slot * st), n > 0 ? (n - 1) * st + D * ES : 0);
-    };
-    // The pages of tiles t + 4 (looked up), t + 3 and t + 2, and the scales of t + 3's.
-    int page_ahead, page_k, page_v;
-    float ks_k = 1.0f, vs_k = 1.0f, ks_v, vs_v;
-    auto scales = [&](int page) {
-      if constexpr (EIGHT) {
-        if ((uint32_t)page >= (uint64_t)g.pages) return;  // (those of another tile: nothing takes them)
-        const int64_t i = (int64_t)page * g.kv_heads + head;
-        ks_k = ((ScalarFloats)(uintptr_t)g.k_scale)[i];
-        vs_k = ((ScalarFloats)(uintptr_t)g.v_scale)[i];
+    // This wave's keys of the tiles from `window` on, a tile to a lane: where they lie in K and V, how far from there their
+    // bytes go (0: none), and what they share.  (Found here for 64 tiles at once: scalar code between two steps' loads was
+    // what a step waited for.)
+    int window;
+    int64_t k_at, v_at;
+    int k_bytes, v_bytes;
+    ChunkFactors shared;
+    auto look = [&](int t0) __attribute__((always_inline)) {
+      window = t0;
+      const bool inside = t0 + lane < p.t1;
+      const int first = inside ? (t0 + lane) * BN + wave * KEYS : 0;
+      const int nth = g.page_shift >= 0 ? first >> g.page_shift : first / g.page_size, slot = first - nth * g.page_size;
+      const bool any = inside && first < p.Sk;
+      int64_t page = any ? table[nth] : -1;
+      const bool there = page >= 0 && page < g.pages;
+      const int keys = there ? min(KEYS, p.Sk - first) : 0;
+      if (!there) page = 0;
+      k_at = (int64_t)(uintptr_t)kbase + page * g.ks[0] * ES + (int64_t)slot * kst;
+      v_at = (int64_t)(uintptr_t)vbase + page * g.vs[0] * ES + (int64_t)slot * vst;
+      k_bytes = keys > 0 ? (keys - 1) * kst + D * ES : 0;
+      v_bytes = keys > 0 ? (keys - 1) * vst + D * ES : 0;
+      float ks = 1.0f, vs = 1.0f;
+      if (EIGHT && there) {
+        ks = g.k_scale[page * g.kv_heads + head];
+        vs = g.v_scale[page * g.kv_heads + head];
+        if (vs < LEAST_SCALE) v_bytes = 0;
       }
+      shared = chunk_factors(c, ks, vs, there || !any);
     };
-    // What tile t's keys share, from the wave that has the first of each sixteen.
-    auto share = [&](int t, int page) {
-      const bool there = t * BN + wave * KEYS >= p.Sk || (uint32_t)page < (uint64_t)g.pages;
-      if ((wave & 1) == 0 && lane == 0) factors[t & 3][wave >> 1] = chunk_factors(c, ks_v, vs_v, there);
+    // The keys of one lane, as a buffer that ends with the last key.
+    auto keys_of = [&](int64_t at, int bytes, int i) {
+      const uint32_t lo = __builtin_amdgcn_readlane((int)at, i), hi = __builtin_amdgcn_readlane((int)(at >> 32), i);
+      return buffer_of((const char*)((uint64_t)hi << 32 | lo), __builtin_amdgcn_readlane(bytes, i));
     };
     auto send_k = [&](int t) __attribute__((always_inline)) {
-      const u32x4 rs = keys_of(kbase, g.ks[0], kst, page_k, t);
+      const u32x4 rs = keys_of(k_at, k_bytes, t - window);
 #pragma unroll
       for (int u = 0; u < LOADS; ++u)
         buffer_to_lds(rs, lds_at + RAW + (t & 3) * SENT + (wave * LOADS + u) * 1024, k_off[u], 0);
     };
+    // (and what tile t's keys share, from the wave that has the first of each sixteen)
     auto send_v = [&](int t) __attribute__((always_inline)) {
-      const u32x4 rs = keys_of(vbase, g.vs[0], vst, EIGHT && vs_v < LEAST_SCALE ? -1 : page_v, t);
+      const u32x4 rs = keys_of(v_at, v_bytes, t - window);
+      if ((wave & 1) == 0 && lane == t - window) factors[t & 3][wave >> 1] = shared;
 #pragma unroll
       for (int u = 0; u < LOADS; ++u)
         buffer_to_lds(rs, lds_at + RAW + (4 + (t & 3)) * SENT + (wave * LOADS + u) * 1024, v_off[u], 0);
     };
-    // Tiles t + 3 and t + 2 sent for, and what comes after them looked up.
     auto send = [&](int t) __attribute__((always_inline)) {
-      page_v = page_k;
-      ks_v = ks_k;
-      vs_v = vs_k;
-      page_k = page_ahead;
-      page_ahead = look(t + 4);
-      share(t + 2, page_v);
-      send_k(t + 3);
       send_v(t + 2);
-      scales(page_k);
+      if (t + 3 == window + 64) look(t + 3);
+      send_k(t + 3);
     };
     auto mark_of = [&](int t) { return marked + (t - p.t0) + 1; };
     // 8 bits: this wave's keys of a tile, which have come, into its wide stage.
@@ -777,9 +773,7 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
     // Tiles t0 to t0 + 2 of K and the first two of V under way.
     frag qf[DM / 16];
     chunk_queries<T, DM>(g, s, p, qf);
-    page_k = look(p.t0);
-    scales(page_k);
-    page_ahead = look(p.t0 + 1);
+    look(p.t0);
     send_k(p.t0);
     send(p.t0 - 2);
     send(p.t0 - 1);
