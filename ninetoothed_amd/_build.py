@@ -41,10 +41,11 @@ COMMON_FLAGS = (
 # Per-source flags.  attention.hip: builtin MFMAs keep their accumulators in VGPRs (its
 # one-wave-per-SIMD kernel puts only the output accumulators in AGPRs, through inline
 # assembly); without this the compiler would move every MFMA to AGPRs in that kernel and
-# copy the scores back and forth.  The other attentions: as attention.hip.
+# copy the scores back and forth.  The other attentions, and linear4.hip (its groups' sums): as attention.hip.
 _MFMA_IN_VGPRS = ("-mllvm", "-amdgpu-mfma-vgpr-form=1")
 FILE_FLAGS = {"attention.hip": _MFMA_IN_VGPRS, "prompt_attention.hip": _MFMA_IN_VGPRS,
-              "cache_attention.hip": _MFMA_IN_VGPRS, "chunk_attention.hip": _MFMA_IN_VGPRS}
+              "cache_attention.hip": _MFMA_IN_VGPRS, "chunk_attention.hip": _MFMA_IN_VGPRS,
+              "linear4.hip": _MFMA_IN_VGPRS}
 
 
 def hipcc() -> str:

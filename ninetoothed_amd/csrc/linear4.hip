@@ -1,4 +1,5 @@
 // Products with weights of 4 bits and a scale (and zero point) for each group of a row's elements.
+#include "attention_rows.h"
 #include "packed.h"
 #include "mfma_core.h"
 
@@ -18,6 +19,7 @@ struct Linear4Args {
 namespace l4 {
 
 constexpr int WAVES = 8;
+constexpr int TILE_WAVES = 4, TILE_ROWS = 64;  // of linear4_tiles_kernel
 constexpr int STEP = 128;  // elements of k a wave takes at a time: 16 bytes of weights a lane
 
 template <typename T>
@@ -79,6 +81,19 @@ __device__ __forceinline__ u32x4 across_quads(u32x4 w) {
   swap32(b, d);
   return u32x4{a, b, c, d};
 }
+// The sum over N neighbouring lanes (4, 8 or 16), in each of them.
+template <int N>
+__device__ __forceinline__ float over_lanes(float v) {
+  auto from = [&](auto code) __attribute__((always_inline)) {
+    constexpr int C = decltype(code)::value;
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), C, 0xf, 0xf, true));
+  };
+  v += from(std::integral_constant<int, 0xb1>());  // lane ^ 1
+  v += from(std::integral_constant<int, 0x4e>());  // lane ^ 2
+  if constexpr (N > 4) v += from(std::integral_constant<int, 0x141>());  // 7 - lane, of eight
+  if constexpr (N > 8) v += from(std::integral_constant<int, 0x140>());  // 15 - lane, of sixteen
+  return v;
+}
 
 }  // namespace l4
 
@@ -87,15 +102,16 @@ __device__ __forceinline__ u32x4 across_quads(u32x4 w) {
 //   out[m][n] = c[m][n] + sum_g scale[n][g] (sum_k x[m][k] (16 + q[n][k]) - (16 + zero[n][g]) sum_k x[m][k]),
 // where 16 + q is made from the bits, exact in either type, and the sums of x are a product with ones.
 // Bound by HBM for few rows: the weights are read once, 16 bytes a lane, by waves that share 16 NB columns and take
-// turns of 128 elements of k; x comes from the L2 for each of those workgroups.  A wave's 16 x 16 x 32 products take
+// turns of 128 elements of k; x comes from the L2 for each of those workgroups, the most of what is loaded beyond a
+// few rows (24 rows, k of 11,008, 4,096 columns: 24 us, of which the weights are 5; one row, k of 4,096: 5 us, a launch).  A wave's 16 x 16 x 32 products take
 // 32 neighbouring elements of k, which lie in one group, so a turn's four dwords go across the quads first.
 // MB: blocks of 16 rows; SUB: products of a turn that share a group.
-template <typename T, int MB, int NB, int SUB>
+template <typename T, int MB, int SUB>
 __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) {
   using namespace l4;
   typedef mma16<T> M;
   typedef typename M::frag frag;
-  constexpr int ROWS = MB * 16, COLS = NB * 16;
+  constexpr int NB = 1, ROWS = MB * 16, COLS = NB * 16;
   __shared__ float sums[WAVES][ROWS][COLS + 1];
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -124,14 +140,14 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       t.w[j] = u32x4{0u, 0u, 0u, 0u};
-      if (k0 + quad * 32 < k) t.w[j] = *(const u32x4*)(W[j] + k0 / 2);
+      if (SUB == 4 || k0 + quad * 32 < k) t.w[j] = *(const u32x4*)(W[j] + k0 / 2);
     }
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         t.x[i][p] = u32x4{0u, 0u, 0u, 0u};
-        if (k0 + p * 32 < k) t.x[i][p] = *(const u32x4*)(X[i] + k0 + p * 32);
+        if (SUB == 4 || k0 + p * 32 < k) t.x[i][p] = *(const u32x4*)(X[i] + k0 + p * 32);
       }
 #pragma unroll
     for (int p = 0; p < 4; p += SUB) {
@@ -187,12 +203,20 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
       }
     }
   };
-  Turn now, next;
-  if (wave < steps) load(now, wave);
-  for (int step = wave; step < steps; step += WAVES) {
-    if (step + WAVES < steps) load(next, step + WAVES);
-    take(now);
-    now = next;
+  // (each turn's registers keep their place: a copy would wait for what they were sent for)
+  constexpr int AHEAD = MB == 4 ? 2 : MB == 2 ? 3 : 4;
+  Turn turns[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (wave + i * WAVES < steps) load(turns[i], wave + i * WAVES);
+  for (int step0 = wave; step0 < steps; step0 += AHEAD * WAVES) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int step = step0 + i * WAVES;
+      if (step >= steps) break;
+      take(turns[i]);
+      if (step + AHEAD * WAVES < steps) load(turns[i], step + AHEAD * WAVES);
+    }
   }
   // (row quad * 4 + r, column col of a block)
 #pragma unroll
@@ -211,6 +235,156 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
     if (g.c) y += elem<T>::to_float(((const uint16_t*)g.c)[(m0 + m) * g.cs[0] + (n0 + n) * g.cs[1]]);
     ((uint16_t*)g.out)[(m0 + m) * g.os[0] + (n0 + n) * g.os[1]] = elem<T>::from_float(y);
   }
+}
+
+// The same for many rows, where the MFMAs bound it: a workgroup takes 32 MB rows and 128 columns, a wave 32 of those, so that
+// each weight is widened once for all of the rows, from the registers that it was loaded into.  x passes through two
+// LDS stages of 128 elements of k, in the weights' order of pairs, and is summed on its way.  A lane's weights of a
+// 32 x 32 x 16 product are its next eight: which of k's elements a product takes is free, if both operands agree.  A
+// group's sum starts at -(16 + zero) sum x and is scaled once.  300 rows by 11,008 columns, k of 4,096: 56 us, 480 TFLOP/s
+// (267 us in the blocks above); no one part bounds it: without its loads, without the staging of x or without the products
+// with their widening it is 10 to 25 us shorter, and eight waves beside each other (256 columns) or twice the rows, with
+// as many registers, gain nothing.
+template <typename T, int SUB>
+__global__ __launch_bounds__(l4::TILE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear4_tiles_kernel(Linear4Args g) {
+  using namespace l4;
+  typedef typename mfma_traits<T>::frag frag;
+  constexpr int NW = TILE_WAVES, MB = TILE_ROWS / 32, ROWS = TILE_ROWS, ROW = STEP * 2, CHUNKS = ROWS / (NW * 4), PARTS = 4 / SUB;
+  constexpr int PIECES = SUB == 1 ? 4 : 2, DWORDS = 8 / PIECES;  // loads of a lane's weights, and their size
+  typedef Vec<uint32_t, DWORDS> Piece;
+  __shared__ __attribute__((aligned(1024))) char tiles[2][ROWS * ROW];
+  __shared__ __attribute__((aligned(16))) float sums[2][PARTS][ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // The row tiles of a column tile go to one XCD, one after the other (workgroups go round the eight).
+  const int64_t m_tiles = (g.rows + ROWS - 1) / ROWS, id = g.first + blockIdx.x;
+  const int64_t n0 = (id / 8 / m_tiles * 8 + id % 8) * (NW * 32), m0 = id / 8 % m_tiles * ROWS;
+  if (n0 >= g.n) return;
+  const int k = (int)g.k, steps = (k + STEP - 1) / STEP;
+  const int64_t n = min(n0 + wave * 32 + col, g.n - 1);  // (columns past the end repeat the last, and rows too)
+  const uint8_t* W = g.weight + n * g.ws[0] + half * DWORDS * 4;
+  // (a lane loads a scale, or for its other half the zero point, and gets the other's)
+  const bool of_zeros = half && g.zeros;
+  const uint16_t* SZ = of_zeros ? (const uint16_t*)g.zeros + n * g.zs[0] : (const uint16_t*)g.scales + n * g.ss[0];
+  const int64_t sz_stride = of_zeros ? g.zs[1] : g.ss[1];
+  const uint16_t* X[CHUNKS];
+#pragma unroll
+  for (int u = 0; u < CHUNKS; ++u)
+    X[u] = (const uint16_t*)g.x + min(m0 + u * (NW * 4) + tid / 16, g.rows - 1) * g.xs[0] + tid % 16 * 8;
+
+  struct Weights {
+    Piece w[PIECES];
+    uint16_t sz[PARTS];
+  };
+  auto load = [&](Weights& t, int step) __attribute__((always_inline)) {
+    const int k0 = step * STEP;
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      t.w[j] = Piece{};
+      if (SUB == 4 || k0 + j * (STEP / PIECES) + half * (SUB == 1 ? 0 : 32) < k) t.w[j] = *(const Piece*)(W + k0 / 2 + j * (STEP / 2 / PIECES));
+    }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      const int64_t group = (uint32_t)min(k0 + p * SUB * 32, k - 1) / (uint32_t)g.group;
+      t.sz[p] = SZ[group * sz_stride];
+    }
+  };
+  u32x4 held[CHUNKS];
+  auto load_x = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < CHUNKS; ++u) {
+      held[u] = u32x4{0u, 0u, 0u, 0u};
+      if (SUB == 4 || step * STEP + tid % 16 * 8 < k) held[u] = *(const u32x4*)(X[u] + step * STEP);
+    }
+  };
+  auto store_x = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < CHUNKS; ++u) {
+      const int row = u * (NW * 4) + tid / 16, chunk = tid % 16;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum = lane_rows::add2<T>(held[u][w], sum);
+      sum = over_lanes<SUB * 4>(sum);
+      *(u32x4*)(tiles[step & 1] + row * ROW + ((chunk ^ (row & 15)) * 16)) = paired(held[u]);
+      if (chunk % (SUB * 4) == 0) sums[step & 1][chunk / (SUB * 4)][row] = sum;
+    }
+  };
+  floatx16 acc[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  auto take = [&](const Weights& t, int step) __attribute__((always_inline)) {
+    const char* tile = tiles[step & 1] + col * ROW;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      const auto both = __builtin_amdgcn_permlane32_swap(t.sz[p], t.sz[p], false, false);
+      const float s = elem<T>::to_float((uint16_t)both[0]);
+      const float z = -16.0f - (g.zeros ? elem<T>::to_float((uint16_t)both[1]) : 8.0f);
+      floatx16 part[MB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 all = *(const float4*)&sums[step & 1][p][i * 32 + q * 8 + half * 4];
+          part[i][q * 4] = z * all.x;
+          part[i][q * 4 + 1] = z * all.y;
+          part[i][q * 4 + 2] = z * all.z;
+          part[i][q * 4 + 3] = z * all.w;
+        }
+#pragma unroll
+      for (int e = p * SUB * 2; e < (p + 1) * SUB * 2; ++e) {  // products
+        const int j = e / DWORDS, d = e % DWORDS, chunk = j * (16 / PIECES) + half * DWORDS + d;
+        const frag fw = __builtin_bit_cast(frag, wide8<T>(t.w[j].e[d]));
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const frag fx = __builtin_bit_cast(frag, *(const u32x4*)(tile + i * 32 * ROW + ((chunk ^ (col & 15)) * 16)));
+          part[i] = mfma_traits<T>::mma(fx, fw, part[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = __builtin_fmaf(s, part[i][r], acc[i][r]);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);  // (a part's fragments at a time: there are registers for no more)
+    }
+  };
+  // Weights are sent for some steps ahead, and x two; each set of registers keeps its place (a copy would wait for them).
+  constexpr int AHEAD = SUB == 1 ? 2 : 3;
+  Weights w[AHEAD];
+  if (steps > 0) {
+    load_x(0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < steps) load(w[i], i);
+    store_x(0);
+    if (steps > 1) load_x(1);
+  }
+  __syncthreads();
+  for (int step0 = 0; step0 < steps; step0 += AHEAD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int step = step0 + i;
+      if (step >= steps) break;
+      take(w[i], step);
+      if (step + 1 < steps) store_x(step + 1);
+      if (step + 2 < steps) load_x(step + 2);
+      if (step + AHEAD < steps) load(w[i], step + AHEAD);
+      __syncthreads();
+    }
+  }
+  if (n0 + wave * 32 + col >= g.n) return;
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t m = m0 + i * 32 + r / 4 * 8 + half * 4 + r % 4;
+      if (m >= g.rows) continue;
+      float y = acc[i][r];
+      if (g.c) y += elem<T>::to_float(((const uint16_t*)g.c)[m * g.cs[0] + n * g.cs[1]]);
+      ((uint16_t*)g.out)[m * g.os[0] + n * g.os[1]] = elem<T>::from_float(y);
+    }
 }
 
 // The same element by element, for any strides and alignment: a wave a column, ROWS rows at a time, its lanes along k.
@@ -244,18 +418,32 @@ __global__ __launch_bounds__(256) void linear4_elements_kernel(Linear4Args g) {
   }
 }
 
-template <typename T, int MB, int NB>
+template <typename T, int MB>
 static void linear4_blocks(Linear4Args g, hipStream_t stream) {
-  const int64_t workgroups = cdiv(g.rows, MB * 16) * cdiv(g.n, NB * 16);
+  const int64_t workgroups = cdiv(g.rows, MB * 16) * cdiv(g.n, 16);
   in_launches(workgroups, l4::WAVES * 64, [&](int64_t first, unsigned count) {
     g.first = first;
     const dim3 grid(count), block(l4::WAVES * 64);
     if (g.group % 128 == 0)
-      hipLaunchKernelGGL((linear4_kernel<T, MB, NB, 4>), grid, block, 0, stream, g);
+      hipLaunchKernelGGL((linear4_kernel<T, MB, 4>), grid, block, 0, stream, g);
     else if (g.group % 64 == 0)
-      hipLaunchKernelGGL((linear4_kernel<T, MB, NB, 2>), grid, block, 0, stream, g);
+      hipLaunchKernelGGL((linear4_kernel<T, MB, 2>), grid, block, 0, stream, g);
     else
-      hipLaunchKernelGGL((linear4_kernel<T, MB, NB, 1>), grid, block, 0, stream, g);
+      hipLaunchKernelGGL((linear4_kernel<T, MB, 1>), grid, block, 0, stream, g);
+  });
+}
+
+template <typename T>
+static void linear4_tiles(Linear4Args g, hipStream_t stream) {
+  constexpr int block = l4::TILE_WAVES * 64, cols = l4::TILE_WAVES * 32;
+  in_launches(cdiv(g.rows, l4::TILE_ROWS) * cdiv(cdiv(g.n, cols), 8) * 8, block, [&](int64_t first, unsigned count) {
+    g.first = first;
+    if (g.group % 128 == 0)
+      hipLaunchKernelGGL((linear4_tiles_kernel<T, 4>), dim3(count), dim3(block), 0, stream, g);
+    else if (g.group % 64 == 0)
+      hipLaunchKernelGGL((linear4_tiles_kernel<T, 2>), dim3(count), dim3(block), 0, stream, g);
+    else
+      hipLaunchKernelGGL((linear4_tiles_kernel<T, 1>), dim3(count), dim3(block), 0, stream, g);
   });
 }
 
@@ -271,12 +459,17 @@ static int linear4_launch(Linear4Args g, hipStream_t stream) {
     });
     return launch_status();
   }
-  if (g.rows <= 16)
-    linear4_blocks<T, 1, 1>(g, stream);
+  // Tiles of 64 rows take their weights once for all of them, but whole rows of k: they win where there is one for every
+  // third CU or so (us, tiles against blocks: 128 rows by 11008, 172 tiles: 49 | 117; 256 by 4096, 128 tiles: 49 | 79;
+  // 100 by 4096, 64 tiles: 48 | 40; 300 by 1024 with k of 11008, 40 tiles: 115 | 87).
+  if (g.rows > 64 && cdiv(g.rows, l4::TILE_ROWS) * cdiv(g.n, l4::TILE_WAVES * 32) >= 96)
+    linear4_tiles<T>(g, stream);
+  else if (g.rows <= 16)
+    linear4_blocks<T, 1>(g, stream);
   else if (g.rows <= 32)
-    linear4_blocks<T, 2, 1>(g, stream);
+    linear4_blocks<T, 2>(g, stream);
   else
-    linear4_blocks<T, 4, 1>(g, stream);
+    linear4_blocks<T, 4>(g, stream);
   return launch_status();
 }
 

@@ -133,7 +133,7 @@ def test_norm_odd_values(dim, eight):
 
 
 # -------------------------------------------------------------------------------------------- linear
-def check_linear(x, weight, scales, out, zeros, c):
+def check_linear(x, weight, scales, out, zeros, c, roundings=None):
     n, k = weight.shape[0], x.shape[1]
     group = k // scales.shape[1]
     q = torch.stack((weight & 15, weight >> 4), -1).reshape(n, -1, group).double()
@@ -143,7 +143,7 @@ def check_linear(x, weight, scales, out, zeros, c):
     size = x.double().abs() @ ((32 + q + abs(z)) * s.abs()).reshape(n, k).t()
     if c is not None:
         want, size = want + c.double(), size + c.double().abs()
-    tol = 2.0**-23 * (group + scales.shape[1] / 8 + 16) * size + want.abs() * half_step(x.dtype)
+    tol = 2.0**-23 * (roundings or group + scales.shape[1] / 8 + 16) * size + want.abs() * half_step(x.dtype)
     close(out, want, tol + (2.0**-25 if x.dtype == F16 else 0), f"{x.shape[0]} rows of {k}, {n} columns")
 
 
@@ -215,6 +215,46 @@ def test_linear_odd_values(rows):
     assert (out == 0).all()
     kernels.linear_4bit(x[:, :0], weight[:, :0], scales[:, :0], out, c=want.nan_to_num())
     assert torch.equal(out, want.nan_to_num())
+
+
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("dtype", (F16, BF16))
+@pytest.mark.parametrize("rows,k,n,group", (
+    (65, 32, 6100, 32), (130, 160, 4100, 32), (129, 4064, 4000, 32), (70, 96, 6145, 96), (200, 192, 3000, 64),
+    (200, 1152, 3050, 64), (257, 2048, 2500, 128), (90, 640, 6200, 128), (300, 768, 2500, 256), (128, 128, 6144, 128)))
+def test_linear_of_many_rows(rows, k, n, group, dtype, zeros):
+    """Tiles of 64 rows.  Sums in fp32: of 128 products at most and of as many x (their order is the matrix core's: twice
+    the roundings), two products with scale and zero point, and then a sum for every 32, 64 or 128 elements of k."""
+    x, (weight, scales, z) = randn(rows, k, dtype=dtype), weights(n, k, group, dtype, zeros)
+    piece = 128 if group % 128 == 0 else 64 if group % 64 == 0 else 32
+    for c in (None, randn(n, rows, dtype=dtype, seed=5).t()):
+        out = torch.full((rows, n), math.nan, dtype=dtype, device=DEV)
+        kernels.linear_4bit(x, weight, scales, out, zeros=z, c=c)
+        check_linear(x, weight, scales, out, z, c, roundings=2 * piece + 2 + k / piece)
+    again = c.clone()  # onto c itself, the same bits
+    assert torch.equal(kernels.linear_4bit(x, weight, scales, again, zeros=z, c=again), out)
+    # columns of a wider output, groups along the other side, rows of a wider x
+    wide = torch.full((rows, 2 * n), 3.0, dtype=dtype, device=DEV)
+    xs = torch.cat([x, x], 1)[:, k:]
+    kernels.linear_4bit(xs, weight, scales.t().contiguous().t(), wide[:, ::2], c=c,
+                        zeros=None if z is None else z.t().contiguous().t())
+    assert torch.equal(wide[:, ::2], out) and (wide[:, 1::2] == 3).all()
+
+
+def test_linear_odd_values_of_many_rows():
+    rows, k, n = 130, 256, 4200
+    weight, scales, z = weights(n, k, 64, BF16, True)
+    x = randn(rows, k, dtype=BF16)
+    x[70, 7] = math.nan
+    scales[3, 2] = math.inf
+    out = torch.empty(rows, n, dtype=BF16, device=DEV)
+    kernels.linear_4bit(x, weight, scales, out, zeros=z)
+    assert out[70].isnan().all() and not out[:, 3].isfinite().any()
+    rest, keep = [i for i in range(rows) if i != 70], [i for i in range(n) if i != 3]
+    check_linear(x[rest], weight[keep], scales[keep], out[rest][:, keep], z[keep], None, roundings=2 * 64 + 2 + 4)
+    none = torch.full((rows, n), 7.0, dtype=BF16, device=DEV)  # k of zero
+    kernels.linear_4bit(x[:, :0], weight[:, :0], scales[:, :0], none)
+    assert (none == 0).all()
 
 
 def test_linear_of_quantized_weights():
