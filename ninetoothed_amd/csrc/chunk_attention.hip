@@ -706,7 +706,7 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       const u32x4 rs = keys_of(k_at, k_bytes, t - window);
 #pragma unroll
       for (int u = 0; u < LOADS; ++u)
-        buffer_to_lds(rs, lds_at + RAW + (t & 3) * SENT + (wave * LOADS + u) * 1024, k_off[u], 0);
+        new_buffer_to_lds(rs, lds_at + RAW + (t & 3) * SENT + (wave * LOADS + u) * 1024, k_off[u]);
     };
     // (and what tile t's keys share, from the wave that has the first of each sixteen)
     auto send_v = [&](int t) __attribute__((always_inline)) {
@@ -714,7 +714,7 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
       if ((wave & 1) == 0 && lane == t - window) factors[t & 3][wave >> 1] = shared;
 #pragma unroll
       for (int u = 0; u < LOADS; ++u)
-        buffer_to_lds(rs, lds_at + RAW + (4 + (t & 3)) * SENT + (wave * LOADS + u) * 1024, v_off[u], 0);
+        new_buffer_to_lds(rs, lds_at + RAW + (4 + (t & 3)) * SENT + (wave * LOADS + u) * 1024, v_off[u]);
     };
     auto send = [&](int t) __attribute__((always_inline)) {
       send_v(t + 2);

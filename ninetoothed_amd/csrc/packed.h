@@ -107,6 +107,14 @@ __device__ __forceinline__ void buffer_to_lds(u32x4 rs, uint32_t lds_addr, int o
                  "s"(__builtin_amdgcn_readfirstlane(soffset))
                : "memory", "m0");
 }
+// The same for a buffer that a vector instruction may have made just before (v_readlane, also where the compiler takes
+// spilled scalars back): a load reads such scalars five wait states later at the soonest.
+__device__ __forceinline__ void new_buffer_to_lds(u32x4 rs, uint32_t lds_addr, int offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(offset), "s"(rs)
+               : "memory", "m0");
+}
 __device__ __forceinline__ void global_to_lds(const void* p, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
