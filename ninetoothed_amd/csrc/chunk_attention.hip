@@ -58,6 +58,7 @@ struct ChunkArgs {
   bool q_vectors, o_vectors;
   float scale_log2;        // softmax scale * log2(e)
   float *part_o, *part_ml;  // partial states, two a workgroup: [slot][row][DM], [slot][row][2]
+  int4* joins;              // of a workgroup: states to join (or 0), rows, the sequence's first row of q, block
 };
 
 // The work of a head of k and v is a line of blocks of 256 rows, sequence by sequence, in which a block is as long as
@@ -564,13 +565,13 @@ __device__ __forceinline__ void chunk_products(const ChunkTile<DM>& at, const ch
 
 // The stretch of a workgroup, piece by piece: f(sequence, its number, block) for each.
 struct ChunkStretch {
-  int64_t begin, stop, seq_at;
+  int64_t begin, stop, seq_at, share;
   int b, nth;
   ChunkSequence s;
   bool there;
   template <int THREADS>
   __device__ __forceinline__ ChunkStretch(const ChunkArgs& g, ChunkLds<THREADS>& lds, int part) {
-    int64_t share = 0;
+    share = 0;
     const ChunkPlace place = chunk_place(g, lds, [&](int64_t length) {
       share = chunk_share(g, length);
       return min(part * share, length - 1);  // (a workgroup past the end has nothing to do)
@@ -584,6 +585,20 @@ struct ChunkStretch {
     seq_at = place.before;
     s = chunk_sequence(g, b);
     nth = chunk_block(s, begin - seq_at);
+  }
+  // For chunk_join_kernel: the block inside of which the stretch begins, if no stretch before it begins there.  The states
+  // are that of the stretch before, the second of its two, and the first of each stretch up to the one in which the
+  // block ends.
+  __device__ __forceinline__ void note_join(const ChunkArgs& g) const {
+    if (g.parts == 1) return;
+    int4 join = {0, 0, 0, 0};
+    if (there) {
+      const int64_t block_at = seq_at + chunk_line(s, nth), block_end = seq_at + chunk_line(s, nth + 1);
+      if (block_at < begin && block_at >= begin - share)
+        join = {1 + (int)((uint64_t)(block_end - begin + share - 1) / (uint64_t)share), min(ch::BM, s.rows - nth * ch::BM),
+                s.begin, nth};
+    }
+    if (threadIdx.x == 0) g.joins[blockIdx.x] = join;
   }
   // To the block behind one that ends at `end`; false if that is past the stretch.
   __device__ __forceinline__ bool next(const ChunkArgs& g, int64_t end) {
@@ -643,6 +658,7 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   int marked = 0;  // tiles of the pieces before this one
   if (EIGHT && tid < RING) odd_tile[tid] = 0;
   ChunkStretch at(g, place_lds, blockIdx.x / g.kv_heads);
+  at.note_join(g);
   if (!at.there) return;
   const Tile tile;
   const float c = fmaxf(fabsf(g.scale_log2), LEAST_FACTOR);  // (of a scale of 0 times minus infinity would be NaN)
@@ -885,6 +901,7 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = g.dim, head = blockIdx.x % g.kv_heads;
   ChunkStretch at(g, place_lds, blockIdx.x / g.kv_heads);
+  at.note_join(g);
   if (!at.there) return;
   const Tile tile;
   const float c = fmaxf(fabsf(g.scale_log2), LEAST_FACTOR);  // (of a scale of 0 times minus infinity would be NaN)
@@ -1042,30 +1059,17 @@ __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 
   }
 }
 
-// Joins the partial states of blocks whose keys were split.  A workgroup takes JOIN_ROWS rows of the block inside of
-// which stretch `part` begins, if it is the first stretch that begins there: the states are that of the stretch
-// before, the second of its two, and the first of each stretch up to the one in which the block ends.
+// Joins the partial states of blocks whose keys were split.  A workgroup takes JOIN_ROWS rows of the block that stretch
+// `part` has noted.  (Finding it here again took 8 us of the launch's 13.)
 template <typename T, int DM>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs g) {
   using namespace ch;
   constexpr int LANES = DM / 4, GROUPS = 256 / LANES;
-  __shared__ ChunkLds<256> lds;
   const int tid = threadIdx.x;
   const int head = blockIdx.x % g.kv_heads, rest = blockIdx.x / g.kv_heads;
   const int part = rest / (BM / JOIN_ROWS) + 1, chunk = rest % (BM / JOIN_ROWS);
-  int64_t share = 0;
-  const ChunkPlace place = chunk_place(g, lds, [&](int64_t length) {
-    share = chunk_share(g, length);
-    return min(part * share, length - 1);
-  });
-  const int64_t begin = part * share;
-  if (begin >= place.length) return;
-  const ChunkSequence s = chunk_sequence(g, place.sequence);
-  const int nth = chunk_block(s, begin - place.before);
-  const int64_t block_at = place.before + chunk_line(s, nth), block_end = place.before + chunk_line(s, nth + 1);
-  if (block_at == begin || block_at < begin - share) return;
-  const int states = 1 + (int)((block_end - begin + share - 1) / share);
-  const int rows = min(BM, s.rows - nth * BM);
+  const int4 join = g.joins[part * g.kv_heads + head];
+  const int states = join.x, rows = join.y, begin = join.z, nth = join.w;
   const int d = tid % LANES * 4;
   for (int r = chunk * JOIN_ROWS + tid / LANES; r < (chunk + 1) * JOIN_ROWS && r < rows; r += GROUPS) {
     auto slot = [&](int i) {  // of the i-th state
@@ -1089,7 +1093,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs g) {
     if (d >= g.dim) continue;
     const float inv = sum != 0.f ? 1.0f / sum : 0.f;
     const int row = nth * BM + r, tok = row / g.group;
-    uint16_t* O = (uint16_t*)g.o + (int64_t)(s.begin + tok) * g.os[0] + (head * g.group + (row - tok * g.group)) * g.os[1];
+    uint16_t* O = (uint16_t*)g.o + (int64_t)(begin + tok) * g.os[0] + (head * g.group + (row - tok * g.group)) * g.os[1];
     const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     if (g.o_vectors) {
       *(u32x2*)(O + d) = u32x2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
@@ -1110,7 +1114,7 @@ static int64_t chunk_parts(int64_t tokens, int64_t sequences, int64_t kv_heads, 
   return std::max<int64_t>(1, std::min<int64_t>(256 * a_cu / kv_heads, most));
 }
 static int64_t chunk_state_bytes(int64_t parts, int64_t kv_heads, int64_t dim) {
-  return parts == 1 ? 0 : parts * kv_heads * 2 * ch::BM * ((dim <= 64 ? 64 : 128) + 2) * 4;
+  return parts == 1 ? 0 : parts * kv_heads * (2 * ch::BM * ((dim <= 64 ? 64 : 128) + 2) * 4 + (int64_t)sizeof(int4));
 }
 
 template <typename T, bool EIGHT, int DM>
@@ -1202,6 +1206,7 @@ extern "C" int nt_chunk_attention(const void* q, const int64_t* q_strides, const
   g.parts = (int)parts;
   g.part_o = (float*)workspace;
   g.part_ml = need ? g.part_o + parts * kv_heads * 2 * nt::ch::BM * (dim <= 64 ? 64 : 128) : nullptr;
+  g.joins = need ? (int4*)(g.part_ml + parts * kv_heads * 2 * nt::ch::BM * 2) : nullptr;
 #define NT_CHUNK(T, E)                          \
   if (dim <= 64)                                \
     nt::chunk_launch<T, E, 64>(g, stream);      \
