@@ -633,10 +633,16 @@ struct ChunkStretch {
 //   - What lies past a sequence's end or in no page is stored as zeros.  A causally masked key meets p = 0, which an
 //     infinite or NaN v would still turn into NaN: rows of a tile that is masked and holds one are taken key by key, each
 //     over the keys that it sees (8 bits: such values are stored as zeros, and the tile is marked).
-// This kernel: pages of whole multiples of 16 keys, so that the 8 keys of a tile that a wave stages lie in one page, which it
-// looks up by a scalar load.  A step takes tile t - 1's values and tile t's scores and weights.  K(t + 3) and V(t + 2) are sent
-// for in it, by loads into LDS: four stages; with 8 bits they are raw, and each wave widens its own keys' into two more
-// as they come.
+// This kernel: pages of whole multiples of 16 keys, so that the 8 keys of a tile that a wave stages lie in one page.  A step
+// takes the products of tile t - 1's values and tile t's keys, and then tile t's weights.  Waves 4 to 7 are half a step behind,
+// so that of a SIMD's two waves one is at its products while the other is at its exponentials (all eight in step: prompts
+// 648 us, so 601 to 630).  K(t + 3) and V(t + 2) are sent for in step t, by loads into LDS: four stages; with 8 bits they are
+// raw, and each wave widens its own keys' into two more as they come.  Waves 4 to 7 send and widen a step ahead, as the
+// others' products come half a step before theirs.
+// Measured: three prompts' pieces of 2,000 tokens over 3,500 to 7,000 keys (32 heads on 8 of 128, bf16) 630 us, 918 TFLOP/s,
+// at 1.8 GHz (a library product of 8192^3: 1,133); 512 tokens over 60,001 keys of 8 bits 458 us, 966 TFLOP/s; five tokens
+// of each of 32 sequences of 500 to 6,000 keys of 8 bits 109 us, 2.1 TB/s: there one wave has rows, and a tile takes it some
+// 3,500 cycles of products, widening and weights, one after the other.
 template <typename T, bool EIGHT, int DM>
 __global__ __launch_bounds__(ch::NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_pages_kernel(ChunkArgs g) {
   using namespace ch;

@@ -101,10 +101,11 @@ __device__ __forceinline__ float over_lanes(float v) {
 // lower four bits first).  Sums in fp32, rounded once:
 //   out[m][n] = c[m][n] + sum_g scale[n][g] (sum_k x[m][k] (16 + q[n][k]) - (16 + zero[n][g]) sum_k x[m][k]),
 // where 16 + q is made from the bits, exact in either type, and the sums of x are a product with ones.
-// Bound by HBM for few rows: the weights are read once, 16 bytes a lane, by waves that share 16 NB columns and take
-// turns of 128 elements of k; x comes from the L2 for each of those workgroups, the most of what is loaded beyond a
-// few rows (24 rows, k of 11,008, 4,096 columns: 24 us, of which the weights are 5; one row, k of 4,096: 5 us, a launch).  A wave's 16 x 16 x 32 products take
-// 32 neighbouring elements of k, which lie in one group, so a turn's four dwords go across the quads first.
+// Bound by HBM for one row or a few: the weights are read once, 16 bytes a lane, by waves that share 16 columns and take
+// turns of 128 elements of k; x comes from the L2 for each of those workgroups, and is most of what is loaded beyond some
+// rows (24 rows, k of 11,008, 4,096 columns: 24 us, of which the weights are 5; 32 columns a workgroup, which halves that,
+// leave half of the CUs without one: 33; one row, k of 4,096, 4,096 columns: 5 us, a launch).  A wave's 16 x 16 x 32 products
+// take 32 neighbouring elements of k, which lie in one group, so a turn's four dwords go across the quads first.
 // MB: blocks of 16 rows; SUB: products of a turn that share a group.
 template <typename T, int MB, int SUB>
 __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) {
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
 // each weight is widened once for all of the rows, from the registers that it was loaded into.  x passes through two
 // LDS stages of 128 elements of k, in the weights' order of pairs, and is summed on its way.  A lane's weights of a
 // 32 x 32 x 16 product are its next eight: which of k's elements a product takes is free, if both operands agree.  A
-// group's sum starts at -(16 + zero) sum x and is scaled once.  300 rows by 11,008 columns, k of 4,096: 56 us, 480 TFLOP/s
+// group's sum starts at -(16 + zero) sum x and is scaled once.  300 rows by 11,008 columns, k of 4,096: 53 us, 510 TFLOP/s
 // (267 us in the blocks above); no one part bounds it: without its loads, without the staging of x or without the products
 // with their widening it is 10 to 25 us shorter, and eight waves beside each other (256 columns) or twice the rows, with
 // as many registers, gain nothing.
