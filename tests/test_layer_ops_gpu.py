@@ -437,6 +437,21 @@ def test_chunk_split_keys(new, cached, cache):
         run_chunk(new, [a + b for a, b in zip(new, cached)], heads, kv_heads, dim, 64, F16, cache, width=700)
 
 
+@pytest.mark.parametrize("page", (16, 64))
+@pytest.mark.parametrize("cache", (F16, E4M3))
+def test_chunk_of_many_tiles_a_workgroup(cache, page):
+    """64 heads share the CUs, so that a stretch is some hundred tiles long; pages are missing here and there, among them
+    those around each 64th tile."""
+    def edit(q, kc, vc, tables):
+        kc[0], vc[0] = math.nan, math.nan
+        tables[tables == 0] = -1
+        tables[:, ::63 * 64 // page] = -3
+        tables[:, 64 * 64 // page] = 1 << 30
+        tables[0, 100:100 + 64 // page] = -1
+
+    run_chunk([3, 0, 40], [20000, 50, 17001], 64, 64, 64, page, F16, cache, edit=edit)
+
+
 @pytest.mark.parametrize("cache", (BF16, E4M3))
 def test_chunk_many_sequences(cache):
     g = torch.Generator().manual_seed(7)
