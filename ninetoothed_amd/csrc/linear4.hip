@@ -113,7 +113,11 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
   typedef mma16<T> M;
   typedef typename M::frag frag;
   constexpr int NB = 1, ROWS = MB * 16, COLS = NB * 16;
-  __shared__ float sums[WAVES][ROWS][COLS + 1];
+  constexpr int STAGES = MB == 4 ? 1 : 2, STAGE = ROWS * STEP * 2, LOADS = STAGE / 1024;  // of x, each wave's own
+  typedef float Sums[WAVES][ROWS][COLS + 1];
+  __shared__ __attribute__((aligned(1024))) char lds[WAVES * STAGES * STAGE];
+  static_assert(sizeof(Sums) <= sizeof(lds), "the sums lie where x did");
+  Sums& sums = *(Sums*)lds;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t m_tiles = (g.rows + ROWS - 1) / ROWS, id = g.first + blockIdx.x;
@@ -121,7 +125,7 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
   const int k = (int)g.k, steps = (k + STEP - 1) / STEP;
 
   const uint8_t* W[NB];
-  const uint16_t *S[NB], *Z[NB], *X[MB];
+  const uint16_t *S[NB], *Z[NB], *X[LOADS];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int64_t n = min(n0 + j * 16 + col, g.n - 1);  // (columns past the end repeat the last)
@@ -129,27 +133,33 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
     S[j] = (const uint16_t*)g.scales + n * g.ss[0];
     Z[j] = (const uint16_t*)g.zeros + n * g.zs[0];
   }
+  // A load takes 8 rows' 64 neighbouring elements into LDS, a row's 16-byte chunks XORed by row for the fragments' reads.
 #pragma unroll
-  for (int i = 0; i < MB; ++i) X[i] = (const uint16_t*)g.x + min(m0 + i * 16 + col, g.rows - 1) * g.xs[0] + quad * 8;
+  for (int u = 0; u < LOADS; ++u) {
+    const int row = u / 2 * 8 + lane / 8;
+    X[u] = (const uint16_t*)g.x + min(m0 + row, g.rows - 1) * g.xs[0];
+  }
+  char* stages = lds + wave * (STAGES * STAGE);
+  const uint32_t stages_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)stages;
 
   struct Turn {
-    u32x4 w[NB], x[MB][4];
+    u32x4 w[NB];
     uint16_t s[NB][4 / SUB], z[NB][4 / SUB];
   };
-  auto load = [&](Turn& t, int step) __attribute__((always_inline)) {
+  auto load = [&](Turn& t, int step, int stage) __attribute__((always_inline)) {
     const int k0 = step * STEP;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the stage has been read)
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {  // (past k: what is there, which no product takes)
+      const int swz = (u / 2 * 8 + lane / 8) >> 1 & 7;
+      const int at = k0 + (u & 1) * 64 + ((lane & 7) ^ swz) * 8;
+      global_to_lds(X[u] + (SUB == 4 ? at : min(at, k - 8)), stages_at + stage * STAGE + u * 1024);
+    }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       t.w[j] = u32x4{0u, 0u, 0u, 0u};
       if (SUB == 4 || k0 + quad * 32 < k) t.w[j] = *(const u32x4*)(W[j] + k0 / 2);
     }
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        t.x[i][p] = u32x4{0u, 0u, 0u, 0u};
-        if (SUB == 4 || k0 + p * 32 < k) t.x[i][p] = *(const u32x4*)(X[i] + k0 + p * 32);
-      }
 #pragma unroll
     for (int p = 0; p < 4; p += SUB) {
       const int64_t group = min(k0 + p * 32, k - 1) / g.group;
@@ -166,12 +176,17 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   const frag ones = __builtin_bit_cast(frag, u32x4{M::ONES, M::ONES, M::ONES, M::ONES});
-  auto take = [&](const Turn& t) __attribute__((always_inline)) {
+  // x of the turn has come when its weights have, which were sent for behind it (loads end in order).
+  auto take = [&](Turn& t, int step, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) asm volatile("" : "+v"(t.w[j])::"memory");
+    const char* x = stages + stage * STAGE;
     u32x4 w[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) w[j] = across_quads(t.w[j]);
 #pragma unroll
     for (int p0 = 0; p0 < 4; p0 += SUB) {
+      if (SUB != 4 && step * STEP + p0 * 32 >= k) break;
       floatx4 part[MB][NB], all[MB];
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
@@ -186,7 +201,9 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
         for (int j = 0; j < NB; ++j) fw[j] = __builtin_bit_cast(frag, wide8<T>(w[j][p]));
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-          const frag fx = __builtin_bit_cast(frag, paired(t.x[i][p]));
+          const int row = i * 16 + col, chunk = (p & 1) * 4 + quad;
+          const u32x4 raw = *(const u32x4*)(x + (row / 8 * 2 + p / 2) * 1024 + (row & 7) * 128 + ((chunk ^ (row >> 1 & 7)) * 16));
+          const frag fx = __builtin_bit_cast(frag, paired(raw));
           all[i] = M::mma(fx, ones, all[i]);
 #pragma unroll
           for (int j = 0; j < NB; ++j) part[i][j] = M::mma(fx, fw[j], part[i][j]);
@@ -205,20 +222,20 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
     }
   };
   // (each turn's registers keep their place: a copy would wait for what they were sent for)
-  constexpr int AHEAD = MB == 4 ? 2 : MB == 2 ? 3 : 4;
-  Turn turns[AHEAD];
+  Turn turns[STAGES];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (wave + i * WAVES < steps) load(turns[i], wave + i * WAVES);
-  for (int step0 = wave; step0 < steps; step0 += AHEAD * WAVES) {
+  for (int i = 0; i < STAGES; ++i)
+    if (wave + i * WAVES < steps) load(turns[i], wave + i * WAVES, i);
+  for (int step0 = wave; step0 < steps; step0 += STAGES * WAVES) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       const int step = step0 + i * WAVES;
       if (step >= steps) break;
-      take(turns[i]);
-      if (step + AHEAD * WAVES < steps) load(turns[i], step + AHEAD * WAVES);
+      take(turns[i], step, i);
+      if (step + STAGES * WAVES < steps) load(turns[i], step + STAGES * WAVES, i);
     }
   }
+  __syncthreads();
   // (row quad * 4 + r, column col of a block)
 #pragma unroll
   for (int i = 0; i < MB; ++i)
