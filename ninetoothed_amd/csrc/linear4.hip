@@ -102,10 +102,11 @@ __device__ __forceinline__ float over_lanes(float v) {
 //   out[m][n] = c[m][n] + sum_g scale[n][g] (sum_k x[m][k] (16 + q[n][k]) - (16 + zero[n][g]) sum_k x[m][k]),
 // where 16 + q is made from the bits, exact in either type, and the sums of x are a product with ones.
 // Bound by HBM for one row or a few: the weights are read once, 16 bytes a lane, by waves that share 16 columns and take
-// turns of 128 elements of k; x comes from the L2 for each of those workgroups, and is most of what is loaded beyond some
-// rows (24 rows, k of 11,008, 4,096 columns: 24 us, of which the weights are 5; 32 columns a workgroup, which halves that,
-// leave half of the CUs without one: 33; one row, k of 4,096, 4,096 columns: 5 us, a launch).  A wave's 16 x 16 x 32 products
-// take 32 neighbouring elements of k, which lie in one group, so a turn's four dwords go across the quads first.
+// turns of 128 elements of k.  x comes from the L2 for each of those workgroups, by loads into LDS with a row's elements
+// in neighbouring lanes: as fragments, with a row to each lane, it took longer than all the rest (24 rows, k of 11,008,
+// 4,096 columns: 24 us, now 18, of which the weights are 5; 64 rows by 11,008 columns, k of 4,096: 59, now 28).  One row,
+// k of 4,096, 4,096 columns: 5 us, a launch.  A wave's 16 x 16 x 32 products take 32 neighbouring elements of k, which
+// lie in one group, so a turn's four dwords go across the quads first.
 // MB: blocks of 16 rows; SUB: products of a turn that share a group.
 template <typename T, int MB, int SUB>
 __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) {
@@ -125,13 +126,16 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
   const int k = (int)g.k, steps = (k + STEP - 1) / STEP;
 
   const uint8_t* W[NB];
-  const uint16_t *S[NB], *Z[NB], *X[LOADS];
+  const uint16_t *SZ[NB], *X[LOADS];
+  // (of a turn's first and second group, or third and fourth, quads 0 and 2 load the scale and quads 1 and 3 the zero point)
+  constexpr int PARTS = 4 / SUB, PAIRS = PARTS == 4 ? 2 : 1;
+  const bool of_zeros = (quad & 1) && g.zeros;
+  const int64_t sz_stride = of_zeros ? g.zs[1] : g.ss[1];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int64_t n = min(n0 + j * 16 + col, g.n - 1);  // (columns past the end repeat the last)
     W[j] = g.weight + n * g.ws[0] + quad * 16;
-    S[j] = (const uint16_t*)g.scales + n * g.ss[0];
-    Z[j] = (const uint16_t*)g.zeros + n * g.zs[0];
+    SZ[j] = of_zeros ? (const uint16_t*)g.zeros + n * g.zs[0] : (const uint16_t*)g.scales + n * g.ss[0];
   }
   // A load takes 8 rows' 64 neighbouring elements into LDS, a row's 16-byte chunks XORed by row for the fragments' reads.
 #pragma unroll
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
 
   struct Turn {
     u32x4 w[NB];
-    uint16_t s[NB][4 / SUB], z[NB][4 / SUB];
+    uint16_t sz[NB][PAIRS];
   };
   auto load = [&](Turn& t, int step, int stage) __attribute__((always_inline)) {
     const int k0 = step * STEP;
@@ -161,13 +165,11 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
       if (SUB == 4 || k0 + quad * 32 < k) t.w[j] = *(const u32x4*)(W[j] + k0 / 2);
     }
 #pragma unroll
-    for (int p = 0; p < 4; p += SUB) {
-      const int64_t group = min(k0 + p * 32, k - 1) / g.group;
+    for (int q = 0; q < PAIRS; ++q) {
+      const int k1 = k0 + q * 64, k2 = PARTS == 1 ? k1 : k1 + SUB * 32;
+      const int first = min(k1, k - 1) / g.group, second = min(k2, k - 1) / g.group;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        t.s[j][p / SUB] = S[j][group * g.ss[1]];
-        t.z[j][p / SUB] = g.zeros ? Z[j][group * g.zs[1]] : (uint16_t)0;
-      }
+      for (int j = 0; j < NB; ++j) t.sz[j][q] = SZ[j][(int64_t)(quad < 2 ? first : second) * sz_stride];
     }
   };
   floatx4 acc[MB][NB];
@@ -211,8 +213,16 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
       }
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        const float s = elem<T>::to_float(t.s[j][p0 / SUB]);
-        const float z = 16.0f + (g.zeros ? elem<T>::to_float(t.z[j][p0 / SUB]) : 8.0f);
+        constexpr bool PAIR = PARTS > 1;
+        const int part_at = p0 / SUB, q = part_at / 2;
+        const auto both = __builtin_amdgcn_permlane16_swap(t.sz[j][q], t.sz[j][q], false, false);
+        uint32_t s_bits = both[0], z_bits = both[1];
+        if (PAIR) {
+          s_bits = __builtin_amdgcn_permlane32_swap(s_bits, s_bits, false, false)[part_at & 1];
+          z_bits = __builtin_amdgcn_permlane32_swap(z_bits, z_bits, false, false)[part_at & 1];
+        }
+        const float s = elem<T>::to_float((uint16_t)s_bits);
+        const float z = 16.0f + (g.zeros ? elem<T>::to_float((uint16_t)z_bits) : 8.0f);
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -260,7 +270,7 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
 // LDS stages of 128 elements of k, in the weights' order of pairs, and is summed on its way.  A lane's weights of a
 // 32 x 32 x 16 product are its next eight: which of k's elements a product takes is free, if both operands agree.  A
 // group's sum starts at -(16 + zero) sum x and is scaled once.  300 rows by 11,008 columns, k of 4,096: 53 us, 510 TFLOP/s
-// (267 us in the blocks above); no one part bounds it: without its loads, without the staging of x or without the products
+// (115 us in the blocks above); no one part bounds it: without its loads, without the staging of x or without the products
 // with their widening it is 10 to 25 us shorter, and eight waves beside each other (256 columns) or twice the rows, with
 // as many registers, gain nothing.
 template <typename T, int SUB>
@@ -477,10 +487,10 @@ static int linear4_launch(Linear4Args g, hipStream_t stream) {
     });
     return launch_status();
   }
-  // Tiles of 64 rows take their weights once for all of them, but whole rows of k: they win where there is one for every
-  // third CU or so (us, tiles against blocks: 128 rows by 11008, 172 tiles: 49 | 117; 256 by 4096, 128 tiles: 49 | 79;
-  // 100 by 4096, 64 tiles: 48 | 40; 300 by 1024 with k of 11008, 40 tiles: 115 | 87).
-  if (g.rows > 64 && cdiv(g.rows, l4::TILE_ROWS) * cdiv(g.n, l4::TILE_WAVES * 32) >= 96)
+  // Tiles of 64 rows take their weights once for all of them, but whole rows of k: they win where there is one for more
+  // than every second CU (us, tiles against blocks: 300 rows by 11,008, 430 tiles: 56 | 115; 128 by 11,008, 172 tiles: 41 | 50;
+  // 256 by 4,096, 128 tiles: 41 | 35; 192 by 4,096, 96 tiles: 51 | 32).
+  if (g.rows > 64 && cdiv(g.rows, l4::TILE_ROWS) * cdiv(g.n, l4::TILE_WAVES * 32) >= 150)
     linear4_tiles<T>(g, stream);
   else if (g.rows <= 16)
     linear4_blocks<T, 1>(g, stream);

@@ -220,8 +220,8 @@ def test_linear_odd_values(rows):
 @pytest.mark.parametrize("zeros", (False, True))
 @pytest.mark.parametrize("dtype", (F16, BF16))
 @pytest.mark.parametrize("rows,k,n,group", (
-    (65, 32, 6100, 32), (130, 160, 4100, 32), (129, 4064, 4000, 32), (70, 96, 6145, 96), (200, 192, 3000, 64),
-    (200, 1152, 3050, 64), (257, 2048, 2500, 128), (90, 640, 6200, 128), (300, 768, 2500, 256), (128, 128, 6144, 128)))
+    (65, 32, 9601, 32), (130, 160, 6401, 32), (129, 4064, 6300, 32), (70, 96, 9545, 96), (200, 192, 4800, 64),
+    (200, 1152, 4750, 64), (257, 2048, 3800, 128), (90, 640, 9600, 128), (300, 768, 3800, 256), (128, 128, 9600, 128)))
 def test_linear_of_many_rows(rows, k, n, group, dtype, zeros):
     """Tiles of 64 rows.  Sums in fp32: of 128 products at most and of as many x (their order is the matrix core's: twice
     the roundings), two products with scale and zero point, and then a sum for every 32, 64 or 128 elements of k."""
@@ -242,7 +242,7 @@ def test_linear_of_many_rows(rows, k, n, group, dtype, zeros):
 
 
 def test_linear_odd_values_of_many_rows():
-    rows, k, n = 130, 256, 4200
+    rows, k, n = 130, 256, 6400
     weight, scales, z = weights(n, k, 64, BF16, True)
     x = randn(rows, k, dtype=BF16)
     x[70, 7] = math.nan
