@@ -1144,7 +1144,7 @@ extern "C" int64_t nt_chunk_attention_workspace_size(int64_t tokens, int64_t seq
                                                      int cache_dtype) {
   (void)cache_dtype;
   if (tokens <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim > 128 ||
-      page_size <= 0 || table_width <= 0 || sequences > (1 << 24) || heads > (1 << 20) || page_size > 0x7fffff00LL ||
+      page_size <= 0 || table_width < 0 || sequences > (1 << 24) || heads > (1 << 20) || page_size > 0x7fffff00LL ||
       table_width > 0x7fffff00LL || tokens > 0x7fffff00LL)
     return 0;
   return nt::chunk_state_bytes(nt::chunk_parts(tokens, sequences, kv_heads, heads / kv_heads, dim, page_size, table_width),
