@@ -486,9 +486,10 @@ int nt_cache_attention(const void* q, const int64_t* q_strides, const void* k_ca
  * Otherwise as nt_cache_attention: layouts, types, scales and pages that the cache does not have.  A query that
  * sees no key gives zeros; rows behind the last sequence are left alone.  dim a multiple of 16 up to 128; caches 16-byte
  * aligned, with strides of multiples of 16 bytes.  Weights are rounded to the cache's type (8 bits: F16); their sum is
- * of the rounded ones in 16 bits, of the others in 8, where a v scale below 2^-64 counts as 0.  Less than 2^31 - 255 tokens times heads / kv_heads.  The workspace (16-byte aligned,
- * nt_chunk_attention_workspace_size bytes, 0: none needed) holds partial states of rows whose keys are split over
- * workgroups; nothing between calls, but calls that may run at once need one each.  o must not overlap the inputs. */
+ * of the rounded ones in 16 bits, of the others in 8, where the values of a v scale below 2^-64 are zeros.  Less than
+ * 2^31 - 255 tokens times heads / kv_heads.  The workspace (16-byte aligned, nt_chunk_attention_workspace_size bytes, 0:
+ * none needed) holds partial states of rows whose keys are split over workgroups; nothing between calls, but calls that
+ * may run at once need one each.  o must not overlap the inputs. */
 int64_t nt_chunk_attention_workspace_size(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads,
                                           int64_t dim, int64_t page_size, int64_t table_width, int cache_dtype);
 int nt_chunk_attention(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,

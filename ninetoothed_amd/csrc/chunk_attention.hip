@@ -243,6 +243,7 @@ __device__ __forceinline__ void chunk_rows_by_key(const ChunkArgs& g, const int3
       s *= g.k_scale[page * g.kv_heads + head];
       v_scale = g.v_scale[page * g.kv_heads + head];
     }
+    const bool counts = v_scale >= ch::LEAST_SCALE;  // (else its values are zeros, whatever they are)
     const bool seen = key <= last;
     const float m_new = seen ? fmaxf(m, s) : m, shift = m_new == -INFINITY ? 0.f : m_new;
     const float alpha = __builtin_amdgcn_exp2f(m - shift), p = seen ? __builtin_amdgcn_exp2f(s - shift) : 0.f;
@@ -254,7 +255,7 @@ __device__ __forceinline__ void chunk_rows_by_key(const ChunkArgs& g, const int3
       eight(V, i, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (seen) o[i * 8 + e] = __builtin_fmaf(p * v_scale, x[e], o[i * 8 + e] * alpha);
+        if (seen) o[i * 8 + e] = __builtin_fmaf(p * v_scale, counts ? x[e] : 0.f, o[i * 8 + e] * alpha);
     }
   }
 }

@@ -1007,11 +1007,11 @@ def bind_chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_sc
     Sequence b's tokens are rows starts[b] to starts[b + 1]; it has lengths[b] keys in the cache, the new tokens'
     own last (call :func:`cache_append` first, and count on).  ``causal``: query i sees the keys up to
     i + (keys - queries), so that the last query sees them all.  heads is a multiple of the caches' heads, ``scale``
-    defaults to dim ** -0.5.  8-bit caches count times their scales (any that are not negative).  Scores, softmax and sums
-    are in fp32; the weights are rounded to the cache's type (to fp16 for 8-bit caches) for the product with v, and for
-    16-bit caches in their sum.  Lengths past a table's pages are cut, page numbers the cache does not have hold no keys, a
-    query without keys gives zeros, and rows behind the last sequence are left alone.  ``out`` must not overlap the
-    inputs.  A call takes a workspace for keys that are split over workgroups from torch's allocator."""
+    defaults to dim ** -0.5.  8-bit caches count times their scales (any that are not negative; values of a v scale below
+    2^-64 are zeros).  Scores, softmax and sums are in fp32; the weights are rounded to the cache's type (to fp16 for 8-bit
+    caches) for the product with v, and for 16-bit caches in their sum.  Lengths past a table's pages are cut, page numbers
+    the cache does not have hold no keys, a query without keys gives zeros, and rows behind the last sequence are left
+    alone.  ``out`` must not overlap the inputs.  A call takes a workspace for keys that are split over workgroups from torch's allocator."""
     cache_code = check_chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale, causal, scale)
     device = _check_device(q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale)
     import torch

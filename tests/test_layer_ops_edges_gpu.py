@@ -5,12 +5,14 @@ Tolerances are those of test_layer_ops_gpu, where the norm's sum of squares may 
 which reaches the root, and two more of fp32 in each of root, quotient and products: (133 + 8) 2^-24 < 2^-16.
 """
 
+import math
+
 import pytest
 import torch
 
 from ninetoothed_amd import kernels
 
-from test_cache_ops_gpu import DEV, E4M3, F16, caches, i32, randn
+from test_cache_ops_gpu import BF16, DEV, E4M3, F16, caches, i32, paged, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +30,21 @@ def test_chunk_of_many_tokens_without_keys(tokens, cache):
         kernels.chunk_attention(q, kc[:pages], vc[:pages], t, lengths, starts, out,
                                 *(s if s is None else s[:pages] for s in scales))
         assert (out[:tokens] == 0).all() and (out[tokens:] == 7).all()
+
+
+@pytest.mark.parametrize("page", (16, 24))
+def test_chunk_a_v_scale_of_zero_holds_nothing(page):
+    # ... whatever its values are, and whether or not a masked NaN elsewhere has the rows taken key by key
+    tables, pages = paged([110], page)
+    kc, vc = caches((pages, page, 2, 64), E4M3)
+    ks, vs = (torch.full((pages, 2), 2.0**-6, device=DEV) for _ in range(2))
+    q, starts, at = randn(60, 4, 64, dtype=BF16), i32([0, 60]), lambda key: (int(tables[0, key // page]), key % page)
+    vs[at(page)[0]] = 0.0
+    vc[at(100) + (0, 5)] = math.nan
+    outs = []
+    for value in (1.0, math.nan):
+        vc[at(page + 3) + (0, 9)] = value
+        outs.append(kernels.chunk_attention(q, kc, vc, tables, i32([110]), starts, torch.empty_like(q), ks, vs))
+    seen = 100 - (110 - 60)  # the first query that sees key 100
+    assert outs[0][:seen].isfinite().all() and outs[0][seen:, :2, 5].isnan().all()
+    assert torch.equal(outs[0].nan_to_num(), outs[1].nan_to_num())
