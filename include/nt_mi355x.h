@@ -511,8 +511,9 @@ int nt_cache_copy(void* k_cache, const int64_t* k_strides, void* v_cache, const 
 
 /* What a layer runs beside its attention.
  *
- * Root-mean-square norm of rows: s = x + residual (null: x), y = s / sqrt(mean(s^2) + eps) * weight, all in fp32; total =
- * s rounded (written where there is a residual; it may lie on x or residual exactly), out = y rounded, or for out_dtype
+ * Root-mean-square norm of rows: s = x + residual (null: x), y = s / sqrt(mean(s^2) + eps) * weight, all in fp32 (the
+ * squares of elements times a power of two where their sum would pass its range); total = s rounded (written where there
+ * is a residual; it may lie on x or residual exactly), out = y rounded, or for out_dtype
  * E4M3 y / scale with scale = the largest finite |y| / 448 (2^-64 at least) of a row, or with `group` (32, 64 or 128) of
  * each so many elements: scale is [rows] or [rows, dim / group], side by side.  Infinite y are stored as NaN.  dtype F32,
  * F16 or BF16 (x, weight, residual, total; out too where it is not E4M3).  Strides are those of (row, element).

@@ -37,6 +37,13 @@ __device__ __forceinline__ uint8_t e4m3_byte(float q) {
   return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, 0.f, 0, false);
 }
 
+// A sum of squares that passes fp32's range, or has lost what lies below it and has no eps beside which that does not
+// count, is taken again of elements times a power of two, of which any 65,536 squares stay inside.
+__device__ __forceinline__ bool out_of_range(float sum, float eps) {
+  return sum > 0x1p126f || (sum < 0x1p-100f && eps < 0x1p-100f);
+}
+__device__ __forceinline__ float into_range(float sum) { return sum > 1.0f ? 0x1p-80f : 0x1p100f; }
+
 // f over the workgroup's (or for 64 lanes a row the wave's) lanes; slots: SLOTS floats of LDS that nobody
 // reads any more.  Every lane gets the same, in an order that does not change.
 template <int LANES, typename W, typename F>
@@ -67,7 +74,8 @@ __device__ __forceinline__ float row_max(float v, float* slots) {
 //   scale = max(|y| of the row or group) / 448.
 // Bound by HBM: x and residual read, total and the output written once.  A row is held in the registers of LANES
 // lanes, VECS vectors of N elements each (16 bytes of x) a lane, so that it is read once whatever comes of its sum
-// and its largest value; the weight stays in registers from row to row.
+// and its largest value; the weight stays in registers from row to row, up to four vectors a lane (of eight and more, which
+// leave no registers for it, it is read again for each row: 500 rows of 65,536 in bf16 149 us, held 278).
 template <typename T, int MODE, int LANES, int VECS>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(NormArgs g) {
   using namespace rn;
@@ -75,12 +83,13 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(NormArg
   typedef typename E::storage S;
   constexpr int N = 16 / sizeof(S), BLOCK = LANES < 256 ? 256 : LANES, ROWS = BLOCK / LANES;
   typedef Vec<S, N> V;
-  __shared__ float sums[2][SLOTS], mosts[2][SLOTS];
+  __shared__ float sums[2][SLOTS], mosts[2][SLOTS], again[SLOTS];
   const int lane = threadIdx.x % LANES;
   const int64_t step = (int64_t)gridDim.x * ROWS;
-  V w[VECS];
+  constexpr bool HELD = VECS < 8;
+  V w[HELD ? VECS : 1];
 #pragma unroll
-  for (int v = 0; v < VECS; ++v) {
+  for (int v = 0; HELD && v < VECS; ++v) {
     const int at = (v * LANES + lane) * N;
     if (at < g.dim) w[v] = *(const V*)((const S*)g.weight + at);
   }
@@ -120,15 +129,32 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(NormArg
       }
     }
     sum = row_sum<LANES>(sum, sums[turn]);
-    const float factor = 1.0f / sqrtf(sum / (float)g.dim + g.eps);
+    float eps = g.eps;
+    if (out_of_range(sum, eps)) {  // (the same in all of the row's lanes)
+      const float times = into_range(sum);
+      eps = eps * times * times;
+      sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < VECS; ++v)
+        if ((v * LANES + lane) * N < g.dim) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            s[v][e] *= times;
+            sum = __builtin_fmaf(s[v][e], s[v][e], sum);
+          }
+        }
+      sum = row_sum<LANES>(sum, again);
+    }
+    const float factor = 1.0f / sqrtf(sum / (float)g.dim + eps);
     float most = 0.f;
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
       const int at = (v * LANES + lane) * N;
       if (at < g.dim) {
+        const V by = HELD ? w[HELD ? v : 0] : *(const V*)((const S*)g.weight + at);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          s[v][e] = s[v][e] * factor * E::to_float(w[v].e[e]);
+          s[v][e] = s[v][e] * factor * E::to_float(by.e[e]);
           if (MODE == ROW8) most = fmaxf(most, finite_size(s[v][e]));
         }
       }
@@ -181,7 +207,7 @@ __global__ __launch_bounds__(256) void norm_elements_kernel(NormArgs g) {
   using namespace rn;
   typedef elem<T> E;
   typedef typename E::storage S;
-  __shared__ float sums[SLOTS], mosts[SLOTS];
+  __shared__ float sums[SLOTS], mosts[SLOTS], again[SLOTS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = g.first_row + blockIdx.x;
   const S* x = (const S*)g.x + row * g.xs[0];
@@ -196,8 +222,19 @@ __global__ __launch_bounds__(256) void norm_elements_kernel(NormArgs g) {
     sum = __builtin_fmaf(s, s, sum);
   }
   sum = row_sum<256>(sum, sums);
-  const float factor = 1.0f / sqrtf(sum / (float)g.dim + g.eps);
-  auto normed = [&](int i, float s) { return s * factor * E::to_float(((const S*)g.weight)[i * g.ws]); };
+  float eps = g.eps, times = 1.0f;
+  if (out_of_range(sum, eps)) {
+    times = into_range(sum);
+    eps = eps * times * times;
+    sum = 0.f;
+    for (int i = tid; i < g.dim; i += 256) {
+      const float s = value(i) * times;
+      sum = __builtin_fmaf(s, s, sum);
+    }
+    sum = row_sum<256>(sum, again);
+  }
+  const float factor = 1.0f / sqrtf(sum / (float)g.dim + eps);
+  auto normed = [&](int i, float s) { return s * times * factor * E::to_float(((const S*)g.weight)[i * g.ws]); };
   auto write = [&](int i, float inverse) {
     const float s = value(i), y = normed(i, s);
     if (g.residual) ((S*)g.total)[row * g.ts[0] + i * g.ts[1]] = E::from_float(s);

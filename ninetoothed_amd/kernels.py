@@ -1011,7 +1011,8 @@ def bind_chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_sc
     2^-64 are zeros).  Scores, softmax and sums are in fp32; the weights are rounded to the cache's type (to fp16 for 8-bit
     caches) for the product with v, and for 16-bit caches in their sum.  Lengths past a table's pages are cut, page numbers
     the cache does not have hold no keys, a query without keys gives zeros, and rows behind the last sequence are left
-    alone.  ``out`` must not overlap the inputs.  A call takes a workspace for keys that are split over workgroups from torch's allocator."""
+    alone.  ``out`` must not overlap the inputs.  A call takes a workspace for keys that are split over workgroups from
+    torch's allocator."""
     cache_code = check_chunk_attention(q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale, causal, scale)
     device = _check_device(q, k_cache, v_cache, tables, lengths, starts, out, k_scale, v_scale)
     import torch
@@ -1149,7 +1150,8 @@ def bind_rms_norm(x, weight, out, residual=None, total=None, scale=None, eps=1e-
     x, weight, residual and total share one dtype (fp32, fp16 or bf16), as out does, or out is ``torch.float8_e4m3fn``:
     then it holds y / scale, with scale [rows], or [rows, dim / group] for groups of 32, 64 or 128 elements, the largest
     finite |y| of the row or group over 448 (2^-64 at least).  Infinities are stored as NaN there.  Squares
-    and their sum are in fp32, so elements past 2^63 give rows of zeros.  Any strides; up to 65536 elements.
+    and their sum are in fp32, of elements times a power of two where they would pass its range.  Any strides; up to 65536
+    elements.
     ``out`` may be x, and ``total`` x or the residual; else what is written must not overlap anything."""
     group = check_rms_norm(x, weight, out, residual, total, scale, eps)
     device = _check_device(x, weight, out, residual, total, scale)

@@ -12,9 +12,47 @@ import torch
 
 from ninetoothed_amd import kernels
 
-from test_cache_ops_gpu import BF16, DEV, E4M3, F16, caches, i32, paged, randn
+from test_cache_ops_gpu import BF16, DEV, E4M3, F16, F32, caches, i32, paged, randn
+from test_layer_ops_gpu import check_norm
 
 pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- norm
+@pytest.mark.parametrize("out", ("same", "row", 64))
+@pytest.mark.parametrize("residual", (False, True))
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("rows,dim,step", ((5, 64, 1), (4, 1024, 1), (3, 4096, 1), (2, 16384, 1), (1, 65536, 1), (3, 4096, 2)))
+def test_norm_of_elements_whose_squares_pass_fp32(rows, dim, step, dtype, residual, out):
+    # Sums of squares from 2^112 to 2^256, and (with an eps of zero) down to 2^-194.
+    for power, eps in ((56, 1e-5), (58, 1e-5), (63, 1e-5), (64, 1e-5), (100, 1e-5), (120, 1e-5), (58, 0.0), (-40, 0.0), (-50, 0.0),
+                       (-60, 1e-35), (-75, 0.0), (-100, 0.0)):
+        x, weight = randn(rows, dim * step, dtype=dtype)[:, ::step].mul_(2.0**power), randn(dim, dtype=dtype, seed=1)
+        r = randn(rows, dim, dtype=dtype, seed=2).mul_(2.0**power) if residual else None
+        total = torch.full_like(r, math.nan) if residual else None
+        y = torch.full((rows, dim), 7.0, device=DEV).to(dtype if out == "same" else E4M3)
+        group = out if isinstance(out, int) else 0
+        scale = None if out == "same" else torch.full((rows, dim // group) if group else (rows,), math.nan, device=DEV)
+        kernels.rms_norm(x, weight, y, residual=r, total=total, scale=scale, eps=eps)
+        check_norm(x, weight, y, r, total, scale, group, eps)
+
+
+@pytest.mark.parametrize("dim", (128, 1000, 4096))
+def test_norm_beside_rows_whose_squares_pass_fp32(dim):
+    # ordinary rows keep their bits, whatever their neighbours hold; infinities and NaN as ever
+    x, weight = randn(300, dim, dtype=BF16), randn(dim, dtype=BF16, seed=1)
+    want = kernels.rms_norm(x, weight, torch.empty_like(x))
+    odd = x.clone()
+    odd[::3] *= 2.0**70
+    odd[1, 3], odd[4, 5], odd[7, 0] = math.inf, math.nan, -math.inf
+    odd[1, 9] = odd[4, 9] = 2.0**100
+    got = kernels.rms_norm(odd, weight, torch.empty_like(x))
+    keep = [i for i in range(300) if i % 3 and i not in (1, 4, 7)]
+    assert torch.equal(got[keep], want[keep])
+    check_norm(odd[::3], weight, got[::3], None, None, None, 0, 1e-6)
+    assert got[4].isnan().all()
+    for row, at in ((1, 3), (7, 0)):
+        assert got[row, at].isnan() and (got[row, :at] == 0).all() and (got[row, at + 1:] == 0).all()
 
 
 # --------------------------------------------------------------------------------------------- chunk
