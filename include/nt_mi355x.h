@@ -526,8 +526,9 @@ int nt_rms_norm(const void* x, const int64_t* x_strides, const void* weight, int
 /* out [rows, n] = c + x [rows, k] W^T, W[n][k] = scales[n][k / group] * (q[n][k] - zeros[n][k / group]) with q of 4
  * bits, two to a byte of weight [n, k / 2] (element 2 i in the lower half of byte i); zeros null: 8, c null: 0.
  * x, scales, zeros, c and out are of dtype F16 or BF16.  Strides are those of (row, element), in elements (weight:
- * bytes).  group a multiple of 32 that divides k.  Sums in fp32, rounded once.  A row of x that holds an infinity
- * gives NaN.  out may lie on c exactly, and must not overlap the others. */
+ * bytes).  group a multiple of 32 that divides k.  Sums in fp32, of (16 + q) x and (16 + zero) x, rounded once: a row of x
+ * that holds an infinity gives NaN (zeros above -16), and one of which 32 times the magnitudes of a group sum to more than
+ * fp32 holds may.  out may lie on c exactly, and must not overlap the others. */
 int nt_linear_4bit(const void* x, const int64_t* x_strides, const void* weight, const int64_t* weight_strides,
                    const void* scales, const int64_t* scale_strides, const void* zeros, const int64_t* zero_strides,
                    const void* c, const int64_t* c_strides, void* out, const int64_t* out_strides, int dtype,

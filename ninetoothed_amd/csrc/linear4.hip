@@ -416,13 +416,14 @@ __global__ __launch_bounds__(l4::TILE_WAVES * 64) __attribute__((amdgpu_waves_pe
 }
 
 // The same element by element, for any strides and alignment: a wave a column, ROWS rows at a time, its lanes along k.
+// (An infinite x is NaN here too, as it is in the sums above: zero times it is added.)
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void linear4_elements_kernel(Linear4Args g) {
   const int lane = threadIdx.x & 63;
   const int64_t m_tiles = (g.rows + ROWS - 1) / ROWS, id = (g.first + blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t m0 = id % m_tiles * ROWS, n = id / m_tiles;
   if (n >= g.n) return;
-  float acc[ROWS] = {};
+  float acc[ROWS] = {}, none[ROWS] = {};
   for (int64_t k = 2 * lane; k < g.k; k += 128) {
     const uint32_t byte = g.weight[n * g.ws[0] + k / 2 * g.ws[1]];
     const int64_t group = k / g.group;  // (an even number of elements)
@@ -433,13 +434,14 @@ __global__ __launch_bounds__(256) void linear4_elements_kernel(Linear4Args g) {
     for (int m = 0; m < ROWS; ++m) {
       if (m0 + m >= g.rows) break;
       const uint16_t* x = (const uint16_t*)g.x + (m0 + m) * g.xs[0];
-      acc[m] = __builtin_fmaf(w0, elem<T>::to_float(x[k * g.xs[1]]), acc[m]);
-      acc[m] = __builtin_fmaf(w1, elem<T>::to_float(x[(k + 1) * g.xs[1]]), acc[m]);
+      const float x0 = elem<T>::to_float(x[k * g.xs[1]]), x1 = elem<T>::to_float(x[(k + 1) * g.xs[1]]);
+      acc[m] = __builtin_fmaf(w1, x1, __builtin_fmaf(w0, x0, acc[m]));
+      none[m] = __builtin_fmaf(0.f, x1, __builtin_fmaf(0.f, x0, none[m]));
     }
   }
 #pragma unroll
   for (int m = 0; m < ROWS; ++m) {
-    float y = wave_sum(acc[m]);
+    float y = wave_sum(acc[m] + none[m]);
     if (lane != m || m0 + m >= g.rows) continue;
     if (g.c) y += elem<T>::to_float(((const uint16_t*)g.c)[(m0 + m) * g.cs[0] + n * g.cs[1]]);
     ((uint16_t*)g.out)[(m0 + m) * g.os[0] + n * g.os[1]] = elem<T>::from_float(y);

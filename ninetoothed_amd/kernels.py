@@ -1237,8 +1237,10 @@ def bind_linear_4bit(x, weight, scales, out, zeros=None, c=None):
 
     ``weight`` [n, k // 2] (``torch.uint8``) holds two values q of 0 to 15 a byte, element 2 i in the lower four bits
     of byte i; the group, k // scales.shape[1], is a multiple of 32.  ``zeros`` of None are 8.  ``c`` (None: nothing) may be
-    a residual or an expanded bias.  All else is of one dtype, fp16 or bf16.  Sums are in fp32 and rounded once; a row
-    of x that holds an infinity gives NaN.  ``out`` may be c, and must not overlap the others.
+    a residual or an expanded bias.  All else is of one dtype, fp16 or bf16.  Sums are in fp32, of (16 + q) x and
+    (16 + zero) x, and rounded once; a row of x that holds an infinity gives NaN (with zeros above -16), and one of
+    which 32 times the magnitudes of a group sum to more than fp32 holds may.  ``out`` may be c, and must not overlap
+    the others.
     :func:`quantize_4bit` makes the weights."""
     group = check_linear_4bit(x, weight, scales, out, zeros, c)
     device = _check_device(x, weight, scales, out, zeros, c)

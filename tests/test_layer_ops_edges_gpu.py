@@ -13,7 +13,7 @@ import torch
 from ninetoothed_amd import kernels
 
 from test_cache_ops_gpu import BF16, DEV, E4M3, F16, F32, caches, i32, paged, randn
-from test_layer_ops_gpu import check_norm
+from test_layer_ops_gpu import check_linear, check_norm, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -53,6 +53,32 @@ def test_norm_beside_rows_whose_squares_pass_fp32(dim):
     assert got[4].isnan().all()
     for row, at in ((1, 3), (7, 0)):
         assert got[row, at].isnan() and (got[row, :at] == 0).all() and (got[row, at + 1:] == 0).all()
+
+
+# -------------------------------------------------------------------------------------------- linear
+def unaligned(t):
+    return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("dtype", (F16, BF16))
+@pytest.mark.parametrize("rows,n", ((2, 40), (20, 40), (90, 40), (130, 6400)))
+def test_linear_of_infinite_x(rows, n, dtype, zeros):
+    """A row with an infinity is NaN, whichever form the call's strides and sizes take; the other rows keep their bits."""
+    k = 256
+    weight, scales, z = weights(n, k, 64, dtype, zeros)
+    x = randn(rows, k, dtype=dtype)
+    odd = x.clone()
+    odd[1, 7], odd[rows - 1, k - 1] = math.inf, -math.inf
+    rest = [i for i in range(rows) if i not in (1, rows - 1)]
+    for form in (lambda t: t, unaligned, lambda t: t.t().contiguous().t(), lambda t: t.repeat_interleave(2, 1)[:, ::2]):
+        for w in (weight, weight.t().contiguous().t()):
+            for c in (None, randn(rows, n, dtype=dtype, seed=4)):
+                want = kernels.linear_4bit(form(x), w, scales, torch.empty(rows, n, dtype=dtype, device=DEV), zeros=z, c=c)
+                got = kernels.linear_4bit(form(odd), w, scales, torch.empty_like(want), zeros=z, c=c)
+                assert got[1].isnan().all() and got[rows - 1].isnan().all()
+                assert torch.equal(got[rest], want[rest])
+                check_linear(x, weight, scales, want, z, c)
 
 
 # --------------------------------------------------------------------------------------------- chunk
