@@ -284,10 +284,13 @@ __global__ __launch_bounds__(l4::TILE_WAVES * 64) __attribute__((amdgpu_waves_pe
   __shared__ __attribute__((aligned(16))) float sums[2][PARTS][ROWS];
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // The row tiles of a column tile go to one XCD, one after the other (workgroups go round the eight).
-  const int64_t m_tiles = (g.rows + ROWS - 1) / ROWS, id = g.first + blockIdx.x;
-  const int64_t n0 = (id / 8 / m_tiles * 8 + id % 8) * (NW * 32), m0 = id / 8 % m_tiles * ROWS;
-  if (n0 >= g.n) return;
+  // Tiles one below the other share their weights: an XCD takes an eighth of them all, in that order (workgroups go round
+  // the eight).  (With whole columns of tiles to an XCD, as many of them idle as there are columns short of a multiple of
+  // eight: k of 4,096, 9,700 rows by 128 columns 140 us, so 47; 4,800 by 512 90 and 57; 1,300 by 1,152 52 and 42.)
+  const int64_t m_tiles = (g.rows + ROWS - 1) / ROWS, tiles_all = m_tiles * ((g.n + NW * 32 - 1) / (NW * 32));
+  const int64_t id = g.first + blockIdx.x, tile = id % 8 * ((tiles_all + 7) / 8) + id / 8;
+  if (tile >= tiles_all) return;
+  const int64_t n0 = tile / m_tiles * (NW * 32), m0 = tile % m_tiles * ROWS;
   const int k = (int)g.k, steps = (k + STEP - 1) / STEP;
   const int64_t n = min(n0 + wave * 32 + col, g.n - 1);  // (columns past the end repeat the last, and rows too)
   const uint8_t* W = g.weight + n * g.ws[0] + half * DWORDS * 4;
@@ -343,7 +346,7 @@ __global__ __launch_bounds__(l4::TILE_WAVES * 64) __attribute__((amdgpu_waves_pe
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
   auto take = [&](const Weights& t, int step) __attribute__((always_inline)) {
-    const char* tile = tiles[step & 1] + col * ROW;
+    const char* x = tiles[step & 1] + col * ROW;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
       const auto both = __builtin_amdgcn_permlane32_swap(t.sz[p], t.sz[p], false, false);
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(l4::TILE_WAVES * 64) __attribute__((amdgpu_waves_pe
         const frag fw = __builtin_bit_cast(frag, wide8<T>(t.w[j].e[d]));
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-          const frag fx = __builtin_bit_cast(frag, *(const u32x4*)(tile + i * 32 * ROW + ((chunk ^ (col & 15)) * 16)));
+          const frag fx = __builtin_bit_cast(frag, *(const u32x4*)(x + i * 32 * ROW + ((chunk ^ (col & 15)) * 16)));
           part[i] = mfma_traits<T>::mma(fx, fw, part[i]);
         }
       }
@@ -466,7 +469,7 @@ static void linear4_blocks(Linear4Args g, hipStream_t stream) {
 template <typename T>
 static void linear4_tiles(Linear4Args g, hipStream_t stream) {
   constexpr int block = l4::TILE_WAVES * 64, cols = l4::TILE_WAVES * 32;
-  in_launches(cdiv(g.rows, l4::TILE_ROWS) * cdiv(cdiv(g.n, cols), 8) * 8, block, [&](int64_t first, unsigned count) {
+  in_launches(cdiv(cdiv(g.rows, l4::TILE_ROWS) * cdiv(g.n, cols), 8) * 8, block, [&](int64_t first, unsigned count) {
     g.first = first;
     if (g.group % 128 == 0)
       hipLaunchKernelGGL((linear4_tiles_kernel<T, 4>), dim3(count), dim3(block), 0, stream, g);
@@ -490,8 +493,10 @@ static int linear4_launch(Linear4Args g, hipStream_t stream) {
     return launch_status();
   }
   // Tiles of 64 rows take their weights once for all of them, but whole rows of k: they win where there is one for more
-  // than every second CU (us, tiles against blocks: 300 rows by 11,008, 430 tiles: 56 | 115; 128 by 11,008, 172 tiles: 41 | 50;
-  // 256 by 4,096, 128 tiles: 41 | 35; 192 by 4,096, 96 tiles: 51 | 32).
+  // than every second CU.  Both sides' time grows with k, and the border hardly moves with it, or with the group: the rule is
+  // within a fifth of the better side.  (us, tiles | blocks, at 96, 128, 160 and 192 tiles; k of 4,096, groups of 128: 41 | 28,
+  // 42 | 36, 43 | 43, 42 | 52; k of 1,024: 14 | 12, 14 | 16, 14 | 20, 15 | 23; k of 11,008: 100 | 62, 100 | 82, 100 | 101,
+  // 100 | 122; in groups of 32: 164 | 85, 164 | 110, 165 | 138, 166 | 165.)
   if (g.rows > 64 && cdiv(g.rows, l4::TILE_ROWS) * cdiv(g.n, l4::TILE_WAVES * 32) >= 150)
     linear4_tiles<T>(g, stream);
   else if (g.rows <= 16)

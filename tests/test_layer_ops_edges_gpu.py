@@ -81,6 +81,17 @@ def test_linear_of_infinite_x(rows, n, dtype, zeros):
                 check_linear(x, weight, scales, want, z, c)
 
 
+@pytest.mark.parametrize("rows,k,n,group", ((9700, 4096, 128, 128), (4800, 1024, 512, 64), (1300, 1024, 1152, 32), (9601, 256, 100, 128),
+                                            (1210, 384, 1030, 128), (4736, 128, 257, 32)))
+def test_linear_of_many_rows_and_few_columns(rows, k, n, group):
+    """As test_linear_of_many_rows, of up to 9 tiles of columns."""
+    x, (weight, scales, z) = randn(rows, k, dtype=BF16), weights(n, k, group, BF16, True)
+    for c in (None, randn(n, rows, dtype=BF16, seed=5).t()):
+        out = torch.full((rows, n), math.nan, dtype=BF16, device=DEV)
+        kernels.linear_4bit(x, weight, scales, out, zeros=z, c=c)
+        check_linear(x, weight, scales, out, z, c, roundings=2 * group + 2 + k / group)
+
+
 # --------------------------------------------------------------------------------------------- chunk
 @pytest.mark.parametrize("cache", (F16, E4M3))
 @pytest.mark.parametrize("tokens", (1, 300, 2000))
