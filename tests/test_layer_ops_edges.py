@@ -3,8 +3,9 @@
 import ctypes
 
 import pytest
+import torch
 
-from ninetoothed_amd import _lib
+from ninetoothed_amd import _lib, kernels
 
 INVALID, P = 1, 1 << 12  # (an address that nothing reads: each call returns before a launch)
 
@@ -21,3 +22,10 @@ def test_chunk_workspace_of_calls_without_keys(tokens, pages, width):
         assert lib.nt_chunk_attention(P, strides, P, strides, P, strides, 1, None, None, P, strides, 1, P, width, P, P, tokens, 2,
                                       8, 2, 64, pages, 16, width, 1.0, 1, None, P, without - 1) == INVALID
     assert lib.nt_chunk_attention_workspace_size(tokens, 2, 8, 2, 64, 16, -1, _lib.DTYPE_F16) == 0
+
+
+def test_quantized_weights_keep_no_graph():
+    # (of a parameter: scales that ask for a gradient would keep its copy in fp32 alive)
+    w = torch.nn.Parameter(torch.randn(8, 64).to(torch.float16))
+    for symmetric in (False, True):
+        assert not any(t.requires_grad for t in kernels.quantize_4bit(w, 32, symmetric) if t is not None)
