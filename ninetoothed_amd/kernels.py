@@ -1187,7 +1187,8 @@ def quantize_4bit(w, group=128, symmetric=False):
     n, k = w.shape
     if group < 32 or group % 32 or k % group:
         raise ValueError("the group must be a multiple of 32 that divides k")
-    x = w.detach().float().view(n, k // group, group)
+    # (contiguous: linear_4bit reads rows of 16 bytes, whatever order w lies in)
+    x = w.detach().float().contiguous().view(n, k // group, group)
     if symmetric:
         scales = (x.abs().amax(-1) / 7).to(w.dtype)
         zeros, shift = None, 8.0

@@ -29,3 +29,14 @@ def test_quantized_weights_keep_no_graph():
     w = torch.nn.Parameter(torch.randn(8, 64).to(torch.float16))
     for symmetric in (False, True):
         assert not any(t.requires_grad for t in kernels.quantize_4bit(w, 32, symmetric) if t is not None)
+
+
+def test_quantized_weights_lie_row_by_row():
+    # linear_4bit reads rows of 16 bytes at a time; what the weights were made from may lie in any order
+    w = torch.randn(64, 128, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    for symmetric in (False, True):
+        want = kernels.quantize_4bit(w, 32, symmetric)
+        for other in (w.t().contiguous().t(), torch.cat([w, w], 1)[:, :128], w.repeat_interleave(2, 0)[::2]):
+            got = kernels.quantize_4bit(other, 32, symmetric)
+            for a, b in zip(got, want):
+                assert a is b is None or (torch.equal(a, b) and a.is_contiguous())
