@@ -12,8 +12,9 @@ import torch
 
 from ninetoothed_amd import kernels
 
-from test_cache_ops_gpu import BF16, DEV, E4M3, F16, F32, caches, i32, paged, randn
-from test_layer_ops_gpu import check_linear, check_norm, weights
+from test_cache_ops_gpu import (BF16, DEV, E4M3, F16, F32, attended, caches, check_append, close, half_step, i32, paged, randn,
+                                starts_of)
+from test_layer_ops_gpu import Layer, check_linear, check_norm, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +124,109 @@ def test_chunk_a_v_scale_of_zero_holds_nothing(page):
     seen = 100 - (110 - 60)  # the first query that sees key 100
     assert outs[0][:seen].isfinite().all() and outs[0][seen:, :2, 5].isnan().all()
     assert torch.equal(outs[0].nan_to_num(), outs[1].nan_to_num())
+
+
+# ------------------------------------------------------------------------------------------ together
+def prompts(cache, dtype, pages, width, pieces):
+    """A layer with the prompts' pieces of three sequences in its cache, and a function that goes on from there."""
+    layer = Layer(cache, dtype, pages)
+    n, total = layer.heads * layer.dim, [sum(p[b] for p in pieces) for b in range(3)]
+    x, r = ([randn(total[b], n, dtype=dtype, seed=s + b, scale=scale) for b in range(3)] for s, scale in ((0, 1.0), (10, 2.0)))
+    tables, lengths, at = torch.arange(3 * width, device=DEV).view(3, width).to(torch.int32), i32([0, 0, 0]), [0, 0, 0]
+    for rows in pieces:
+        take = lambda t: torch.cat([t[b][at[b]:at[b] + m] for b, m in enumerate(rows)])  # noqa: E731
+        positions = torch.cat([torch.arange(at[b], at[b] + m) for b, m in enumerate(rows)]).to(DEV)
+        layer.step(layer.buffers(sum(rows)), take(x), take(r), tables, lengths, starts_of(rows), positions)
+        at = [a + m for a, m in zip(at, rows)]
+    return layer, tables, lengths, at
+
+
+@pytest.mark.parametrize("cache,dtype", ((BF16, BF16), (F16, F16), (E4M3, BF16)))
+def test_a_fork_gives_what_a_cache_of_its_own_gives(cache, dtype):
+    """Sequence 1 forks, and both go on.  The fork shares its full pages and has a copy of the begun one, or has all of its
+    pages to itself, filled byte for byte: the same bits.  Without the copy, or without the copied scales, others."""
+    pages, width, page = 60, 12, Layer.page
+    layer, tables, lengths, at = prompts(cache, dtype, pages, width, ([20, 33, 1], [60, 0, 7], [1, 40, 30]))
+    full, begun = at[1] // page, at[1] % page
+    assert full > 1 and 1 < begun < page - 3
+    n, own = layer.heads * layer.dim, pages - 1
+    held = [t.clone() for t in (*layer.caches, *layer.scales) if t is not None]
+    new = [[randn(4, n, dtype=dtype, seed=50 + 2 * i + j, scale=1.0 + j) for j in range(2)] for i in range(3)]
+
+    def go_on(how):
+        for t, was in zip((*layer.caches, *layer.scales), held):
+            t.copy_(was)
+        fork = tables[1].clone()
+        if how == "pages of its own":
+            fork[:full + 1] = torch.arange(pages - full - 2, own, device=DEV)
+            for t in (*layer.caches, *layer.scales):
+                if t is not None:
+                    t = t.view(torch.uint8) if t.dtype == E4M3 else t
+                    t[fork[:full + 1].long()] = t[tables[1, :full + 1].long()]
+        else:
+            fork[full] = own
+            if how != "no copy":
+                kernels.cache_copy(*layer.caches, tables[1, full:full + 1].contiguous(), i32([own]), *layer.scales,
+                                   counts=i32([begun]))
+            if how == "no scales":
+                for s in layer.scales:
+                    s[own] = 1.0
+        all_tables, all_lengths, got = torch.cat([tables, fork[None]]), torch.cat([lengths, lengths[1:2]]), []
+        for x, r in new:
+            b = layer.buffers(4)
+            residual, up = layer.step(b, x, r.clone(), all_tables, all_lengths, starts_of([1] * 4), all_lengths.long())
+            got += [residual, up, b["out"]]
+        return got
+
+    want = go_on("pages of its own")
+    for a, b in zip(go_on("copy"), want):
+        assert torch.equal(a, b)
+    for how in ("no copy", "no scales") if layer.eight else ("no copy",):
+        for a, b in zip(go_on(how), want):
+            assert torch.equal(a[:3], b[:3]) and not torch.equal(a[3], b[3]), how
+
+
+@pytest.mark.parametrize("cache,dtype", ((BF16, BF16), (F16, F16), (E4M3, BF16)))
+def test_each_stage_of_a_layer(cache, dtype):
+    """Each operator of a layer's step against 64 bits of what it was given, for a mix of pieces and single tokens."""
+    pages, width = 40, 12
+    layer, tables, lengths, at = prompts(cache, dtype, pages, width, ([20, 33, 1], [60, 0, 7]))
+    n, kv, rows = layer.heads * layer.dim, layer.kv_heads * layer.dim, [1, 40, 30]
+    b, starts = layer.buffers(sum(rows)), starts_of(rows)
+    positions = torch.cat([torch.arange(a, a + m) for a, m in zip(at, rows)]).to(DEV)
+    x, residual = randn(sum(rows), n, dtype=dtype, seed=3), randn(sum(rows), n, dtype=dtype, seed=4, scale=2.0)
+    was = residual.clone()
+    kernels.rms_norm(x, layer.norms[0], b["h"], residual=residual)
+    check_norm(x, layer.norms[0], b["h"], was, residual, None, 0, 1e-6)
+    kernels.linear_4bit(b["h"], *layer.qkv[:2], b["qkv"], zeros=layer.qkv[2])
+    check_linear(b["h"], *layer.qkv[:2], b["qkv"], layer.qkv[2], None)
+    q = b["qkv"][:, :n].view(-1, layer.heads, layer.dim)
+    k, v = (b["qkv"][:, n + i * kv:n + (i + 1) * kv].view(-1, layer.kv_heads, layer.dim) for i in range(2))
+    before = [None if t is None else t.clone() for t in (*layer.caches, *layer.scales)]
+    kernels.rotary(q, positions, layer.freqs, q)
+    kernels.cache_append(k, v, *layer.caches, tables, lengths, starts, *layer.scales, freqs=layer.freqs)
+    check_append(k, v, *layer.caches, *layer.scales, before, tables, at, rows, layer.page, layer.freqs, False)
+    lengths.add_(starts[1:] - starts[:-1])
+    o = b["out"].view(-1, layer.heads, layer.dim)
+    kernels.chunk_attention(q, *layer.caches, tables, lengths, starts, o, *layer.scales)
+    weight_type, first = F16 if layer.eight else dtype, 0
+    for s, (a, m) in enumerate(zip(at, rows)):
+        held = tables[s].long()
+        kk, vv = ((c.double() * (1.0 if e is None else e.double()[:, None, :, None]))[held].flatten(0, 1)[:a + m]
+                  for c, e in zip(layer.caches, layer.scales))
+        for h in range(layer.heads):
+            g = h // (layer.heads // layer.kv_heads)
+            want, size = attended(q[first:first + m, h], kk[:, g], vv[:, g], layer.dim**-0.5, torch.arange(a, a + m, device=DEV))
+            tol = half_step(dtype) * want.abs() + half_step(weight_type) * (want.abs() + size) + 2.0**-12 * size
+            close(o[first:first + m, h], want, tol + (a + m) * 2.0**-25 * float(vv.abs().max()) + 1e-30, f"sequence {s}, head {h}")
+        first += m
+    was = residual.clone()
+    kernels.linear_4bit(b["out"], *layer.o[:2], residual, zeros=layer.o[2], c=residual)
+    check_linear(b["out"], *layer.o[:2], residual, layer.o[2], was)
+    kernels.rms_norm(residual, layer.norms[1], b["y"], scale=b["scale"])
+    check_norm(residual, layer.norms[1], b["y"], None, None, b["scale"], 0, 1e-6)
+    kernels.gemm(b["y"], layer.up, b["up"])
+    y, up = b["y"].double(), layer.up.double()
+    # (sums of n products in fp32, twice the roundings for the matrix core's order, and one rounding to fp16)
+    tol = (y @ up).abs() * 2.0**-11 + y.abs() @ up.abs() * n * 2.0**-23 + 2.0**-25
+    close(b["up"], y @ up, tol, "up")
