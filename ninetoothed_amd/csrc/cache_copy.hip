@@ -22,8 +22,9 @@ constexpr int COPY_AHEAD = 4;  // vectors a lane
 // destination[:, slots] = source[:, slots] for the first counts[i] slots of pairs of pages, and the pages' scales.
 // Bound by HBM: what is copied is read and written once.  A workgroup takes a piece of one page of one cache, up to
 // COPY_AHEAD vectors a lane, all under way before the first is stored, and stored past the caches: few of a page's slots
-// are read again soon.  1,500 pages of 32 KiB in both caches 36 us (5.5 TB/s), 60 begun ones 6.2; eight vectors a lane
-// 36.7 and 6.5, stores that the caches keep 49 and 8 (eight vectors a lane 65), loads past the caches too 41 and 6.6.
+// are read again soon.  1,500 pages of 32 KiB in both caches 35 us (5.6 TB/s), 60 begun ones 5, a launch; tried beside 36 and
+// 6.2 of another measurement: eight vectors a lane 36.7 and 6.5, stores that the caches keep 49 and 8 (eight vectors a lane
+// 65), loads past the caches too 41 and 6.6.
 // B: bytes of a vector.
 template <int B>
 __global__ __launch_bounds__(256) void cache_copy_kernel(CopyArgs g) {

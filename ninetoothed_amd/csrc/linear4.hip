@@ -104,8 +104,10 @@ __device__ __forceinline__ float over_lanes(float v) {
 // Bound by HBM for one row or a few: the weights are read once, 16 bytes a lane, by waves that share 16 columns and take
 // turns of 128 elements of k.  x comes from the L2 for each of those workgroups, by loads into LDS with a row's elements
 // in neighbouring lanes: as fragments, with a row to each lane, it took longer than all the rest (24 rows, k of 11,008,
-// 4,096 columns: 24 us, now 18, of which the weights are 5; 64 rows by 11,008 columns, k of 4,096: 59, now 28).  One row,
-// k of 4,096, 4,096 columns: 5 us, a launch.  A wave's 16 x 16 x 32 products take 32 neighbouring elements of k, which
+// 4,096 columns: 24 us, now 16, of which the weights are 5; 64 rows by 11,008 columns, k of 4,096: 59, now 29).  One row,
+// k of 4,096, 4,096 columns: 5 us, a launch.  Two turns are sent for at a time, but not kept under way over each other's
+// products: a load into LDS is not in the compiler's count, and where the last turn is not sent its waits take the smallest
+// count, so that each turn's products wait for all that was sent.  A wave's 16 x 16 x 32 products take 32 neighbouring elements of k, which
 // lie in one group, so a turn's four dwords go across the quads first.
 // MB: blocks of 16 rows; SUB: products of a turn that share a group.
 template <typename T, int MB, int SUB>
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
       }
     }
   };
-  // (each turn's registers keep their place: a copy would wait for what they were sent for)
+  // (each turn's registers keep their place, without copies)
   Turn turns[STAGES];
 #pragma unroll
   for (int i = 0; i < STAGES; ++i)
@@ -269,10 +271,11 @@ __global__ __launch_bounds__(l4::WAVES * 64) void linear4_kernel(Linear4Args g) 
 // each weight is widened once for all of the rows, from the registers that it was loaded into.  x passes through two
 // LDS stages of 128 elements of k, in the weights' order of pairs, and is summed on its way.  A lane's weights of a
 // 32 x 32 x 16 product are its next eight: which of k's elements a product takes is free, if both operands agree.  A
-// group's sum starts at -(16 + zero) sum x and is scaled once.  300 rows by 11,008 columns, k of 4,096: 53 us, 510 TFLOP/s
-// (115 us in the blocks above); no one part bounds it: without its loads, without the staging of x or without the products
-// with their widening it is 10 to 25 us shorter, and eight waves beside each other (256 columns) or twice the rows, with
-// as many registers, gain nothing.
+// group's sum starts at -(16 + zero) sum x and is scaled once.  300 rows by 11,008 columns, k of 4,096: 53 to 56 us, 480 to
+// 510 TFLOP/s (114 in the blocks above); 5,000 rows: 731, 617 TFLOP/s.  No one part bounds it: without its loads, without the
+// staging of x or without the products with their widening the 300 rows take 10 to 25 us less, as each waits for the
+// others (where a step ahead may not be sent, the waits for x take in the weights sent behind it); eight waves beside each
+// other (256 columns) or twice the rows, with as many registers, gain nothing.
 template <typename T, int SUB>
 __global__ __launch_bounds__(l4::TILE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear4_tiles_kernel(Linear4Args g) {
   using namespace l4;
@@ -381,7 +384,7 @@ __global__ __launch_bounds__(l4::TILE_WAVES * 64) __attribute__((amdgpu_waves_pe
       __builtin_amdgcn_sched_barrier(0);  // (a part's fragments at a time: there are registers for no more)
     }
   };
-  // Weights are sent for some steps ahead, and x two; each set of registers keeps its place (a copy would wait for them).
+  // Weights are sent for some steps ahead, and x two; each set of registers keeps its place, without copies.
   constexpr int AHEAD = SUB == 1 ? 2 : 3;
   Weights w[AHEAD];
   if (steps > 0) {
