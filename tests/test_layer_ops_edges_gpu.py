@@ -230,3 +230,102 @@ def test_each_stage_of_a_layer(cache, dtype):
     # (sums of n products in fp32, twice the roundings for the matrix core's order, and one rounding to fp16)
     tol = (y @ up).abs() * 2.0**-11 + y.abs() @ up.abs() * n * 2.0**-23 + 2.0**-25
     close(b["up"], y @ up, tol, "up")
+
+
+# --------------------------------------------------------------------------------------------- large
+def test_norm_past_32_bits():
+    rows, dim = 540_000, 4096  # x, residual and output of 4.4 GB each
+    x = torch.empty(rows, dim, dtype=BF16, device=DEV).normal_()
+    r, weight, out = x.flip(1), randn(dim, dtype=BF16, seed=1), torch.empty_like(x)
+    tail = [t[-50:].clone() for t in (x, r)]
+    kernels.rms_norm(x, weight, out, residual=r)
+    check_norm(tail[0], weight, out[-50:], tail[1], r[-50:], None, 0, 1e-6)
+    scale, y = torch.empty(rows, dim // 32, device=DEV), torch.empty(rows, dim, dtype=E4M3, device=DEV)
+    kernels.rms_norm(x, weight, y, scale=scale)
+    check_norm(x[-50:], weight, y[-50:], None, None, scale[-50:], 32, 1e-6)
+    columns = x.view(dim, rows).t()  # (the form for any strides)
+    kernels.rms_norm(columns, weight, r)
+    check_norm(columns[-50:], weight, r[-50:], None, None, None, 0, 1e-6)
+
+
+@pytest.mark.parametrize("rows,k,n", ((540_000, 4096, 64), (300_000, 64, 8192), (3, 8192, 1_100_000), (70, 8192, 1_100_000)))
+def test_linear_past_32_bits(rows, k, n):
+    # x, the output, or the weights, of more than 4 GB
+    x, (weight, scales, z) = torch.empty(rows, k, dtype=BF16, device=DEV).normal_(), weights(32, k, 32, BF16, True)
+    weight, scales, z = (t.repeat(-(-n // 32), 1)[:n] for t in (weight, scales, z))
+    out = torch.full((rows, n), math.nan, dtype=BF16, device=DEV)
+    kernels.linear_4bit(x, weight, scales, out, zeros=z)
+    for at in (slice(0, 3), slice(rows - 3, rows)):
+        for cols in (slice(0, 40), slice(n - 40, n)):
+            check_linear(x[at], weight[cols], scales[cols], out[at, cols], z[cols], None, roundings=2 * 32 + 2 + k / 32)
+
+
+def test_chunk_past_32_bits():
+    tokens, heads, kv_heads, dim = 540_000, 32, 8, 128  # q and out of 4.4 GB
+    q = torch.empty(tokens, heads, dim, dtype=BF16, device=DEV).normal_()
+    kc, vc = caches((6, 32, kv_heads, dim), BF16)
+    tables, keys, starts = i32([[0, 1, 2], [3, 4, 5]]), [70, 90], i32([0, tokens - 100, tokens])
+    out = torch.full_like(q, math.nan)
+    kernels.chunk_attention(q, kc, vc, tables, i32(keys), starts, out, causal=False)
+    for b, rows in ((0, slice(tokens - 150, tokens - 100)), (1, slice(tokens - 100, tokens))):
+        for head in (0, 13, 31):
+            kk, vv = (c[tables[b].long(), :, head // 4].flatten(0, 1)[:keys[b]] for c in (kc, vc))
+            want, size = attended(q[rows, head], kk, vv, dim**-0.5)
+            tol = half_step(BF16) * (2 * want.abs() + size) + 2.0**-12 * size
+            close(out[rows, head], want, tol + keys[b] * 2.0**-25 * float(vv.abs().max()) + 1e-30)
+
+
+# --------------------------------------------------------------------------------------- other calls
+@pytest.mark.parametrize("cache", (F16, E4M3))
+@pytest.mark.parametrize("heads,kv_heads", ((300, 1), (3, 3), (64, 2)))
+def test_chunk_of_wide_groups_and_shared_pages(heads, kv_heads, cache):
+    """More heads of q to one of k than a block has rows; tables that share pages, among them one row for all sequences."""
+    for dim, page in ((16, 16), (48, 24), (128, 128)):
+        new, keys = [2, 0, 5, 1], [150, 9, 200, 40]
+        kc, vc = caches((9, page, kv_heads, dim), cache)
+        ks, vs = ((torch.full((9, kv_heads), 2.0**-7, device=DEV) for _ in range(2)) if cache == E4M3 else (None, None))
+        q = randn(8, heads, dim, dtype=F16)
+        row = (torch.arange(14, device=DEV) % 9).to(torch.int32)
+        outs = [kernels.chunk_attention(q, kc, vc, t, i32(keys), starts_of(new), torch.empty_like(q), ks, vs)
+                for t in (row.expand(4, 14), row.repeat(4, 1), torch.stack([row] * 8)[::2])]
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+        first = 0
+        for m, n in zip(new, keys):
+            last = torch.arange(n - m, n, device=DEV)
+            for head in range(0, heads, 7):
+                h = head // (heads // kv_heads)
+                kk, vv = ((c[row.long(), :, h].double() * (1.0 if s is None else s[0, 0].double())).flatten(0, 1)[:n]
+                          for c, s in ((kc, ks), (vc, vs)))
+                want, size = attended(q[first:first + m, head], kk, vv, dim**-0.5, last)
+                tol = half_step(F16) * (2 * want.abs() + size) + 2.0**-12 * size
+                close(outs[0][first:first + m, head], want, tol + n * 2.0**-25 * float(vv.abs().max()) + 1e-30)
+            first += m
+
+
+@pytest.mark.parametrize("cache", (BF16, E4M3))
+def test_a_captured_chunk_replays_with_other_lengths(cache):
+    """A padded batch: sequences, tables and lengths change between the replays, and the rows behind the last one stay."""
+    q, (kc, vc) = randn(60, 8, 64, dtype=BF16), caches((200, 16, 2, 64), cache)
+    scales = [torch.full((200, 2), 2.0**-6, device=DEV) for _ in range(2)] if cache == E4M3 else [None, None]
+    order = torch.randperm(200, generator=torch.Generator().manual_seed(1)).to(torch.int32).to(DEV)
+    tables, lengths, starts, out = torch.zeros(4, 50, dtype=torch.int32, device=DEV), i32([0] * 4), i32([0] * 5), torch.zeros_like(q)
+    steps = (([5, 1, 0, 40], [100, 800, 0, 77]), ([1, 1, 1, 1], [700, 3, 9, 50]), ([0, 0, 0, 0], [4, 4, 4, 4]),
+             ([60, 0, 0, 0], [790, 0, 0, 0]), ([1, 30, 2, 1], [-1, 31, 600, 1]))
+    call = lambda o: kernels.chunk_attention(q, kc, vc, tables, lengths, starts, o, *scales)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(torch.zeros_like(q))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for i, (new, keys) in enumerate(steps * 2):
+        tables.copy_(order.roll(i).view(4, 50))
+        lengths.copy_(i32(keys))
+        starts.copy_(starts_of(new))
+        want = call(torch.full_like(q, 7.0))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and (out[sum(new):] == 7).all()
